@@ -399,6 +399,78 @@ int lbi_matrix_norms(const void* mats, float* spectral, float* frobenius,
                      void* workspace, size_t workspace_bytes,
                      int64_t N, int64_t d, int dtype, void* stream);
 
+/*
+ * The addition to the residual stream with its RMS norm, and its pullback.  The forward counterpart of lbi_rmsnorm_pullback
+ * (TransformerBlock._prenorm with RMSNorm.forward, reference backbones/transformer/block.py:12-23, :66-76), the sum kept in fp32 up to the
+ * one rounding of each result.
+ *
+ *   s = hidden + residual (residual may be NULL = 0);   y = s * rsqrt(mean(s^2) + eps) * weight
+ *   hidden, normed [rows,D] in dtype; residual, residual_out [rows,D] in residual_dtype (dtype or fp32); weight [D] in weight_dtype (dtype
+ *   or fp32).  residual_out = s, not written if NULL.  With scales [rows] (fp32) normed is e4m3, one byte an element: y divided by the
+ *   row's scale max|y| / 448 (1 for a row of zeros, at least 2^-126 otherwise).
+ *   residual_out may be residual, and hidden where the types are the same; normed may be hidden.
+ *
+ * Pullback, from residual_out:
+ *   i = rsqrt(mean(s^2) + eps), u = s i, p = g_normed * weight:   g_s = i (p - u mean(u p)) + g_residual_out (NULL = 0)
+ *   g_hidden [rows,D] (dtype) and g_residual [rows,D] (residual_dtype) are both g_s, either may be NULL;
+ *   g_weight [D] (fp32) = sum over rows of g_normed * u, in a fixed order.
+ *   g_hidden may be g_normed, g_residual may be g_residual_out.
+ *
+ * D up to 16384, fewer than 2^31 rows; tensors aligned to their elements.
+ */
+int lbi_residual_rmsnorm(const void* hidden, const void* residual, const void* weight, void* normed, void* residual_out, float* scales,
+                         int64_t rows, int64_t D, float eps, int dtype, int residual_dtype, int weight_dtype, void* stream);
+
+size_t lbi_residual_rmsnorm_pullback_workspace_bytes(int64_t rows, int64_t D);
+int lbi_residual_rmsnorm_pullback(const void* g_normed, const void* residual_out, const void* g_residual_out, const void* weight,
+                                  void* g_hidden, void* g_residual, float* g_weight, void* workspace, size_t workspace_bytes,
+                                  int64_t rows, int64_t D, float eps, int dtype, int residual_dtype, int weight_dtype, void* stream);
+
+/*
+ * The gated MLP (GatedMLP.forward, reference backbones/transformer/mlp.py:10-32; with its cache backends/transformer.py:172-188):
+ *
+ *   fc1_output = x fc1_weight^T + fc1_bias,  [up | gate] = fc1_output;  down_input = up * silu(gate);  out = down_input fc2_weight^T + fc2_bias
+ *   x [rows,D], fc1_weight [2 hidden,D], fc2_weight [width,hidden], fc1_output [rows,2 hidden] (not written if NULL),
+ *   down_input [rows,hidden] (always written: the second product reads it), out [rows,width]; a bias may be NULL.
+ *   Sums, biases and the activation in fp32; fc1_output, down_input and out are rounded once each.
+ *
+ * Pullback for one cotangent g_out [rows,width], from fc1_output and down_input as the forward left them:
+ *   g_x [rows,D], g_fc1_weight, g_fc2_weight as the weights, g_fc1_bias [2 hidden] and g_fc2_bias [width] unless NULL.
+ *   The cotangent of fc1_output is rounded once, where it is stored between the products; the weights' gradients are lbi_weight_gradient's.
+ *
+ * 16-bit types; widths multiples of 8 (pad with zeros: neither results nor gradients change), tensors 16-byte aligned, workspace
+ * 256-byte.  rows up to 2^23, widths up to 2^20; the pullback takes what lbi_weight_gradient takes, and at least one row.
+ */
+int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* fc1_bias, const void* fc2_weight, const void* fc2_bias,
+                  void* fc1_output, void* down_input, void* out, int64_t rows, int64_t D, int64_t hidden, int64_t width, int dtype,
+                  void* stream);
+
+size_t lbi_gated_mlp_vjp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width);
+int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* fc1_output, const void* down_input, const void* fc1_weight,
+                      const void* fc2_weight, void* g_x, void* g_fc1_weight, void* g_fc2_weight, void* g_fc1_bias, void* g_fc2_bias,
+                      void* workspace, size_t workspace_bytes, int64_t rows, int64_t D, int64_t hidden, int64_t width, int dtype,
+                      void* stream);
+
+/*
+ * Clipping of n gradients by their global norm (what the reference's training loop does after its backward pass, train/runners.py:378-380):
+ *
+ *   norm = sqrt(sum of the squares of all elements);   out = in * min(1, max_norm / (norm + 1e-6))
+ *
+ *   dtype of each tensor as above, mixed as they come; out may be in (nothing is written then if the factor is 1) or NULL (the tensor only
+ *   counts), and overlaps no other in and no other out (LBI_ERR_INVALID).  norm: one fp32 on the device.  Squares are added in 64 bits, in a
+ *   fixed order.  The list is read before the call returns; workspace 8-byte aligned, tensors aligned to their elements.
+ */
+typedef struct lbi_gradient {
+    const void* in;
+    void* out;
+    int64_t count; /* elements, contiguous */
+    int64_t dtype;
+} lbi_gradient;
+
+size_t lbi_clip_gradients_workspace_bytes(const lbi_gradient* gradients, int64_t n);
+int lbi_clip_gradients(const lbi_gradient* gradients, int64_t n, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

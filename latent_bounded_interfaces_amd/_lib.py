@@ -122,6 +122,26 @@ SYMBOLS = {
         _c.c_int,
         [_c.c_void_p] * 4 + [_c.c_size_t] + [_c.c_int64] * 4 + [_c.c_int, _c.c_void_p],
     ),
+    "lbi_residual_rmsnorm": (
+        _c.c_int,
+        [_c.c_void_p] * 6 + [_c.c_int64] * 2 + [_c.c_float] + [_c.c_int] * 3 + [_c.c_void_p],
+    ),
+    "lbi_residual_rmsnorm_pullback_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 2),
+    "lbi_residual_rmsnorm_pullback": (
+        _c.c_int,
+        [_c.c_void_p] * 8 + [_c.c_size_t] + [_c.c_int64] * 2 + [_c.c_float] + [_c.c_int] * 3 + [_c.c_void_p],
+    ),
+    "lbi_gated_mlp": (_c.c_int, [_c.c_void_p] * 8 + [_c.c_int64] * 4 + [_c.c_int, _c.c_void_p]),
+    "lbi_gated_mlp_vjp_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 4),
+    "lbi_gated_mlp_vjp": (
+        _c.c_int,
+        [_c.c_void_p] * 12 + [_c.c_size_t] + [_c.c_int64] * 4 + [_c.c_int, _c.c_void_p],
+    ),
+    "lbi_clip_gradients_workspace_bytes": (_c.c_size_t, [_c.c_void_p, _c.c_int64]),
+    "lbi_clip_gradients": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_int64, _c.c_float, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p],
+    ),
 }
 
 
