@@ -436,14 +436,15 @@ int lbi_residual_rmsnorm_pullback(const void* g_normed, const void* residual_out
  *
  * Pullback for one cotangent g_out [rows,width], from fc1_output and down_input as the forward left them:
  *   g_x [rows,D], g_fc1_weight, g_fc2_weight as the weights, g_fc1_bias [2 hidden] and g_fc2_bias [width] unless NULL.
- *   The cotangent of fc1_output is rounded once, where it is stored between the products; the weights' gradients are lbi_weight_gradient's.
+ *   The cotangent of fc1_output is rounded once, where it is stored between the products.
  *
  * 16-bit types; widths multiples of 8 (pad with zeros: neither results nor gradients change), tensors 16-byte aligned, workspace
- * 256-byte.  rows up to 2^23, widths up to 2^20; the pullback takes what lbi_weight_gradient takes, and at least one row.
+ * 256-byte.  rows up to 2^23, widths up to 2^20; at least one row for the pullback.
  */
+size_t lbi_gated_mlp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width);
 int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* fc1_bias, const void* fc2_weight, const void* fc2_bias,
-                  void* fc1_output, void* down_input, void* out, int64_t rows, int64_t D, int64_t hidden, int64_t width, int dtype,
-                  void* stream);
+                  void* fc1_output, void* down_input, void* out, void* workspace, size_t workspace_bytes, int64_t rows, int64_t D,
+                  int64_t hidden, int64_t width, int dtype, void* stream);
 
 size_t lbi_gated_mlp_vjp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width);
 int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* fc1_output, const void* down_input, const void* fc1_weight,

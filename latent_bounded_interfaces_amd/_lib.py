@@ -131,7 +131,8 @@ SYMBOLS = {
         _c.c_int,
         [_c.c_void_p] * 8 + [_c.c_size_t] + [_c.c_int64] * 2 + [_c.c_float] + [_c.c_int] * 3 + [_c.c_void_p],
     ),
-    "lbi_gated_mlp": (_c.c_int, [_c.c_void_p] * 8 + [_c.c_int64] * 4 + [_c.c_int, _c.c_void_p]),
+    "lbi_gated_mlp_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 4),
+    "lbi_gated_mlp": (_c.c_int, [_c.c_void_p] * 9 + [_c.c_size_t] + [_c.c_int64] * 4 + [_c.c_int, _c.c_void_p]),
     "lbi_gated_mlp_vjp_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 4),
     "lbi_gated_mlp_vjp": (
         _c.c_int,

@@ -1,13 +1,13 @@
 // The gated MLP of a Transformer block and its pullback, in one 16-bit type, sums in fp32:
 //
 //   forward    z = x W1^T + b1,  [u | g] = z,  a = u * g * sigmoid(g),  out = a W2^T + b2
-//   pullback   g_a = g_out W2;  g_u = g_a silu(g), g_g = g_a u silu'(g);  g_x = [g_u | g_g] W1
+//   pullback   g_a = g_out W2;  g_u = g_a silu(g), g_g = g_a u silu'(g);  g_x = [g_u | g_g] W1;  g_W1 = [g_u | g_g]^T x;  g_W2 = g_out^T a
 //
-// (the weights' gradients are lbi_weight_gradient's).  All four products are one kernel: a workgroup of four waves owns a tile of results,
-// 32 FM x 32 FN of them a wave, and takes 32 terms of the sums a step through LDS, in a ring of four steps.  Operands arrive by
-// buffer_load ... lds (what lies past the end of an operand is zero, so ragged sizes take the same loop); one whose terms lie side by side is
-// read in 16-byte pieces, one whose terms are its rows through transposing reads.  The product is formed as C^T: a lane ends up with four
-// neighbouring columns of one row.  Up and gate of one column meet in one lane, so the gate costs no pass of its own in either direction.
+// All six products are one kernel: a workgroup of four waves owns a tile of results, 32 FM x 32 FN of them a wave, and takes 64 terms of
+// the sums a step through LDS, in a ring of two steps.  Operands arrive by buffer_load ... lds, whole 128-byte lines of them (what lies past the
+// end of an operand is zero, so ragged sizes take the same loop); one whose terms lie side by side is read in 16-byte pieces, one whose
+// terms are its rows through transposing reads.  The product is formed as C^T: a lane ends up with four neighbouring columns of one row.
+// Up and gate of one column meet in one lane, so the gate costs no pass of its own in either direction.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -26,9 +26,9 @@ using attn_mfma::tile_off;
 using attn_mfma::u32x2;
 using attn_mfma::u32x4;
 
-constexpr int STEP = 32, RING = 4, NT = 256;
+constexpr int STEP = 64, RING = 2, NT = 256;
 constexpr unsigned PAST_END = 1u << 31;
-constexpr int PIECE = 1024;  // bytes that a wave's load brings: 16 rows of 32 terms, or 8 terms of 64 columns
+constexpr int PIECE = 1024;  // bytes that a wave's load brings: 8 rows of 64 terms, or 8 terms of 64 columns
 
 // What becomes of the sums.
 enum Finish {
@@ -38,20 +38,74 @@ enum Finish {
 };
 
 struct Task {
-    const void *a, *b, *bias;  // A [M, K]; B [N, K] or, transposed, [K, N]; GATED: B [2N, K]
+    const void *a, *b, *bias;  // A [M, K] or, by rows, [K, M]; B [N, K] or, by rows, [K, N]; GATED: B [2N, K]
     void *out, *z;             // GATED: z [M, 2N] written if given; UNGATED: z [M, 2N] read, out [M, 2N]
     long long M, N, K;
+    float* partial;
     int m_tiles, n_tiles;
+    int whole;              // tiles that one workgroup each sums up; the others' sums are cut into `parts` ranges of `part_steps` steps
+    int parts, part_steps;
 };
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
 
-template <typename T> __device__ __forceinline__ f32x4 load_four(const T* p) {
-    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-    return f32x4{Mma<T>::lo(w[0]), Mma<T>::hi(w[0]), Mma<T>::lo(w[1]), Mma<T>::hi(w[1])};
+struct Eight { float v[8]; };
+__device__ __forceinline__ Eight operator+(const Eight& a, const Eight& b) {
+    Eight r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.v[e] = a.v[e] + b.v[e];
+    return r;
 }
-template <typename T> __device__ __forceinline__ void store_four(T* p, f32x4 v) {
-    *reinterpret_cast<u32x2*>(p) = u32x2{Mma<T>::pack2(v[0], v[1]), Mma<T>::pack2(v[2], v[3])};
+template <typename T> __device__ __forceinline__ Eight load8(const T* p) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+    return Eight{{Mma<T>::lo(w[0]), Mma<T>::hi(w[0]), Mma<T>::lo(w[1]), Mma<T>::hi(w[1]), Mma<T>::lo(w[2]), Mma<T>::hi(w[2]),
+                  Mma<T>::lo(w[3]), Mma<T>::hi(w[3])}};
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const Eight& x) {
+    *reinterpret_cast<u32x4*>(p) = u32x4{Mma<T>::pack2(x.v[0], x.v[1]), Mma<T>::pack2(x.v[2], x.v[3]), Mma<T>::pack2(x.v[4], x.v[5]),
+                                         Mma<T>::pack2(x.v[6], x.v[7])};
+}
+__device__ __forceinline__ void store8(float* p, const Eight& x) {
+    reinterpret_cast<f32x4*>(p)[0] = f32x4{x.v[0], x.v[1], x.v[2], x.v[3]};
+    reinterpret_cast<f32x4*>(p)[1] = f32x4{x.v[4], x.v[5], x.v[6], x.v[7]};
+}
+__device__ __forceinline__ Eight load8(const float* p) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+    return Eight{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+}
+
+// Eight columns of one row of the result, from their sums (GATED: up's and gate's).
+template <typename T, Finish FINISH>
+__device__ __forceinline__ void finish(const Task& task, long long row, long long col, const Eight& x, const Eight& y) {
+    const long long N = task.N;
+    if (row >= task.M || col >= N) return;
+    const T* bias = static_cast<const T*>(task.bias);
+    T* out = static_cast<T*>(task.out);
+    T* z = static_cast<T*>(task.z);
+    if constexpr (FINISH == PLAIN) {
+        store8(out + row * N + col, bias ? x + load8(bias + col) : x);
+    } else if constexpr (FINISH == GATED) {
+        const Eight up = bias ? x + load8(bias + col) : x, gate = bias ? y + load8(bias + N + col) : y;
+        Eight act;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) act.v[e] = up.v[e] * (gate.v[e] * sigmoid(gate.v[e]));
+        store8(out + row * N + col, act);
+        if (z) {
+            store8(z + row * 2 * N + col, up);
+            store8(z + row * 2 * N + N + col, gate);
+        }
+    } else {
+        const Eight up = load8(z + row * 2 * N + col), gate = load8(z + row * 2 * N + N + col);
+        Eight g_up, g_gate;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float open = sigmoid(gate.v[e]);
+            g_up.v[e] = x.v[e] * (gate.v[e] * open);
+            g_gate.v[e] = x.v[e] * up.v[e] * (open * (1.0f + gate.v[e] * (1.0f - open)));
+        }
+        store8(out + row * 2 * N + col, g_up);
+        store8(out + row * 2 * N + N + col, g_gate);
+    }
 }
 
 // 1 KiB from memory to LDS by one wave: lane l brings the 16 bytes at `base` + `off`, zeros from `bytes` on.
@@ -59,55 +113,74 @@ __device__ __forceinline__ void bring(const char* base, unsigned off, unsigned b
     attn_mfma::dma_tile<true>(base, off, bytes, lds);
 }
 
-// Rows of an operand whose terms lie side by side.  In LDS a row of a step is 64 bytes, four rows a bank line, its four chunks swapped by row.
-__device__ __forceinline__ int row_chunk(int row, int chunk) { return row * 64 + ((chunk ^ ((row >> 2) & 3)) << 4); }
-
-// Workgroup -> tile.  Ids equal mod 8 share an L2: they get neighbouring tiles, eight rows of them at a time.
-__device__ __forceinline__ void tile_of(int id, int m_tiles, int n_tiles, int& mt, int& nt) {
-    const int count = m_tiles * n_tiles, lot = count / 8, left = count % 8, x = id % 8;
-    const int at = x * lot + min(x, left) + id / 8;
+// Ids equal mod 8 share an L2: they get neighbouring places.
+__device__ __forceinline__ int place(int id, int count) {
+    const int lot = count / 8, left = count % 8, x = id % 8;
+    return x * lot + min(x, left) + id / 8;
+}
+// Place -> tile: eight rows of tiles at a time.
+__device__ __forceinline__ void tile_at(int at, int m_tiles, int n_tiles, int& mt, int& nt) {
     constexpr int ROWS = 8;
     const int band = at / (ROWS * n_tiles), in = at - band * ROWS * n_tiles, rows = min(ROWS, m_tiles - band * ROWS);
     mt = band * ROWS + in % rows;
     nt = in / rows;
 }
+// What one wave leaves of 32 rows of a part of a tile: columns in eights, GATED up's first.
+template <int FM, int FN> __device__ __forceinline__ size_t partial_at(int item, int wave, int i) {
+    return ((size_t)(item * 4 + wave) * FM + i) * (32 * 32 * FN);
+}
 
-template <typename T, int FM, int FN, bool B_ROWS, Finish FINISH>  // B_ROWS: the terms of B are its rows
+template <typename T, int FM, int FN, bool A_ROWS, bool B_ROWS, Finish FINISH>  // ..._ROWS: the terms are the operand's rows
 __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     constexpr int BM = 64 * FM, BN = 64 * FN;  // rows and columns of B's tile
-    constexpr int A_BYTES = BM * 64, SLOT = A_BYTES + BN * 64, LOADS = FM + FN;
+    constexpr int A_BYTES = BM * 128, SLOT = A_BYTES + BN * 128, READS = FM + FN, LOADS = 2 * READS, BESIDE = (READS + FM * FN - 1) / (FM * FN);
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 31, h = lane >> 5, wm = wave >> 1, wn = wave & 1;
     constexpr int COLUMNS = FINISH == GATED ? BN / 2 : BN;
     const long long M = task.M, N = task.N, K = task.K;
-    int mt, nt;
-    tile_of((int)blockIdx.x, task.m_tiles, task.n_tiles, mt, nt);
-    const long long row0 = (long long)mt * BM, col0 = (long long)nt * COLUMNS;
     const int steps = (int)((K + STEP - 1) / STEP);
+    int at, first = 0, last = steps, item = -1;
+    if ((int)blockIdx.x < task.whole) {
+        at = place((int)blockIdx.x, task.whole);
+    } else {
+        const int rest = task.m_tiles * task.n_tiles - task.whole, p = place((int)blockIdx.x - task.whole, rest * task.parts), part = p / rest;
+        at = task.whole + p % rest;
+        first = part * task.part_steps;
+        last = min(first + task.part_steps, steps);
+        item = p;
+    }
+    int mt, nt;
+    tile_at(at, task.m_tiles, task.n_tiles, mt, nt);
+    const long long row0 = (long long)mt * BM, col0 = (long long)nt * COLUMNS;
     const unsigned row_bytes = (unsigned)K * 2;
     // sources: A's rows, B's rows (GATED: up's and gate's) or B's terms
     const int a_rows = (int)(M - row0 < BM ? M - row0 : BM), b_cols = (int)(N - col0 < COLUMNS ? N - col0 : COLUMNS);
-    const char* a_src = static_cast<const char*>(task.a) + row0 * K * 2;
+    const char* a_src = static_cast<const char*>(task.a) + (A_ROWS ? row0 : row0 * K) * 2;
     const char* b_src = static_cast<const char*>(task.b) + (B_ROWS ? col0 : col0 * K) * 2;
-    unsigned a_off[FM], b_off[FN];
-    const char* b_from[FN];
-    const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+    unsigned a_off[2 * FM], b_off[2 * FN];
+    const char* b_from[2 * FN];
+    const int chunk = (lane & 7) ^ swz<64>(8 * wave + lane / 8);  // the same for each of the wave's pieces: they are 32 rows apart
 #pragma unroll
-    for (int u = 0; u < FM; ++u) {
-        const int row = 16 * (wave + 4 * u) + lane / 4;
-        a_off[u] = row < a_rows ? (unsigned)row * row_bytes + chunk * 16 : PAST_END;
+    for (int u = 0; u < 2 * FM; ++u) {
+        const int q = wave + 4 * u, row = 8 * q + lane / 8;
+        if constexpr (A_ROWS) {
+            const int term = 8 * (q % 8) + lane / 8, col = 64 * (q / 8) + 8 * chunk;
+            a_off[u] = col < a_rows ? (unsigned)(term * M + col) * 2 : PAST_END;
+        } else {
+            a_off[u] = row < a_rows ? (unsigned)row * row_bytes + chunk * 16 : PAST_END;
+        }
     }
 #pragma unroll
-    for (int u = 0; u < FN; ++u) {
+    for (int u = 0; u < 2 * FN; ++u) {
         const int q = wave + 4 * u;
         b_from[u] = b_src;
         if constexpr (B_ROWS) {
-            const int term = 8 * (q % 4) + lane / 8, col = 64 * (q / 4) + 8 * ((lane % 8) ^ swz<64>(term));
+            const int term = 8 * (q % 8) + lane / 8, col = 64 * (q / 8) + 8 * chunk;
             b_off[u] = col < b_cols ? (unsigned)(term * N + col) * 2 : PAST_END;
         } else {
-            int row = 16 * q + lane / 4;
-            if (FINISH == GATED && 16 * q >= COLUMNS) {  // the same for the whole wave
+            int row = 8 * q + lane / 8;
+            if (FINISH == GATED && 8 * q >= COLUMNS) {  // the same for the whole wave
                 row -= COLUMNS;
                 b_from[u] += N * K * 2;
             }
@@ -115,23 +188,20 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
         }
     }
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
-    auto fetch = [&](int it, int slot) __attribute__((always_inline)) {
+    // The loads of a step, one after the other: `u` below 2 FM A's, then B's.
+    auto fetch = [&](int it, int slot, int u) __attribute__((always_inline)) {
         const unsigned to = lds0 + slot * SLOT + wave * PIECE;
-        const bool there = it < steps;
-        const long long k = (long long)it * STEP;
+        const bool there = it < last;
+        const long long k = (long long)it * STEP, terms = K - k < STEP ? K - k : STEP;
         const bool cut = k + 8 * chunk >= K;  // pieces past the end of a row
-        const unsigned a_bytes = there ? (unsigned)(a_rows * (long long)row_bytes - k * 2) : 0;
-#pragma unroll
-        for (int u = 0; u < FM; ++u) bring(a_src + k * 2, cut ? PAST_END : a_off[u], a_bytes, to + u * 4 * PIECE);
-        if constexpr (B_ROWS) {
-            const long long terms = K - k < STEP ? K - k : STEP;
-            const unsigned b_bytes = there ? (unsigned)((terms * N - col0) * 2) : 0;
-#pragma unroll
-            for (int u = 0; u < FN; ++u) bring(b_src + k * N * 2, b_off[u], b_bytes, to + A_BYTES + u * 4 * PIECE);
+        if (u < 2 * FM) {
+            if constexpr (A_ROWS) bring(a_src + k * M * 2, a_off[u], there ? (unsigned)((terms * M - row0) * 2) : 0, to + u * 4 * PIECE);
+            else bring(a_src + k * 2, cut ? PAST_END : a_off[u], there ? (unsigned)(a_rows * (long long)row_bytes - k * 2) : 0, to + u * 4 * PIECE);
+        } else if constexpr (B_ROWS) {
+            bring(b_src + k * N * 2, b_off[u - 2 * FM], there ? (unsigned)((terms * N - col0) * 2) : 0, to + A_BYTES + (u - 2 * FM) * 4 * PIECE);
         } else {
-            const unsigned b_bytes = there ? (unsigned)(b_cols * (long long)row_bytes - k * 2) : 0;
-#pragma unroll
-            for (int u = 0; u < FN; ++u) bring(b_from[u] + k * 2, cut ? PAST_END : b_off[u], b_bytes, to + A_BYTES + u * 4 * PIECE);
+            bring(b_from[u - 2 * FM] + k * 2, cut ? PAST_END : b_off[u - 2 * FM], there ? (unsigned)(b_cols * (long long)row_bytes - k * 2) : 0,
+                  to + A_BYTES + (u - 2 * FM) * 4 * PIECE);
         }
     };
     // first row of B's tile (column of the product) of a wave's j-th fragment
@@ -140,26 +210,28 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
         return 32 * FN * wn + 32 * j;
     };
     u32x4 af[2][FM], bf[2][FN];
-    auto read = [&](int ks, int slot) __attribute__((always_inline)) {
+    // 16 terms of 32 columns of an operand whose terms are its rows, LDS holding 64 columns side by side
+    auto by_rows = [&](const char* tile, int ks, int n0) __attribute__((always_inline)) {
+        tile += n0 / 64 * 8 * PIECE;
+        const int s = lane & 15, term = 16 * ks + 8 * h + (s >> 2), c = (n0 % 64 >> 3) + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_off<64>(term, c) + ((s & 1) << 3))));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_off<64>(term + 4, c) + ((s & 1) << 3))));
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    // The reads of a quarter of a step, in the order in which the products need them: A's first fragment, B's, A's others.
+    auto read = [&](int ks, int slot, int u) __attribute__((always_inline)) {
         const char* at_a = lds + slot * SLOT;
         const char* at_b = at_a + A_BYTES;
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-            af[ks][i] = *reinterpret_cast<const u32x4*>(at_a + row_chunk(32 * FM * wm + 32 * i + m, 2 * ks + h));
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            if constexpr (B_ROWS) {
-                const int n0 = b_row(j);
-                const char* tile = at_b + n0 / 64 * 4 * PIECE;
-                const int s = lane & 15, term = 16 * ks + 8 * h + (s >> 2), c = (n0 % 64 >> 3) + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
-                typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_off<64>(term, c) + ((s & 1) << 3))));
-                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_off<64>(term + 4, c) + ((s & 1) << 3))));
-                bf[ks][j] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-            } else {
-                bf[ks][j] = *reinterpret_cast<const u32x4*>(at_b + row_chunk(b_row(j) + m, 2 * ks + h));
-            }
+        if (u == 0 || u > FN) {
+            const int i = u == 0 ? 0 : u - FN, n0 = 32 * FM * wm + 32 * i;
+            if constexpr (A_ROWS) af[ks & 1][i] = by_rows(at_a, ks, n0);
+            else af[ks & 1][i] = *reinterpret_cast<const u32x4*>(at_a + tile_off<64>(n0 + m, 2 * ks + h));
+            return;
         }
+        const int j = u - 1, n0 = b_row(j);
+        if constexpr (B_ROWS) bf[ks & 1][j] = by_rows(at_b, ks, n0);
+        else bf[ks & 1][j] = *reinterpret_cast<const u32x4*>(at_b + tile_off<64>(n0 + m, 2 * ks + h));
     };
     f32x16 acc[FM][FN];
 #pragma unroll
@@ -168,99 +240,172 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
         for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    auto multiply = [&](int ks) __attribute__((always_inline)) {
+    // The products of a quarter of a step, and behind each what may run beside it (the compiler would put a read right before its use).
+    auto multiply = [&](int ks, auto beside) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::mma(bf[ks][j], af[ks][i], acc[i][j]);
+            for (int j = 0; j < FN; ++j) {
+                acc[i][j] = Mma<T>::mma(bf[ks & 1][j], af[ks & 1][i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = (i * FN + j) * BESIDE; u < (i * FN + j + 1) * BESIDE; ++u)
+                    if (u < READS) beside(u);
+                __builtin_amdgcn_sched_barrier(0);
+            }
     };
 #pragma unroll
-    for (int u = 0; u < RING; ++u) fetch(u, u);
-    __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((RING - 1) * LOADS));
+    for (int s = 0; s < RING; ++s)
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) fetch(first + s, s, u);
+    __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm(LOADS));
     asm volatile("s_barrier" ::: "memory");
-    read(0, 0);
-    int slot = 0;
-    for (int it = 0; it < steps; ++it) {
-        const int next = slot + 1 == RING ? 0 : slot + 1;
-        read(1, slot);
-        multiply(0);
-        // this wave's loads of the next step have landed and its reads of this one are done, and behind the barrier everyone's: the next
-        // step can be read, and this one's place filled
-        __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((RING - 2) * LOADS));
+#pragma unroll
+    for (int u = 0; u < READS; ++u) read(0, 0, u);
+    for (int it = first, slot = 0; it < last; ++it, slot ^= 1) {
+        // A step's place is free for the one after the next from the barrier on.  Half of its loads go beside the quarter behind it, half beside
+        // the quarter after that: all at once they queue up and hold up the products (tiles of 256 x 256, 6007 x 4096 x 11008: 525 -> 486 us).
+        multiply(0, [&](int u) __attribute__((always_inline)) {
+            read(1, slot, u);
+            if (it > first) fetch(it + 1, slot ^ 1, READS + u);
+        });
+        multiply(1, [&](int u) __attribute__((always_inline)) { read(2, slot, u); });
+        multiply(2, [&](int u) __attribute__((always_inline)) { read(3, slot, u); });
+        // this wave's loads of the next step have landed and its reads of this one are done, and behind the barrier everyone's
+        __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm(0));
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        fetch(it + RING, slot);
-        read(0, next);
-        multiply(1);
-        slot = next;
+        multiply(3, [&](int u) __attribute__((always_inline)) {
+            read(0, slot ^ 1, u);
+            fetch(it + 2, slot, u);
+        });
     }
-    __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm(0));  // nothing is under way into LDS when the workgroup ends
-    // lane (m, h): columns 8 g + 4 h ... + 3 of row m of each 32 x 32 results
-    const T* bias = static_cast<const T*>(task.bias);
-    T* out = static_cast<T*>(task.out);
-    T* z = static_cast<T*>(task.z);
+    // Nothing is under way into LDS any more, and behind the barrier nothing is read from it: from here on each wave has a part of its own, in
+    // which 32 rows of its results turn from four columns a lane to eight, so that a wave's stores (and z's loads) are whole lines.
+    __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm(0));
+    asm volatile("s_barrier" ::: "memory");
+    constexpr int ROW = 32 * FN + 4;  // floats
+    float* turn = reinterpret_cast<float*>(lds) + wave * 32 * ROW;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        const long long row = row0 + 32 * FM * wm + 32 * i + m;
-        if (row >= M) continue;
 #pragma unroll
-        for (int j = 0; j < (FINISH == GATED ? FN / 2 : FN); ++j)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const long long col = col0 + b_row(j) + 8 * g + 4 * h;
-                if (col >= N) continue;
-                auto four = [&](const f32x16& c) { return f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]}; };
-                f32x4 c = four(acc[i][j]);
-                if constexpr (FINISH == PLAIN) {
-                    if (bias) {
-                        const f32x4 b = load_four(bias + col);
+            for (int g = 0; g < 4; ++g)  // lane (m, h): columns 8 g + 4 h ... + 3 of row m
+                *reinterpret_cast<f32x4*>(turn + m * ROW + 32 * j + 8 * g + 4 * h) =
+                    f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        constexpr int WIDTH = (FINISH == GATED ? 16 : 32) * FN, EIGHTS = WIDTH / 8;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) c[e] += b[e];
-                    }
-                    store_four(out + row * N + col, c);
-                } else if constexpr (FINISH == GATED) {
-                    f32x4 gate = four(acc[i][j + FN / 2]), act;
-                    if (bias) {
-                        const f32x4 b = load_four(bias + col), bg = load_four(bias + N + col);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) c[e] += b[e], gate[e] += bg[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) act[e] = c[e] * (gate[e] * sigmoid(gate[e]));
-                    store_four(out + row * N + col, act);
-                    if (z) {
-                        store_four(z + row * 2 * N + col, c);
-                        store_four(z + row * 2 * N + N + col, gate);
-                    }
-                } else {
-                    const f32x4 up = load_four(z + row * 2 * N + col), gate = load_four(z + row * 2 * N + N + col);
-                    f32x4 g_up, g_gate;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float open = sigmoid(gate[e]);
-                        g_up[e] = c[e] * (gate[e] * open);
-                        g_gate[e] = c[e] * up[e] * (open * (1.0f + gate[e] * (1.0f - open)));
-                    }
-                    store_four(out + row * 2 * N + col, g_up);
-                    store_four(out + row * 2 * N + N + col, g_gate);
-                }
+        for (int u = 0; u < 32 * EIGHTS / 64; ++u) {
+            const int eight = 64 * u + lane, r = eight / EIGHTS, c = eight % EIGHTS * 8;
+            const Eight x = load8(turn + r * ROW + c);
+            Eight y;
+            if constexpr (FINISH == GATED) y = load8(turn + r * ROW + WIDTH + c);
+            if (item < 0) {
+                finish<T, FINISH>(task, row0 + 32 * FM * wm + 32 * i + r, col0 + WIDTH * wn + c, x, y);
+            } else {
+                float* to = task.partial + partial_at<FM, FN>(item, wave, i) + eight * 8;
+                store8(to, x);
+                if constexpr (FINISH == GATED) store8(to + 32 * WIDTH, y);
             }
+        }
     }
 }
 
-template <typename T, int FM, int FN, bool B_ROWS, Finish FINISH> int launch_tile(Task task, hipStream_t stream) {
-    constexpr auto kernel = product_kernel<T, FM, FN, B_ROWS, FINISH>;
-    constexpr int BM = 64 * FM, COLUMNS = FINISH == GATED ? 32 * FN : 64 * FN;
-    constexpr size_t bytes = (size_t)RING * 4096 * (FM + FN);
+// Adds the parts of the tiles whose sums were cut, in order, and finishes them: a thread takes eight columns of a row.
+template <typename T, int FM, int FN, Finish FINISH> __global__ __launch_bounds__(256) void add_parts_kernel(Task task) {
+    constexpr int WIDTH = (FINISH == GATED ? 16 : 32) * FN, EIGHTS = WIDTH / 8, COUNT = 32 * EIGHTS;
+    const int rest = task.m_tiles * task.n_tiles - task.whole;
+    const int id = blockIdx.x * 256 + threadIdx.x, eight = id % COUNT, i = id / COUNT % FM, wave = id / (COUNT * FM) % 4, tile = id / (COUNT * FM * 4);
+    if (tile >= rest) return;
+    int mt, nt;
+    tile_at(task.whole + tile, task.m_tiles, task.n_tiles, mt, nt);
+    const long long row = (long long)mt * 64 * FM + 32 * FM * (wave >> 1) + 32 * i + eight / EIGHTS;
+    const long long col = (long long)nt * (FINISH == GATED ? 32 : 64) * FN + WIDTH * (wave & 1) + eight % EIGHTS * 8;
+    if (row >= task.M || col >= task.N) return;
+    Eight x{}, y{};
+#pragma unroll 4
+    for (int part = 0; part < task.parts; ++part) {
+        const float* from = task.partial + partial_at<FM, FN>(part * rest + tile, wave, i) + eight * 8;
+        x = x + load8(from);
+        if constexpr (FINISH == GATED) y = y + load8(from + 32 * WIDTH);
+    }
+    finish<T, FINISH>(task, row, col, x, y);
+}
+
+// How a product is laid out: the tile, and into how many parts the sums of those tiles are cut that do not fill the chip once more.
+struct Layout {
+    int form;  // FM x FN: 0: 4 x 4, 1: 2 x 2, 2: 1 x 2
+    int m_tiles, n_tiles, whole, parts, part_steps;
+    double us;
+    size_t bytes() const {
+        constexpr int sizes[3] = {256 * 256, 128 * 128, 64 * 128};
+        return parts > 1 ? (size_t)(m_tiles * n_tiles - whole) * parts * sizes[form] * sizeof(float) : 0;
+    }
+};
+
+// By what a call takes, in us: for each round of workgroups over the chip its steps, a start of 2 to 2.5 and the results on their way out (20 GB/s
+// a CU, since all finish together); for parts a second launch and their sums out and back.  A step of 256 x 256 takes 1.5 us with both operands
+// by columns, 1.7 and 1.8 with one and both by rows (twice the reads); of 128 x 128, two workgroups a CU, 1.03 ... 1.07 and alone on its CU
+// 0.5 ... 0.85; of 64 x 128, three a CU, 0.95 ... 1.08 and 0.4 ... 0.75.  Of 16 calls with 1 ... 8192 rows, each with 13 layouts, what is chosen
+// took 1.01 times the best on average, 1.09 at most.
+Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
+    constexpr struct { int rows, columns, a_cu; double step[3], alone[3], start; } forms[3] = {
+        {256, 256, 1, {1.5, 1.68, 1.8}, {1.5, 1.68, 1.8}, 2.5},
+        {128, 128, 2, {1.03, 1.04, 1.07}, {0.5, 0.6, 0.85}, 2.0},
+        {64, 128, 3, {0.98, 1.08, 1.0}, {0.4, 0.5, 0.75}, 2.0}};
+    const int cus = device_compute_units(), steps = (int)((K + STEP - 1) / STEP);
+    Layout best{};
+    best.us = -1.0;
+    for (int f = 0; f < 3; ++f) {
+        const auto& form = forms[f];
+        const int columns = finish == GATED ? form.columns / 2 : form.columns, slots = cus * form.a_cu;
+        const int64_t m_tiles = (M + form.rows - 1) / form.rows, n_tiles = (N + columns - 1) / columns, tiles = m_tiles * n_tiles;
+        if (tiles >= 1 << 24) continue;
+        const double full = form.step[by_rows], alone = form.alone[by_rows];
+        const double fixed = form.start + (finish == GATED ? 6 : finish == UNGATED ? 8 : 2) * form.rows * columns * form.a_cu / 20e3;
+        const auto rounds = [&](int64_t items, int of) {
+            const int deep = (int)((items % slots + cus - 1) / cus);  // workgroups that share a CU in the last round
+            const double step = deep <= 1 || form.a_cu == 1 ? alone : alone + (full - alone) * (deep - 1) / (form.a_cu - 1);
+            return (double)(items / slots) * (of * full + fixed) + (deep ? of * step + fixed : 0.0);
+        };
+        for (int s = 1; s <= 32; ++s) {
+            const int part_steps = (steps + s - 1) / s, parts = (steps + part_steps - 1) / part_steps;
+            if (parts != s || (s > 1 && part_steps < 2)) continue;
+            const int64_t whole = s == 1 ? tiles : tiles / slots * slots, rest = tiles - whole;
+            if (s > 1 && rest == 0) break;
+            double us = rounds(whole, steps);
+            if (rest) us += rounds(rest * s, part_steps) + 8.0 + (double)rest * s * form.rows * form.columns * 8.0 / 8e6;
+            if (best.us < 0.0 || us < best.us) best = {f, (int)m_tiles, (int)n_tiles, (int)whole, s, part_steps, us};
+        }
+    }
+    return best;
+}
+
+template <typename T, int FM, int FN, bool A_ROWS, bool B_ROWS, Finish FINISH> int launch_tile(const Task& task, hipStream_t stream) {
+    constexpr auto kernel = product_kernel<T, FM, FN, A_ROWS, B_ROWS, FINISH>;
+    constexpr size_t bytes = (size_t)RING * 8192 * (FM + FN);
+    static_assert(bytes >= 4 * 32 * (32 * FN + 4) * sizeof(float), "the turn of the results fits the ring");
     if (int status = ensure_dynamic_lds<kernel>(bytes)) return status;
-    task.m_tiles = (int)((task.M + BM - 1) / BM);
-    task.n_tiles = (int)((task.N + COLUMNS - 1) / COLUMNS);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(task.m_tiles * task.n_tiles)), dim3(NT), bytes, stream, task);
+    const int rest = task.m_tiles * task.n_tiles - task.whole;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(task.whole + rest * task.parts)), dim3(NT), bytes, stream, task);
+    if (rest) {
+        const int eights = rest * 4 * FM * 32 * (FINISH == GATED ? 2 : 4) * FN;
+        hipLaunchKernelGGL((add_parts_kernel<T, FM, FN, FINISH>), dim3((unsigned)((eights + 255) / 256)), dim3(256), 0, stream, task);
+    }
     LBI_HIP_CHECK(hipGetLastError());
     return LBI_OK;
 }
 
-template <typename T, bool B_ROWS, Finish FINISH> int launch(const Task& task, hipStream_t stream) {
-    return launch_tile<T, 2, 2, B_ROWS, FINISH>(task, stream);
+// `partial`: layout_of(...).bytes()
+template <typename T, bool A_ROWS, bool B_ROWS, Finish FINISH>
+int launch(const void* a, const void* b, const void* bias, void* out, void* z, int64_t M, int64_t N, int64_t K, void* partial,
+           hipStream_t stream) {
+    const Layout l = layout_of(M, N, K, FINISH, A_ROWS + B_ROWS);
+    if (l.us < 0.0) return fail(LBI_ERR_UNSUPPORTED, "lbi_gated_mlp: too many tiles");
+    const Task task{a, b, bias, out, z, M, N, K, static_cast<float*>(partial), l.m_tiles, l.n_tiles, l.whole, l.parts, l.part_steps};
+    if (l.form == 0) return launch_tile<T, 4, 4, A_ROWS, B_ROWS, FINISH>(task, stream);
+    if (l.form == 1) return launch_tile<T, 2, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
+    return launch_tile<T, 1, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
 }
 
 // Sums over the rows of x [rows, N]: the gradient of a bias.  A workgroup takes 64 columns, eight to a thread's load, and a slab of rows;
@@ -335,34 +480,47 @@ bool on_grid(std::initializer_list<const void*> tensors) {
 }
 
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
+size_t forward_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
+    return up(std::max(layout_of(rows, hidden, D, GATED, 0).bytes(), layout_of(rows, width, hidden, PLAIN, 0).bytes()));
+}
 struct Parts {  // of the pullback's workspace, in bytes
-    size_t g_fc1, sums, gradient;
+    size_t g_fc1, sums, partial;
 };
 Parts parts_of(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
     return {up((size_t)rows * 2 * hidden * 2), up((size_t)slabs_of(rows) * std::max(2 * hidden, width) * sizeof(float)),
-            up(std::max(lbi_weight_gradient_workspace_bytes(2 * hidden, D, rows), lbi_weight_gradient_workspace_bytes(width, hidden, rows)))};
+            up(std::max({layout_of(rows, hidden, width, UNGATED, 1).bytes(), layout_of(rows, D, 2 * hidden, PLAIN, 1).bytes(),
+                         layout_of(2 * hidden, D, rows, PLAIN, 2).bytes(), layout_of(width, hidden, rows, PLAIN, 2).bytes()}))};
 }
 
 }  // namespace
 }  // namespace block_mlp
 }  // namespace lbi
 
+extern "C" size_t lbi_gated_mlp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
+    using namespace lbi::block_mlp;
+    if (check("lbi_gated_mlp", rows, D, hidden, width, LBI_BF16) || rows == 0) return 0;
+    return forward_bytes(rows, D, hidden, width);
+}
+
 extern "C" int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* fc1_bias, const void* fc2_weight, const void* fc2_bias,
-                             void* fc1_output, void* down_input, void* out, int64_t rows, int64_t D, int64_t hidden, int64_t width,
-                             int dtype, void* stream) {
+                             void* fc1_output, void* down_input, void* out, void* workspace, size_t workspace_bytes, int64_t rows,
+                             int64_t D, int64_t hidden, int64_t width, int dtype, void* stream) {
     using namespace lbi;
     using namespace lbi::block_mlp;
     clear_error();
     if (int bad = check("lbi_gated_mlp", rows, D, hidden, width, dtype)) return bad;
     if (rows == 0) return LBI_OK;
     if (!x || !fc1_weight || !fc2_weight || !down_input || !out) return fail(LBI_ERR_INVALID, "lbi_gated_mlp: null pointer");
-    if (!on_grid({x, fc1_weight, fc1_bias, fc2_weight, fc2_bias, fc1_output, down_input, out}))
+    if (!on_grid({x, fc1_weight, fc1_bias, fc2_weight, fc2_bias, fc1_output, down_input, out, workspace}))
         return fail(LBI_ERR_INVALID, "lbi_gated_mlp: tensors must be 16-byte aligned");
+    const size_t need = forward_bytes(rows, D, hidden, width);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(LBI_ERR_WORKSPACE, "lbi_gated_mlp: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     const hipStream_t on = static_cast<hipStream_t>(stream);
     const auto run = [&](auto t) {
         using T = decltype(t);
-        if (int status = launch<T, false, GATED>(Task{x, fc1_weight, fc1_bias, down_input, fc1_output, rows, hidden, D, 0, 0}, on)) return status;
-        return launch<T, false, PLAIN>(Task{down_input, fc2_weight, fc2_bias, out, nullptr, rows, width, hidden, 0, 0}, on);
+        if (int s = launch<T, false, false, GATED>(x, fc1_weight, fc1_bias, down_input, fc1_output, rows, hidden, D, workspace, on)) return s;
+        return launch<T, false, false, PLAIN>(down_input, fc2_weight, fc2_bias, out, nullptr, rows, width, hidden, workspace, on);
     };
     return dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{});
 }
@@ -371,7 +529,7 @@ extern "C" size_t lbi_gated_mlp_vjp_workspace_bytes(int64_t rows, int64_t D, int
     using namespace lbi::block_mlp;
     if (check("lbi_gated_mlp_vjp", rows, D, hidden, width, LBI_BF16) || rows == 0) return 0;
     const Parts p = parts_of(rows, D, hidden, width);
-    return p.g_fc1 + p.sums + p.gradient;
+    return p.g_fc1 + p.sums + p.partial;
 }
 
 extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* fc1_output, const void* down_input, const void* fc1_weight,
@@ -389,23 +547,24 @@ extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* f
         reinterpret_cast<uintptr_t>(workspace) % 256)
         return fail(LBI_ERR_INVALID, "lbi_gated_mlp_vjp: tensors must be 16-byte aligned, the workspace 256");
     const Parts p = parts_of(rows, D, hidden, width);
-    if (!workspace || workspace_bytes < p.g_fc1 + p.sums + p.gradient)
-        return fail(LBI_ERR_WORKSPACE, "lbi_gated_mlp_vjp: workspace of %zu bytes needed, %zu given", p.g_fc1 + p.sums + p.gradient, workspace_bytes);
+    if (!workspace || workspace_bytes < p.g_fc1 + p.sums + p.partial)
+        return fail(LBI_ERR_WORKSPACE, "lbi_gated_mlp_vjp: workspace of %zu bytes needed, %zu given", p.g_fc1 + p.sums + p.partial, workspace_bytes);
     const hipStream_t on = static_cast<hipStream_t>(stream);
     char* g_fc1 = static_cast<char*>(workspace);
     float* sums = reinterpret_cast<float*>(g_fc1 + p.g_fc1);
-    char* gradient = g_fc1 + p.g_fc1 + p.sums;
+    char* partial = g_fc1 + p.g_fc1 + p.sums;
     const auto run = [&](auto t) {
         using T = decltype(t);
-        if (int s = launch<T, true, UNGATED>(Task{g_out, fc2_weight, nullptr, g_fc1, const_cast<void*>(fc1_output), rows, hidden, width, 0, 0}, on)) return s;
-        if (int s = launch<T, true, PLAIN>(Task{g_fc1, fc1_weight, nullptr, g_x, nullptr, rows, D, 2 * hidden, 0, 0}, on)) return s;
+        void* z = const_cast<void*>(fc1_output);
+        if (int s = launch<T, false, true, UNGATED>(g_out, fc2_weight, nullptr, g_fc1, z, rows, hidden, width, partial, on)) return s;
+        if (int s = launch<T, false, true, PLAIN>(g_fc1, fc1_weight, nullptr, g_x, nullptr, rows, D, 2 * hidden, partial, on)) return s;
+        if (int s = launch<T, true, true, PLAIN>(g_fc1, x, nullptr, g_fc1_weight, nullptr, 2 * hidden, D, rows, partial, on)) return s;
+        if (int s = launch<T, true, true, PLAIN>(g_out, down_input, nullptr, g_fc2_weight, nullptr, width, hidden, rows, partial, on)) return s;
         if (g_fc1_bias)
             if (int s = column_sums<T>(g_fc1, g_fc1_bias, sums, rows, 2 * hidden, on)) return s;
         if (g_fc2_bias)
             if (int s = column_sums<T>(g_out, g_fc2_bias, sums, rows, width, on)) return s;
         return (int)LBI_OK;
     };
-    if (int s = dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{})) return s;
-    if (int s = lbi_weight_gradient(g_fc1, x, g_fc1_weight, gradient, p.gradient, 2 * hidden, D, rows, dtype, stream)) return s;
-    return lbi_weight_gradient(g_out, down_input, g_fc2_weight, gradient, p.gradient, width, hidden, rows, dtype, stream);
+    return dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{});
 }

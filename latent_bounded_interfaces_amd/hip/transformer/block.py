@@ -173,11 +173,15 @@ def gated_mlp(x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight: torch.Tenso
         x = _ready(x.reshape(rows, dim), dtype, rows, d)
         fc1_weight, fc1_bias = _halves(fc1_weight, dtype, hd, d), _halves(fc1_bias, dtype, hd)
         fc2_weight, fc2_bias = _ready(fc2_weight, dtype, w, hd), _ready(fc2_bias, dtype, w)
+        lib = _lib.load()
         with _lib.device_guard(x.device):
-            status = _lib.load().lbi_gated_mlp(
+            need = int(lib.lbi_gated_mlp_workspace_bytes(rows, d, hd, w))
+            workspace = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
+            status = lib.lbi_gated_mlp(
                 x.data_ptr(), fc1_weight.data_ptr(), None if fc1_bias is None else fc1_bias.data_ptr(), fc2_weight.data_ptr(),
                 None if fc2_bias is None else fc2_bias.data_ptr(), None if fc1_output is None else fc1_output.data_ptr(),
-                down.data_ptr(), out.data_ptr(), rows, d, hd, w, _lib.dtype_code(dtype), _stream(x))
+                down.data_ptr(), out.data_ptr(), None if workspace is None else workspace.data_ptr(), need, rows, d, hd, w,
+                _lib.dtype_code(dtype), _stream(x))
         _lib.check(status, "lbi_gated_mlp")
     out = out[:, :width].reshape(*outer, width)
     if not keep:
