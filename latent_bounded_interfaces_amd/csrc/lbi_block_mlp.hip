@@ -26,7 +26,11 @@ using attn_mfma::tile_off;
 using attn_mfma::u32x2;
 using attn_mfma::u32x4;
 
-constexpr int STEP = 64, RING = 2, NT = 256;
+constexpr int STEP = 64, NT = 256;
+// Steps of a tile's ring, what LDS holds for the workgroups that share a CU: one of 256 x 256, two of the others.  Small tiles multiply little in
+// a step: the fragments of a whole step are read while the last one's are multiplied (77 x 2048 x 5632 in tiles of 64 x 128, 88 steps: 36 us
+// with two steps in the ring, 27 with three, no less with four or six; reading by quarters 41 whatever the ring.  128 x 128: no difference).
+template <int FM, int FN> constexpr int RING = FM == 1 ? 3 : 2;
 constexpr unsigned PAST_END = 1u << 31;
 constexpr int PIECE = 1024;  // bytes that a wave's load brings: 8 rows of 64 terms, or 8 terms of 64 columns
 
@@ -36,6 +40,8 @@ enum Finish {
     GATED,   // C is up and gate of one column: activation, and z where it is kept
     UNGATED  // C is the activation's cotangent: that of z
 };
+
+template <int N> using Count = std::integral_constant<int, N>;
 
 struct Task {
     const void *a, *b, *bias;  // A [M, K] or, by rows, [K, M]; B [N, K] or, by rows, [K, N]; GATED: B [2N, K]
@@ -133,11 +139,11 @@ template <int FM, int FN> __device__ __forceinline__ size_t partial_at(int item,
 template <typename T, int FM, int FN, bool A_ROWS, bool B_ROWS, Finish FINISH>  // ..._ROWS: the terms are the operand's rows
 __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     constexpr int BM = 64 * FM, BN = 64 * FN;  // rows and columns of B's tile
-    constexpr int A_BYTES = BM * 128, SLOT = A_BYTES + BN * 128, READS = FM + FN, LOADS = 2 * READS, BESIDE = (READS + FM * FN - 1) / (FM * FN);
+    constexpr int DEEP = RING<FM, FN>, A_BYTES = BM * 128, SLOT = A_BYTES + BN * 128, READS = FM + FN, LOADS = 2 * READS, BESIDE = (READS + FM * FN - 1) / (FM * FN);
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 31, h = lane >> 5, wm = wave >> 1, wn = wave & 1;
-    constexpr int COLUMNS = FINISH == GATED ? BN / 2 : BN;
+    constexpr int WIDE = FINISH == GATED ? BN / 2 : BN;
     const long long M = task.M, N = task.N, K = task.K;
     const int steps = (int)((K + STEP - 1) / STEP);
     int at, first = 0, last = steps, item = -1;
@@ -152,10 +158,10 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     }
     int mt, nt;
     tile_at(at, task.m_tiles, task.n_tiles, mt, nt);
-    const long long row0 = (long long)mt * BM, col0 = (long long)nt * COLUMNS;
+    const long long row0 = (long long)mt * BM, col0 = (long long)nt * WIDE;
     const unsigned row_bytes = (unsigned)K * 2;
     // sources: A's rows, B's rows (GATED: up's and gate's) or B's terms
-    const int a_rows = (int)(M - row0 < BM ? M - row0 : BM), b_cols = (int)(N - col0 < COLUMNS ? N - col0 : COLUMNS);
+    const int a_rows = (int)(M - row0 < BM ? M - row0 : BM), b_cols = (int)(N - col0 < WIDE ? N - col0 : WIDE);
     const char* a_src = static_cast<const char*>(task.a) + (A_ROWS ? row0 : row0 * K) * 2;
     const char* b_src = static_cast<const char*>(task.b) + (B_ROWS ? col0 : col0 * K) * 2;
     unsigned a_off[2 * FM], b_off[2 * FN];
@@ -180,8 +186,8 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
             b_off[u] = col < b_cols ? (unsigned)(term * N + col) * 2 : PAST_END;
         } else {
             int row = 8 * q + lane / 8;
-            if (FINISH == GATED && 8 * q >= COLUMNS) {  // the same for the whole wave
-                row -= COLUMNS;
+            if (FINISH == GATED && 8 * q >= WIDE) {  // the same for the whole wave
+                row -= WIDE;
                 b_from[u] += N * K * 2;
             }
             b_off[u] = row < b_cols ? (unsigned)row * row_bytes + chunk * 16 : PAST_END;
@@ -206,10 +212,12 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     };
     // first row of B's tile (column of the product) of a wave's j-th fragment
     auto b_row = [&](int j) __attribute__((always_inline)) {
-        if (FINISH == GATED) return (j / (FN / 2)) * COLUMNS + 16 * FN * wn + 32 * (j % (FN / 2));
+        if (FINISH == GATED) return (j / (FN / 2)) * WIDE + 16 * FN * wn + 32 * (j % (FN / 2));
         return 32 * FN * wn + 32 * j;
     };
-    u32x4 af[2][FM], bf[2][FN];
+    constexpr bool AHEAD = FM == 1;  // the fragments of a whole step are read while the last one's are multiplied
+    constexpr int SETS = AHEAD ? 8 : 2;
+    u32x4 af[SETS][FM], bf[SETS][FN];
     // 16 terms of 32 columns of an operand whose terms are its rows, LDS holding 64 columns side by side
     auto by_rows = [&](const char* tile, int ks, int n0) __attribute__((always_inline)) {
         tile += n0 / 64 * 8 * PIECE;
@@ -220,18 +228,18 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
     // The reads of a quarter of a step, in the order in which the products need them: A's first fragment, B's, A's others.
-    auto read = [&](int ks, int slot, int u) __attribute__((always_inline)) {
+    auto read = [&](int set, int ks, int slot, int u) __attribute__((always_inline)) {
         const char* at_a = lds + slot * SLOT;
         const char* at_b = at_a + A_BYTES;
         if (u == 0 || u > FN) {
             const int i = u == 0 ? 0 : u - FN, n0 = 32 * FM * wm + 32 * i;
-            if constexpr (A_ROWS) af[ks & 1][i] = by_rows(at_a, ks, n0);
-            else af[ks & 1][i] = *reinterpret_cast<const u32x4*>(at_a + tile_off<64>(n0 + m, 2 * ks + h));
+            if constexpr (A_ROWS) af[set][i] = by_rows(at_a, ks, n0);
+            else af[set][i] = *reinterpret_cast<const u32x4*>(at_a + tile_off<64>(n0 + m, 2 * ks + h));
             return;
         }
         const int j = u - 1, n0 = b_row(j);
-        if constexpr (B_ROWS) bf[ks & 1][j] = by_rows(at_b, ks, n0);
-        else bf[ks & 1][j] = *reinterpret_cast<const u32x4*>(at_b + tile_off<64>(n0 + m, 2 * ks + h));
+        if constexpr (B_ROWS) bf[set][j] = by_rows(at_b, ks, n0);
+        else bf[set][j] = *reinterpret_cast<const u32x4*>(at_b + tile_off<64>(n0 + m, 2 * ks + h));
     };
     f32x16 acc[FM][FN];
 #pragma unroll
@@ -241,12 +249,12 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     // The products of a quarter of a step, and behind each what may run beside it (the compiler would put a read right before its use).
-    auto multiply = [&](int ks, auto beside) __attribute__((always_inline)) {
+    auto multiply = [&](int set, auto beside) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                acc[i][j] = Mma<T>::mma(bf[ks & 1][j], af[ks & 1][i], acc[i][j]);
+                acc[i][j] = Mma<T>::mma(bf[set][j], af[set][i], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = (i * FN + j) * BESIDE; u < (i * FN + j + 1) * BESIDE; ++u)
@@ -255,29 +263,59 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
             }
     };
 #pragma unroll
-    for (int s = 0; s < RING; ++s)
+    for (int s = 0; s < DEEP; ++s)
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) fetch(first + s, s, u);
-    __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm(LOADS));
+    __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((DEEP - 1) * LOADS));
     asm volatile("s_barrier" ::: "memory");
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int u = 0; u < READS; ++u) read(0, 0, u);
-    for (int it = first, slot = 0; it < last; ++it, slot ^= 1) {
-        // A step's place is free for the one after the next from the barrier on.  Half of its loads go beside the quarter behind it, half beside
-        // the quarter after that: all at once they queue up and hold up the products (tiles of 256 x 256, 6007 x 4096 x 11008: 525 -> 486 us).
-        multiply(0, [&](int u) __attribute__((always_inline)) {
-            read(1, slot, u);
-            if (it > first) fetch(it + 1, slot ^ 1, READS + u);
-        });
-        multiply(1, [&](int u) __attribute__((always_inline)) { read(2, slot, u); });
-        multiply(2, [&](int u) __attribute__((always_inline)) { read(3, slot, u); });
-        // this wave's loads of the next step have landed and its reads of this one are done, and behind the barrier everyone's
-        __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm(0));
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        multiply(3, [&](int u) __attribute__((always_inline)) {
-            read(0, slot ^ 1, u);
-            fetch(it + 2, slot, u);
-        });
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int u = 0; u < READS; ++u) read(ks, ks, 0, u);
+        int slot = 0;
+        auto step = [&](auto parity, int it) __attribute__((always_inline)) {
+            constexpr int now = 4 * decltype(parity)::value, then = 4 - now;
+            const int next = slot + 1 == DEEP ? 0 : slot + 1;
+            // this wave's loads of the next step have landed and its reads of this one are done, and behind the barrier everyone's
+            __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((DEEP - 2) * LOADS));
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+                multiply(now + ks, [&](int u) __attribute__((always_inline)) {
+                    read(then + ks, ks, next, u);
+                    if (ks & 1) fetch(it + DEEP, slot, ks / 2 * READS + u);
+                });
+            slot = next;
+        };
+        for (int it = first; it < last; it += 2) {
+            step(Count<0>{}, it);
+            if (it + 1 < last) step(Count<1>{}, it + 1);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < READS; ++u) read(0, 0, 0, u);
+        for (int it = first, slot = 0, before = DEEP - 1; it < last; ++it) {
+            const int next = slot + 1 == DEEP ? 0 : slot + 1;
+            // A step's place is free for the one a ring later from the barrier on.  Half of its loads go beside the quarter behind it, half
+            // beside the quarter after that: all at once they queue up and hold up the products (tiles of 256 x 256, 6007 x 4096 x 11008:
+            // 525 -> 486 us).
+            multiply(0, [&](int u) __attribute__((always_inline)) {
+                read(1, 1, slot, u);
+                if (it > first) fetch(it - 1 + DEEP, before, READS + u);
+            });
+            multiply(1, [&](int u) __attribute__((always_inline)) { read(0, 2, slot, u); });
+            multiply(0, [&](int u) __attribute__((always_inline)) { read(1, 3, slot, u); });
+            // this wave's loads of the next step have landed and its reads of this one are done, and behind the barrier everyone's
+            __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((DEEP - 2) * LOADS));
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            multiply(1, [&](int u) __attribute__((always_inline)) {
+                read(0, 0, next, u);
+                fetch(it + DEEP, slot, u);
+            });
+            before = slot;
+            slot = next;
+        }
     }
     // Nothing is under way into LDS any more, and behind the barrier nothing is read from it: from here on each wave has a part of its own, in
     // which 32 rows of its results turn from four columns a lane to eight, so that a wave's stores (and z's loads) are whole lines.
@@ -332,7 +370,97 @@ template <typename T, int FM, int FN, Finish FINISH> __global__ __launch_bounds_
     finish<T, FINISH>(task, row, col, x, y);
 }
 
+// Products of a few rows, both operands' terms side by side: a weight comes through once, and what counts is that all of the chip asks for it
+// at once.  KW waves share the sums of COLUMNS columns (GATED: pairs of them) of all rows, each lane 16 bytes of every 512 KW terms; lanes are
+// added by exchange, waves in order.  One token, 768 -> 2 x 2048 -> 768 in bf16: @@.
+constexpr int FEW = 4, COLUMNS = 2;
+constexpr int64_t FEW_TERMS = 4 << 20;  // of a weight, from three rows on
+template <typename T, int ROWS, Finish FINISH, int KW> __global__ __launch_bounds__(256) void few_rows_kernel(Task task) {
+    constexpr int HALVES = FINISH == GATED ? 2 : 1;
+    __shared__ float sums[4][HALVES][COLUMNS][ROWS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kw = wave % KW;
+    const long long M = task.M, N = task.N, K = task.K, col0 = ((long long)blockIdx.x * (4 / KW) + wave / KW) * COLUMNS;
+    const T* x = static_cast<const T*>(task.a);
+    const T* w = static_cast<const T*>(task.b);
+    const T *x_row[ROWS], *w_row[HALVES][COLUMNS];  // past the end: the last one again
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) x_row[r] = x + (r < M ? r : M - 1) * K;
+#pragma unroll
+    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c) w_row[s][c] = w + (s * N + (col0 + c < N ? col0 + c : N - 1)) * K;
+    float acc[HALVES][COLUMNS][ROWS] = {};
+#pragma unroll 2
+    for (long long k = (kw * 64 + lane) * 8; k < K; k += KW * 512) {
+        Eight wv[HALVES][COLUMNS];
+#pragma unroll
+        for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+            for (int c = 0; c < COLUMNS; ++c) wv[s][c] = load8(w_row[s][c] + k);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const Eight xv = load8(x_row[r] + k);
+#pragma unroll
+            for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[s][c][r] = fmaf(wv[s][c].v[e], xv.v[e], acc[s][c][r]);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+                for (int off = 32; off >= 1; off >>= 1) acc[s][c][r] += __shfl_xor(acc[s][c][r], off, 64);
+                if (lane == 0) sums[wave][s][c][r] = acc[s][c][r];
+            }
+    __syncthreads();
+    const int c = lane / ROWS, r = lane % ROWS;
+    const long long col = col0 + c;
+    if (kw || c >= COLUMNS || r >= M || col >= N) return;
+    float total[HALVES];
+#pragma unroll
+    for (int s = 0; s < HALVES; ++s) {
+        total[s] = sums[wave][s][c][r];
+#pragma unroll
+        for (int q = 1; q < KW; ++q) total[s] += sums[wave + q][s][c][r];
+        if (task.bias) total[s] += to_f32(static_cast<const T*>(task.bias)[s * N + col]);
+    }
+    const auto store = [](T* p, float v) { *reinterpret_cast<unsigned short*>(p) = (unsigned short)Mma<T>::pack2(v, 0.0f); };
+    T* out = static_cast<T*>(task.out) + r * N + col;
+    if constexpr (FINISH == PLAIN) {
+        store(out, total[0]);
+    } else {
+        store(out, total[0] * (total[1] * sigmoid(total[1])));
+        if (T* z = static_cast<T*>(task.z)) {
+            store(z + r * 2 * N + col, total[0]);
+            store(z + r * 2 * N + N + col, total[1]);
+        }
+    }
+}
+
+template <typename T, Finish FINISH> int launch_few(const Task& task, hipStream_t stream) {
+    const auto with = [&](auto rows, auto kw) {
+        constexpr int ROWS = decltype(rows)::value, KW = decltype(kw)::value, COUNT = COLUMNS * (4 / KW);
+        hipLaunchKernelGGL((few_rows_kernel<T, ROWS, FINISH, KW>), dim3((unsigned)((task.N + COUNT - 1) / COUNT)), dim3(256), 0, stream, task);
+        LBI_HIP_CHECK(hipGetLastError());
+        return (int)LBI_OK;
+    };
+    const auto with_rows = [&](auto rows) {  // sums so long that a wave's share takes two loads and more are shared
+        if (task.K <= 1024) return with(rows, Count<1>{});
+        return task.K <= 2048 ? with(rows, Count<2>{}) : with(rows, Count<4>{});
+    };
+    if (task.M <= 1) return with_rows(Count<1>{});
+    if (task.M <= 2) return with_rows(Count<2>{});
+    return with_rows(Count<4>{});
+}
+
 // How a product is laid out: the tile, and into how many parts the sums of those tiles are cut that do not fill the chip once more.
+constexpr int NONE = -1, FEW_ROWS = 3;
 struct Layout {
     int form;  // FM x FN: 0: 4 x 4, 1: 2 x 2, 2: 1 x 2
     int m_tiles, n_tiles, whole, parts, part_steps;
@@ -343,39 +471,38 @@ struct Layout {
     }
 };
 
-// By what a call takes, in us: for each round of workgroups over the chip its steps, a start of 2 to 2.5 and the results on their way out (20 GB/s
-// a CU, since all finish together); for parts a second launch and their sums out and back.  A step of 256 x 256 takes 1.5 us with both operands
-// by columns, 1.7 and 1.8 with one and both by rows (twice the reads); of 128 x 128, two workgroups a CU, 1.03 ... 1.07 and alone on its CU
-// 0.5 ... 0.85; of 64 x 128, three a CU, 0.95 ... 1.08 and 0.4 ... 0.75.  Of 16 calls with 1 ... 8192 rows, each with 13 layouts, what is chosen
-// took 1.01 times the best on average, 1.09 at most.
+// By what a call takes, in us: for each round of workgroups over the chip its steps, its start and the results on their way out (20 GB/s a CU, since
+// all finish together); for parts a second launch and their sums out and back.  The constants are fitted to 254 products of 35 blocks (1 ... 16896
+// rows, widths 128 ... 11008), each in up to 27 layouts: what is chosen took 1.005 times the best on average, 1.10 at most.  A step of 256 x 256
+// takes 1.5 us with the terms of both operands side by side, 1.7 with both by rows (twice the reads); of 128 x 128, two workgroups a CU, 1.0
+// and alone on its CU 0.6 ... 0.8; of 64 x 128 0.6 and 0.2 ... 0.4.
 Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
     constexpr struct { int rows, columns, a_cu; double step[3], alone[3], start; } forms[3] = {
-        {256, 256, 1, {1.5, 1.68, 1.8}, {1.5, 1.68, 1.8}, 2.5},
-        {128, 128, 2, {1.03, 1.04, 1.07}, {0.5, 0.6, 0.85}, 2.0},
-        {64, 128, 3, {0.98, 1.08, 1.0}, {0.4, 0.5, 0.75}, 2.0}};
+        {256, 256, 1, {1.50, 1.47, 1.66}, {1.30, 1.52, 1.75}, 5.1},
+        {128, 128, 2, {0.99, 0.94, 1.01}, {0.59, 0.60, 0.78}, 1.35},
+        {64, 128, 2, {0.56, 0.62, 0.65}, {0.18, 0.40, 0.43}, 2.5}};
     const int cus = device_compute_units(), steps = (int)((K + STEP - 1) / STEP);
-    Layout best{};
-    best.us = -1.0;
+    Layout best{NONE, 0, 0, 0, 1, 0, 0.0};
+    if (by_rows == 0 && M <= FEW && (M <= 2 || N * K <= FEW_TERMS)) return {FEW_ROWS, 0, 0, 0, 1, 0, 0.0};
     for (int f = 0; f < 3; ++f) {
         const auto& form = forms[f];
         const int columns = finish == GATED ? form.columns / 2 : form.columns, slots = cus * form.a_cu;
         const int64_t m_tiles = (M + form.rows - 1) / form.rows, n_tiles = (N + columns - 1) / columns, tiles = m_tiles * n_tiles;
         if (tiles >= 1 << 24) continue;
         const double full = form.step[by_rows], alone = form.alone[by_rows];
-        const double fixed = form.start + (finish == GATED ? 6 : finish == UNGATED ? 8 : 2) * form.rows * columns * form.a_cu / 20e3;
+        const double fixed = form.start + (finish == GATED ? 5.1 : finish == UNGATED ? 3.5 : 2.1) * form.rows * columns * form.a_cu / 20e3;
         const auto rounds = [&](int64_t items, int of) {
             const int deep = (int)((items % slots + cus - 1) / cus);  // workgroups that share a CU in the last round
-            const double step = deep <= 1 || form.a_cu == 1 ? alone : alone + (full - alone) * (deep - 1) / (form.a_cu - 1);
-            return (double)(items / slots) * (of * full + fixed) + (deep ? of * step + fixed : 0.0);
+            return (double)(items / slots) * (of * full + fixed) + (deep ? of * (deep == 1 ? alone : full) + fixed : 0.0);
         };
-        for (int s = 1; s <= 32; ++s) {
+        for (int s : {1, 2, 3, 4, 5, 6, 8, 12, 16}) {
             const int part_steps = (steps + s - 1) / s, parts = (steps + part_steps - 1) / part_steps;
-            if (parts != s || (s > 1 && part_steps < 2)) continue;
+            if (parts != s) continue;
             const int64_t whole = s == 1 ? tiles : tiles / slots * slots, rest = tiles - whole;
-            if (s > 1 && rest == 0) break;
+            if (s > 1 && (rest == 0 || part_steps < 2 || rest * s > 2 * slots)) break;  // parts for two rounds at most
             double us = rounds(whole, steps);
-            if (rest) us += rounds(rest * s, part_steps) + 8.0 + (double)rest * s * form.rows * form.columns * 8.0 / 8e6;
-            if (best.us < 0.0 || us < best.us) best = {f, (int)m_tiles, (int)n_tiles, (int)whole, s, part_steps, us};
+            if (rest) us += rounds(rest * s, part_steps) + 2.35 + (double)rest * s * form.rows * form.columns * 8.0 / 6.8e6;
+            if (best.form == NONE || us < best.us) best = {f, (int)m_tiles, (int)n_tiles, (int)whole, s, part_steps, us};
         }
     }
     return best;
@@ -383,7 +510,7 @@ Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
 
 template <typename T, int FM, int FN, bool A_ROWS, bool B_ROWS, Finish FINISH> int launch_tile(const Task& task, hipStream_t stream) {
     constexpr auto kernel = product_kernel<T, FM, FN, A_ROWS, B_ROWS, FINISH>;
-    constexpr size_t bytes = (size_t)RING * 8192 * (FM + FN);
+    constexpr size_t bytes = (size_t)RING<FM, FN> * 8192 * (FM + FN);
     static_assert(bytes >= 4 * 32 * (32 * FN + 4) * sizeof(float), "the turn of the results fits the ring");
     if (int status = ensure_dynamic_lds<kernel>(bytes)) return status;
     const int rest = task.m_tiles * task.n_tiles - task.whole;
@@ -396,13 +523,14 @@ template <typename T, int FM, int FN, bool A_ROWS, bool B_ROWS, Finish FINISH> i
     return LBI_OK;
 }
 
-// `partial`: layout_of(...).bytes()
+// `partial`: l.bytes()
 template <typename T, bool A_ROWS, bool B_ROWS, Finish FINISH>
-int launch(const void* a, const void* b, const void* bias, void* out, void* z, int64_t M, int64_t N, int64_t K, void* partial,
+int launch(const Layout& l, const void* a, const void* b, const void* bias, void* out, void* z, int64_t M, int64_t N, int64_t K, void* partial,
            hipStream_t stream) {
-    const Layout l = layout_of(M, N, K, FINISH, A_ROWS + B_ROWS);
-    if (l.us < 0.0) return fail(LBI_ERR_UNSUPPORTED, "lbi_gated_mlp: too many tiles");
+    if (l.form == NONE) return fail(LBI_ERR_UNSUPPORTED, "lbi_gated_mlp: too many tiles");
     const Task task{a, b, bias, out, z, M, N, K, static_cast<float*>(partial), l.m_tiles, l.n_tiles, l.whole, l.parts, l.part_steps};
+    if constexpr (!A_ROWS && !B_ROWS)
+        if (l.form == FEW_ROWS) return launch_few<T, FINISH>(task, stream);
     if (l.form == 0) return launch_tile<T, 4, 4, A_ROWS, B_ROWS, FINISH>(task, stream);
     if (l.form == 1) return launch_tile<T, 2, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
     return launch_tile<T, 1, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
@@ -480,17 +608,22 @@ bool on_grid(std::initializer_list<const void*> tensors) {
 }
 
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
-size_t forward_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
-    return up(std::max(layout_of(rows, hidden, D, GATED, 0).bytes(), layout_of(rows, width, hidden, PLAIN, 0).bytes()));
-}
-struct Parts {  // of the pullback's workspace, in bytes
-    size_t g_fc1, sums, partial;
+struct Forward {
+    Layout fc1, fc2;
+    Forward(int64_t rows, int64_t D, int64_t hidden, int64_t width)
+        : fc1(layout_of(rows, hidden, D, GATED, 0)), fc2(layout_of(rows, width, hidden, PLAIN, 0)) {}
+    size_t bytes() const { return up(std::max(fc1.bytes(), fc2.bytes())); }
 };
-Parts parts_of(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
-    return {up((size_t)rows * 2 * hidden * 2), up((size_t)slabs_of(rows) * std::max(2 * hidden, width) * sizeof(float)),
-            up(std::max({layout_of(rows, hidden, width, UNGATED, 1).bytes(), layout_of(rows, D, 2 * hidden, PLAIN, 1).bytes(),
-                         layout_of(2 * hidden, D, rows, PLAIN, 2).bytes(), layout_of(width, hidden, rows, PLAIN, 2).bytes()}))};
-}
+struct Pullback {
+    Layout a, x, fc1, fc2;
+    size_t g_fc1, sums, partial;  // parts of the workspace, in bytes
+    Pullback(int64_t rows, int64_t D, int64_t hidden, int64_t width)
+        : a(layout_of(rows, hidden, width, UNGATED, 1)), x(layout_of(rows, D, 2 * hidden, PLAIN, 1)),
+          fc1(layout_of(2 * hidden, D, rows, PLAIN, 2)), fc2(layout_of(width, hidden, rows, PLAIN, 2)), g_fc1(up((size_t)rows * 2 * hidden * 2)),
+          sums(up((size_t)slabs_of(rows) * std::max(2 * hidden, width) * sizeof(float))),
+          partial(up(std::max({a.bytes(), x.bytes(), fc1.bytes(), fc2.bytes()}))) {}
+    size_t bytes() const { return g_fc1 + sums + partial; }
+};
 
 }  // namespace
 }  // namespace block_mlp
@@ -499,7 +632,7 @@ Parts parts_of(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
 extern "C" size_t lbi_gated_mlp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
     using namespace lbi::block_mlp;
     if (check("lbi_gated_mlp", rows, D, hidden, width, LBI_BF16) || rows == 0) return 0;
-    return forward_bytes(rows, D, hidden, width);
+    return Forward(rows, D, hidden, width).bytes();
 }
 
 extern "C" int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* fc1_bias, const void* fc2_weight, const void* fc2_bias,
@@ -513,14 +646,15 @@ extern "C" int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* 
     if (!x || !fc1_weight || !fc2_weight || !down_input || !out) return fail(LBI_ERR_INVALID, "lbi_gated_mlp: null pointer");
     if (!on_grid({x, fc1_weight, fc1_bias, fc2_weight, fc2_bias, fc1_output, down_input, out, workspace}))
         return fail(LBI_ERR_INVALID, "lbi_gated_mlp: tensors must be 16-byte aligned");
-    const size_t need = forward_bytes(rows, D, hidden, width);
+    const Forward l(rows, D, hidden, width);
+    const size_t need = l.bytes();
     if (need && (!workspace || workspace_bytes < need))
         return fail(LBI_ERR_WORKSPACE, "lbi_gated_mlp: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     const hipStream_t on = static_cast<hipStream_t>(stream);
     const auto run = [&](auto t) {
         using T = decltype(t);
-        if (int s = launch<T, false, false, GATED>(x, fc1_weight, fc1_bias, down_input, fc1_output, rows, hidden, D, workspace, on)) return s;
-        return launch<T, false, false, PLAIN>(down_input, fc2_weight, fc2_bias, out, nullptr, rows, width, hidden, workspace, on);
+        if (int s = launch<T, false, false, GATED>(l.fc1, x, fc1_weight, fc1_bias, down_input, fc1_output, rows, hidden, D, workspace, on)) return s;
+        return launch<T, false, false, PLAIN>(l.fc2, down_input, fc2_weight, fc2_bias, out, nullptr, rows, width, hidden, workspace, on);
     };
     return dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{});
 }
@@ -528,8 +662,7 @@ extern "C" int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* 
 extern "C" size_t lbi_gated_mlp_vjp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
     using namespace lbi::block_mlp;
     if (check("lbi_gated_mlp_vjp", rows, D, hidden, width, LBI_BF16) || rows == 0) return 0;
-    const Parts p = parts_of(rows, D, hidden, width);
-    return p.g_fc1 + p.sums + p.partial;
+    return Pullback(rows, D, hidden, width).bytes();
 }
 
 extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* fc1_output, const void* down_input, const void* fc1_weight,
@@ -546,9 +679,9 @@ extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* f
     if (!on_grid({g_out, x, fc1_output, down_input, fc1_weight, fc2_weight, g_x, g_fc1_weight, g_fc2_weight, g_fc1_bias, g_fc2_bias}) ||
         reinterpret_cast<uintptr_t>(workspace) % 256)
         return fail(LBI_ERR_INVALID, "lbi_gated_mlp_vjp: tensors must be 16-byte aligned, the workspace 256");
-    const Parts p = parts_of(rows, D, hidden, width);
-    if (!workspace || workspace_bytes < p.g_fc1 + p.sums + p.partial)
-        return fail(LBI_ERR_WORKSPACE, "lbi_gated_mlp_vjp: workspace of %zu bytes needed, %zu given", p.g_fc1 + p.sums + p.partial, workspace_bytes);
+    const Pullback p(rows, D, hidden, width);
+    if (!workspace || workspace_bytes < p.bytes())
+        return fail(LBI_ERR_WORKSPACE, "lbi_gated_mlp_vjp: workspace of %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
     const hipStream_t on = static_cast<hipStream_t>(stream);
     char* g_fc1 = static_cast<char*>(workspace);
     float* sums = reinterpret_cast<float*>(g_fc1 + p.g_fc1);
@@ -556,10 +689,10 @@ extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* f
     const auto run = [&](auto t) {
         using T = decltype(t);
         void* z = const_cast<void*>(fc1_output);
-        if (int s = launch<T, false, true, UNGATED>(g_out, fc2_weight, nullptr, g_fc1, z, rows, hidden, width, partial, on)) return s;
-        if (int s = launch<T, false, true, PLAIN>(g_fc1, fc1_weight, nullptr, g_x, nullptr, rows, D, 2 * hidden, partial, on)) return s;
-        if (int s = launch<T, true, true, PLAIN>(g_fc1, x, nullptr, g_fc1_weight, nullptr, 2 * hidden, D, rows, partial, on)) return s;
-        if (int s = launch<T, true, true, PLAIN>(g_out, down_input, nullptr, g_fc2_weight, nullptr, width, hidden, rows, partial, on)) return s;
+        if (int s = launch<T, false, true, UNGATED>(p.a, g_out, fc2_weight, nullptr, g_fc1, z, rows, hidden, width, partial, on)) return s;
+        if (int s = launch<T, false, true, PLAIN>(p.x, g_fc1, fc1_weight, nullptr, g_x, nullptr, rows, D, 2 * hidden, partial, on)) return s;
+        if (int s = launch<T, true, true, PLAIN>(p.fc1, g_fc1, x, nullptr, g_fc1_weight, nullptr, 2 * hidden, D, rows, partial, on)) return s;
+        if (int s = launch<T, true, true, PLAIN>(p.fc2, g_out, down_input, nullptr, g_fc2_weight, nullptr, width, hidden, rows, partial, on)) return s;
         if (g_fc1_bias)
             if (int s = column_sums<T>(g_fc1, g_fc1_bias, sums, rows, 2 * hidden, on)) return s;
         if (g_fc2_bias)

@@ -24,41 +24,49 @@ def _flat(t: torch.Tensor) -> bool:
     return t.permute(order).is_contiguous()
 
 
-def _check(tensors: Sequence[torch.Tensor], what: str) -> None:
+def _check(tensors: Sequence[torch.Tensor], what: str, device: torch.device | None = None) -> torch.device:
+    """The one device of ``tensors``."""
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what} must be torch.Tensors")
-        if t.layout != torch.strided:
+        if t.layout is not torch.strided:
             raise TypeError(f"{what} must be dense tensors")
-        _lib.dtype_code(t.dtype)
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} must be CUDA tensors (this build has no CPU execution path)")
-        if t.device != tensors[0].device:
-            raise ValueError(f"{what} must be on one device")
+        if t.dtype not in _lib._DTYPE_CODES:
+            _lib.dtype_code(t.dtype)
+        if device is None or t.device != device:
+            if not t.is_cuda:
+                raise RuntimeError(f"{what} must be CUDA tensors (this build has no CPU execution path)")
+            if device is not None:
+                raise ValueError(f"{what} must be on one device")
+            device = t.device
+    return device
 
 
 def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor | None], max_norm: float) -> torch.Tensor:
     device = grads[0].device
+    codes = _lib._DTYPE_CODES
     words, held, late = [], [], []
     for g, out in zip(grads, outs):
         to = out
-        if not _flat(g) or not (out is None or out is g or out.stride() == g.stride() or (g.is_contiguous() and out.is_contiguous())):
+        if not (g.is_contiguous() and (out is None or out is g or out.is_contiguous())) and not (
+                _flat(g) and (out is None or out is g or out.stride() == g.stride())):
             g = g.contiguous()
             if out is not None and (out is g or not out.is_contiguous()):
                 to = torch.empty_like(g)
                 late.append((out, to))
             # a contiguous `out` of its own is written by the kernel
-        held.append((g, to))  # copies live until the kernels are queued
-        words += (g.data_ptr(), 0 if to is None else to.data_ptr(), g.numel(), _lib.dtype_code(g.dtype))
-    if len({(o.data_ptr(), o.shape, o.stride()) for o, _ in late}) != len(late):
+            held.append((g, to))  # copies live until the kernels are queued
+        words += (g.data_ptr(), 0 if to is None else to.data_ptr(), g.numel(), codes[g.dtype])
+    count = len(words) // 4
+    if late and len({(o.data_ptr(), o.shape, o.stride()) for o, _ in late}) != len(late):
         raise ValueError("a result overlaps another tensor")
     table = (ctypes.c_int64 * len(words))(*words)
     norm = torch.empty((), device=device, dtype=torch.float32)
     lib = _lib.load()
     with _lib.device_guard(device):
-        need = int(lib.lbi_clip_gradients_workspace_bytes(table, len(held)))
+        need = int(lib.lbi_clip_gradients_workspace_bytes(table, count))
         workspace = torch.empty(max(need, 8), device=device, dtype=torch.uint8)
-        status = lib.lbi_clip_gradients(table, len(held), max_norm, norm.data_ptr(), workspace.data_ptr(), need,
+        status = lib.lbi_clip_gradients(table, count, max_norm, norm.data_ptr(), workspace.data_ptr(), need,
                                         _lib.current_stream_ptr(device))
     _lib.check(status, "lbi_clip_gradients")
     for out, to in late:
@@ -94,15 +102,15 @@ def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, *, out: Seque
             raise ValueError("out must hold one tensor for each gradient")
     if not grads:
         return torch.zeros(())
-    _check(grads, "grads")
+    device = _check(grads, "grads")
     if out is None:
         out = grads
     else:
-        _check([grads[0], *out], "out")
+        _check(out, "out", device)
         for g, o in zip(grads, out):
             if g.shape != o.shape or g.dtype != o.dtype:
                 raise ValueError("out must have the shapes and types of the gradients")
-    if torch.is_grad_enabled() and any(o.requires_grad for o in out):
+    if any(o.requires_grad for o in out) and torch.is_grad_enabled():
         raise RuntimeError("clip_gradients writes tensors that require grad: call it under torch.no_grad()")
     return _clip(grads, out, max_norm)
 

@@ -22,14 +22,19 @@ _PRODUCT_TYPES = (torch.float16, torch.bfloat16)
 
 
 def _no_graph(what: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} records no autograd graph: call it under torch.no_grad(), with its pullback for the gradients")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} records no autograd graph: call it under torch.no_grad(), with its pullback for the gradients")
 
 
 def _one_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
-    _require_cuda(first, *(t for t in others if t is not None))
-    if any(t is not None and t.device != first.device for t in others):
-        raise ValueError(f"{what}: tensors must be on one device")
+    device = first.device
+    if device.type != "cuda":
+        _require_cuda(first)
+    for t in others:
+        if t is not None and t.device != device:
+            _require_cuda(t)
+            raise ValueError(f"{what}: tensors must be on one device")
 
 
 def _norm_types(what: str, branch: torch.dtype, stream: torch.dtype, weight: torch.Tensor) -> torch.Tensor:
@@ -55,21 +60,22 @@ def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight
         raise ValueError("residual_rmsnorm: residual must be shaped like hidden")
     _one_device("residual_rmsnorm", hidden, residual, weight)
     _no_graph("residual_rmsnorm", hidden, residual, weight)
-    stream = residual_dtype or (hidden if residual is None else residual).dtype
-    weight = _norm_types("residual_rmsnorm", hidden.dtype, stream, weight).contiguous()
+    branch = hidden.dtype
+    stream = residual_dtype or (branch if residual is None else residual.dtype)
+    weight = _norm_types("residual_rmsnorm", branch, stream, weight).contiguous()
     hidden = hidden.contiguous()
     if residual is not None:
-        residual = residual.to(stream).contiguous()
-    total = torch.empty(hidden.shape, device=hidden.device, dtype=stream)
-    normed = torch.empty(hidden.shape, device=hidden.device, dtype=torch.float8_e4m3fn if scaled else hidden.dtype)
+        residual = (residual if residual.dtype == stream else residual.to(stream)).contiguous()
+    total = torch.empty_like(hidden, dtype=stream)
+    normed = torch.empty_like(hidden, dtype=torch.float8_e4m3fn) if scaled else torch.empty_like(hidden)
     scales = torch.empty(hidden.shape[:-1], device=hidden.device, dtype=torch.float32) if scaled else None
-    width = int(hidden.shape[-1])
-    if hidden.numel():
+    count, width = hidden.numel(), hidden.shape[-1]
+    if count:
         with _lib.device_guard(hidden.device):
             status = _lib.load().lbi_residual_rmsnorm(
                 hidden.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), normed.data_ptr(),
-                total.data_ptr(), None if scales is None else scales.data_ptr(), hidden.numel() // width, width, float(eps),
-                _lib.dtype_code(hidden.dtype), _lib.dtype_code(stream), _lib.dtype_code(weight.dtype), _stream(hidden))
+                total.data_ptr(), None if scales is None else scales.data_ptr(), count // width, width, eps,
+                _lib.dtype_code(branch), _lib.dtype_code(stream), _lib.dtype_code(weight.dtype), _stream(hidden))
         _lib.check(status, "lbi_residual_rmsnorm")
     elif scales is not None:
         scales.fill_(1.0)
@@ -94,7 +100,7 @@ def residual_rmsnorm_pullback(g_normed: torch.Tensor, residual_out: torch.Tensor
     g_normed, residual_out = g_normed.contiguous(), residual_out.contiguous()
     if g_residual is not None:
         g_residual = g_residual.contiguous()
-    g_stream = torch.empty(g_normed.shape, device=g_normed.device, dtype=stream)
+    g_stream = torch.empty_like(residual_out)
     g_hidden = g_stream if stream == branch else torch.empty_like(g_normed)
     width = int(g_normed.shape[-1])
     g_weight = torch.empty(width, device=g_normed.device, dtype=torch.float32)
@@ -130,10 +136,10 @@ def _check_mlp(what: str, x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight:
 
 def _ready(t: torch.Tensor | None, dtype: torch.dtype, *to: int) -> torch.Tensor | None:
     """``t`` in ``dtype``, padded with zeros to the shape ``to``, contiguous and on the kernels' 16-byte grid."""
-    if t is None:
-        return None
+    if t is None or (t.dtype == dtype and t.shape == to and t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
     t = t.detach().to(dtype)
-    if tuple(t.shape) != to:
+    if t.shape != to:
         pad = [extent for have, want in zip(reversed(t.shape), reversed(to)) for extent in (0, want - have)]
         t = torch.nn.functional.pad(t, pad)
     t = t.contiguous()
@@ -146,8 +152,8 @@ def _eights(n: int) -> int:
 
 def _halves(t: torch.Tensor | None, dtype: torch.dtype, hidden: int, *rest: int) -> torch.Tensor | None:
     """``[2 * hidden, ...]`` with each half padded (see :func:`_ready`)."""
-    if t is None:
-        return None
+    if t is None or t.shape[0] == 2 * hidden and t.shape[1:] == rest:  # nothing to pad between the halves
+        return _ready(t, dtype, 2 * hidden, *rest)
     halves = _ready(t.reshape(2, t.shape[0] // 2, *t.shape[1:]), dtype, 2, hidden, *rest)
     return halves.view(2 * hidden, *rest)
 
@@ -170,7 +176,7 @@ def gated_mlp(x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight: torch.Tenso
     out, down = x.new_empty(rows, w), x.new_empty(rows, hd)
     fc1_output = x.new_empty(rows, 2 * hd) if keep else None
     if rows:
-        x = _ready(x.reshape(rows, dim), dtype, rows, d)
+        x = _ready(x if x.dim() == 2 else x.reshape(rows, dim), dtype, rows, d)
         fc1_weight, fc1_bias = _halves(fc1_weight, dtype, hd, d), _halves(fc1_bias, dtype, hd)
         fc2_weight, fc2_bias = _ready(fc2_weight, dtype, w, hd), _ready(fc2_bias, dtype, w)
         lib = _lib.load()
@@ -183,10 +189,13 @@ def gated_mlp(x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight: torch.Tenso
                 down.data_ptr(), out.data_ptr(), None if workspace is None else workspace.data_ptr(), need, rows, d, hd, w,
                 _lib.dtype_code(dtype), _stream(x))
         _lib.check(status, "lbi_gated_mlp")
-    out = out[:, :width].reshape(*outer, width)
+    if width != w or len(outer) != 1:
+        out = out[:, :width].reshape(*outer, width)
     if not keep:
         return out
-    return out, fc1_output.view(rows, 2, hd)[:, :, :hidden].reshape(*outer, 2 * hidden), down[:, :hidden].reshape(*outer, hidden)
+    if hidden != hd or len(outer) != 1:
+        fc1_output, down = fc1_output.view(rows, 2, hd)[:, :, :hidden].reshape(*outer, 2 * hidden), down[:, :hidden].reshape(*outer, hidden)
+    return out, fc1_output, down
 
 
 def gated_mlp_vjp(g_out: torch.Tensor, x: torch.Tensor, fc1_output: torch.Tensor, down_input: torch.Tensor, fc1_weight: torch.Tensor,
@@ -206,8 +215,10 @@ def gated_mlp_vjp(g_out: torch.Tensor, x: torch.Tensor, fc1_output: torch.Tensor
         empty = [torch.zeros_like(x), x.new_zeros(fc1_weight.shape), x.new_zeros(fc2_weight.shape)]
         return tuple(empty + [x.new_zeros(2 * hidden), x.new_zeros(width)] if bias else empty)
     d, hd, w = _eights(dim), _eights(hidden), _eights(width)
-    g_out, x, down_input = (_ready(t.reshape(rows, -1), dtype, rows, to) for t, to in ((g_out, w), (x, d), (down_input, hd)))
-    fc1_output = _ready(fc1_output.reshape(rows, 2, hidden), dtype, rows, 2, hd)
+    if len(outer) != 1:
+        g_out, x, fc1_output, down_input = (t.reshape(rows, t.shape[-1]) for t in (g_out, x, fc1_output, down_input))
+    g_out, x, down_input = _ready(g_out, dtype, rows, w), _ready(x, dtype, rows, d), _ready(down_input, dtype, rows, hd)
+    fc1_output = _ready(fc1_output if hidden == hd else fc1_output.reshape(rows, 2, hidden), dtype, rows, *((2 * hd,) if hidden == hd else (2, hd)))
     fc1_weight, fc2_weight = _halves(fc1_weight, dtype, hd, d), _ready(fc2_weight, dtype, w, hd)
     g_x, g_fc1, g_fc2 = x.new_empty(rows, d), x.new_empty(2 * hd, d), x.new_empty(w, hd)
     g_fc1_bias, g_fc2_bias = (x.new_empty(2 * hd), x.new_empty(w)) if bias else (None, None)
@@ -220,11 +231,12 @@ def gated_mlp_vjp(g_out: torch.Tensor, x: torch.Tensor, fc1_output: torch.Tensor
             g_x.data_ptr(), g_fc1.data_ptr(), g_fc2.data_ptr(), g_fc1_bias.data_ptr() if bias else None,
             g_fc2_bias.data_ptr() if bias else None, workspace.data_ptr(), need, rows, d, hd, w, _lib.dtype_code(dtype), _stream(x))
     _lib.check(status, "lbi_gated_mlp_vjp")
-    grads = [g_x[:, :dim].reshape(*outer, dim), g_fc1.view(2, hd, d)[:, :hidden, :dim].reshape(2 * hidden, dim),
-             g_fc2[:width, :hidden].contiguous()]
-    if bias:
-        grads += [g_fc1_bias.view(2, hd)[:, :hidden].reshape(2 * hidden), g_fc2_bias[:width].contiguous()]
-    return tuple(grads)
+    if (dim, hidden, width) != (d, hd, w):
+        g_x, g_fc1, g_fc2 = g_x[:, :dim].contiguous(), g_fc1.view(2, hd, d)[:, :hidden, :dim].reshape(2 * hidden, dim), g_fc2[:width, :hidden].contiguous()
+        if bias:
+            g_fc1_bias, g_fc2_bias = g_fc1_bias.view(2, hd)[:, :hidden].reshape(2 * hidden), g_fc2_bias[:width].contiguous()
+    grads = (g_x if len(outer) == 1 else g_x.view(*outer, dim), g_fc1, g_fc2)
+    return (*grads, g_fc1_bias, g_fc2_bias) if bias else grads
 
 
 __all__ = ["gated_mlp", "gated_mlp_vjp", "residual_rmsnorm", "residual_rmsnorm_pullback"]
