@@ -468,7 +468,7 @@ typedef struct lbi_gradient {
     int64_t dtype;
 } lbi_gradient;
 
-size_t lbi_clip_gradients_workspace_bytes(const lbi_gradient* gradients, int64_t n);
+size_t lbi_clip_gradients_workspace_bytes(int64_t n);
 int lbi_clip_gradients(const lbi_gradient* gradients, int64_t n, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
                        void* stream);
 

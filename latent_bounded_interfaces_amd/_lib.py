@@ -138,7 +138,7 @@ SYMBOLS = {
         _c.c_int,
         [_c.c_void_p] * 12 + [_c.c_size_t] + [_c.c_int64] * 4 + [_c.c_int, _c.c_void_p],
     ),
-    "lbi_clip_gradients_workspace_bytes": (_c.c_size_t, [_c.c_void_p, _c.c_int64]),
+    "lbi_clip_gradients_workspace_bytes": (_c.c_size_t, [_c.c_int64]),
     "lbi_clip_gradients": (
         _c.c_int,
         [_c.c_void_p, _c.c_int64, _c.c_float, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p],

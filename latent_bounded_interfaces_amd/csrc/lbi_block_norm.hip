@@ -6,8 +6,8 @@
 // Everything between load and store is fp32, the sum that the norm sees included: it is rounded only where it is stored.  y comes in the
 // type of `hidden`, or in 8 bits (e4m3) with one scale a row, max|y| / 448.
 //
-// Bound by memory: a row is read once and kept in registers, eight neighbouring elements a lane and piece, by one wave up to 2048 columns,
-// by a workgroup of 256 or 512 threads beyond.  Pieces are loaded at any alignment (an element's own is enough); one that runs past the
+// Bound by memory: a row is read once and kept in registers, eight neighbouring elements a lane and piece, by as many lanes (8 ... 1024) as
+// hold it in one or two pieces: few registers a lane leave room for the waves that hide the loads.  Pieces are loaded at any alignment (an element's own is enough); one that runs past the
 // end of its row goes element by element, so every width takes the same kernel.
 #include <hip/hip_runtime.h>
 
@@ -31,33 +31,49 @@ typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 
 struct Eight { float v[PIECE]; };
 
-// Eight elements from `p` on, `left` of which are in the row (the others are zero).
-__device__ __forceinline__ Eight load8(const float* p, int left) {
-    Eight r;
-    if (left >= PIECE) {
-        const f32x4_any a = reinterpret_cast<const f32x4_any*>(p)[0], b = reinterpret_cast<const f32x4_any*>(p + 4)[0];
+// Eight elements as stored.  They are widened only where they are used: a conversion right behind its load would wait for it, and the loads of
+// a row would come one after the other (2000 x 8192 in bf16, pullback: 46 -> 32 us).
+template <typename T> struct Raw {
+    u32x4_any w;
+    __device__ __forceinline__ Eight wide() const {
+        Eight r;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r.v[e] = a[e], r.v[4 + e] = b[e];
+        for (int e = 0; e < 4; ++e) r.v[2 * e] = Mma<T>::lo(w[e]), r.v[2 * e + 1] = Mma<T>::hi(w[e]);
+        return r;
+    }
+};
+template <> struct Raw<float> {
+    f32x4_any a, b;
+    __device__ __forceinline__ Eight wide() const { return Eight{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}}; }
+};
+// From `p` on, `left` of which are in the row (TAIL: perhaps fewer than eight; the others are zero).
+template <bool TAIL> __device__ __forceinline__ Raw<float> load8(const float* p, int left) {
+    Raw<float> r;
+    if (!TAIL || left >= PIECE) {
+        r.a = reinterpret_cast<const f32x4_any*>(p)[0];
+        r.b = reinterpret_cast<const f32x4_any*>(p + 4)[0];
     } else {
 #pragma unroll
-        for (int e = 0; e < PIECE; ++e) r.v[e] = e < left ? p[e] : 0.0f;
+        for (int e = 0; e < 4; ++e) {
+            r.a[e] = e < left ? p[e] : 0.0f;
+            r.b[e] = 4 + e < left ? p[4 + e] : 0.0f;
+        }
     }
     return r;
 }
-template <typename T> __device__ __forceinline__ Eight load8(const T* p, int left) {
-    Eight r;
-    if (left >= PIECE) {
-        const u32x4_any a = *reinterpret_cast<const u32x4_any*>(p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r.v[2 * e] = Mma<T>::lo(a[e]), r.v[2 * e + 1] = Mma<T>::hi(a[e]);
+template <bool TAIL, typename T> __device__ __forceinline__ Raw<T> load8(const T* p, int left) {
+    Raw<T> r;
+    if (!TAIL || left >= PIECE) {
+        r.w = *reinterpret_cast<const u32x4_any*>(p);
     } else {
+        const unsigned short* raw = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-        for (int e = 0; e < PIECE; ++e) r.v[e] = e < left ? to_f32(p[e]) : 0.0f;
+        for (int e = 0; e < 4; ++e) r.w[e] = (2 * e < left ? raw[2 * e] : 0u) | (2 * e + 1 < left ? (unsigned)raw[2 * e + 1] << 16 : 0u);
     }
     return r;
 }
-__device__ __forceinline__ void store8(float* p, const Eight& x, int left) {
-    if (left >= PIECE) {
+template <bool TAIL> __device__ __forceinline__ void store8(float* p, const Eight& x, int left) {
+    if (!TAIL || left >= PIECE) {
         reinterpret_cast<f32x4_any*>(p)[0] = f32x4_any{x.v[0], x.v[1], x.v[2], x.v[3]};
         reinterpret_cast<f32x4_any*>(p + 4)[0] = f32x4_any{x.v[4], x.v[5], x.v[6], x.v[7]};
     } else {
@@ -66,11 +82,11 @@ __device__ __forceinline__ void store8(float* p, const Eight& x, int left) {
             if (e < left) p[e] = x.v[e];
     }
 }
-template <typename T> __device__ __forceinline__ void store8(T* p, const Eight& x, int left) {
+template <bool TAIL, typename T> __device__ __forceinline__ void store8(T* p, const Eight& x, int left) {
     u32x4_any words;
 #pragma unroll
     for (int e = 0; e < 4; ++e) words[e] = Mma<T>::pack2(x.v[2 * e], x.v[2 * e + 1]);
-    if (left >= PIECE) {
+    if (!TAIL || left >= PIECE) {
         *reinterpret_cast<u32x4_any*>(p) = words;
     } else {
         unsigned short* raw = reinterpret_cast<unsigned short*>(p);
@@ -79,14 +95,14 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const Eight& 
             if (e < left) raw[e] = (unsigned short)(words[e / 2] >> (16 * (e % 2)));
     }
 }
-__device__ __forceinline__ void store8_e4m3(unsigned char* p, const Eight& x, int left) {
+template <bool TAIL> __device__ __forceinline__ void store8_e4m3(unsigned char* p, const Eight& x, int left) {
     u32x2_any words;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         int w = __builtin_amdgcn_cvt_pk_fp8_f32(x.v[4 * e], x.v[4 * e + 1], 0, false);
         words[e] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x.v[4 * e + 2], x.v[4 * e + 3], w, true);
     }
-    if (left >= PIECE) {
+    if (!TAIL || left >= PIECE) {
         *reinterpret_cast<u32x2_any*>(p) = words;
     } else {
 #pragma unroll
@@ -101,60 +117,85 @@ __device__ __forceinline__ float larger(float a, float b) { return b > a || b !=
 struct Add { static __device__ __forceinline__ float of(float a, float b) { return a + b; } };
 struct Larger { static __device__ __forceinline__ float of(float a, float b) { return larger(a, b); } };
 
-// One value over the NT threads that share a row, the same in all of them: lanes by exchange, waves in order.  `spare`: NT / 64 floats that no
-// other exchange of the row uses.
+// One value over the threads that share a row, the same in all of them: lanes by exchange, waves in order.  Rows of up to 64 threads have NT of
+// them, wider ones the whole workgroup, which is at most NT.  `spare`: NT / 64 floats that no other exchange of the row uses.
 template <typename Op, int NT> __device__ __forceinline__ float over_row(float x, float* spare) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x = Op::of(x, __shfl_xor(x, off, 64));
+    for (int off = (NT < 64 ? NT : 64) / 2; off >= 1; off >>= 1) x = Op::of(x, __shfl_xor(x, off, 64));
     if constexpr (NT > 64) {
         if ((threadIdx.x & 63) == 0) spare[threadIdx.x >> 6] = x;
         __syncthreads();
         x = spare[0];
-#pragma unroll
-        for (int w = 1; w < NT / 64; ++w) x = Op::of(x, spare[w]);
+        for (int w = 1; w < (int)blockDim.x / 64; ++w) x = Op::of(x, spare[w]);
     }
     return x;
 }
 
-template <typename T> __device__ __forceinline__ Eight load_weight(const void* weight, int c, int left, bool wide) {
-    return wide ? load8(static_cast<const float*>(weight) + c, left) : load8(static_cast<const T*>(weight) + c, left);
+// Two sums at once.
+template <int NT> __device__ __forceinline__ void sums_over_row(float& x, float& y, float (*spare)[2]) {
+#pragma unroll
+    for (int off = (NT < 64 ? NT : 64) / 2; off >= 1; off >>= 1) {
+        const float a = __shfl_xor(x, off, 64), b = __shfl_xor(y, off, 64);
+        x += a;
+        y += b;
+    }
+    if constexpr (NT > 64) {
+        if ((threadIdx.x & 63) == 0) spare[threadIdx.x >> 6][0] = x, spare[threadIdx.x >> 6][1] = y;
+        __syncthreads();
+        x = spare[0][0];
+        y = spare[0][1];
+        for (int w = 1; w < (int)blockDim.x / 64; ++w) x += spare[w][0], y += spare[w][1];
+    }
 }
 
-// NT threads a row (a workgroup of 256 holds four rows of 64), PIECES pieces a lane.
-template <typename T, typename R, bool SCALED, int NT, int PIECES>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const T* __restrict__ hidden, const R* __restrict__ residual,
-                                                                   const void* __restrict__ weight, void* __restrict__ normed,
-                                                                   R* __restrict__ stream_out, float* __restrict__ scales, long long rows,
-                                                                   int D, float eps, int weight_wide) {
-    __shared__ float spare[2][NT / 64];
-    const int t = threadIdx.x % NT;
-    const long long row = NT < 256 ? (long long)blockIdx.x * (256 / NT) + threadIdx.x / NT : (long long)blockIdx.x;
-    if (row >= rows) return;  // whole waves, and no barrier below is theirs alone
+// rows that a workgroup holds side by side: 256 threads of rows that need no more than a wave each, one row otherwise
+template <int NT> constexpr int SIDE = NT <= 64 ? 256 / NT : 1;
+
+template <bool TAIL, typename T> __device__ __forceinline__ Eight load_weight(const void* weight, int c, int left, bool wide) {
+    return wide ? load8<TAIL>(static_cast<const float*>(weight) + c, left).wide() : load8<TAIL>(static_cast<const T*>(weight) + c, left).wide();
+}
+
+// NT threads a row (beyond 64: up to NT, the workgroup's), PIECES pieces a lane.  TAIL: D is no whole number of pieces.
+template <typename T, typename R, bool SCALED, bool TAIL, int NT, int PIECES>
+__global__ __launch_bounds__(NT * SIDE<NT>) void norm_kernel(const T* __restrict__ hidden, const R* __restrict__ residual,
+                                                             const void* __restrict__ weight, void* __restrict__ normed,
+                                                             R* __restrict__ stream_out, float* __restrict__ scales, long long rows, int D,
+                                                             float eps, int weight_wide) {
+    __shared__ float spare[2][NT <= 64 ? 1 : NT / 64];
+    const int threads = NT <= 64 ? NT : (int)blockDim.x, t = threadIdx.x % threads;
+    const long long row = (long long)blockIdx.x * SIDE<NT> + threadIdx.x / threads;
+    if (row >= rows) return;  // all lanes of a row, and with barriers below the row is the workgroup's only one
+    Raw<T> h[PIECES];
+    Raw<R> r[PIECES];
     Eight s[PIECES], w[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int c = (p * NT + t) * PIECE;
-        if (c < D) s[p] = load8(hidden + row * D + c, D - c);
+        const int c = (p * threads + t) * PIECE;
+        if (c < D) h[p] = load8<TAIL>(hidden + row * D + c, D - c);
     }
-    if (residual) {
-        Eight r[PIECES];
+    if (residual)
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int c = (p * NT + t) * PIECE;
-            if (c < D) r[p] = load8(residual + row * D + c, D - c);
+            const int c = (p * threads + t) * PIECE;
+            if (c < D) r[p] = load8<TAIL>(residual + row * D + c, D - c);
         }
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-#pragma unroll
-            for (int e = 0; e < PIECE; ++e) s[p].v[e] += r[p].v[e];
+    for (int p = 0; p < PIECES; ++p) {
+        const int c = (p * threads + t) * PIECE;
+        if (c < D) w[p] = load_weight<TAIL, T>(weight, c, D - c, weight_wide != 0);
     }
     float sum = 0.0f;
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int c = (p * NT + t) * PIECE;
+        const int c = (p * threads + t) * PIECE;
         if (c >= D) continue;
-        w[p] = load_weight<T>(weight, c, D - c, weight_wide != 0);
-        if (stream_out) store8(stream_out + row * D + c, s[p], D - c);
+        s[p] = h[p].wide();
+        if (residual) {
+            const Eight more = r[p].wide();
+#pragma unroll
+            for (int e = 0; e < PIECE; ++e) s[p].v[e] += more.v[e];
+        }
+        if (stream_out) store8<TAIL>(stream_out + row * D + c, s[p], D - c);
 #pragma unroll
         for (int e = 0; e < PIECE; ++e) sum = fmaf(s[p].v[e], s[p].v[e], sum);
     }
@@ -162,14 +203,14 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const T* __re
     float most = 0.0f;
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int c = (p * NT + t) * PIECE;
+        const int c = (p * threads + t) * PIECE;
         if (c >= D) continue;
 #pragma unroll
         for (int e = 0; e < PIECE; ++e) {
             s[p].v[e] = s[p].v[e] * inv * w[p].v[e];
             if (SCALED) most = larger(most, fabsf(s[p].v[e]));
         }
-        if (!SCALED) store8(static_cast<T*>(normed) + row * D + c, s[p], D - c);
+        if (!SCALED) store8<TAIL>(static_cast<T*>(normed) + row * D + c, s[p], D - c);
     }
     if constexpr (SCALED) {
         most = over_row<Larger, NT>(most, spare[1]);
@@ -178,131 +219,156 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(const T* __re
         if (t == 0) scales[row] = scale;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int c = (p * NT + t) * PIECE;
+            const int c = (p * threads + t) * PIECE;
             if (c >= D) continue;
 #pragma unroll
             for (int e = 0; e < PIECE; ++e) s[p].v[e] *= back;
-            store8_e4m3(static_cast<unsigned char*>(normed) + row * D + c, s[p], D - c);
+            store8_e4m3<TAIL>(static_cast<unsigned char*>(normed) + row * D + c, s[p], D - c);
         }
     }
 }
 
-// A workgroup takes the rows of one slab, NT threads a row, and leaves its share of the weight's gradient in `partials` [slabs, D].
-template <typename T, typename R, int NT, int PIECES>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_pullback_kernel(const T* __restrict__ g_normed, const R* __restrict__ stream,
-                                                                            const R* __restrict__ g_stream, const void* __restrict__ weight,
-                                                                            T* __restrict__ g_hidden, R* __restrict__ g_residual,
-                                                                            float* __restrict__ partials, long long rows, int D, float eps,
-                                                                            int weight_wide, int slab) {
-    constexpr int SIDE = NT < 256 ? 256 / NT : 1;  // rows side by side
-    extern __shared__ __align__(16) float lds[];   // SIDE > 1: [SIDE][D]
-    __shared__ float spare[2][2][NT / 64];
-    const int t = threadIdx.x % NT, side = threadIdx.x / NT;
+// A workgroup takes the rows of one slab, NT threads a row, and leaves its share of the weight's gradient in `partials` [slabs, D].  The next
+// row is on its way while one is worked on; its loads stand in no branch, since the compiler waits for every load under way where branches meet
+// (past the end of a row or of the slab they fetch again what is there).  MORE: there is a g_stream.
+template <typename T, typename R, bool MORE, bool TAIL, int NT, int PIECES>
+__global__ __launch_bounds__(NT * SIDE<NT>) void norm_pullback_kernel(const T* __restrict__ g_normed, const R* __restrict__ stream,
+                                                                      const R* __restrict__ g_stream, const void* __restrict__ weight,
+                                                                      T* __restrict__ g_hidden, R* __restrict__ g_residual,
+                                                                      float* __restrict__ partials, long long rows, int D, float eps,
+                                                                      int weight_wide, int slab) {
+    extern __shared__ __align__(16) float lds[];  // SIDE > 1: [SIDE][D]
+    __shared__ float spare[2][NT <= 64 ? 1 : NT / 64][2];
+    const int threads = NT <= 64 ? NT : (int)blockDim.x, t = threadIdx.x % threads, side = threadIdx.x / threads;
     const long long first = (long long)blockIdx.x * slab, last = first + slab < rows ? first + slab : rows;
+    struct Row {
+        Raw<R> x[PIECES], more[PIECES];
+        Raw<T> g[PIECES];
+    };
+    auto bring = [&](long long row) __attribute__((always_inline)) {
+        Row r;
+        const long long from = (row < last ? row : last - 1) * D;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int at = (p * threads + t) * PIECE, c = at < D ? at : 0;
+            r.x[p] = load8<TAIL>(stream + from + c, D - c);
+            r.g[p] = load8<TAIL>(g_normed + from + c, D - c);
+            if constexpr (MORE) r.more[p] = load8<TAIL>(g_stream + from + c, D - c);
+        }
+        return r;
+    };
+    constexpr bool AHEAD = NT * PIECES <= 1024;  // the widest rows leave no registers for it
+    Row next;
+    if constexpr (AHEAD) next = bring(first + side);
     Eight w[PIECES], total[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int c = (p * NT + t) * PIECE;
-        if (c < D) w[p] = load_weight<T>(weight, c, D - c, weight_wide != 0);
+        const int c = (p * threads + t) * PIECE;
+        if (c < D) w[p] = load_weight<TAIL, T>(weight, c, D - c, weight_wide != 0);
 #pragma unroll
         for (int e = 0; e < PIECE; ++e) total[p].v[e] = 0.0f;
     }
     int turn = 0;
-    for (long long row = first + side; row < last; row += SIDE, turn ^= 1) {
-        Eight x[PIECES], g[PIECES], more[PIECES];
-#pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-            const int c = (p * NT + t) * PIECE;
-            if (c >= D) continue;
-            x[p] = load8(stream + row * D + c, D - c);
-            g[p] = load8(g_normed + row * D + c, D - c);
-            if (g_stream) more[p] = load8(g_stream + row * D + c, D - c);
-        }
+    for (long long row = first + side; row < last; row += SIDE<NT>, turn ^= 1) {
+        const Row now = AHEAD ? next : bring(row);
+        if constexpr (AHEAD) next = bring(row + SIDE<NT>);
         float squares = 0.0f, along = 0.0f;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            if ((p * NT + t) * PIECE >= D) continue;
+            if ((p * threads + t) * PIECE >= D) continue;
+            const Eight x = now.x[p].wide(), g = now.g[p].wide();
 #pragma unroll
             for (int e = 0; e < PIECE; ++e) {
-                squares = fmaf(x[p].v[e], x[p].v[e], squares);
-                along = fmaf(x[p].v[e], g[p].v[e] * w[p].v[e], along);
+                squares = fmaf(x.v[e], x.v[e], squares);
+                along = fmaf(x.v[e], g.v[e] * w[p].v[e], along);
             }
         }
-        squares = over_row<Add, NT>(squares, spare[turn][0]);
-        along = over_row<Add, NT>(along, spare[turn][1]);
+        sums_over_row<NT>(squares, along, spare[turn]);
         const float inv = rsqrtf(squares / (float)D + eps), mean = along * inv / (float)D;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int c = (p * NT + t) * PIECE;
+            const int c = (p * threads + t) * PIECE;
             if (c >= D) continue;
-            Eight out;
+            const Eight x = now.x[p].wide(), g = now.g[p].wide();
+            Eight out, more;
+            if constexpr (MORE) more = now.more[p].wide();
 #pragma unroll
             for (int e = 0; e < PIECE; ++e) {
-                const float unit = x[p].v[e] * inv;
-                total[p].v[e] = fmaf(g[p].v[e], unit, total[p].v[e]);
-                out.v[e] = inv * (g[p].v[e] * w[p].v[e] - unit * mean) + (g_stream ? more[p].v[e] : 0.0f);
+                const float unit = x.v[e] * inv;
+                total[p].v[e] = fmaf(g.v[e], unit, total[p].v[e]);
+                out.v[e] = inv * (g.v[e] * w[p].v[e] - unit * mean);
+                if constexpr (MORE) out.v[e] += more.v[e];
             }
-            if (g_residual) store8(g_residual + row * D + c, out, D - c);
-            if (g_hidden) store8(g_hidden + row * D + c, out, D - c);
+            if (g_residual) store8<TAIL>(g_residual + row * D + c, out, D - c);
+            if (g_hidden) store8<TAIL>(g_hidden + row * D + c, out, D - c);
         }
     }
-    if constexpr (SIDE > 1) {
+    if constexpr (SIDE<NT> > 1) {
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int c = (p * NT + t) * PIECE;
-            if (c < D) store8(lds + side * D + c, total[p], D - c);
+            const int c = (p * threads + t) * PIECE;
+            if (c < D) store8<TAIL>(lds + side * D + c, total[p], D - c);
         }
         __syncthreads();
         for (int c = threadIdx.x; c < D; c += 256) {
             float sum = lds[c];
 #pragma unroll
-            for (int q = 1; q < SIDE; ++q) sum += lds[q * D + c];
+            for (int q = 1; q < SIDE<NT>; ++q) sum += lds[q * D + c];
             partials[(size_t)blockIdx.x * D + c] = sum;
         }
     } else {
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int c = (p * NT + t) * PIECE;
-            if (c < D) store8(partials + (size_t)blockIdx.x * D + c, total[p], D - c);
+            const int c = (p * threads + t) * PIECE;
+            if (c < D) store8<TAIL>(partials + (size_t)blockIdx.x * D + c, total[p], D - c);
         }
     }
 }
 
-// out[c] = sum over slabs of partials[slab][c]: 16 columns a workgroup, 64 threads a column, whose sums are added in order.
-constexpr int FOLD_COLUMNS = 16, FOLD_PARTS = 64;
-__global__ __launch_bounds__(FOLD_COLUMNS * FOLD_PARTS) void fold_kernel(const float* __restrict__ partials, float* __restrict__ out, int slabs,
-                                                                         int D) {
-    __shared__ float part[FOLD_PARTS][FOLD_COLUMNS];
-    const int col = threadIdx.x % FOLD_COLUMNS, q = threadIdx.x / FOLD_COLUMNS, c = blockIdx.x * FOLD_COLUMNS + col;
+// out[c] = sum over slabs of partials[slab][c]: COLUMNS columns a workgroup, PARTS threads a column, whose sums are added in order.
+template <int COLUMNS, int PARTS>
+__global__ __launch_bounds__(COLUMNS * PARTS) void fold_kernel(const float* __restrict__ partials, float* __restrict__ out, int slabs, int D) {
+    __shared__ float part[PARTS][COLUMNS];
+    const int col = threadIdx.x % COLUMNS, q = threadIdx.x / COLUMNS, c = blockIdx.x * COLUMNS + col;
     float sum = 0.0f;
     if (c < D)
 #pragma unroll 8
-        for (int s = q; s < slabs; s += FOLD_PARTS) sum += partials[(size_t)s * D + c];
+        for (int s = q; s < slabs; s += PARTS) sum += partials[(size_t)s * D + c];
     part[q][col] = sum;
     __syncthreads();
-    for (int half = FOLD_PARTS / 2; half >= 1; half /= 2) {
+    for (int half = PARTS / 2; half >= 1; half /= 2) {
         if (q < half) part[q][col] += part[q + half][col];
         __syncthreads();
     }
     if (q == 0 && c < D) out[c] = part[0][col];
 }
 
-constexpr int64_t MOST_COLUMNS = 512 * 4 * PIECE, MOST_ROWS = (int64_t)1 << 31;
-constexpr int SLABS = 512;  // two workgroups a CU
+constexpr int64_t MOST_COLUMNS = 1024 * 2 * PIECE, MOST_ROWS = (int64_t)1 << 31;
 
-// rows of a slab of the pullback, and how many slabs that makes
-int slab_rows(int64_t rows) { return (int)std::max<int64_t>((rows + SLABS - 1) / SLABS, 4); }
-int slab_count(int64_t rows) { return (int)((rows + slab_rows(rows) - 1) / slab_rows(rows)); }
+// Slabs of the pullback, and the rows of one: four workgroups a CU of narrow rows, two of wide ones, whose shares of the weight's gradient
+// would be as many bytes as a twentieth of the rows themselves.
+int slab_rows(int64_t rows, int64_t D) {
+    const int64_t slabs = D <= 1024 ? 1024 : 512;
+    const int64_t least = D <= 512 ? 2048 / D : 1;  // rows that a workgroup holds side by side, about
+    return (int)std::max<int64_t>((rows + slabs - 1) / slabs, least);
+}
+int slab_count(int64_t rows, int64_t D) { return (int)((rows + slab_rows(rows, D) - 1) / slab_rows(rows, D)); }
 
 template <int NT_, int PIECES_> struct Form { static constexpr int NT = NT_, PIECES = PIECES_; };
 // What holds a row of D columns in registers.
-template <typename F> int by_width(int64_t D, F&& launch) {
+// Threads of a row: as few waves as hold it where that is more than one.
+template <int NT, int PIECES> int threads_of(int64_t D) {
+    return NT <= 64 ? NT : (int)((D + 64 * PIECE * PIECES - 1) / (64 * PIECE * PIECES)) * 64;
+}
+template <bool PULLBACK, typename F> int by_width(int64_t D, F&& launch) {
+    if (D <= 64) return launch(Form<8, 1>{});
+    if (D <= 128) return launch(Form<16, 1>{});
+    if (D <= 256) return launch(Form<32, 1>{});
     if (D <= 512) return launch(Form<64, 1>{});
     if (D <= 1024) return launch(Form<64, 2>{});
-    if (D <= 2048) return launch(Form<64, 4>{});
-    if (D <= 4096) return launch(Form<256, 2>{});
-    if (D <= 8192) return launch(Form<256, 4>{});
-    return launch(Form<512, 4>{});
+    // a slab's rows come one after the other: twice the waves (6000 x 5120 in fp16: 74 -> 68 us, and 53 with the next row ahead)
+    if (D <= 8192) return launch(Form<PULLBACK ? 1024 : 512, PULLBACK ? 1 : 2>{});
+    return launch(Form<1024, 2>{});
 }
 
 template <typename T> struct Type { using type = T; };
@@ -343,10 +409,11 @@ extern "C" int lbi_residual_rmsnorm(const void* hidden, const void* residual, co
     return by_types(dtype, residual_dtype, [&](auto t, auto r) {
         using T = typename decltype(t)::type;
         using R = typename decltype(r)::type;
-        return by_width(D, [&](auto form) {
-            constexpr int NT = decltype(form)::NT, PIECES = decltype(form)::PIECES, SIDE = NT < 256 ? 256 / NT : 1;
-            const auto kernel = scales ? norm_kernel<T, R, true, NT, PIECES> : norm_kernel<T, R, false, NT, PIECES>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + SIDE - 1) / SIDE)), dim3(NT * SIDE), 0, static_cast<hipStream_t>(stream),
+        return by_width<false>(D, [&](auto form) {
+            constexpr int NT = decltype(form)::NT, PIECES = decltype(form)::PIECES, COUNT = SIDE<NT>;
+            const auto kernel = D % PIECE ? (scales ? norm_kernel<T, R, true, true, NT, PIECES> : norm_kernel<T, R, false, true, NT, PIECES>)
+                                          : (scales ? norm_kernel<T, R, true, false, NT, PIECES> : norm_kernel<T, R, false, false, NT, PIECES>);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + COUNT - 1) / COUNT)), dim3((unsigned)(threads_of<NT, PIECES>(D) * COUNT)), 0, static_cast<hipStream_t>(stream),
                                static_cast<const T*>(hidden), static_cast<const R*>(residual), weight, normed, static_cast<R*>(residual_out),
                                scales, (long long)rows, (int)D, eps, (int)(weight_dtype == LBI_F32));
             LBI_HIP_CHECK(hipGetLastError());
@@ -358,7 +425,7 @@ extern "C" int lbi_residual_rmsnorm(const void* hidden, const void* residual, co
 extern "C" size_t lbi_residual_rmsnorm_pullback_workspace_bytes(int64_t rows, int64_t D) {
     using namespace lbi::block_norm;
     if (rows < 0 || D < 1 || D > MOST_COLUMNS || rows >= MOST_ROWS) return 0;
-    return (size_t)slab_count(rows) * (size_t)D * sizeof(float);
+    return (size_t)slab_count(rows, D) * (size_t)D * sizeof(float);
 }
 
 extern "C" int lbi_residual_rmsnorm_pullback(const void* g_normed, const void* residual_out, const void* g_residual_out, const void* weight,
@@ -371,7 +438,7 @@ extern "C" int lbi_residual_rmsnorm_pullback(const void* g_normed, const void* r
     if (int bad = check("lbi_residual_rmsnorm_pullback", rows, D, dtype, residual_dtype, weight_dtype)) return bad;
     if (!g_weight || (rows && (!g_normed || !residual_out || !weight || (!g_hidden && !g_residual))))
         return fail(LBI_ERR_INVALID, "lbi_residual_rmsnorm_pullback: null pointer");
-    const int slabs = slab_count(rows);
+    const int slabs = slab_count(rows, D);
     const size_t need = lbi_residual_rmsnorm_pullback_workspace_bytes(rows, D);
     if (need && (!workspace || workspace_bytes < need))
         return fail(LBI_ERR_WORKSPACE, "lbi_residual_rmsnorm_pullback: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
@@ -384,21 +451,27 @@ extern "C" int lbi_residual_rmsnorm_pullback(const void* g_normed, const void* r
         const int status = by_types(dtype, residual_dtype, [&](auto t, auto r) {
             using T = typename decltype(t)::type;
             using R = typename decltype(r)::type;
-            return by_width(D, [&](auto form) {
-                constexpr int NT = decltype(form)::NT, PIECES = decltype(form)::PIECES, SIDE = NT < 256 ? 256 / NT : 1;
-                const size_t bytes = SIDE > 1 ? SIDE * (size_t)D * sizeof(float) : 0;  // 32 KiB at most
-                hipLaunchKernelGGL((norm_pullback_kernel<T, R, NT, PIECES>), dim3((unsigned)slabs), dim3(NT * SIDE), bytes,
+            return by_width<true>(D, [&](auto form) {
+                constexpr int NT = decltype(form)::NT, PIECES = decltype(form)::PIECES, COUNT = SIDE<NT>;
+                const size_t bytes = COUNT > 1 ? COUNT * (size_t)D * sizeof(float) : 0;  // 16 KiB at most
+                const auto kernel = D % PIECE ? (g_residual_out ? norm_pullback_kernel<T, R, true, true, NT, PIECES>
+                                                                : norm_pullback_kernel<T, R, false, true, NT, PIECES>)
+                                              : (g_residual_out ? norm_pullback_kernel<T, R, true, false, NT, PIECES>
+                                                                : norm_pullback_kernel<T, R, false, false, NT, PIECES>);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)slabs), dim3((unsigned)(threads_of<NT, PIECES>(D) * COUNT)), bytes,
                                    static_cast<hipStream_t>(stream), static_cast<const T*>(g_normed), static_cast<const R*>(residual_out),
                                    static_cast<const R*>(g_residual_out), weight, static_cast<T*>(g_hidden), static_cast<R*>(g_residual),
-                                   partials, (long long)rows, (int)D, eps, (int)(weight_dtype == LBI_F32), slab_rows(rows));
+                                   partials, (long long)rows, (int)D, eps, (int)(weight_dtype == LBI_F32), slab_rows(rows, D));
                 LBI_HIP_CHECK(hipGetLastError());
                 return (int)LBI_OK;
             });
         });
         if (status) return status;
     }
-    hipLaunchKernelGGL(fold_kernel, dim3((unsigned)((D + FOLD_COLUMNS - 1) / FOLD_COLUMNS)), dim3(FOLD_COLUMNS * FOLD_PARTS), 0,
-                       static_cast<hipStream_t>(stream), partials, g_weight, slabs, (int)D);
+    const bool wide = D >= 4096;  // enough columns to fill the chip in whole lines
+    const auto fold = wide ? fold_kernel<32, 32> : fold_kernel<16, 64>;
+    hipLaunchKernelGGL(fold, dim3((unsigned)((D + (wide ? 31 : 15)) / (wide ? 32 : 16))), dim3(1024), 0, static_cast<hipStream_t>(stream),
+                       partials, g_weight, slabs, (int)D);
     LBI_HIP_CHECK(hipGetLastError());
     return LBI_OK;
 }

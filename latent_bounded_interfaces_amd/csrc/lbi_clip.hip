@@ -1,10 +1,13 @@
 // Clipping of a list of gradients by their global 2-norm:  n = sqrt(sum of all squares),  out = g * min(1, max_norm / (n + 1e-6)).
 //
-// Two kernels: one leaves the sums of squares of its workgroups in the workspace, the other adds them (every workgroup for itself: some
+// Two kernels: one leaves the sums of squares of its workgroups in the workspace, the other adds them (every workgroup for itself: a
 // thousand numbers out of the cache cost less than a launch) and scales.  Both walk the same chunks of up to CHUNK elements of one tensor,
 // the table of tensors coming as a kernel argument, TABLE tensors a launch, so nothing is copied to the device and the call can be captured.
 // Squares are formed and added in 64 bits: no gradient of fp32 overflows or vanishes in them, and the norm does not depend on how the chunks
-// fall.  Chunks go to workgroups in a fixed order and sums are added in a fixed order: reruns are bit-identical.
+// fall (fp32 sums of eight would be no faster).  Chunks go to workgroups in a fixed order and sums are added in a fixed order: reruns are bit-identical.
+//
+// Bound by memory: 162 M elements of bf16 are read twice, which the caches cannot hold, and written once, 980 MB in 200 us, the rate of a
+// large copy.  A call of a few small tensors is two launches, 4 + 5 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -21,34 +24,37 @@ namespace {
 using attn_mfma::Mma;
 
 constexpr int THREADS = 256, PIECE = 8, UNROLL = 4, CHUNK = THREADS * PIECE * UNROLL;
-constexpr int TABLE = 100, MOST_GROUPS = 1024;
+constexpr int TABLE = 140, MOST_GROUPS = 1024;
 
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-struct Tensor {
-    const void* in;
-    void* out;
-    long long count;
-    unsigned first;  // chunk of the launch with which it begins
-    int dtype;
-};
 struct Table {
-    Tensor tensor[TABLE];
+    const void* in[TABLE];
+    void* out[TABLE];
+    long long count_type[TABLE];  // elements * 4 + type
+    unsigned first[TABLE];        // chunk with which the tensor begins
     int tensors;
     unsigned chunks;
 };
 static_assert(sizeof(Table) <= 4000, "kernel arguments");
 
+struct Piece {  // a chunk's part of a tensor
+    const void* in;
+    void* out;
+    long long at;
+    int count, dtype;
+};
 // the tensor that a chunk lies in: the last one that begins no later
-__device__ __forceinline__ int tensor_of(const Table& table, unsigned chunk) {
+__device__ __forceinline__ Piece piece_of(const Table& table, unsigned chunk) {
     int low = 0, high = table.tensors - 1;
     while (low < high) {
         const int mid = (low + high + 1) / 2;
-        if (table.tensor[mid].first <= chunk) low = mid;
+        if (table.first[mid] <= chunk) low = mid;
         else high = mid - 1;
     }
-    return low;
+    const long long at = (long long)(chunk - table.first[low]) * CHUNK, left = (table.count_type[low] >> 2) - at;
+    return Piece{table.in[low], table.out[low], at, (int)(left < CHUNK ? left : CHUNK), (int)(table.count_type[low] & 3)};
 }
 
 struct Eight { float v[PIECE]; };
@@ -140,12 +146,10 @@ __global__ __launch_bounds__(THREADS) void squares_kernel(Table table, double* _
     __shared__ double spare[THREADS / 64];
     double sum = 0.0;
     for (unsigned chunk = blockIdx.x; chunk < table.chunks; chunk += gridDim.x) {
-        const Tensor& t = table.tensor[tensor_of(table, chunk)];
-        const long long at = (long long)(chunk - t.first) * CHUNK;
-        const int count = (int)(t.count - at < CHUNK ? t.count - at : CHUNK);
-        if (t.dtype == LBI_F32) sum += squares_of(static_cast<const float*>(t.in) + at, count);
-        else if (t.dtype == LBI_F16) sum += squares_of(static_cast<const _Float16*>(t.in) + at, count);
-        else sum += squares_of(static_cast<const bf16_raw*>(t.in) + at, count);
+        const Piece p = piece_of(table, chunk);
+        if (p.dtype == LBI_F32) sum += squares_of(static_cast<const float*>(p.in) + p.at, p.count);
+        else if (p.dtype == LBI_F16) sum += squares_of(static_cast<const _Float16*>(p.in) + p.at, p.count);
+        else sum += squares_of(static_cast<const bf16_raw*>(p.in) + p.at, p.count);
     }
     sum = over_group(sum, spare);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
@@ -160,17 +164,15 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(Table table, const doubl
     const float factor = (float)(ratio > 1.0 ? 1.0 : ratio);  // not a number stays one
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     for (unsigned chunk = blockIdx.x; chunk < table.chunks; chunk += gridDim.x) {
-        const Tensor& t = table.tensor[tensor_of(table, chunk)];
-        if (!t.out || (t.in == t.out && factor == 1.0f)) continue;
-        const long long at = (long long)(chunk - t.first) * CHUNK;
-        const int count = (int)(t.count - at < CHUNK ? t.count - at : CHUNK);
-        if (t.dtype == LBI_F32) scale(static_cast<const float*>(t.in) + at, static_cast<float*>(t.out) + at, count, factor);
-        else if (t.dtype == LBI_F16) scale(static_cast<const _Float16*>(t.in) + at, static_cast<_Float16*>(t.out) + at, count, factor);
-        else scale(static_cast<const bf16_raw*>(t.in) + at, static_cast<bf16_raw*>(t.out) + at, count, factor);
+        const Piece p = piece_of(table, chunk);
+        if (!p.out || (p.in == p.out && factor == 1.0f)) continue;
+        if (p.dtype == LBI_F32) scale(static_cast<const float*>(p.in) + p.at, static_cast<float*>(p.out) + p.at, p.count, factor);
+        else if (p.dtype == LBI_F16) scale(static_cast<const _Float16*>(p.in) + p.at, static_cast<_Float16*>(p.out) + p.at, p.count, factor);
+        else scale(static_cast<const bf16_raw*>(p.in) + p.at, static_cast<bf16_raw*>(p.out) + p.at, p.count, factor);
     }
 }
 
-// Tensors from list[first] on that one launch takes: TABLE tensors with elements, fewer than 2^31 chunks.
+// The next TABLE tensors of the list that have elements.
 Table table_of(const lbi_gradient* list, int64_t n, int64_t& first) {
     Table table;
     table.tensors = 0;
@@ -178,21 +180,26 @@ Table table_of(const lbi_gradient* list, int64_t n, int64_t& first) {
     for (; first < n && table.tensors < TABLE; ++first) {
         const lbi_gradient& g = list[first];
         if (g.count == 0) continue;
-        const int64_t chunks = (g.count + CHUNK - 1) / CHUNK;
-        if (table.tensors && table.chunks + chunks >= (int64_t)1 << 31) break;
-        table.tensor[table.tensors++] = Tensor{g.in, g.out, (long long)g.count, table.chunks, (int)g.dtype};
-        table.chunks += (unsigned)chunks;
+        table.in[table.tensors] = g.in;
+        table.out[table.tensors] = g.out;
+        table.count_type[table.tensors] = (long long)g.count * 4 + g.dtype;
+        table.first[table.tensors++] = table.chunks;
+        table.chunks += (unsigned)((g.count + CHUNK - 1) / CHUNK);
     }
     return table;
 }
 int groups_of(const Table& table) { return (int)std::min<unsigned>(table.chunks, MOST_GROUPS); }
 
+constexpr int64_t MOST_ELEMENTS = (int64_t)1 << 40;  // of a list: more than any memory holds, and 32 bits count its chunks
+
 int check(const char* who, const lbi_gradient* list, int64_t n) {
     if (n < 0 || (n && !list)) return fail(LBI_ERR_INVALID, "%s: bad list", who);
+    int64_t all = 0;
     for (int64_t i = 0; i < n; ++i) {
         const lbi_gradient& g = list[i];
         if (g.dtype < LBI_F32 || g.dtype > LBI_BF16) return fail(LBI_ERR_INVALID, "%s: bad dtype %lld", who, (long long)g.dtype);
-        if (g.count < 0 || g.count >= (int64_t)1 << 43) return fail(LBI_ERR_INVALID, "%s: bad size %lld", who, (long long)g.count);
+        if (g.count < 0 || g.count > MOST_ELEMENTS || (all += g.count) > MOST_ELEMENTS)
+            return fail(LBI_ERR_INVALID, "%s: bad size %lld", who, (long long)g.count);
         if (g.count && !g.in) return fail(LBI_ERR_INVALID, "%s: null pointer", who);
         const uintptr_t grid = dtype_size((int)g.dtype);
         if (reinterpret_cast<uintptr_t>(g.in) % grid || reinterpret_cast<uintptr_t>(g.out) % grid)
@@ -233,12 +240,9 @@ bool apart(const lbi_gradient* list, int64_t n) {
 }  // namespace clip
 }  // namespace lbi
 
-extern "C" size_t lbi_clip_gradients_workspace_bytes(const lbi_gradient* gradients, int64_t n) {
+extern "C" size_t lbi_clip_gradients_workspace_bytes(int64_t n) {
     using namespace lbi::clip;
-    if (check("lbi_clip_gradients", gradients, n)) return 0;
-    size_t sums = 0;
-    for (int64_t first = 0; first < n;) sums += (size_t)groups_of(table_of(gradients, n, first));
-    return std::max<size_t>(sums, 1) * sizeof(double);
+    return (size_t)(std::max<int64_t>(n, 0) / TABLE + 1) * MOST_GROUPS * sizeof(double);
 }
 
 extern "C" int lbi_clip_gradients(const lbi_gradient* gradients, int64_t n, float max_norm, float* norm, void* workspace,
@@ -251,7 +255,7 @@ extern "C" int lbi_clip_gradients(const lbi_gradient* gradients, int64_t n, floa
     if (!norm) return fail(LBI_ERR_INVALID, "lbi_clip_gradients: null pointer");
     if (reinterpret_cast<uintptr_t>(norm) % 4 || reinterpret_cast<uintptr_t>(workspace) % 8)
         return fail(LBI_ERR_INVALID, "lbi_clip_gradients: norm or workspace is not aligned");
-    const size_t need = lbi_clip_gradients_workspace_bytes(gradients, n);
+    const size_t need = lbi_clip_gradients_workspace_bytes(n);
     if (!workspace || workspace_bytes < need)
         return fail(LBI_ERR_WORKSPACE, "lbi_clip_gradients: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     try {

@@ -7,7 +7,7 @@ norm stays on the device.
 """
 from __future__ import annotations
 
-import ctypes
+import array
 import math
 from typing import Sequence
 
@@ -24,50 +24,65 @@ def _flat(t: torch.Tensor) -> bool:
     return t.permute(order).is_contiguous()
 
 
-def _check(tensors: Sequence[torch.Tensor], what: str, device: torch.device | None = None) -> torch.device:
-    """The one device of ``tensors``."""
+def _refuse(tensors: Sequence[torch.Tensor], what: str, index: int) -> None:
+    """Raises for the first of ``tensors`` that the kernels do not take on the device ``index``."""
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what} must be torch.Tensors")
-        if t.layout is not torch.strided:
+        if t.layout != torch.strided:
             raise TypeError(f"{what} must be dense tensors")
-        if t.dtype not in _lib._DTYPE_CODES:
-            _lib.dtype_code(t.dtype)
-        if device is None or t.device != device:
-            if not t.is_cuda:
-                raise RuntimeError(f"{what} must be CUDA tensors (this build has no CPU execution path)")
-            if device is not None:
-                raise ValueError(f"{what} must be on one device")
-            device = t.device
-    return device
+        _lib.dtype_code(t.dtype)
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} must be CUDA tensors (this build has no CPU execution path)")
+        if t.get_device() != index:
+            raise ValueError(f"{what} must be on one device")
 
 
-def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor | None], max_norm: float) -> torch.Tensor:
-    device = grads[0].device
-    codes = _lib._DTYPE_CODES
+def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None, max_norm: float) -> torch.Tensor:
+    """``outs``: where the results go (``grads`` itself: in place; ``None``: nowhere, the norm alone)."""
+    if not isinstance(grads[0], torch.Tensor) or not grads[0].is_cuda:
+        _refuse(grads[:1], "grads", 0)
+    index, codes, changing = grads[0].get_device(), _lib._DTYPE_CODES, torch.is_grad_enabled()
     words, held, late = [], [], []
-    for g, out in zip(grads, outs):
+    for i, g in enumerate(grads):
+        out = None if outs is None else outs[i]
+        try:  # most calls: a tensor costs less than a microsecond
+            dtype = g.dtype
+            if out is not None and out is not g:
+                if g.shape != out.shape or out.dtype is not dtype:
+                    raise ValueError("out must have the shapes and types of the gradients")
+                plain = g.is_contiguous() and out.is_contiguous() and out.get_device() == index
+            else:
+                plain = g.is_contiguous()
+            if plain and g.get_device() == index and not (changing and out is not None and out.requires_grad):
+                words += (g.data_ptr(), 0 if out is None else out.data_ptr(), g.numel(), codes[dtype])
+                continue
+        except (AttributeError, KeyError, RuntimeError):
+            pass  # said below
+        _refuse([g], "grads", index)
         to = out
-        if not (g.is_contiguous() and (out is None or out is g or out.is_contiguous())) and not (
-                _flat(g) and (out is None or out is g or out.stride() == g.stride())):
+        if out is not None:
+            _refuse([out], "out", index)
+            if out.requires_grad and changing:
+                raise RuntimeError("clip_gradients writes tensors that require grad: call it under torch.no_grad()")
+        if not _flat(g) or not (out is None or out is g or out.stride() == g.stride()):
             g = g.contiguous()
-            if out is not None and (out is g or not out.is_contiguous()):
+            if out is not None and (out is grads[i] or not out.is_contiguous()):
                 to = torch.empty_like(g)
                 late.append((out, to))
             # a contiguous `out` of its own is written by the kernel
             held.append((g, to))  # copies live until the kernels are queued
         words += (g.data_ptr(), 0 if to is None else to.data_ptr(), g.numel(), codes[g.dtype])
-    count = len(words) // 4
     if late and len({(o.data_ptr(), o.shape, o.stride()) for o, _ in late}) != len(late):
         raise ValueError("a result overlaps another tensor")
-    table = (ctypes.c_int64 * len(words))(*words)
+    count, device = len(grads), grads[0].device
+    table = array.array("q", words)  # lbi_gradient of include/lbi_hip.h: four words of 64 bits
     norm = torch.empty((), device=device, dtype=torch.float32)
     lib = _lib.load()
     with _lib.device_guard(device):
-        need = int(lib.lbi_clip_gradients_workspace_bytes(table, count))
-        workspace = torch.empty(max(need, 8), device=device, dtype=torch.uint8)
-        status = lib.lbi_clip_gradients(table, count, max_norm, norm.data_ptr(), workspace.data_ptr(), need,
-                                        _lib.current_stream_ptr(device))
+        need = lib.lbi_clip_gradients_workspace_bytes(count)
+        workspace = torch.empty(need, device=device, dtype=torch.uint8)
+        status = lib.lbi_clip_gradients(table.buffer_info()[0], count, max_norm, norm.data_ptr(), workspace.data_ptr(), need, _lib.current_stream_ptr(device))
     _lib.check(status, "lbi_clip_gradients")
     for out, to in late:
         out.copy_(to)
@@ -80,8 +95,7 @@ def gradient_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     grads = list(grads)
     if not grads:
         return torch.zeros(())
-    _check(grads, "grads")
-    return _clip(grads, [None] * len(grads), math.inf)
+    return _clip(grads, None, math.inf)
 
 
 def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, *, out: Sequence[torch.Tensor] | None = None) -> torch.Tensor:
@@ -102,17 +116,7 @@ def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, *, out: Seque
             raise ValueError("out must hold one tensor for each gradient")
     if not grads:
         return torch.zeros(())
-    device = _check(grads, "grads")
-    if out is None:
-        out = grads
-    else:
-        _check(out, "out", device)
-        for g, o in zip(grads, out):
-            if g.shape != o.shape or g.dtype != o.dtype:
-                raise ValueError("out must have the shapes and types of the gradients")
-    if any(o.requires_grad for o in out) and torch.is_grad_enabled():
-        raise RuntimeError("clip_gradients writes tensors that require grad: call it under torch.no_grad()")
-    return _clip(grads, out, max_norm)
+    return _clip(grads, grads if out is None else out, max_norm)
 
 
 __all__ = ["clip_gradients", "gradient_norm"]
