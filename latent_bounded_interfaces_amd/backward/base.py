@@ -3,7 +3,8 @@
 Same names, fields and behaviour as reference backward/base.py:10-90 so that code written
 against the reference's ``backward`` package finds them here: ``ADResult``,
 ``LBIBackwardResult``, the structural model protocol ``ScanBackpropModel`` and the three
-helpers that move gradients between ``param.grad`` and a ``{name: grad}`` map.
+helpers that move gradients between ``param.grad`` and a ``{name: grad}`` map; and two that clip them by their global
+norm on the way.
 """
 from __future__ import annotations
 
@@ -12,6 +13,8 @@ from typing import Any, Protocol, runtime_checkable
 
 import torch
 from torch import nn
+
+from ..hip.gradients import clip_gradients
 
 GradMap = dict  # {parameter name: gradient tensor or None}
 
@@ -77,6 +80,25 @@ def assign_grad_map(model: nn.Module, grad_map: GradMap) -> None:
         p.grad = None if grad is None else grad.detach().clone()
 
 
+def clip_grad_map(grad_map: GradMap, max_norm: float) -> torch.Tensor:
+    """Clips the gradients of a map in place by their global norm, which is returned (a scalar tensor on their device; the
+    reference's loop calls ``clip_grad_norm_`` on the parameters, train/runners.py:378-380).  ``None`` entries count as zero."""
+    return clip_gradients([grad for grad in grad_map.values() if grad is not None], max_norm)
+
+
+def assign_clipped_grad_map(model: nn.Module, grad_map: GradMap, max_norm: float) -> torch.Tensor:
+    """:func:`assign_grad_map` of the clipped gradients: scaled on their way into ``param.grad``, the map is left as it is.
+    Returns the norm, over the trainable parameters' gradients and before clipping."""
+    grads, copies = [], []
+    for name, p in _trainable(model):
+        grad = grad_map.get(name)
+        p.grad = None if grad is None else torch.empty_like(grad, requires_grad=False)
+        if grad is not None:
+            grads.append(grad.detach())
+            copies.append(p.grad)
+    return clip_gradients(grads, max_norm, out=copies)
+
+
 def store_named_grads(grad_map: GradMap, param_name_map: dict[int, str], params, grads) -> None:
     """Files ``grads`` (as ``torch.autograd.grad`` returns them for ``params``) under the parameters' names."""
     for p, grad in zip(params, grads):
@@ -89,7 +111,9 @@ __all__ = [
     "GradMap",
     "LBIBackwardResult",
     "ScanBackpropModel",
+    "assign_clipped_grad_map",
     "assign_grad_map",
+    "clip_grad_map",
     "collect_named_grads",
     "store_named_grads",
 ]

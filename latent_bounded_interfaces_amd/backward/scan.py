@@ -26,7 +26,7 @@ import torch
 from torch import nn
 
 from ..hip.interface import suffix_apply, suffix_scan_cotangents, suffix_scan_pullbacks
-from .base import ADResult, LBIBackwardResult, ScanBackpropModel, assign_grad_map
+from .base import ADResult, LBIBackwardResult, ScanBackpropModel, assign_clipped_grad_map, assign_grad_map
 from .local_vjp import TorchAutogradLocalVJPProvider, build_local_vjp_provider
 from .pullbacks import STRUCTURED_MODE_NAMES, build_interface_pullback_provider
 from .suffix_scan import (
@@ -128,6 +128,7 @@ class ScanADEngine:
         compute_interface_jacobian_stats: bool = False,
         include_interface_jacobian_suffix: bool = False,
         local_vjp_mode: str = "autograd",
+        max_grad_norm: float | None = None,
     ) -> None:
         # ``state_jacobian_basis_chunk=None``: the provider's own default, which is the reference's 1 for its
         # autograd modes and "all d directions in one call" for the structured provider
@@ -138,9 +139,13 @@ class ScanADEngine:
         self.local_vjp_provider = local_vjp_provider or build_local_vjp_provider(local_vjp_mode)
         self.compute_interface_jacobian_stats = bool(compute_interface_jacobian_stats)
         self.include_interface_jacobian_suffix = bool(include_interface_jacobian_suffix)
+        # ``param.grad`` gets the gradients clipped to this global norm (the returned map is not clipped), and the diagnostics
+        # ``grad_norm``, a scalar tensor on the device; ``None``: the caller clips, as in the reference
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
 
     @classmethod
-    def from_config(cls, cfg: Any, *, compute_interface_jacobian_stats: bool = False) -> "ScanADEngine":
+    def from_config(cls, cfg: Any, *, compute_interface_jacobian_stats: bool = False,
+                    max_grad_norm: float | None = None) -> "ScanADEngine":
         """Reads ``interface_jacobian_mode``, ``jacobian_basis_chunk`` and ``log_interface_jacobian_suffix``
         of the reference's training configuration (train/config.py:164-171).
 
@@ -160,6 +165,7 @@ class ScanADEngine:
             local_vjp_provider=build_local_vjp_provider(str(getattr(cfg, "local_vjp_mode", "autograd"))),
             compute_interface_jacobian_stats=compute_interface_jacobian_stats,
             include_interface_jacobian_suffix=bool(cfg.log_interface_jacobian_suffix),
+            max_grad_norm=max_grad_norm,
         )
 
     def backward(self, *, model: nn.Module, loss: torch.Tensor, cache: Any | None = None) -> ADResult:
@@ -177,7 +183,11 @@ class ScanADEngine:
             compute_interface_jacobian_stats=self.compute_interface_jacobian_stats,
             include_interface_jacobian_suffix=self.include_interface_jacobian_suffix,
         )
-        assign_grad_map(model, result.grad_map)
+        grad_norm = None
+        if self.max_grad_norm is None:
+            assign_grad_map(model, result.grad_map)
+        else:
+            grad_norm = assign_clipped_grad_map(model, result.grad_map, self.max_grad_norm)
         diagnostics: dict[str, Any] = {
             "interface_scan_rms": result.interface_scan_rms,
             "interface_pullback_provider": self.pullback_provider.name,
@@ -185,6 +195,8 @@ class ScanADEngine:
         }
         if result.interface_jacobian_stats is not None:
             diagnostics["interface_jacobian_stats"] = dict(result.interface_jacobian_stats)
+        if grad_norm is not None:
+            diagnostics["grad_norm"] = grad_norm
         return ADResult(grad_map=result.grad_map, diagnostics=diagnostics)
 
 

@@ -167,3 +167,33 @@ def test_captured(device):
         want = [clip_gradients(grads, 1.0, out=eager), *eager]
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+def test_the_engine_clips_what_it_assigns(device):
+    """``ScanADEngine(max_grad_norm=)`` leaves the clipped gradients on the parameters, the whole ones in the map."""
+    from latent_bounded_interfaces_amd.backends import HipTransformerLowering
+    from latent_bounded_interfaces_amd.backward import ScanADEngine, clip_grad_map
+    from oracle import lbi_model as olbi
+
+    model = olbi.OracleLBIModel(vocab_size=61, dim=32, n_heads=4, n_kv_heads=2, layers=4, layers_per_region=2, interface_width=8, hidden=48,
+                                d_conv=4, interface_hidden=12, seed=31, lowering=HipTransformerLowering()).to(device)
+    ids = torch.randint(0, 61, (2, 10), generator=torch.Generator().manual_seed(3)).to(device)
+    whole = None
+    for max_norm in (None, 0.01):
+        logits, cache = model.forward_with_cache(ids)
+        result = ScanADEngine(max_grad_norm=max_norm).backward(model=model, loss=olbi.token_loss(logits, ids), cache=cache)
+        grads = {n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None}
+        if max_norm is None:
+            assert "grad_norm" not in result.diagnostics
+            whole = grads
+    assert set(grads) == set(whole)
+    names = list(whole)
+    want_norm, want = truth.clip([whole[n].cpu() for n in names], 0.01)
+    assert float(want_norm[0]) > 0.01
+    truth.assert_near(result.diagnostics["grad_norm"], want_norm)
+    for n, one in zip(names, want):
+        truth.assert_near(grads[n], one, n)
+        assert torch.equal(result.grad_map[n], whole[n])
+    clip_grad_map(result.grad_map, 0.01)
+    for n in names:
+        assert torch.equal(result.grad_map[n], grads[n])
