@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 #include "lbi_attn_mfma.h"
 #include "lbi_attn_dkdv128.h"
@@ -31,7 +33,7 @@ constexpr int STEP = 64, NT = 256;
 // a step: the fragments of a whole step are read while the last one's are multiplied (77 x 2048 x 5632 in tiles of 64 x 128, 88 steps: 36 us
 // with two steps in the ring, 27 with three, no less with four or six; reading by quarters 41 whatever the ring.  128 x 128: no difference).
 template <int FM, int FN> constexpr int RING = FM == 1 ? 3 : 2;
-constexpr unsigned PAST_END = 1u << 31;
+constexpr unsigned PAST_END = 1u << 31;  // no operand's step reaches this far
 constexpr int PIECE = 1024;  // bytes that a wave's load brings: 8 rows of 64 terms, or 8 terms of 64 columns
 
 // What becomes of the sums.
@@ -114,10 +116,34 @@ __device__ __forceinline__ void finish(const Task& task, long long row, long lon
     }
 }
 
-// 1 KiB from memory to LDS by one wave: lane l brings the 16 bytes at `base` + `off`, zeros from `bytes` on.
-__device__ __forceinline__ void bring(const char* base, unsigned off, unsigned bytes, unsigned lds) {
-    attn_mfma::dma_tile<true>(base, off, bytes, lds);
+template <typename F, int... I> __device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) { (f(Count<I>{}), ...); }
+// f(Count<0>{}), ... f(Count<N - 1>{})
+template <int N, typename F> __device__ __forceinline__ void each(F&& f) { each(f, std::make_integer_sequence<int, N>{}); }
+
+// 1 KiB from memory to LDS by one wave: lane l brings the 16 bytes at `off` of what `words` describe, zeros past its end.
+template <int AT> __device__ __forceinline__ void bring(const u32x4& words, unsigned off, unsigned lds) {
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+                 :
+                 : "s"(lds), "i"(AT), "v"(off), "s"(words)
+                 : "memory", "scc");
 }
+
+// Where an operand's steps lie: the bytes from its tile's part of a step to the end of the tile (terms side by side) or of the operand (by rows).
+struct Source {
+    const char* at;
+    long long left, step;
+    __device__ __forceinline__ void skip(int steps) {
+        at += steps * step;
+        left -= steps * step;
+    }
+    // words 0 and 1 the address, 2 the bytes that may be read, 3 the format (32 bits); then on to the next step
+    __device__ __forceinline__ u32x4 next(bool there) {
+        constexpr long long most = PAST_END - 16;
+        const u32x4 words = {(unsigned)(size_t)at, (unsigned)((size_t)at >> 32) & 0xffffu, there ? (unsigned)(left < most ? left : most) : 0u, 4u << 15};
+        skip(1);
+        return words;
+    }
+};
 
 // Ids equal mod 8 share an L2: they get neighbouring places.
 __device__ __forceinline__ int place(int id, int count) {
@@ -139,7 +165,7 @@ template <int FM, int FN> __device__ __forceinline__ size_t partial_at(int item,
 template <typename T, int FM, int FN, bool A_ROWS, bool B_ROWS, Finish FINISH>  // ..._ROWS: the terms are the operand's rows
 __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     constexpr int BM = 64 * FM, BN = 64 * FN;  // rows and columns of B's tile
-    constexpr int DEEP = RING<FM, FN>, A_BYTES = BM * 128, SLOT = A_BYTES + BN * 128, READS = FM + FN, LOADS = 2 * READS, BESIDE = (READS + FM * FN - 1) / (FM * FN);
+    constexpr int DEEP = RING<FM, FN>, A_BYTES = BM * 128, SLOT = A_BYTES + BN * 128, READS = FM + FN, LOADS = 2 * READS;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 31, h = lane >> 5, wm = wave >> 1, wn = wave & 1;
@@ -160,86 +186,94 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     tile_at(at, task.m_tiles, task.n_tiles, mt, nt);
     const long long row0 = (long long)mt * BM, col0 = (long long)nt * WIDE;
     const unsigned row_bytes = (unsigned)K * 2;
-    // sources: A's rows, B's rows (GATED: up's and gate's) or B's terms
     const int a_rows = (int)(M - row0 < BM ? M - row0 : BM), b_cols = (int)(N - col0 < WIDE ? N - col0 : WIDE);
-    const char* a_src = static_cast<const char*>(task.a) + (A_ROWS ? row0 : row0 * K) * 2;
-    const char* b_src = static_cast<const char*>(task.b) + (B_ROWS ? col0 : col0 * K) * 2;
-    unsigned a_off[2 * FM], b_off[2 * FN];
-    const char* b_from[2 * FN];
+    Source a_src = A_ROWS ? Source{static_cast<const char*>(task.a) + row0 * 2, (K * M - row0) * 2, STEP * M * 2}
+                          : Source{static_cast<const char*>(task.a) + row0 * K * 2, (long long)a_rows * row_bytes, STEP * 2};
+    Source b_src = B_ROWS ? Source{static_cast<const char*>(task.b) + col0 * 2, (K * N - col0) * 2, STEP * N * 2}
+                          : Source{static_cast<const char*>(task.b) + col0 * K * 2, (long long)b_cols * row_bytes, STEP * 2};
+    a_src.skip(first);
+    b_src.skip(first);
+    // Each wave brings every fourth piece.  GATED: B's tile is up's rows, then gate's, the same pieces further on.
+    unsigned a_off[2 * FM], b_off[FINISH == GATED ? FN : 2 * FN];
+    constexpr int B_OFFS = FINISH == GATED ? FN : 2 * FN;
     const int chunk = (lane & 7) ^ swz<64>(8 * wave + lane / 8);  // the same for each of the wave's pieces: they are 32 rows apart
 #pragma unroll
     for (int u = 0; u < 2 * FM; ++u) {
-        const int q = wave + 4 * u, row = 8 * q + lane / 8;
-        if constexpr (A_ROWS) {
-            const int term = 8 * (q % 8) + lane / 8, col = 64 * (q / 8) + 8 * chunk;
-            a_off[u] = col < a_rows ? (unsigned)(term * M + col) * 2 : PAST_END;
-        } else {
-            a_off[u] = row < a_rows ? (unsigned)row * row_bytes + chunk * 16 : PAST_END;
-        }
+        const int q = wave + 4 * u, col = 64 * (q / 8) + 8 * chunk;
+        if constexpr (A_ROWS) a_off[u] = col < a_rows ? (unsigned)((8 * (q % 8) + lane / 8) * M + col) * 2 : PAST_END;
+        else a_off[u] = (unsigned)(8 * q + lane / 8) * row_bytes + chunk * 16;
     }
 #pragma unroll
-    for (int u = 0; u < 2 * FN; ++u) {
-        const int q = wave + 4 * u;
-        b_from[u] = b_src;
-        if constexpr (B_ROWS) {
-            const int term = 8 * (q % 8) + lane / 8, col = 64 * (q / 8) + 8 * chunk;
-            b_off[u] = col < b_cols ? (unsigned)(term * N + col) * 2 : PAST_END;
-        } else {
-            int row = 8 * q + lane / 8;
-            if (FINISH == GATED && 8 * q >= WIDE) {  // the same for the whole wave
-                row -= WIDE;
-                b_from[u] += N * K * 2;
-            }
-            b_off[u] = row < b_cols ? (unsigned)row * row_bytes + chunk * 16 : PAST_END;
-        }
+    for (int u = 0; u < B_OFFS; ++u) {
+        const int q = wave + 4 * u, col = 64 * (q / 8) + 8 * chunk;
+        if constexpr (B_ROWS) b_off[u] = col < b_cols ? (unsigned)((8 * (q % 8) + lane / 8) * N + col) * 2 : PAST_END;
+        else b_off[u] = (unsigned)(8 * q + lane / 8) * row_bytes + chunk * 16;
     }
-    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
-    // The loads of a step, one after the other: `u` below 2 FM A's, then B's.
-    auto fetch = [&](int it, int slot, int u) __attribute__((always_inline)) {
-        const unsigned to = lds0 + slot * SLOT + wave * PIECE;
-        const bool there = it < last;
-        const long long k = (long long)it * STEP, terms = K - k < STEP ? K - k : STEP;
-        const bool cut = k + 8 * chunk >= K;  // pieces past the end of a row
-        if (u < 2 * FM) {
-            if constexpr (A_ROWS) bring(a_src + k * M * 2, a_off[u], there ? (unsigned)((terms * M - row0) * 2) : 0, to + u * 4 * PIECE);
-            else bring(a_src + k * 2, cut ? PAST_END : a_off[u], there ? (unsigned)(a_rows * (long long)row_bytes - k * 2) : 0, to + u * 4 * PIECE);
-        } else if constexpr (B_ROWS) {
-            bring(b_src + k * N * 2, b_off[u - 2 * FM], there ? (unsigned)((terms * N - col0) * 2) : 0, to + A_BYTES + (u - 2 * FM) * 4 * PIECE);
-        } else {
-            bring(b_from[u - 2 * FM] + k * 2, cut ? PAST_END : b_off[u - 2 * FM], there ? (unsigned)(b_cols * (long long)row_bytes - k * 2) : 0,
-                  to + A_BYTES + (u - 2 * FM) * 4 * PIECE);
+    const int rest_terms = (int)(K % STEP), cut = rest_terms ? steps - 1 : -1;  // the step that ends early
+    const unsigned past = 8 * chunk >= rest_terms ? PAST_END : 0;
+    const unsigned lds_wave = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds + wave * PIECE;
+    u32x4 a_words, b_words, gate_words;
+    auto aim = [&](int it) __attribute__((always_inline)) {  // at the loads of step `it`, which follows the last one aimed at
+        a_words = a_src.next(it < last);
+        b_words = b_src.next(it < last);
+        if constexpr (FINISH == GATED) {
+            const size_t gate = ((size_t)b_words[1] << 32 | b_words[0]) + (size_t)(N * K * 2);
+            gate_words = u32x4{(unsigned)gate, (unsigned)(gate >> 32) & 0xffffu, b_words[2], b_words[3]};
         }
+        if (it == cut) {  // the last step of all: what comes behind it reads nothing
+            if constexpr (!A_ROWS)
+#pragma unroll
+                for (int u = 0; u < 2 * FM; ++u) a_off[u] |= past;
+            if constexpr (!B_ROWS)
+#pragma unroll
+                for (int u = 0; u < B_OFFS; ++u) b_off[u] |= past;
+        }
+    };
+    // The loads of a step, one after the other: U below 2 FM A's, then B's.
+    auto fetch = [&](auto slot_, auto u_) __attribute__((always_inline)) {
+        constexpr int SLOT_AT = decltype(slot_)::value * SLOT, U = decltype(u_)::value, V = U - 2 * FM;
+        if constexpr (U < 2 * FM) bring<SLOT_AT + U * 4 * PIECE>(a_words, a_off[U], lds_wave);
+        else if constexpr (V < B_OFFS) bring<SLOT_AT + A_BYTES + V * 4 * PIECE>(b_words, b_off[V], lds_wave);
+        else bring<SLOT_AT + A_BYTES + V * 4 * PIECE>(gate_words, b_off[V - B_OFFS], lds_wave);
     };
     // first row of B's tile (column of the product) of a wave's j-th fragment
     auto b_row = [&](int j) __attribute__((always_inline)) {
         if (FINISH == GATED) return (j / (FN / 2)) * WIDE + 16 * FN * wn + 32 * (j % (FN / 2));
         return 32 * FN * wn + 32 * j;
     };
+    // Where a lane reads.  Terms side by side: a row is 128 bytes, its 16-byte pieces swapped by row, which 32 rows further on is the same; a
+    // place for each quarter of a step.  By rows: 64 columns are 8 KiB, 16 terms 2 KiB; two places for each fragment.
+    int a_lane[A_ROWS ? 2 * FM : 4], b_lane[B_ROWS ? 2 * FN : 4];
+    auto by_rows = [&](int n0, int half) __attribute__((always_inline)) {
+        const int s = lane & 15, term = 8 * h + (s >> 2) + 4 * half, c = (n0 % 64 >> 3) + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
+        return n0 / 64 * 8 * PIECE + tile_off<64>(term, c) + ((s & 1) << 3);
+    };
+#pragma unroll
+    for (int u = 0; u < (A_ROWS ? 2 * FM : 4); ++u) a_lane[u] = A_ROWS ? by_rows(32 * FM * wm + 32 * (u / 2), u % 2) : tile_off<64>(32 * FM * wm + m, 2 * u + h);
+#pragma unroll
+    for (int u = 0; u < (B_ROWS ? 2 * FN : 4); ++u)
+        b_lane[u] = A_BYTES + (B_ROWS ? by_rows(b_row(u / 2), u % 2) : tile_off<64>((FINISH == GATED ? 16 : 32) * FN * wn + m, 2 * u + h));
+    auto transposed = [&](int lo_at, int hi_at) __attribute__((always_inline)) {
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + lo_at)));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + hi_at)));
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
     constexpr bool AHEAD = FM == 1;  // the fragments of a whole step are read while the last one's are multiplied
     constexpr int SETS = AHEAD ? 8 : 2;
     u32x4 af[SETS][FM], bf[SETS][FN];
-    // 16 terms of 32 columns of an operand whose terms are its rows, LDS holding 64 columns side by side
-    auto by_rows = [&](const char* tile, int ks, int n0) __attribute__((always_inline)) {
-        tile += n0 / 64 * 8 * PIECE;
-        const int s = lane & 15, term = 16 * ks + 8 * h + (s >> 2), c = (n0 % 64 >> 3) + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
-        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_off<64>(term, c) + ((s & 1) << 3))));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_off<64>(term + 4, c) + ((s & 1) << 3))));
-        return u32x4{lo[0], lo[1], hi[0], hi[1]};
-    };
     // The reads of a quarter of a step, in the order in which the products need them: A's first fragment, B's, A's others.
-    auto read = [&](int set, int ks, int slot, int u) __attribute__((always_inline)) {
-        const char* at_a = lds + slot * SLOT;
-        const char* at_b = at_a + A_BYTES;
-        if (u == 0 || u > FN) {
-            const int i = u == 0 ? 0 : u - FN, n0 = 32 * FM * wm + 32 * i;
-            if constexpr (A_ROWS) af[set][i] = by_rows(at_a, ks, n0);
-            else af[set][i] = *reinterpret_cast<const u32x4*>(at_a + tile_off<64>(n0 + m, 2 * ks + h));
-            return;
+    auto read = [&](auto set_, auto ks_, auto slot_, auto u_) __attribute__((always_inline)) {
+        constexpr int set = decltype(set_)::value, ks = decltype(ks_)::value, from = decltype(slot_)::value * SLOT, U = decltype(u_)::value;
+        if constexpr (U == 0 || U > FN) {
+            constexpr int i = U == 0 ? 0 : U - FN;
+            if constexpr (A_ROWS) af[set][i] = transposed(a_lane[2 * i] + (from + ks * 2048), a_lane[2 * i + 1] + (from + ks * 2048));
+            else af[set][i] = *reinterpret_cast<const u32x4*>(lds + a_lane[ks] + (from + i * 4096));
+        } else {
+            constexpr int j = U - 1, further = FINISH == GATED ? j / (FN / 2) * WIDE * 128 + j % (FN / 2) * 4096 : j * 4096;
+            if constexpr (B_ROWS) bf[set][j] = transposed(b_lane[2 * j] + (from + ks * 2048), b_lane[2 * j + 1] + (from + ks * 2048));
+            else bf[set][j] = *reinterpret_cast<const u32x4*>(lds + b_lane[ks] + (from + further));
         }
-        const int j = u - 1, n0 = b_row(j);
-        if constexpr (B_ROWS) bf[set][j] = by_rows(at_b, ks, n0);
-        else bf[set][j] = *reinterpret_cast<const u32x4*>(at_b + tile_off<64>(n0 + m, 2 * ks + h));
     };
     f32x16 acc[FM][FN];
 #pragma unroll
@@ -249,72 +283,80 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     // The products of a quarter of a step, and behind each what may run beside it (the compiler would put a read right before its use).
-    auto multiply = [&](int set, auto beside) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                acc[i][j] = Mma<T>::mma(bf[set][j], af[set][i], acc[i][j]);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int u = (i * FN + j) * BESIDE; u < (i * FN + j + 1) * BESIDE; ++u)
-                    if (u < READS) beside(u);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+    auto multiply = [&](auto set_, auto beside) __attribute__((always_inline)) {
+        constexpr int set = decltype(set_)::value;
+        each<FM * FN>([&](auto n) __attribute__((always_inline)) {
+            constexpr int i = decltype(n)::value / FN, j = decltype(n)::value % FN, BESIDE = (READS + FM * FN - 1) / (FM * FN);
+            acc[i][j] = Mma<T>::mma(bf[set][j], af[set][i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+            each<BESIDE>([&](auto e) __attribute__((always_inline)) {
+                constexpr int U = decltype(n)::value * BESIDE + decltype(e)::value;
+                if constexpr (U < READS) beside(Count<U>{});
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
     };
-#pragma unroll
-    for (int s = 0; s < DEEP; ++s)
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) fetch(first + s, s, u);
-    __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((DEEP - 1) * LOADS));
+    // This wave's loads of the next step have landed and its reads of this one are done, and behind the barrier everyone's.
+    auto meet = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((DEEP - 2) * LOADS));
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    // The ring is filled, up to half of its last step; that one's other half goes beside the first products.
+    each<DEEP>([&](auto s) __attribute__((always_inline)) {
+        aim(first + decltype(s)::value);
+        each<(decltype(s)::value == DEEP - 1 && !AHEAD ? READS : LOADS)>([&](auto u) __attribute__((always_inline)) { fetch(s, u); });
+    });
+    __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm(AHEAD ? (DEEP - 1) * LOADS : (DEEP - 2) * LOADS + READS));
     asm volatile("s_barrier" ::: "memory");
     if constexpr (AHEAD) {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-            for (int u = 0; u < READS; ++u) read(ks, ks, 0, u);
-        int slot = 0;
-        auto step = [&](auto parity, int it) __attribute__((always_inline)) {
-            constexpr int now = 4 * decltype(parity)::value, then = 4 - now;
-            const int next = slot + 1 == DEEP ? 0 : slot + 1;
-            // this wave's loads of the next step have landed and its reads of this one are done, and behind the barrier everyone's
-            __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((DEEP - 2) * LOADS));
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-                multiply(now + ks, [&](int u) __attribute__((always_inline)) {
-                    read(then + ks, ks, next, u);
-                    if (ks & 1) fetch(it + DEEP, slot, ks / 2 * READS + u);
+        each<4>([&](auto ks) __attribute__((always_inline)) { each<READS>([&](auto u) __attribute__((always_inline)) { read(ks, ks, Count<0>{}, u); }); });
+        auto step = [&](auto n, int it) __attribute__((always_inline)) {
+            constexpr int S = decltype(n)::value % DEEP, NEXT = (S + 1) % DEEP, now = decltype(n)::value % 2 * 4, then = 4 - now;
+            meet();
+            aim(it + DEEP);
+            each<4>([&](auto ks) __attribute__((always_inline)) {
+                constexpr int KS = decltype(ks)::value;
+                multiply(Count<now + KS>{}, [&](auto u) __attribute__((always_inline)) {
+                    read(Count<then + KS>{}, ks, Count<NEXT>{}, u);
+                    if constexpr (KS % 2) fetch(Count<S>{}, Count<KS / 2 * READS + decltype(u)::value>{});
                 });
-            slot = next;
+            });
         };
-        for (int it = first; it < last; it += 2) {
-            step(Count<0>{}, it);
-            if (it + 1 < last) step(Count<1>{}, it + 1);
+        constexpr int TURN = DEEP % 2 ? 2 * DEEP : DEEP;  // after which places and sets are as before
+        for (int it = first;;) {
+            bool more = true;
+            each<TURN>([&](auto n) __attribute__((always_inline)) {
+                if (more) {
+                    step(n, it);
+                    more = ++it < last;
+                }
+            });
+            if (!more) break;
         }
     } else {
-#pragma unroll
-        for (int u = 0; u < READS; ++u) read(0, 0, 0, u);
-        for (int it = first, slot = 0, before = DEEP - 1; it < last; ++it) {
-            const int next = slot + 1 == DEEP ? 0 : slot + 1;
+        static_assert(AHEAD || DEEP == 2, "two steps a turn");
+        each<READS>([&](auto u) __attribute__((always_inline)) { read(Count<0>{}, Count<0>{}, Count<0>{}, u); });
+        auto step = [&](auto s, int it) __attribute__((always_inline)) {
+            constexpr int S = decltype(s)::value, NEXT = 1 - S;
             // A step's place is free for the one a ring later from the barrier on.  Half of its loads go beside the quarter behind it, half
             // beside the quarter after that: all at once they queue up and hold up the products (tiles of 256 x 256, 6007 x 4096 x 11008:
             // 525 -> 486 us).
-            multiply(0, [&](int u) __attribute__((always_inline)) {
-                read(1, 1, slot, u);
-                if (it > first) fetch(it - 1 + DEEP, before, READS + u);
+            multiply(Count<0>{}, [&](auto u) __attribute__((always_inline)) {
+                read(Count<1>{}, Count<1>{}, s, u);
+                fetch(Count<NEXT>{}, Count<READS + decltype(u)::value>{});
             });
-            multiply(1, [&](int u) __attribute__((always_inline)) { read(0, 2, slot, u); });
-            multiply(0, [&](int u) __attribute__((always_inline)) { read(1, 3, slot, u); });
-            // this wave's loads of the next step have landed and its reads of this one are done, and behind the barrier everyone's
-            __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm((DEEP - 2) * LOADS));
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            multiply(1, [&](int u) __attribute__((always_inline)) {
-                read(0, 0, next, u);
-                fetch(it + DEEP, slot, u);
+            multiply(Count<1>{}, [&](auto u) __attribute__((always_inline)) { read(Count<0>{}, Count<2>{}, s, u); });
+            multiply(Count<0>{}, [&](auto u) __attribute__((always_inline)) { read(Count<1>{}, Count<3>{}, s, u); });
+            meet();
+            aim(it + 2);
+            multiply(Count<1>{}, [&](auto u) __attribute__((always_inline)) {
+                read(Count<0>{}, Count<0>{}, Count<NEXT>{}, u);
+                fetch(s, u);
             });
-            before = slot;
-            slot = next;
+        };
+        for (int it = first; it < last; it += 2) {  // behind the last of an odd number of steps comes one of zeros
+            step(Count<0>{}, it);
+            step(Count<1>{}, it + 1);
         }
     }
     // Nothing is under way into LDS any more, and behind the barrier nothing is read from it: from here on each wave has a part of its own, in
@@ -460,37 +502,41 @@ template <typename T, Finish FINISH> int launch_few(const Task& task, hipStream_
 }
 
 // How a product is laid out: the tile, and into how many parts the sums of those tiles are cut that do not fill the chip once more.
-constexpr int NONE = -1, FEW_ROWS = 3;
+constexpr int NONE = -1, FEW_ROWS = 5, FORMS = 5;
+// A tile's fragments, how many workgroups share a CU, and what it takes there, in us (see layout_of).
+struct Form {
+    int fm, fn, a_cu;
+    double step[3], alone[3], start;
+};
+constexpr Form forms[FORMS] = {{4, 4, 1, {1.45, 1.37, 1.46}, {1.00, 1.20, 1.69}, 4.1}, {3, 2, 2, {1.08, 1.11, 1.12}, {0.55, 0.79, 0.70}, 1.3},
+                               {2, 3, 2, {1.05, 1.20, 1.12}, {0.57, 0.79, 0.72}, 1.4}, {2, 2, 2, {0.79, 0.82, 0.91}, {0.50, 0.56, 0.63}, 1.5},
+                               {1, 2, 2, {0.51, 0.58, 0.65}, {0.30, 0.30, 0.37}, 2.0}};
 struct Layout {
-    int form;  // FM x FN: 0: 4 x 4, 1: 2 x 2, 2: 1 x 2
+    int form;
     int m_tiles, n_tiles, whole, parts, part_steps;
     double us;
     size_t bytes() const {
-        constexpr int sizes[3] = {256 * 256, 128 * 128, 64 * 128};
-        return parts > 1 ? (size_t)(m_tiles * n_tiles - whole) * parts * sizes[form] * sizeof(float) : 0;
+        return parts > 1 ? (size_t)(m_tiles * n_tiles - whole) * parts * (64 * forms[form].fm) * (64 * forms[form].fn) * sizeof(float) : 0;
     }
 };
 
 // By what a call takes, in us: for each round of workgroups over the chip its steps, its start and the results on their way out (20 GB/s a CU, since
-// all finish together); for parts a second launch and their sums out and back.  The constants are fitted to 254 products of 35 blocks (1 ... 16896
-// rows, widths 128 ... 11008), each in up to 27 layouts: what is chosen took 1.005 times the best on average, 1.10 at most.  A step of 256 x 256
-// takes 1.5 us with the terms of both operands side by side, 1.7 with both by rows (twice the reads); of 128 x 128, two workgroups a CU, 1.0
-// and alone on its CU 0.6 ... 0.8; of 64 x 128 0.6 and 0.2 ... 0.4.
+// all finish together); for parts a second launch and their sums out and back.  The constants are fitted to 340 products of 58 blocks (1 ... 16384
+// rows, widths 128 ... 11008), each in up to 45 layouts: what is chosen took 1.007 times the best on average, 1.15 at most.  A step of 256 x 256
+// takes 1.45 us where it fills the chip, 1 where it does not; of 192 x 128 two on a CU 1.1, one 0.55 ... 0.8; of 128 x 128 0.8 ... 0.9 and 0.5 ... 0.6;
+// of 64 x 128 0.5 ... 0.65 and 0.3.  More with operands by rows, whose reads are twice as many.
 Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
-    constexpr struct { int rows, columns, a_cu; double step[3], alone[3], start; } forms[3] = {
-        {256, 256, 1, {1.50, 1.47, 1.66}, {1.30, 1.52, 1.75}, 5.1},
-        {128, 128, 2, {0.99, 0.94, 1.01}, {0.59, 0.60, 0.78}, 1.35},
-        {64, 128, 2, {0.56, 0.62, 0.65}, {0.18, 0.40, 0.43}, 2.5}};
     const int cus = device_compute_units(), steps = (int)((K + STEP - 1) / STEP);
     Layout best{NONE, 0, 0, 0, 1, 0, 0.0};
     if (by_rows == 0 && M <= FEW && (M <= 2 || N * K <= FEW_TERMS)) return {FEW_ROWS, 0, 0, 0, 1, 0, 0.0};
-    for (int f = 0; f < 3; ++f) {
-        const auto& form = forms[f];
-        const int columns = finish == GATED ? form.columns / 2 : form.columns, slots = cus * form.a_cu;
-        const int64_t m_tiles = (M + form.rows - 1) / form.rows, n_tiles = (N + columns - 1) / columns, tiles = m_tiles * n_tiles;
+    for (int f = 0; f < FORMS; ++f) {
+        const Form& form = forms[f];
+        if (finish == GATED && form.fn % 2) continue;  // up and gate are half of a wave's columns each
+        const int rows = 64 * form.fm, wide = 64 * form.fn, columns = finish == GATED ? wide / 2 : wide, slots = cus * form.a_cu;
+        const int64_t m_tiles = (M + rows - 1) / rows, n_tiles = (N + columns - 1) / columns, tiles = m_tiles * n_tiles;
         if (tiles >= 1 << 24) continue;
         const double full = form.step[by_rows], alone = form.alone[by_rows];
-        const double fixed = form.start + (finish == GATED ? 5.1 : finish == UNGATED ? 3.5 : 2.1) * form.rows * columns * form.a_cu / 20e3;
+        const double fixed = form.start + (finish == GATED ? 4.4 : finish == UNGATED ? 2.6 : 1.9) * rows * columns * form.a_cu / 20e3;
         const auto rounds = [&](int64_t items, int of) {
             const int deep = (int)((items % slots + cus - 1) / cus);  // workgroups that share a CU in the last round
             return (double)(items / slots) * (of * full + fixed) + (deep ? of * (deep == 1 ? alone : full) + fixed : 0.0);
@@ -501,7 +547,7 @@ Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
             const int64_t whole = s == 1 ? tiles : tiles / slots * slots, rest = tiles - whole;
             if (s > 1 && (rest == 0 || part_steps < 2 || rest * s > 2 * slots)) break;  // parts for two rounds at most
             double us = rounds(whole, steps);
-            if (rest) us += rounds(rest * s, part_steps) + 2.35 + (double)rest * s * form.rows * form.columns * 8.0 / 6.8e6;
+            if (rest) us += rounds(rest * s, part_steps) + 4.8 + (double)rest * s * rows * columns * 8.0 / 6.4e6;
             if (best.form == NONE || us < best.us) best = {f, (int)m_tiles, (int)n_tiles, (int)whole, s, part_steps, us};
         }
     }
@@ -532,7 +578,10 @@ int launch(const Layout& l, const void* a, const void* b, const void* bias, void
     if constexpr (!A_ROWS && !B_ROWS)
         if (l.form == FEW_ROWS) return launch_few<T, FINISH>(task, stream);
     if (l.form == 0) return launch_tile<T, 4, 4, A_ROWS, B_ROWS, FINISH>(task, stream);
-    if (l.form == 1) return launch_tile<T, 2, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
+    if (l.form == 1) return launch_tile<T, 3, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
+    if constexpr (FINISH != GATED)
+        if (l.form == 2) return launch_tile<T, 2, 3, A_ROWS, B_ROWS, FINISH>(task, stream);
+    if (l.form == 3) return launch_tile<T, 2, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
     return launch_tile<T, 1, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
 }
 
