@@ -414,7 +414,7 @@ template <typename T, int FM, int FN, Finish FINISH> __global__ __launch_bounds_
 
 // Products of a few rows, both operands' terms side by side: a weight comes through once, and what counts is that all of the chip asks for it
 // at once.  KW waves share the sums of COLUMNS columns (GATED: pairs of them) of all rows, each lane 16 bytes of every 512 KW terms; lanes are
-// added by exchange, waves in order.  One token, 768 -> 2 x 2048 -> 768 in bf16: @@.
+// added by exchange, waves in order.  One token, 768 -> 2 x 2048 -> 768 in bf16: 4.8 and 2.3 us (64 x 128 tiles: 7.5 and 8.6).
 constexpr int FEW = 4, COLUMNS = 2;
 constexpr int64_t FEW_TERMS = 4 << 20;  // of a weight, from three rows on
 template <typename T, int ROWS, Finish FINISH, int KW> __global__ __launch_bounds__(256) void few_rows_kernel(Task task) {
@@ -639,15 +639,119 @@ template <typename T> int column_sums(const void* x, void* out, float* partials,
     return LBI_OK;
 }
 
+// Widths that are no whole 16-byte pieces run on copies padded with zeros, which change neither results nor gradients: one launch pads all
+// operands, one cuts all results (padded one by one, a fill and a copy each, a call for two rows of 503 -> 2 x 159 -> 503 took 48 us, now 20).
+struct Copy {
+    const void* from;
+    void* to;
+    long long from_rows, from_columns, from_ld, to_rows, to_columns, to_ld, first;  // first: row of the launch with which it begins
+};
+struct Copies {
+    Copy copy[8];
+    int count;
+    long long rows;
+};
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+__global__ __launch_bounds__(256) void copy_kernel(Copies all) {
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= all.rows) return;
+    int n = 0;
+    while (n + 1 < all.count && all.copy[n + 1].first <= row) ++n;
+    const Copy& c = all.copy[n];
+    const long long r = row - c.first, there = r < c.from_rows ? c.from_columns : 0;
+    const unsigned short* from = static_cast<const unsigned short*>(c.from) + r * c.from_ld;
+    unsigned short* to = static_cast<unsigned short*>(c.to) + r * c.to_ld;
+    for (long long col = (threadIdx.x & 63) * 8; col < c.to_columns; col += 512) {
+        u32x4_any w = {0, 0, 0, 0};
+        if (col + 8 <= there) {
+            w = *reinterpret_cast<const u32x4_any*>(from + col);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = (col + 2 * e < there ? from[col + 2 * e] : 0u) | (col + 2 * e + 1 < there ? (unsigned)from[col + 2 * e + 1] << 16 : 0u);
+        }
+        if (col + 8 <= c.to_columns) {
+            *reinterpret_cast<u32x4_any*>(to + col) = w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < c.to_columns) to[col + e] = (unsigned short)(w[e / 2] >> (16 * (e % 2)));
+        }
+    }
+}
+
+size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// The copies of a call, and what they take of the workspace.  Without a base it only counts.
+struct Padding {
+    char* base;
+    size_t bytes = 0;
+    Copies in{}, out{};
+    static int64_t eights(int64_t n) { return (n + 7) / 8 * 8; }
+    static void add(Copies& list, const Copy& c) {
+        list.copy[list.count] = c;
+        list.copy[list.count++].first = list.rows;
+        list.rows += c.to_rows;
+    }
+    // Room for `halves` matrices [rows, columns] behind one another, padded; where nothing is to pad, the tensor itself.
+    void* room(const void* tensor, int64_t rows, int64_t columns, int64_t padded_rows, int64_t padded_columns, int halves) {
+        if (!tensor || (rows == padded_rows && columns == padded_columns)) return const_cast<void*>(tensor);
+        void* at = base + bytes;
+        bytes += up((size_t)halves * padded_rows * padded_columns * 2);
+        return at;
+    }
+    // Matrices one behind the other.
+    const void* operand(const void* tensor, int64_t rows, int64_t columns, int64_t padded_rows, int64_t padded_columns, int halves = 1) {
+        char* at = static_cast<char*>(room(tensor, rows, columns, padded_rows, padded_columns, halves));
+        if (at != tensor)
+            for (int half = 0; half < halves; ++half)
+                add(in, {static_cast<const char*>(tensor) + half * rows * columns * 2, at + half * padded_rows * padded_columns * 2, rows, columns,
+                         columns, padded_rows, padded_columns, padded_columns, 0});
+        return at;
+    }
+    void* result(void* tensor, int64_t rows, int64_t columns, int64_t padded_rows, int64_t padded_columns, int halves = 1) {
+        char* at = static_cast<char*>(room(tensor, rows, columns, padded_rows, padded_columns, halves));
+        if (at != tensor)
+            for (int half = 0; half < halves; ++half)
+                add(out, {at + half * padded_rows * padded_columns * 2, static_cast<char*>(tensor) + half * rows * columns * 2, padded_rows,
+                          padded_columns, padded_columns, rows, columns, columns, 0});
+        return at;
+    }
+    // Two matrices side by side, [rows, 2 columns].
+    const void* side_by_side(const void* tensor, int64_t rows, int64_t columns, int64_t padded) {
+        char* at = static_cast<char*>(room(tensor, rows, columns, rows, padded, 2));
+        if (at != tensor)
+            for (int half = 0; half < 2; ++half)
+                add(in, {static_cast<const char*>(tensor) + half * columns * 2, at + half * padded * 2, rows, columns, 2 * columns, rows, padded,
+                         2 * padded, 0});
+        return at;
+    }
+    void* result_side_by_side(void* tensor, int64_t rows, int64_t columns, int64_t padded) {
+        char* at = static_cast<char*>(room(tensor, rows, columns, rows, padded, 2));
+        if (at != tensor)
+            for (int half = 0; half < 2; ++half)
+                add(out, {at + half * padded * 2, static_cast<char*>(tensor) + half * columns * 2, rows, columns, 2 * padded, rows, columns,
+                          2 * columns, 0});
+        return at;
+    }
+    static int run(const Copies& list, hipStream_t stream) {
+        if (!list.rows) return LBI_OK;
+        hipLaunchKernelGGL(copy_kernel, dim3((unsigned)((list.rows + 3) / 4)), dim3(256), 0, stream, list);
+        LBI_HIP_CHECK(hipGetLastError());
+        return LBI_OK;
+    }
+};
+
 constexpr int64_t MOST_WIDTH = 1 << 20, MOST_ROWS = 1 << 23;
 
 int check(const char* who, int64_t rows, int64_t D, int64_t hidden, int64_t width, int dtype) {
-    if (rows < 0 || D < 0 || hidden < 0 || width < 0)
+    if (rows < 0 || D < 1 || hidden < 1 || width < 1)
         return fail(LBI_ERR_INVALID, "%s: bad size (rows=%lld D=%lld hidden=%lld width=%lld)", who, (long long)rows, (long long)D,
                     (long long)hidden, (long long)width);
     if (dtype != LBI_F16 && dtype != LBI_BF16) return fail(LBI_ERR_UNSUPPORTED, "%s: needs half or bfloat16", who);
-    if (D < 8 || hidden < 8 || width < 8 || D % 8 || hidden % 8 || width % 8 || std::max({D, hidden, width}) > MOST_WIDTH || rows > MOST_ROWS)
-        return fail(LBI_ERR_UNSUPPORTED, "%s: widths are multiples of 8, up to 2^20, rows up to 2^23", who);
+    if (std::max({D, hidden, width}) > MOST_WIDTH || rows > MOST_ROWS)
+        return fail(LBI_ERR_UNSUPPORTED, "%s: widths up to 2^20, rows up to 2^23", who);
     return LBI_OK;
 }
 bool on_grid(std::initializer_list<const void*> tensors) {
@@ -656,23 +760,71 @@ bool on_grid(std::initializer_list<const void*> tensors) {
     return true;
 }
 
-size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 struct Forward {
-    Layout fc1, fc2;
-    Forward(int64_t rows, int64_t D, int64_t hidden, int64_t width)
-        : fc1(layout_of(rows, hidden, D, GATED, 0)), fc2(layout_of(rows, width, hidden, PLAIN, 0)) {}
-    size_t bytes() const { return up(std::max(fc1.bytes(), fc2.bytes())); }
+    const void *x, *fc1_weight, *fc1_bias, *fc2_weight, *fc2_bias;
+    void *fc1_output, *down_input, *out;
+    int64_t rows, D, hidden, width;
 };
 struct Pullback {
-    Layout a, x, fc1, fc2;
-    size_t g_fc1, sums, partial;  // parts of the workspace, in bytes
-    Pullback(int64_t rows, int64_t D, int64_t hidden, int64_t width)
-        : a(layout_of(rows, hidden, width, UNGATED, 1)), x(layout_of(rows, D, 2 * hidden, PLAIN, 1)),
-          fc1(layout_of(2 * hidden, D, rows, PLAIN, 2)), fc2(layout_of(width, hidden, rows, PLAIN, 2)), g_fc1(up((size_t)rows * 2 * hidden * 2)),
-          sums(up((size_t)slabs_of(rows) * std::max(2 * hidden, width) * sizeof(float))),
-          partial(up(std::max({a.bytes(), x.bytes(), fc1.bytes(), fc2.bytes()}))) {}
-    size_t bytes() const { return g_fc1 + sums + partial; }
+    const void *g_out, *x, *fc1_output, *down_input, *fc1_weight, *fc2_weight;
+    void *g_x, *g_fc1_weight, *g_fc2_weight, *g_fc1_bias, *g_fc2_bias;
+    int64_t rows, D, hidden, width;
 };
+
+// The calls as they run: tensors padded where that is needed, the products' layouts, the workspace.
+struct ForwardPlan {
+    Padding pad;
+    Forward t;
+    Layout fc1, fc2;
+    size_t partial;
+    ForwardPlan(const Forward& c, void* workspace) : pad{static_cast<char*>(workspace)}, t(c) {
+        t.D = Padding::eights(c.D), t.hidden = Padding::eights(c.hidden), t.width = Padding::eights(c.width);
+        t.x = pad.operand(c.x, c.rows, c.D, c.rows, t.D);
+        t.fc1_weight = pad.operand(c.fc1_weight, c.hidden, c.D, t.hidden, t.D, 2);
+        t.fc1_bias = pad.operand(c.fc1_bias, 1, c.hidden, 1, t.hidden, 2);
+        t.fc2_weight = pad.operand(c.fc2_weight, c.width, c.hidden, t.width, t.hidden);
+        t.fc2_bias = pad.operand(c.fc2_bias, 1, c.width, 1, t.width);
+        t.fc1_output = pad.result_side_by_side(c.fc1_output, c.rows, c.hidden, t.hidden);
+        t.down_input = pad.result(c.down_input, c.rows, c.hidden, c.rows, t.hidden);
+        t.out = pad.result(c.out, c.rows, c.width, c.rows, t.width);
+        fc1 = layout_of(t.rows, t.hidden, t.D, GATED, 0);
+        fc2 = layout_of(t.rows, t.width, t.hidden, PLAIN, 0);
+        partial = pad.bytes;
+    }
+    size_t bytes() const { return partial + up(std::max(fc1.bytes(), fc2.bytes())); }
+};
+struct PullbackPlan {
+    Padding pad;
+    Pullback t;
+    Layout a, x, fc1, fc2;
+    size_t g_fc1, sums, partial;
+    PullbackPlan(const Pullback& c, void* workspace) : pad{static_cast<char*>(workspace)}, t(c) {
+        t.D = Padding::eights(c.D), t.hidden = Padding::eights(c.hidden), t.width = Padding::eights(c.width);
+        t.g_out = pad.operand(c.g_out, c.rows, c.width, c.rows, t.width);
+        t.x = pad.operand(c.x, c.rows, c.D, c.rows, t.D);
+        t.fc1_output = pad.side_by_side(c.fc1_output, c.rows, c.hidden, t.hidden);
+        t.down_input = pad.operand(c.down_input, c.rows, c.hidden, c.rows, t.hidden);
+        t.fc1_weight = pad.operand(c.fc1_weight, c.hidden, c.D, t.hidden, t.D, 2);
+        t.fc2_weight = pad.operand(c.fc2_weight, c.width, c.hidden, t.width, t.hidden);
+        t.g_x = pad.result(c.g_x, c.rows, c.D, c.rows, t.D);
+        t.g_fc1_weight = pad.result(c.g_fc1_weight, c.hidden, c.D, t.hidden, t.D, 2);
+        t.g_fc2_weight = pad.result(c.g_fc2_weight, c.width, c.hidden, t.width, t.hidden);
+        t.g_fc1_bias = pad.result(c.g_fc1_bias, 1, c.hidden, 1, t.hidden, 2);
+        t.g_fc2_bias = pad.result(c.g_fc2_bias, 1, c.width, 1, t.width);
+        a = layout_of(t.rows, t.hidden, t.width, UNGATED, 1);
+        x = layout_of(t.rows, t.D, 2 * t.hidden, PLAIN, 1);
+        fc1 = layout_of(2 * t.hidden, t.D, t.rows, PLAIN, 2);
+        fc2 = layout_of(t.width, t.hidden, t.rows, PLAIN, 2);
+        g_fc1 = pad.bytes;
+        sums = g_fc1 + up((size_t)t.rows * 2 * t.hidden * 2);
+        partial = sums + up((size_t)slabs_of(t.rows) * std::max(2 * t.hidden, t.width) * sizeof(float));
+    }
+    size_t bytes() const { return partial + up(std::max({a.bytes(), x.bytes(), fc1.bytes(), fc2.bytes()})); }
+};
+
+// Every tensor given: what a plan that only counts is told.
+const void* const SOME = reinterpret_cast<const void*>(256);
+void* const SOME_RESULT = reinterpret_cast<void*>(256);
 
 }  // namespace
 }  // namespace block_mlp
@@ -681,7 +833,7 @@ struct Pullback {
 extern "C" size_t lbi_gated_mlp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
     using namespace lbi::block_mlp;
     if (check("lbi_gated_mlp", rows, D, hidden, width, LBI_BF16) || rows == 0) return 0;
-    return Forward(rows, D, hidden, width).bytes();
+    return ForwardPlan({SOME, SOME, SOME, SOME, SOME, SOME_RESULT, SOME_RESULT, SOME_RESULT, rows, D, hidden, width}, nullptr).bytes();
 }
 
 extern "C" int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* fc1_bias, const void* fc2_weight, const void* fc2_bias,
@@ -693,25 +845,31 @@ extern "C" int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* 
     if (int bad = check("lbi_gated_mlp", rows, D, hidden, width, dtype)) return bad;
     if (rows == 0) return LBI_OK;
     if (!x || !fc1_weight || !fc2_weight || !down_input || !out) return fail(LBI_ERR_INVALID, "lbi_gated_mlp: null pointer");
-    if (!on_grid({x, fc1_weight, fc1_bias, fc2_weight, fc2_bias, fc1_output, down_input, out, workspace}))
-        return fail(LBI_ERR_INVALID, "lbi_gated_mlp: tensors must be 16-byte aligned");
-    const Forward l(rows, D, hidden, width);
-    const size_t need = l.bytes();
+    if (!on_grid({x, fc1_weight, fc1_bias, fc2_weight, fc2_bias, fc1_output, down_input, out}) || reinterpret_cast<uintptr_t>(workspace) % 256)
+        return fail(LBI_ERR_INVALID, "lbi_gated_mlp: tensors must be 16-byte aligned, the workspace 256");
+    const ForwardPlan p({x, fc1_weight, fc1_bias, fc2_weight, fc2_bias, fc1_output, down_input, out, rows, D, hidden, width}, workspace);
+    const size_t need = p.bytes();
     if (need && (!workspace || workspace_bytes < need))
         return fail(LBI_ERR_WORKSPACE, "lbi_gated_mlp: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     const hipStream_t on = static_cast<hipStream_t>(stream);
-    const auto run = [&](auto t) {
-        using T = decltype(t);
-        if (int s = launch<T, false, false, GATED>(l.fc1, x, fc1_weight, fc1_bias, down_input, fc1_output, rows, hidden, D, workspace, on)) return s;
-        return launch<T, false, false, PLAIN>(l.fc2, down_input, fc2_weight, fc2_bias, out, nullptr, rows, width, hidden, workspace, on);
+    const auto run = [&](auto type) {
+        using T = decltype(type);
+        const Forward& t = p.t;
+        void* partial = static_cast<char*>(workspace) + p.partial;
+        if (int s = launch<T, false, false, GATED>(p.fc1, t.x, t.fc1_weight, t.fc1_bias, t.down_input, t.fc1_output, rows, t.hidden, t.D, partial, on))
+            return s;
+        return launch<T, false, false, PLAIN>(p.fc2, t.down_input, t.fc2_weight, t.fc2_bias, t.out, nullptr, rows, t.width, t.hidden, partial, on);
     };
-    return dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{});
+    if (int s = Padding::run(p.pad.in, on)) return s;
+    if (int s = dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{})) return s;
+    return Padding::run(p.pad.out, on);
 }
 
 extern "C" size_t lbi_gated_mlp_vjp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width) {
     using namespace lbi::block_mlp;
     if (check("lbi_gated_mlp_vjp", rows, D, hidden, width, LBI_BF16) || rows == 0) return 0;
-    return Pullback(rows, D, hidden, width).bytes();
+    return PullbackPlan({SOME, SOME, SOME, SOME, SOME, SOME, SOME_RESULT, SOME_RESULT, SOME_RESULT, SOME_RESULT, SOME_RESULT, rows, D, hidden, width},
+                        nullptr).bytes();
 }
 
 extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* fc1_output, const void* down_input, const void* fc1_weight,
@@ -728,25 +886,30 @@ extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* f
     if (!on_grid({g_out, x, fc1_output, down_input, fc1_weight, fc2_weight, g_x, g_fc1_weight, g_fc2_weight, g_fc1_bias, g_fc2_bias}) ||
         reinterpret_cast<uintptr_t>(workspace) % 256)
         return fail(LBI_ERR_INVALID, "lbi_gated_mlp_vjp: tensors must be 16-byte aligned, the workspace 256");
-    const Pullback p(rows, D, hidden, width);
+    const PullbackPlan p({g_out, x, fc1_output, down_input, fc1_weight, fc2_weight, g_x, g_fc1_weight, g_fc2_weight, g_fc1_bias, g_fc2_bias, rows, D,
+                          hidden, width}, workspace);
     if (!workspace || workspace_bytes < p.bytes())
         return fail(LBI_ERR_WORKSPACE, "lbi_gated_mlp_vjp: workspace of %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
     const hipStream_t on = static_cast<hipStream_t>(stream);
-    char* g_fc1 = static_cast<char*>(workspace);
-    float* sums = reinterpret_cast<float*>(g_fc1 + p.g_fc1);
-    char* partial = g_fc1 + p.g_fc1 + p.sums;
-    const auto run = [&](auto t) {
-        using T = decltype(t);
-        void* z = const_cast<void*>(fc1_output);
-        if (int s = launch<T, false, true, UNGATED>(p.a, g_out, fc2_weight, nullptr, g_fc1, z, rows, hidden, width, partial, on)) return s;
-        if (int s = launch<T, false, true, PLAIN>(p.x, g_fc1, fc1_weight, nullptr, g_x, nullptr, rows, D, 2 * hidden, partial, on)) return s;
-        if (int s = launch<T, true, true, PLAIN>(p.fc1, g_fc1, x, nullptr, g_fc1_weight, nullptr, 2 * hidden, D, rows, partial, on)) return s;
-        if (int s = launch<T, true, true, PLAIN>(p.fc2, g_out, down_input, nullptr, g_fc2_weight, nullptr, width, hidden, rows, partial, on)) return s;
-        if (g_fc1_bias)
-            if (int s = column_sums<T>(g_fc1, g_fc1_bias, sums, rows, 2 * hidden, on)) return s;
-        if (g_fc2_bias)
-            if (int s = column_sums<T>(g_out, g_fc2_bias, sums, rows, width, on)) return s;
+    char* base = static_cast<char*>(workspace);
+    void *g_fc1 = base + p.g_fc1, *partial = base + p.partial;
+    float* sums = reinterpret_cast<float*>(base + p.sums);
+    const auto run = [&](auto type) {
+        using T = decltype(type);
+        const Pullback& t = p.t;
+        void* z = const_cast<void*>(t.fc1_output);
+        if (int s = launch<T, false, true, UNGATED>(p.a, t.g_out, t.fc2_weight, nullptr, g_fc1, z, rows, t.hidden, t.width, partial, on)) return s;
+        if (int s = launch<T, false, true, PLAIN>(p.x, g_fc1, t.fc1_weight, nullptr, t.g_x, nullptr, rows, t.D, 2 * t.hidden, partial, on)) return s;
+        if (int s = launch<T, true, true, PLAIN>(p.fc1, g_fc1, t.x, nullptr, t.g_fc1_weight, nullptr, 2 * t.hidden, t.D, rows, partial, on)) return s;
+        if (int s = launch<T, true, true, PLAIN>(p.fc2, t.g_out, t.down_input, nullptr, t.g_fc2_weight, nullptr, t.width, t.hidden, rows, partial, on))
+            return s;
+        if (t.g_fc1_bias)
+            if (int s = column_sums<T>(g_fc1, t.g_fc1_bias, sums, rows, 2 * t.hidden, on)) return s;
+        if (t.g_fc2_bias)
+            if (int s = column_sums<T>(t.g_out, t.g_fc2_bias, sums, rows, t.width, on)) return s;
         return (int)LBI_OK;
     };
-    return dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{});
+    if (int s = Padding::run(p.pad.in, on)) return s;
+    if (int s = dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{})) return s;
+    return Padding::run(p.pad.out, on);
 }

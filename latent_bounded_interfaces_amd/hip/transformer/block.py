@@ -134,28 +134,12 @@ def _check_mlp(what: str, x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight:
     return x.numel() // dim, dim, int(hidden), int(width)
 
 
-def _ready(t: torch.Tensor | None, dtype: torch.dtype, *to: int) -> torch.Tensor | None:
-    """``t`` in ``dtype``, padded with zeros to the shape ``to``, contiguous and on the kernels' 16-byte grid."""
-    if t is None or (t.dtype == dtype and t.shape == to and t.is_contiguous() and t.data_ptr() % 16 == 0):
+def _ready(t: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor | None:
+    """``t`` in ``dtype``, contiguous and on the kernels' 16-byte grid."""
+    if t is None or (t.dtype == dtype and t.is_contiguous() and t.data_ptr() % 16 == 0):
         return t
-    t = t.detach().to(dtype)
-    if t.shape != to:
-        pad = [extent for have, want in zip(reversed(t.shape), reversed(to)) for extent in (0, want - have)]
-        t = torch.nn.functional.pad(t, pad)
-    t = t.contiguous()
+    t = t.detach().to(dtype).contiguous()
     return t.clone() if t.data_ptr() % 16 else t
-
-
-def _eights(n: int) -> int:
-    return (n + 7) // 8 * 8
-
-
-def _halves(t: torch.Tensor | None, dtype: torch.dtype, hidden: int, *rest: int) -> torch.Tensor | None:
-    """``[2 * hidden, ...]`` with each half padded (see :func:`_ready`)."""
-    if t is None or t.shape[0] == 2 * hidden and t.shape[1:] == rest:  # nothing to pad between the halves
-        return _ready(t, dtype, 2 * hidden, *rest)
-    halves = _ready(t.reshape(2, t.shape[0] // 2, *t.shape[1:]), dtype, 2, hidden, *rest)
-    return halves.view(2 * hidden, *rest)
 
 
 def gated_mlp(x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight: torch.Tensor, fc1_bias: torch.Tensor | None = None,
@@ -165,37 +149,30 @@ def gated_mlp(x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight: torch.Tenso
 
     Returns ``out [..., width]`` in the dtype of ``x``; with ``keep`` ``(out, fc1_output [..., 2 * hidden], down_input [..., hidden])``,
     what :func:`gated_mlp_vjp` and the region pullback read.  Sums, biases and the activation are fp32; ``down_input``, the
-    operand of the second product, is the one rounding in between.  Widths that are no multiples of 8 run on padded copies."""
+    operand of the second product, is the one rounding in between.  Widths that are no multiples of 8 run on padded copies, a pass over
+    the operands and one over the results."""
     rows, dim, hidden, width = _check_mlp("gated_mlp", x, fc1_weight, fc2_weight)
     if (fc1_bias is not None and fc1_bias.shape != (2 * hidden,)) or (fc2_bias is not None and fc2_bias.shape != (width,)):
         raise ValueError("gated_mlp: fc1_bias must be [2 * hidden] and fc2_bias [width]")
     _one_device("gated_mlp", x, fc1_weight, fc2_weight, fc1_bias, fc2_bias)
     _no_graph("gated_mlp", x, fc1_weight, fc2_weight, fc1_bias, fc2_bias)
     dtype, outer = x.dtype, x.shape[:-1]
-    d, hd, w = _eights(dim), _eights(hidden), _eights(width)
-    out, down = x.new_empty(rows, w), x.new_empty(rows, hd)
-    fc1_output = x.new_empty(rows, 2 * hd) if keep else None
+    out, down = x.new_empty(*outer, width), x.new_empty(*outer, hidden)
+    fc1_output = x.new_empty(*outer, 2 * hidden) if keep else None
     if rows:
-        x = _ready(x if x.dim() == 2 else x.reshape(rows, dim), dtype, rows, d)
-        fc1_weight, fc1_bias = _halves(fc1_weight, dtype, hd, d), _halves(fc1_bias, dtype, hd)
-        fc2_weight, fc2_bias = _ready(fc2_weight, dtype, w, hd), _ready(fc2_bias, dtype, w)
+        x, fc1_weight, fc2_weight = _ready(x, dtype), _ready(fc1_weight, dtype), _ready(fc2_weight, dtype)
+        fc1_bias, fc2_bias = _ready(fc1_bias, dtype), _ready(fc2_bias, dtype)
         lib = _lib.load()
         with _lib.device_guard(x.device):
-            need = int(lib.lbi_gated_mlp_workspace_bytes(rows, d, hd, w))
+            need = lib.lbi_gated_mlp_workspace_bytes(rows, dim, hidden, width)
             workspace = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
             status = lib.lbi_gated_mlp(
                 x.data_ptr(), fc1_weight.data_ptr(), None if fc1_bias is None else fc1_bias.data_ptr(), fc2_weight.data_ptr(),
                 None if fc2_bias is None else fc2_bias.data_ptr(), None if fc1_output is None else fc1_output.data_ptr(),
-                down.data_ptr(), out.data_ptr(), None if workspace is None else workspace.data_ptr(), need, rows, d, hd, w,
+                down.data_ptr(), out.data_ptr(), None if workspace is None else workspace.data_ptr(), need, rows, dim, hidden, width,
                 _lib.dtype_code(dtype), _stream(x))
         _lib.check(status, "lbi_gated_mlp")
-    if width != w or len(outer) != 1:
-        out = out[:, :width].reshape(*outer, width)
-    if not keep:
-        return out
-    if hidden != hd or len(outer) != 1:
-        fc1_output, down = fc1_output.view(rows, 2, hd)[:, :, :hidden].reshape(*outer, 2 * hidden), down[:, :hidden].reshape(*outer, hidden)
-    return out, fc1_output, down
+    return (out, fc1_output, down) if keep else out
 
 
 def gated_mlp_vjp(g_out: torch.Tensor, x: torch.Tensor, fc1_output: torch.Tensor, down_input: torch.Tensor, fc1_weight: torch.Tensor,
@@ -214,29 +191,20 @@ def gated_mlp_vjp(g_out: torch.Tensor, x: torch.Tensor, fc1_output: torch.Tensor
     if not rows:
         empty = [torch.zeros_like(x), x.new_zeros(fc1_weight.shape), x.new_zeros(fc2_weight.shape)]
         return tuple(empty + [x.new_zeros(2 * hidden), x.new_zeros(width)] if bias else empty)
-    d, hd, w = _eights(dim), _eights(hidden), _eights(width)
-    if len(outer) != 1:
-        g_out, x, fc1_output, down_input = (t.reshape(rows, t.shape[-1]) for t in (g_out, x, fc1_output, down_input))
-    g_out, x, down_input = _ready(g_out, dtype, rows, w), _ready(x, dtype, rows, d), _ready(down_input, dtype, rows, hd)
-    fc1_output = _ready(fc1_output if hidden == hd else fc1_output.reshape(rows, 2, hidden), dtype, rows, *((2 * hd,) if hidden == hd else (2, hd)))
-    fc1_weight, fc2_weight = _halves(fc1_weight, dtype, hd, d), _ready(fc2_weight, dtype, w, hd)
-    g_x, g_fc1, g_fc2 = x.new_empty(rows, d), x.new_empty(2 * hd, d), x.new_empty(w, hd)
-    g_fc1_bias, g_fc2_bias = (x.new_empty(2 * hd), x.new_empty(w)) if bias else (None, None)
+    g_out, x, fc1_output, down_input = _ready(g_out, dtype), _ready(x, dtype), _ready(fc1_output, dtype), _ready(down_input, dtype)
+    fc1_weight, fc2_weight = _ready(fc1_weight, dtype), _ready(fc2_weight, dtype)
+    g_x, g_fc1, g_fc2 = torch.empty_like(x), x.new_empty(2 * hidden, dim), x.new_empty(width, hidden)
+    g_fc1_bias, g_fc2_bias = (x.new_empty(2 * hidden), x.new_empty(width)) if bias else (None, None)
     lib = _lib.load()
     with _lib.device_guard(x.device):
-        need = int(lib.lbi_gated_mlp_vjp_workspace_bytes(rows, d, hd, w))
+        need = lib.lbi_gated_mlp_vjp_workspace_bytes(rows, dim, hidden, width)
         workspace = torch.empty(need, device=x.device, dtype=torch.uint8)
         status = lib.lbi_gated_mlp_vjp(
             g_out.data_ptr(), x.data_ptr(), fc1_output.data_ptr(), down_input.data_ptr(), fc1_weight.data_ptr(), fc2_weight.data_ptr(),
             g_x.data_ptr(), g_fc1.data_ptr(), g_fc2.data_ptr(), g_fc1_bias.data_ptr() if bias else None,
-            g_fc2_bias.data_ptr() if bias else None, workspace.data_ptr(), need, rows, d, hd, w, _lib.dtype_code(dtype), _stream(x))
+            g_fc2_bias.data_ptr() if bias else None, workspace.data_ptr(), need, rows, dim, hidden, width, _lib.dtype_code(dtype), _stream(x))
     _lib.check(status, "lbi_gated_mlp_vjp")
-    if (dim, hidden, width) != (d, hd, w):
-        g_x, g_fc1, g_fc2 = g_x[:, :dim].contiguous(), g_fc1.view(2, hd, d)[:, :hidden, :dim].reshape(2 * hidden, dim), g_fc2[:width, :hidden].contiguous()
-        if bias:
-            g_fc1_bias, g_fc2_bias = g_fc1_bias.view(2, hd)[:, :hidden].reshape(2 * hidden), g_fc2_bias[:width].contiguous()
-    grads = (g_x if len(outer) == 1 else g_x.view(*outer, dim), g_fc1, g_fc2)
-    return (*grads, g_fc1_bias, g_fc2_bias) if bias else grads
+    return (g_x, g_fc1, g_fc2, g_fc1_bias, g_fc2_bias) if bias else (g_x, g_fc1, g_fc2)
 
 
 __all__ = ["gated_mlp", "gated_mlp_vjp", "residual_rmsnorm", "residual_rmsnorm_pullback"]

@@ -65,10 +65,9 @@ def test_mlp_statuses():
 
     assert forward(rows=0) == (0, b"") and pullback(rows=0)[0] == -2
     for call in (forward, pullback):
-        for bad in (dict(rows=-1), dict(dim=-8), dict(hidden=-8), dict(width=-8)):
+        for bad in (dict(rows=-1), dict(dim=-8), dict(hidden=-8), dict(width=-8), dict(dim=0), dict(hidden=0), dict(width=0)):
             assert call(**bad)[0] == -1 and b"bad size" in call(**bad)[1], bad
-        for bad in (dict(dtype=F32), dict(dtype=7), dict(dim=60), dict(hidden=60), dict(width=60), dict(dim=0), dict(hidden=0), dict(width=0),
-                    dict(dim=(1 << 20) + 8), dict(rows=(1 << 23) + 1)):
+        for bad in (dict(dtype=F32), dict(dtype=7), dict(dim=(1 << 20) + 8), dict(rows=(1 << 23) + 1)):
             assert call(**bad)[0] == -2, bad
     for name in ("x", "w1", "w2", "a", "out"):
         assert forward(**{name: None})[0] == -1 and b"null" in forward(**{name: None})[1]
@@ -85,7 +84,9 @@ def test_mlp_statuses():
     assert need > 0
     big = dict(rows=64, dim=256, hidden=8192, width=256)
     assert forward(**big, size=need - 1)[0] == -4 and forward(**big, ws=None)[0] == -4
-    for sizes in ((0, 64, 64, 64), (16, 60, 64, 64), (-1, 64, 64, 64)):
+    # widths that are padded: the copies too
+    assert lib.lbi_gated_mlp_workspace_bytes(16, 63, 64, 64) >= 2 * (16 * 64 + 128 * 64) and forward(dim=63, ws=None)[0] == -4
+    for sizes in ((0, 64, 64, 64), (16, 0, 64, 64), (-1, 64, 64, 64)):
         assert lib.lbi_gated_mlp_workspace_bytes(*sizes) == 0 and lib.lbi_gated_mlp_vjp_workspace_bytes(*sizes) == 0
 
 
