@@ -28,11 +28,7 @@ using attn_mfma::tile_off;
 using attn_mfma::u32x2;
 using attn_mfma::u32x4;
 
-constexpr int STEP = 64, NT = 256;
-// Steps of a tile's ring, what LDS holds for the workgroups that share a CU: one of 256 x 256, two of the others.  Small tiles multiply little in
-// a step: the fragments of a whole step are read while the last one's are multiplied (77 x 2048 x 5632 in tiles of 64 x 128, 88 steps: 36 us
-// with two steps in the ring, 27 with three, no less with four or six; reading by quarters 41 whatever the ring.  128 x 128: no difference).
-template <int FM, int FN> constexpr int RING = FM == 1 ? 3 : 2;
+constexpr int STEP = 64, NT = 256;  // terms of a step, threads
 constexpr unsigned PAST_END = 1u << 31;  // no operand's step reaches this far
 constexpr int PIECE = 1024;  // bytes that a wave's load brings: 8 rows of 64 terms, or 8 terms of 64 columns
 
@@ -116,9 +112,9 @@ __device__ __forceinline__ void finish(const Task& task, long long row, long lon
     }
 }
 
-template <typename F, int... I> __device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) { (f(Count<I>{}), ...); }
+template <typename F, int... I> __host__ __device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) { (f(Count<I>{}), ...); }
 // f(Count<0>{}), ... f(Count<N - 1>{})
-template <int N, typename F> __device__ __forceinline__ void each(F&& f) { each(f, std::make_integer_sequence<int, N>{}); }
+template <int N, typename F> __host__ __device__ __forceinline__ void each(F&& f) { each(f, std::make_integer_sequence<int, N>{}); }
 
 // 1 KiB from memory to LDS by one wave: lane l brings the 16 bytes at `off` of what `words` describe, zeros past its end.
 template <int AT> __device__ __forceinline__ void bring(const u32x4& words, unsigned off, unsigned lds) {
@@ -162,10 +158,10 @@ template <int FM, int FN> __device__ __forceinline__ size_t partial_at(int item,
     return ((size_t)(item * 4 + wave) * FM + i) * (32 * 32 * FN);
 }
 
-template <typename T, int FM, int FN, bool A_ROWS, bool B_ROWS, Finish FINISH>  // ..._ROWS: the terms are the operand's rows
+template <typename T, int FM, int FN, int DEEP, bool A_ROWS, bool B_ROWS, Finish FINISH>  // ..._ROWS: the terms are the operand's rows
 __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     constexpr int BM = 64 * FM, BN = 64 * FN;  // rows and columns of B's tile
-    constexpr int DEEP = RING<FM, FN>, A_BYTES = BM * 128, SLOT = A_BYTES + BN * 128, READS = FM + FN, LOADS = 2 * READS;
+    constexpr int A_BYTES = BM * 128, SLOT = A_BYTES + BN * 128, READS = FM + FN, LOADS = 2 * READS;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 31, h = lane >> 5, wm = wave >> 1, wn = wave & 1;
@@ -259,7 +255,9 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
         const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + hi_at)));
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
-    constexpr bool AHEAD = FM == 1;  // the fragments of a whole step are read while the last one's are multiplied
+    // Small tiles multiply little in a step: the fragments of a whole one are read while the last one's are multiplied (77 x 2048 x 5632 in tiles of
+    // 64 x 128: 36 us by quarters, 27 by steps).
+    constexpr bool AHEAD = FM == 1;
     constexpr int SETS = AHEAD ? 8 : 2;
     u32x4 af[SETS][FM], bf[SETS][FN];
     // The reads of a quarter of a step, in the order in which the products need them: A's first fragment, B's, A's others.
@@ -334,29 +332,41 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
             if (!more) break;
         }
     } else {
-        static_assert(AHEAD || DEEP == 2, "two steps a turn");
         each<READS>([&](auto u) __attribute__((always_inline)) { read(Count<0>{}, Count<0>{}, Count<0>{}, u); });
         auto step = [&](auto s, int it) __attribute__((always_inline)) {
-            constexpr int S = decltype(s)::value, NEXT = 1 - S;
+            constexpr int S = decltype(s)::value, NEXT = (S + 1) % DEEP, BEFORE = (S + DEEP - 1) % DEEP;
             // A step's place is free for the one a ring later from the barrier on.  Half of its loads go beside the quarter behind it, half
             // beside the quarter after that: all at once they queue up and hold up the products (tiles of 256 x 256, 6007 x 4096 x 11008:
             // 525 -> 486 us).
             multiply(Count<0>{}, [&](auto u) __attribute__((always_inline)) {
                 read(Count<1>{}, Count<1>{}, s, u);
-                fetch(Count<NEXT>{}, Count<READS + decltype(u)::value>{});
+                fetch(Count<BEFORE>{}, Count<READS + decltype(u)::value>{});
             });
             multiply(Count<1>{}, [&](auto u) __attribute__((always_inline)) { read(Count<0>{}, Count<2>{}, s, u); });
             multiply(Count<0>{}, [&](auto u) __attribute__((always_inline)) { read(Count<1>{}, Count<3>{}, s, u); });
             meet();
-            aim(it + 2);
+            aim(it + DEEP);
             multiply(Count<1>{}, [&](auto u) __attribute__((always_inline)) {
                 read(Count<0>{}, Count<0>{}, Count<NEXT>{}, u);
                 fetch(s, u);
             });
         };
-        for (int it = first; it < last; it += 2) {  // behind the last of an odd number of steps comes one of zeros
-            step(Count<0>{}, it);
-            step(Count<1>{}, it + 1);
+        if constexpr (DEEP == 2) {
+            for (int it = first; it < last; it += 2) {  // behind the last of an odd number of steps comes one of zeros
+                step(Count<0>{}, it);
+                step(Count<1>{}, it + 1);
+            }
+        } else {
+            for (int it = first;;) {
+                bool more = true;
+                each<DEEP>([&](auto n) __attribute__((always_inline)) {
+                    if (more) {
+                        step(n, it);
+                        more = ++it < last;
+                    }
+                });
+                if (!more) break;
+            }
         }
     }
     // Nothing is under way into LDS any more, and behind the barrier nothing is read from it: from here on each wave has a part of its own, in
@@ -502,15 +512,18 @@ template <typename T, Finish FINISH> int launch_few(const Task& task, hipStream_
 }
 
 // How a product is laid out: the tile, and into how many parts the sums of those tiles are cut that do not fill the chip once more.
-constexpr int NONE = -1, FEW_ROWS = 5, FORMS = 5;
-// A tile's fragments, how many workgroups share a CU, and what it takes there, in us (see layout_of).
+constexpr int NONE = -1, FORMS = 7, FEW_ROWS = FORMS;
+// A tile's fragments, the steps of its ring, how many workgroups of it LDS lets share a CU, and what it takes there, in us (see layout_of).  Where
+// there is one workgroup a CU a ring of three is the better one (8192 x 768 x 4096 in tiles of 128 x 192: 64 -> 51 us).
 struct Form {
-    int fm, fn, a_cu;
+    int fm, fn, deep, a_cu;
     double step[3], alone[3], start;
 };
-constexpr Form forms[FORMS] = {{4, 4, 1, {1.45, 1.37, 1.46}, {1.00, 1.20, 1.69}, 4.1}, {3, 2, 2, {1.08, 1.11, 1.12}, {0.55, 0.79, 0.70}, 1.3},
-                               {2, 3, 2, {1.05, 1.20, 1.12}, {0.57, 0.79, 0.72}, 1.4}, {2, 2, 2, {0.79, 0.82, 0.91}, {0.50, 0.56, 0.63}, 1.5},
-                               {1, 2, 2, {0.51, 0.58, 0.65}, {0.30, 0.30, 0.37}, 2.0}};
+constexpr Form forms[FORMS] = {
+    {4, 4, 2, 1, {1.40, 1.29, 1.42}, {1.00, 1.12, 1.64}, 3.5}, {3, 2, 2, 2, {1.10, 1.02, 1.13}, {0.48, 0.52, 0.64}, 0.9},
+    {3, 2, 3, 1, {0.58, 0.63, 0.55}, {0.43, 0.51, 0.58}, 2.5}, {2, 3, 3, 1, {0.57, 0.67, 0.55}, {0.43, 0.50, 0.57}, 2.8},
+    {2, 2, 2, 2, {0.77, 0.84, 0.85}, {0.48, 0.48, 0.60}, 1.4}, {2, 2, 3, 1, {0.40, 0.41, 0.36}, {0.40, 0.39, 0.43}, 2.2},
+    {1, 2, 3, 2, {0.53, 0.54, 0.47}, {0.31, 0.26, 0.31}, 2.3}};
 struct Layout {
     int form;
     int m_tiles, n_tiles, whole, parts, part_steps;
@@ -522,9 +535,8 @@ struct Layout {
 
 // By what a call takes, in us: for each round of workgroups over the chip its steps, its start and the results on their way out (20 GB/s a CU, since
 // all finish together); for parts a second launch and their sums out and back.  The constants are fitted to 340 products of 58 blocks (1 ... 16384
-// rows, widths 128 ... 11008), each in up to 45 layouts: what is chosen took 1.007 times the best on average, 1.15 at most.  A step of 256 x 256
-// takes 1.45 us where it fills the chip, 1 where it does not; of 192 x 128 two on a CU 1.1, one 0.55 ... 0.8; of 128 x 128 0.8 ... 0.9 and 0.5 ... 0.6;
-// of 64 x 128 0.5 ... 0.65 and 0.3.  More with operands by rows, whose reads are twice as many.
+// rows, widths 128 ... 11008), each in up to 70 layouts: what is chosen took 1.007 times the best on average, 1.14 at most.  A step of 256 x 256
+// takes 1.4 us where it fills the chip, 1 where it does not; of 192 x 128 two on a CU 1.1, one 0.6; of 128 x 128 0.8 and 0.4; of 64 x 128 0.5 and 0.3.
 Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
     const int cus = device_compute_units(), steps = (int)((K + STEP - 1) / STEP);
     Layout best{NONE, 0, 0, 0, 1, 0, 0.0};
@@ -536,7 +548,7 @@ Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
         const int64_t m_tiles = (M + rows - 1) / rows, n_tiles = (N + columns - 1) / columns, tiles = m_tiles * n_tiles;
         if (tiles >= 1 << 24) continue;
         const double full = form.step[by_rows], alone = form.alone[by_rows];
-        const double fixed = form.start + (finish == GATED ? 4.4 : finish == UNGATED ? 2.6 : 1.9) * rows * columns * form.a_cu / 20e3;
+        const double fixed = form.start + (finish == GATED ? 4.9 : finish == UNGATED ? 3.4 : 2.1) * rows * columns * form.a_cu / 20e3;
         const auto rounds = [&](int64_t items, int of) {
             const int deep = (int)((items % slots + cus - 1) / cus);  // workgroups that share a CU in the last round
             return (double)(items / slots) * (of * full + fixed) + (deep ? of * (deep == 1 ? alone : full) + fixed : 0.0);
@@ -547,16 +559,16 @@ Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
             const int64_t whole = s == 1 ? tiles : tiles / slots * slots, rest = tiles - whole;
             if (s > 1 && (rest == 0 || part_steps < 2 || rest * s > 2 * slots)) break;  // parts for two rounds at most
             double us = rounds(whole, steps);
-            if (rest) us += rounds(rest * s, part_steps) + 4.8 + (double)rest * s * rows * columns * 8.0 / 6.4e6;
+            if (rest) us += rounds(rest * s, part_steps) + 3.5 + (double)rest * s * rows * columns * 8.0 / 5.6e6;
             if (best.form == NONE || us < best.us) best = {f, (int)m_tiles, (int)n_tiles, (int)whole, s, part_steps, us};
         }
     }
     return best;
 }
 
-template <typename T, int FM, int FN, bool A_ROWS, bool B_ROWS, Finish FINISH> int launch_tile(const Task& task, hipStream_t stream) {
-    constexpr auto kernel = product_kernel<T, FM, FN, A_ROWS, B_ROWS, FINISH>;
-    constexpr size_t bytes = (size_t)RING<FM, FN> * 8192 * (FM + FN);
+template <typename T, int FM, int FN, int DEEP, bool A_ROWS, bool B_ROWS, Finish FINISH> int launch_tile(const Task& task, hipStream_t stream) {
+    constexpr auto kernel = product_kernel<T, FM, FN, DEEP, A_ROWS, B_ROWS, FINISH>;
+    constexpr size_t bytes = (size_t)DEEP * 8192 * (FM + FN);
     static_assert(bytes >= 4 * 32 * (32 * FN + 4) * sizeof(float), "the turn of the results fits the ring");
     if (int status = ensure_dynamic_lds<kernel>(bytes)) return status;
     const int rest = task.m_tiles * task.n_tiles - task.whole;
@@ -577,12 +589,13 @@ int launch(const Layout& l, const void* a, const void* b, const void* bias, void
     const Task task{a, b, bias, out, z, M, N, K, static_cast<float*>(partial), l.m_tiles, l.n_tiles, l.whole, l.parts, l.part_steps};
     if constexpr (!A_ROWS && !B_ROWS)
         if (l.form == FEW_ROWS) return launch_few<T, FINISH>(task, stream);
-    if (l.form == 0) return launch_tile<T, 4, 4, A_ROWS, B_ROWS, FINISH>(task, stream);
-    if (l.form == 1) return launch_tile<T, 3, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
-    if constexpr (FINISH != GATED)
-        if (l.form == 2) return launch_tile<T, 2, 3, A_ROWS, B_ROWS, FINISH>(task, stream);
-    if (l.form == 3) return launch_tile<T, 2, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
-    return launch_tile<T, 1, 2, A_ROWS, B_ROWS, FINISH>(task, stream);
+    int status = LBI_OK;
+    each<FORMS>([&](auto f) {
+        constexpr Form form = forms[decltype(f)::value];
+        if constexpr (FINISH != GATED || form.fn % 2 == 0)
+            if (l.form == decltype(f)::value) status = launch_tile<T, form.fm, form.fn, form.deep, A_ROWS, B_ROWS, FINISH>(task, stream);
+    });
+    return status;
 }
 
 // Sums over the rows of x [rows, N]: the gradient of a bias.  A workgroup takes 64 columns, eight to a thread's load, and a slab of rows;
