@@ -520,10 +520,10 @@ struct Form {
     double step[3], alone[3], start;
 };
 constexpr Form forms[FORMS] = {
-    {4, 4, 2, 1, {1.40, 1.29, 1.42}, {1.00, 1.12, 1.64}, 3.5}, {3, 2, 2, 2, {1.10, 1.02, 1.13}, {0.48, 0.52, 0.64}, 0.9},
-    {3, 2, 3, 1, {0.58, 0.63, 0.55}, {0.43, 0.51, 0.58}, 2.5}, {2, 3, 3, 1, {0.57, 0.67, 0.55}, {0.43, 0.50, 0.57}, 2.8},
-    {2, 2, 2, 2, {0.77, 0.84, 0.85}, {0.48, 0.48, 0.60}, 1.4}, {2, 2, 3, 1, {0.40, 0.41, 0.36}, {0.40, 0.39, 0.43}, 2.2},
-    {1, 2, 3, 2, {0.53, 0.54, 0.47}, {0.31, 0.26, 0.31}, 2.3}};
+    {4, 4, 2, 1, {1.33, 1.33, 1.56}, {1.32, 1.28, 1.82}, 2.8}, {3, 2, 2, 2, {1.10, 1.11, 1.11}, {0.59, 0.64, 0.62}, 1.9},
+    {3, 2, 3, 1, {0.60, 0.64, 0.57}, {0.49, 0.54, 0.51}, 2.2}, {2, 3, 3, 1, {0.60, 0.69, 0.64}, {0.52, 0.54, 0.57}, 2.2},
+    {2, 2, 2, 2, {0.86, 0.89, 0.93}, {0.49, 0.48, 0.62}, 2.0}, {2, 2, 3, 1, {0.48, 0.44, 0.39}, {0.42, 0.36, 0.47}, 2.2},
+    {1, 2, 3, 2, {0.55, 0.59, 0.54}, {0.31, 0.27, 0.32}, 2.8}};
 struct Layout {
     int form;
     int m_tiles, n_tiles, whole, parts, part_steps;
@@ -533,11 +533,13 @@ struct Layout {
     }
 };
 
-// By what a call takes, in us: for each round of workgroups over the chip its steps, its start and the results on their way out (20 GB/s a CU, since
-// all finish together); for parts a second launch and their sums out and back.  The constants are fitted to 340 products of 58 blocks (1 ... 16384
-// rows, widths 128 ... 11008), each in up to 70 layouts: what is chosen took 1.007 times the best on average, 1.14 at most.  A step of 256 x 256
-// takes 1.4 us where it fills the chip, 1 where it does not; of 192 x 128 two on a CU 1.1, one 0.6; of 128 x 128 0.8 and 0.4; of 64 x 128 0.5 and 0.3.
+// By what a call takes, in us: for each round of workgroups over the chip its steps, its start and the results on their way out (20 GB/s a CU, all
+// finishing together; less of it shows where two share a CU); for parts a second launch and their sums out and back.  The constants are fitted to
+// 430 products of 73 blocks (1 ... 16384 rows, widths 128 ... 11264), each in up to 60 layouts: what is chosen took 1.007 times the best on
+// average, 1.19 at most.  A step of 256 x 256 takes 1.3 ... 1.6 us; of 192 x 128 two on a CU 1.1, one 0.6; of 128 x 128 0.9 and 0.4 ... 0.5; of
+// 64 x 128 0.55 and 0.3.
 Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
+    constexpr double out[3][2] = {{2.2, 1.7}, {4.4, 3.5}, {5.6, 2.6}};  // bytes of a result that show
     const int cus = device_compute_units(), steps = (int)((K + STEP - 1) / STEP);
     Layout best{NONE, 0, 0, 0, 1, 0, 0.0};
     if (by_rows == 0 && M <= FEW && (M <= 2 || N * K <= FEW_TERMS)) return {FEW_ROWS, 0, 0, 0, 1, 0, 0.0};
@@ -548,7 +550,7 @@ Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
         const int64_t m_tiles = (M + rows - 1) / rows, n_tiles = (N + columns - 1) / columns, tiles = m_tiles * n_tiles;
         if (tiles >= 1 << 24) continue;
         const double full = form.step[by_rows], alone = form.alone[by_rows];
-        const double fixed = form.start + (finish == GATED ? 4.9 : finish == UNGATED ? 3.4 : 2.1) * rows * columns * form.a_cu / 20e3;
+        const double fixed = form.start + out[finish][form.a_cu - 1] * rows * columns * form.a_cu / 20e3;
         const auto rounds = [&](int64_t items, int of) {
             const int deep = (int)((items % slots + cus - 1) / cus);  // workgroups that share a CU in the last round
             return (double)(items / slots) * (of * full + fixed) + (deep ? of * (deep == 1 ? alone : full) + fixed : 0.0);
@@ -559,7 +561,7 @@ Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
             const int64_t whole = s == 1 ? tiles : tiles / slots * slots, rest = tiles - whole;
             if (s > 1 && (rest == 0 || part_steps < 2 || rest * s > 2 * slots)) break;  // parts for two rounds at most
             double us = rounds(whole, steps);
-            if (rest) us += rounds(rest * s, part_steps) + 3.5 + (double)rest * s * rows * columns * 8.0 / 5.6e6;
+            if (rest) us += rounds(rest * s, part_steps) + 4.2 + (double)rest * s * rows * columns * 8.0 / 6.5e6;
             if (best.form == NONE || us < best.us) best = {f, (int)m_tiles, (int)n_tiles, (int)whole, s, part_steps, us};
         }
     }
