@@ -60,11 +60,11 @@ __device__ __forceinline__ Eight operator+(const Eight& a, const Eight& b) {
     for (int e = 0; e < 8; ++e) r.v[e] = a.v[e] + b.v[e];
     return r;
 }
-template <typename T> __device__ __forceinline__ Eight load8(const T* p) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+template <typename T> __device__ __forceinline__ Eight wide8(const u32x4& w) {
     return Eight{{Mma<T>::lo(w[0]), Mma<T>::hi(w[0]), Mma<T>::lo(w[1]), Mma<T>::hi(w[1]), Mma<T>::lo(w[2]), Mma<T>::hi(w[2]),
                   Mma<T>::lo(w[3]), Mma<T>::hi(w[3])}};
 }
+template <typename T> __device__ __forceinline__ Eight load8(const T* p) { return wide8<T>(*reinterpret_cast<const u32x4*>(p)); }
 template <typename T> __device__ __forceinline__ void store8(T* p, const Eight& x) {
     *reinterpret_cast<u32x4*>(p) = u32x4{Mma<T>::pack2(x.v[0], x.v[1]), Mma<T>::pack2(x.v[2], x.v[3]), Mma<T>::pack2(x.v[4], x.v[5]),
                                          Mma<T>::pack2(x.v[6], x.v[7])};
@@ -78,34 +78,49 @@ __device__ __forceinline__ Eight load8(const float* p) {
     return Eight{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
 }
 
+// What finishing eight columns of one row reads beside their sums, as stored: the bias (GATED: up's and gate's; zero where there is none) or
+// UNGATED up and gate.  Read ahead, and in no branch: at the end of one the compiler would wait for it, one eight after the other.
+struct Beside { u32x4 a, b; };
+template <typename T, Finish FINISH> __device__ __forceinline__ Beside beside(const Task& task, long long row, long long col) {
+    const long long N = task.N;
+    Beside r{};
+    if (col >= N) col = 0;
+    if constexpr (FINISH == UNGATED) {
+        const T* z = static_cast<const T*>(task.z) + (row < task.M ? row : 0) * 2 * N + col;
+        r.a = *reinterpret_cast<const u32x4*>(z);
+        r.b = *reinterpret_cast<const u32x4*>(z + N);
+    } else if (const T* bias = static_cast<const T*>(task.bias)) {
+        r.a = *reinterpret_cast<const u32x4*>(bias + col);
+        if constexpr (FINISH == GATED) r.b = *reinterpret_cast<const u32x4*>(bias + N + col);
+    }
+    return r;
+}
 // Eight columns of one row of the result, from their sums (GATED: up's and gate's).
 template <typename T, Finish FINISH>
-__device__ __forceinline__ void finish(const Task& task, long long row, long long col, const Eight& x, const Eight& y) {
+__device__ __forceinline__ void finish(const Task& task, long long row, long long col, const Eight& x, const Eight& y, const Beside& more) {
     const long long N = task.N;
     if (row >= task.M || col >= N) return;
-    const T* bias = static_cast<const T*>(task.bias);
     T* out = static_cast<T*>(task.out);
-    T* z = static_cast<T*>(task.z);
+    const Eight a = wide8<T>(more.a), b = wide8<T>(more.b);
     if constexpr (FINISH == PLAIN) {
-        store8(out + row * N + col, bias ? x + load8(bias + col) : x);
+        store8(out + row * N + col, x + a);
     } else if constexpr (FINISH == GATED) {
-        const Eight up = bias ? x + load8(bias + col) : x, gate = bias ? y + load8(bias + N + col) : y;
+        const Eight up = x + a, gate = y + b;
         Eight act;
 #pragma unroll
         for (int e = 0; e < 8; ++e) act.v[e] = up.v[e] * (gate.v[e] * sigmoid(gate.v[e]));
         store8(out + row * N + col, act);
-        if (z) {
+        if (T* z = static_cast<T*>(task.z)) {
             store8(z + row * 2 * N + col, up);
             store8(z + row * 2 * N + N + col, gate);
         }
     } else {
-        const Eight up = load8(z + row * 2 * N + col), gate = load8(z + row * 2 * N + N + col);
         Eight g_up, g_gate;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float open = sigmoid(gate.v[e]);
-            g_up.v[e] = x.v[e] * (gate.v[e] * open);
-            g_gate.v[e] = x.v[e] * up.v[e] * (open * (1.0f + gate.v[e] * (1.0f - open)));
+            const float open = sigmoid(b.v[e]);
+            g_up.v[e] = x.v[e] * (b.v[e] * open);
+            g_gate.v[e] = x.v[e] * a.v[e] * (open * (1.0f + b.v[e] * (1.0f - open)));
         }
         store8(out + row * 2 * N + col, g_up);
         store8(out + row * 2 * N + N + col, g_gate);
@@ -374,24 +389,32 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     __builtin_amdgcn_s_waitcnt(attn_mfma::waitcnt_vm(0));
     asm volatile("s_barrier" ::: "memory");
     constexpr int ROW = 32 * FN + 4;  // floats
+    constexpr int WIDTH = (FINISH == GATED ? 16 : 32) * FN, EIGHTS = WIDTH / 8, TURNS = 32 * EIGHTS / 64;
     float* turn = reinterpret_cast<float*>(lds) + wave * 32 * ROW;
+    const auto row_of = [&](int i, int u) { return row0 + 32 * FM * wm + 32 * i + (64 * u + lane) / EIGHTS; };
+    const auto col_of = [&](int u) { return col0 + WIDTH * wn + (64 * u + lane) % EIGHTS * 8; };
+    Beside more[2][TURNS];
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) more[0][u] = beside<T, FINISH>(task, row_of(0, u), col_of(u));
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
+        if (FINISH == UNGATED && i + 1 < FM)
+#pragma unroll
+            for (int u = 0; u < TURNS; ++u) more[(i + 1) & 1][u] = beside<T, FINISH>(task, row_of(i + 1, u), col_of(u));
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int g = 0; g < 4; ++g)  // lane (m, h): columns 8 g + 4 h ... + 3 of row m
                 *reinterpret_cast<f32x4*>(turn + m * ROW + 32 * j + 8 * g + 4 * h) =
                     f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        constexpr int WIDTH = (FINISH == GATED ? 16 : 32) * FN, EIGHTS = WIDTH / 8;
 #pragma unroll
-        for (int u = 0; u < 32 * EIGHTS / 64; ++u) {
+        for (int u = 0; u < TURNS; ++u) {
             const int eight = 64 * u + lane, r = eight / EIGHTS, c = eight % EIGHTS * 8;
             const Eight x = load8(turn + r * ROW + c);
-            Eight y;
+            Eight y{};
             if constexpr (FINISH == GATED) y = load8(turn + r * ROW + WIDTH + c);
             if (item < 0) {
-                finish<T, FINISH>(task, row0 + 32 * FM * wm + 32 * i + r, col0 + WIDTH * wn + c, x, y);
+                finish<T, FINISH>(task, row_of(i, u), col_of(u), x, y, more[FINISH == UNGATED ? i & 1 : 0][u]);
             } else {
                 float* to = task.partial + partial_at<FM, FN>(item, wave, i) + eight * 8;
                 store8(to, x);
@@ -412,6 +435,7 @@ template <typename T, int FM, int FN, Finish FINISH> __global__ __launch_bounds_
     const long long row = (long long)mt * 64 * FM + 32 * FM * (wave >> 1) + 32 * i + eight / EIGHTS;
     const long long col = (long long)nt * (FINISH == GATED ? 32 : 64) * FN + WIDTH * (wave & 1) + eight % EIGHTS * 8;
     if (row >= task.M || col >= task.N) return;
+    const Beside more = beside<T, FINISH>(task, row, col);
     Eight x{}, y{};
 #pragma unroll 4
     for (int part = 0; part < task.parts; ++part) {
@@ -419,7 +443,7 @@ template <typename T, int FM, int FN, Finish FINISH> __global__ __launch_bounds_
         x = x + load8(from);
         if constexpr (FINISH == GATED) y = y + load8(from + 32 * WIDTH);
     }
-    finish<T, FINISH>(task, row, col, x, y);
+    finish<T, FINISH>(task, row, col, x, y, more);
 }
 
 // Products of a few rows, both operands' terms side by side: a weight comes through once, and what counts is that all of the chip asks for it
