@@ -222,6 +222,68 @@ def test_mlp_vjp(rows, dim, hidden, width, dtype, device):
         assert torch.equal(a, b)
 
 
+#: Sizes that between them take every tile of every product of both directions, on 256 compute units, with sums whole and cut into parts
+MLP_TILES = [(5632, 36, 3902, 154), (179, 2558, 2821, 87), (5886, 164, 2394, 26), (3524, 1682, 19, 340), (5461, 2377, 16, 169),
+             (8245, 31, 151, 520), (1435, 172, 4013, 621), (1, 903, 2069, 34), (1, 1698, 1764, 1105), (1, 2100, 1922, 27), (2615, 21, 17, 2370),
+             (1109, 17, 1982, 16), (8623, 411, 16, 69), (5548, 91, 16, 1411), (6510, 17, 23, 939), (1214, 22, 2444, 18), (8274, 697, 16, 20),
+             (3889, 2182, 17, 18), (6409, 16, 965, 20), (8019, 28, 79, 1607), (6898, 29, 638, 513), (254, 1904, 4009, 653), (5, 1108, 18, 201),
+             (75, 1413, 16, 371), (67, 21, 729, 25), (5, 27, 1141, 18), (7711, 34, 527, 22)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,dim,hidden,width", MLP_TILES)
+def test_mlp_tiles(rows, dim, hidden, width, dtype, device):
+    from latent_bounded_interfaces_amd.hip.transformer.block import gated_mlp, gated_mlp_vjp
+
+    x, fc1, fc2, b1, b2, g_out = _on(device, *_mlp_inputs(rows, dim, hidden, width, dtype, True, seed=2))
+    got = gated_mlp(x, fc1, fc2, b1, b2, keep=True)
+    grads = gated_mlp_vjp(g_out, x, got[1], got[2], fc1, fc2, bias=True)
+    want = (*truth.gated_mlp(x, fc1, fc2, b1, b2, dtype), *truth.gated_mlp_vjp(g_out, x, got[1], got[2], fc1, fc2, dtype))
+    names = ("out", "fc1_output", "down_input", "g_x", "g_fc1_weight", "g_fc2_weight", "g_fc1_bias", "g_fc2_bias")
+    for one, (value, bound), what in zip((*got, *grads), want, names):
+        truth.assert_near(one, (value.cpu(), bound.cpu()), what)
+
+
+def test_mlp_offsets_past_32_bits(device):
+    """More than 2^31 elements of fc1_output.  The cotangent is zero but for the last rows, whose weight gradients are all there is."""
+    from latent_bounded_interfaces_amd.hip.transformer.block import gated_mlp, gated_mlp_vjp
+
+    rows, dim, hidden, few = 131075, 64, 8200, 64
+    x, fc1, fc2, _, _, g_out = _on(device, *_mlp_inputs(rows, dim, hidden, dim, BF16, False))
+    g_out[:-few] = 0
+    got = gated_mlp(x, fc1, fc2, keep=True)
+    for part in (slice(0, few), slice(rows - few, rows)):
+        for one, (value, bound), what in zip(got, truth.gated_mlp(x[part], fc1, fc2, None, None, BF16), ("out", "fc1_output", "down_input")):
+            truth.assert_near(one[part], (value.cpu(), bound.cpu()), what)
+    grads = gated_mlp_vjp(g_out, x, got[1], got[2], fc1, fc2, bias=True)
+    last = [t[-few:] for t in (g_out, x, got[1], got[2])]
+    assert not grads[0][:-few].any()
+    for one, (value, bound), what in zip((grads[0][-few:], *grads[1:]), truth.gated_mlp_vjp(*last, fc1, fc2, BF16), range(5)):
+        truth.assert_near(one, (value.cpu(), bound.cpu()), str(what))
+
+
+@pytest.mark.parametrize("scaled", [False, True])
+def test_norm_offsets_past_32_bits(scaled, device):
+    """More than 2^31 elements: a row's results do not depend on where it lies."""
+    from latent_bounded_interfaces_amd.hip.transformer.block import residual_rmsnorm, residual_rmsnorm_pullback
+
+    rows, dim, few = 131100, 16384, 40
+    gen = torch.Generator().manual_seed(5)
+    some, weight = _randn(gen, few, dim).to(BF16).to(device), (1 + _randn(gen, dim, std=0.1)).to(BF16).to(device)
+    hidden = torch.zeros(rows, dim, device=device, dtype=BF16)
+    hidden[-few:] = some
+    got, want = residual_rmsnorm(hidden, None, weight, EPS, scaled=scaled), residual_rmsnorm(some, None, weight, EPS, scaled=scaled)
+    for a, b in zip(got, want):
+        assert torch.equal(a[-few:].float(), b.float())
+    if not scaled:
+        grad = residual_rmsnorm_pullback(hidden, hidden, weight, EPS, g_residual=hidden)
+        alone = residual_rmsnorm_pullback(some, some, weight, EPS, g_residual=some)
+        assert torch.equal(grad[0][-few:], alone[0]) and not grad[0][:-few].any()
+        value, bound = truth.residual_rmsnorm_pullback(some.cpu(), some.cpu(), weight.cpu(), EPS, some.cpu(), BF16, BF16)[2]
+        chain = rows / 512 + 4 + 8 + 12  # the bound's own slabs, of all rows
+        truth.assert_near(grad[2], (value, bound * ((chain * 2 + 50) / 50)), "g_weight")
+
+
 def test_mlp_gradients_of_the_formula(device):
     """Forward and pullback together against autograd of the formula in 64 bits: what the roundings in between add is bounded by that
     of the three 16-bit tensors on the way, 4 half steps of the largest magnitudes."""

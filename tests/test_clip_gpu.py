@@ -81,6 +81,18 @@ def test_values_that_are_not_finite(device):
             assert int((reference[1] == 0).sum()) == 19
 
 
+def test_more_elements_than_32_bits_count(device):
+    from latent_bounded_interfaces_amd.hip.gradients import clip_gradients
+
+    count = 2 ** 31 + 5
+    grads = [torch.full((count,), 0.5, device=device, dtype=torch.bfloat16), torch.full((3,), 2.0, device=device)]
+    total = (count * 0.25 + 12.0) ** 0.5
+    norm = clip_gradients(grads, total / 4)
+    assert abs(float(norm) - total) <= 2 * 2.0 ** -24 * total
+    # a quarter of 0.5 and 2 exactly, but for the factor's own 1e-6 / norm and its rounding, which bf16 rounds away
+    assert bool((grads[0] == 0.125).all()) and bool(((grads[1] - 0.5).abs() <= 2.0 ** -22).all())
+
+
 def test_layouts(device):
     """Tensors off the vector grid, transposed, strided, expanded; one of them twice."""
     from latent_bounded_interfaces_amd.hip.gradients import clip_gradients
