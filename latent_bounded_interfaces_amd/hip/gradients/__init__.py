@@ -2,7 +2,7 @@
 
 What the reference's training loop does between its backward pass and the optimizer (train/runners.py:378-380,
 ``torch.nn.utils.clip_grad_norm_``): the 2-norm over all gradients, and all of them times ``min(1, max_norm / (norm + 1e-6))``.
-``lbi_clip_gradients`` takes the whole list in two launches per hundred tensors, whatever their sizes and types, and the
+``lbi_clip_gradients`` takes the whole list in two launches per 140 tensors, whatever their sizes and types, and the
 norm stays on the device.
 """
 from __future__ import annotations
