@@ -7,8 +7,10 @@
 // type of `hidden`, or in 8 bits (e4m3) with one scale a row, max|y| / 448.
 //
 // Bound by memory: a row is read once and kept in registers, eight neighbouring elements a lane and piece, by as many lanes (8 ... 1024) as
-// hold it in one or two pieces: few registers a lane leave room for the waves that hide the loads.  Pieces are loaded at any alignment (an element's own is enough); one that runs past the
-// end of its row goes element by element, so every width takes the same kernel.
+// hold it in one or two pieces: few registers a lane leave room for the waves that hide the loads.  Pieces are loaded at any alignment (an
+// element's own is enough); one that runs past the end of its row goes element by element, so every width takes the same kernel.
+// Forward 5003 x 8192 in bf16 with 8-bit output: 55 us, 5.2 TB/s; 8192 x 768 in bf16 with an fp32 stream 13 ... 14 us, 5.3 ... 5.8 TB/s, part of it
+// from the cache, and backwards 20.5 us, 4.9 TB/s, and 4 for the fold of the weight's gradient.  One row: 2.4 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

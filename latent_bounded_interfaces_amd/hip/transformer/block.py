@@ -68,7 +68,7 @@ def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight
         residual = (residual if residual.dtype == stream else residual.to(stream)).contiguous()
     total = torch.empty_like(hidden, dtype=stream)
     normed = torch.empty_like(hidden, dtype=torch.float8_e4m3fn) if scaled else torch.empty_like(hidden)
-    scales = torch.empty(hidden.shape[:-1], device=hidden.device, dtype=torch.float32) if scaled else None
+    scales = hidden.new_empty(hidden.shape[:-1], dtype=torch.float32) if scaled else None
     count, width = hidden.numel(), hidden.shape[-1]
     if count:
         with _lib.device_guard(hidden.device):
@@ -103,14 +103,14 @@ def residual_rmsnorm_pullback(g_normed: torch.Tensor, residual_out: torch.Tensor
     g_stream = torch.empty_like(residual_out)
     g_hidden = g_stream if stream == branch else torch.empty_like(g_normed)
     width = int(g_normed.shape[-1])
-    g_weight = torch.empty(width, device=g_normed.device, dtype=torch.float32)
+    g_weight = g_normed.new_empty(width, dtype=torch.float32)
     if not width:
         return g_hidden, g_stream, g_weight
     rows = g_normed.numel() // width
     lib = _lib.load()
     with _lib.device_guard(g_normed.device):
         need = int(lib.lbi_residual_rmsnorm_pullback_workspace_bytes(rows, width))
-        workspace = torch.empty(max(need, 16), device=g_normed.device, dtype=torch.uint8)
+        workspace = g_normed.new_empty(max(need, 16), dtype=torch.uint8)
         status = lib.lbi_residual_rmsnorm_pullback(
             g_normed.data_ptr(), residual_out.data_ptr(), None if g_residual is None else g_residual.data_ptr(), weight.data_ptr(),
             None if g_hidden is g_stream else g_hidden.data_ptr(), g_stream.data_ptr(), g_weight.data_ptr(), workspace.data_ptr(), need,
@@ -165,7 +165,7 @@ def gated_mlp(x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight: torch.Tenso
         lib = _lib.load()
         with _lib.device_guard(x.device):
             need = lib.lbi_gated_mlp_workspace_bytes(rows, dim, hidden, width)
-            workspace = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
+            workspace = x.new_empty(need, dtype=torch.uint8) if need else None
             status = lib.lbi_gated_mlp(
                 x.data_ptr(), fc1_weight.data_ptr(), None if fc1_bias is None else fc1_bias.data_ptr(), fc2_weight.data_ptr(),
                 None if fc2_bias is None else fc2_bias.data_ptr(), None if fc1_output is None else fc1_output.data_ptr(),
@@ -198,7 +198,7 @@ def gated_mlp_vjp(g_out: torch.Tensor, x: torch.Tensor, fc1_output: torch.Tensor
     lib = _lib.load()
     with _lib.device_guard(x.device):
         need = lib.lbi_gated_mlp_vjp_workspace_bytes(rows, dim, hidden, width)
-        workspace = torch.empty(need, device=x.device, dtype=torch.uint8)
+        workspace = x.new_empty(need, dtype=torch.uint8)
         status = lib.lbi_gated_mlp_vjp(
             g_out.data_ptr(), x.data_ptr(), fc1_output.data_ptr(), down_input.data_ptr(), fc1_weight.data_ptr(), fc2_weight.data_ptr(),
             g_x.data_ptr(), g_fc1.data_ptr(), g_fc2.data_ptr(), g_fc1_bias.data_ptr() if bias else None,
