@@ -89,14 +89,18 @@ def clip_grad_map(grad_map: GradMap, max_norm: float) -> torch.Tensor:
 def assign_clipped_grad_map(model: nn.Module, grad_map: GradMap, max_norm: float) -> torch.Tensor:
     """:func:`assign_grad_map` of the clipped gradients: scaled on their way into ``param.grad``, the map is left as it is.
     Returns the norm, over the trainable parameters' gradients and before clipping."""
-    grads, copies = [], []
+    params, grads = [], []
     for name, p in _trainable(model):
         grad = grad_map.get(name)
-        p.grad = None if grad is None else torch.empty_like(grad, requires_grad=False)
+        p.grad = None  # gone before the clipped ones are allocated
         if grad is not None:
+            params.append(p)
             grads.append(grad.detach())
-            copies.append(p.grad)
-    return clip_gradients(grads, max_norm, out=copies)
+    clipped = [torch.empty_like(grad) for grad in grads]
+    norm = clip_gradients(grads, max_norm, out=clipped)
+    for p, grad in zip(params, clipped):
+        p.grad = grad
+    return norm
 
 
 def store_named_grads(grad_map: GradMap, param_name_map: dict[int, str], params, grads) -> None:

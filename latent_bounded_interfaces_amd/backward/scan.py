@@ -142,6 +142,8 @@ class ScanADEngine:
         # ``param.grad`` gets the gradients clipped to this global norm (the returned map is not clipped), and the diagnostics
         # ``grad_norm``, a scalar tensor on the device; ``None``: the caller clips, as in the reference
         self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        if self.max_grad_norm is not None and not self.max_grad_norm >= 0.0:
+            raise ValueError("max_grad_norm must not be negative")
 
     @classmethod
     def from_config(cls, cfg: Any, *, compute_interface_jacobian_stats: bool = False,

@@ -163,3 +163,16 @@ def test_wrappers_refuse_before_touching_a_device():
     with pytest.raises(ValueError, match="one tensor"):
         clip_gradients([w], 1.0, out=[])
     assert gradient_norm([]).item() == 0.0
+
+
+def test_clipping_that_is_refused_leaves_no_gradients_behind():
+    from latent_bounded_interfaces_amd.backward import ScanADEngine, assign_clipped_grad_map
+
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_grad_norm"):
+            ScanADEngine(max_grad_norm=bad)
+    layer = torch.nn.Linear(3, 2)
+    layer.weight.grad = torch.ones(2, 3)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        assign_clipped_grad_map(layer, {"weight": torch.ones(2, 3), "bias": torch.ones(2)}, 1.0)
+    assert layer.weight.grad is None and layer.bias.grad is None
