@@ -3,7 +3,7 @@
 //   forward    z = x W1^T + b1,  [u | g] = z,  a = u * g * sigmoid(g),  out = a W2^T + b2
 //   pullback   g_a = g_out W2;  g_u = g_a silu(g), g_g = g_a u silu'(g);  g_x = [g_u | g_g] W1;  g_W1 = [g_u | g_g]^T x;  g_W2 = g_out^T a
 //
-// All six products are one kernel: a workgroup of four waves owns a tile of results, 32 FM x 32 FN of them a wave, and takes 64 terms of
+// All six products are one kernel, and the last two one launch: a workgroup of four waves owns a tile of results, 32 FM x 32 FN of them a wave, and takes 64 terms of
 // the sums a step through LDS, in a ring of two or three steps.  Operands arrive by buffer_load ... lds, whole 128-byte lines (what lies past the
 // end of an operand is zero, so ragged sizes take the same loop); one whose terms lie side by side is read in 16-byte pieces, one whose
 // terms are its rows through transposing reads.  The product is formed as C^T: a lane ends up with four neighbouring columns of one row.
@@ -45,11 +45,26 @@ struct Task {
     const void *a, *b, *bias;  // A [M, K] or, by rows, [K, M]; B [N, K] or, by rows, [K, N]; GATED: B [2N, K]
     void *out, *z;             // GATED: z [M, 2N] written if given; UNGATED: z [M, 2N] read, out [M, 2N]
     long long M, N, K;
-    float* partial;
     int m_tiles, n_tiles;
+    struct {  // both operands by rows: a second product over the same K, whose tiles follow those of the first
+        const void *a, *b;
+        void* out;
+        long long M, N;
+        int m_tiles, n_tiles;
+    } second;
+    float* partial;
+    int tiles;              // of both
     int whole;              // tiles that one workgroup each sums up; the others' sums are cut into `parts` ranges of `part_steps` steps
     int parts, part_steps;
 };
+// The product that tile `at` belongs to becomes the task's, and `at` its own tile.
+__device__ __forceinline__ void turn_to(Task& task, int& at) {
+    const int of_first = task.m_tiles * task.n_tiles;
+    if (at < of_first) return;
+    at -= of_first;
+    task.a = task.second.a, task.b = task.second.b, task.out = task.second.out, task.M = task.second.M, task.N = task.second.N;
+    task.m_tiles = task.second.m_tiles, task.n_tiles = task.second.n_tiles;
+}
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
 
@@ -181,18 +196,20 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 31, h = lane >> 5, wm = wave >> 1, wn = wave & 1;
     constexpr int WIDE = FINISH == GATED ? BN / 2 : BN;
-    const long long M = task.M, N = task.N, K = task.K;
+    const long long K = task.K;
     const int steps = (int)((K + STEP - 1) / STEP);
     int at, first = 0, last = steps, item = -1;
     if ((int)blockIdx.x < task.whole) {
         at = place((int)blockIdx.x, task.whole);
     } else {
-        const int rest = task.m_tiles * task.n_tiles - task.whole, p = place((int)blockIdx.x - task.whole, rest * task.parts), part = p / rest;
+        const int rest = task.tiles - task.whole, p = place((int)blockIdx.x - task.whole, rest * task.parts), part = p / rest;
         at = task.whole + p % rest;
         first = part * task.part_steps;
         last = min(first + task.part_steps, steps);
         item = p;
     }
+    if constexpr (A_ROWS && B_ROWS) turn_to(task, at);
+    const long long M = task.M, N = task.N;
     int mt, nt;
     tile_at(at, task.m_tiles, task.n_tiles, mt, nt);
     const long long row0 = (long long)mt * BM, col0 = (long long)nt * WIDE;
@@ -425,13 +442,14 @@ __global__ __launch_bounds__(NT) void product_kernel(Task task) {
 }
 
 // Adds the parts of the tiles whose sums were cut, in order, and finishes them: a thread takes eight columns of a row.
-template <typename T, int FM, int FN, Finish FINISH> __global__ __launch_bounds__(256) void add_parts_kernel(Task task) {
+template <typename T, int FM, int FN, Finish FINISH, bool PAIR> __global__ __launch_bounds__(256) void add_parts_kernel(Task task) {
     constexpr int WIDTH = (FINISH == GATED ? 16 : 32) * FN, EIGHTS = WIDTH / 8, COUNT = 32 * EIGHTS;
-    const int rest = task.m_tiles * task.n_tiles - task.whole;
+    const int rest = task.tiles - task.whole;
     const int id = blockIdx.x * 256 + threadIdx.x, eight = id % COUNT, i = id / COUNT % FM, wave = id / (COUNT * FM) % 4, tile = id / (COUNT * FM * 4);
     if (tile >= rest) return;
-    int mt, nt;
-    tile_at(task.whole + tile, task.m_tiles, task.n_tiles, mt, nt);
+    int at = task.whole + tile, mt, nt;
+    if constexpr (PAIR) turn_to(task, at);
+    tile_at(at, task.m_tiles, task.n_tiles, mt, nt);
     const long long row = (long long)mt * 64 * FM + 32 * FM * (wave >> 1) + 32 * i + eight / EIGHTS;
     const long long col = (long long)nt * (FINISH == GATED ? 32 : 64) * FN + WIDTH * (wave & 1) + eight % EIGHTS * 8;
     if (row >= task.M || col >= task.N) return;
@@ -550,10 +568,10 @@ constexpr Form forms[FORMS] = {
     {1, 2, 3, 2, {0.55, 0.59, 0.54}, {0.31, 0.27, 0.32}, 2.8}};
 struct Layout {
     int form;
-    int m_tiles, n_tiles, whole, parts, part_steps;
+    int tiles, whole, parts, part_steps;
     double us;
     size_t bytes() const {
-        return parts > 1 ? (size_t)(m_tiles * n_tiles - whole) * parts * (64 * forms[form].fm) * (64 * forms[form].fn) * sizeof(float) : 0;
+        return parts > 1 ? (size_t)(tiles - whole) * parts * (64 * forms[form].fm) * (64 * forms[form].fn) * sizeof(float) : 0;
     }
 };
 
@@ -562,16 +580,18 @@ struct Layout {
 // 430 products of 73 blocks (1 ... 16384 rows, widths 128 ... 11264), each in up to 60 layouts: what is chosen took 1.007 times the best on
 // average, 1.19 at most.  A step of 256 x 256 takes 1.3 ... 1.6 us; of 192 x 128 two on a CU 1.1, one 0.6; of 128 x 128 0.9 and 0.4 ... 0.5; of
 // 64 x 128 0.55 and 0.3.
-Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
+// M2, N2: of a second product that is laid out together with the first.
+Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows, int64_t M2 = 0, int64_t N2 = 0) {
     constexpr double out[3][2] = {{2.2, 1.7}, {4.4, 3.5}, {5.6, 2.6}};  // bytes of a result that show
     const int cus = device_compute_units(), steps = (int)((K + STEP - 1) / STEP);
-    Layout best{NONE, 0, 0, 0, 1, 0, 0.0};
-    if (by_rows == 0 && M <= FEW && (M <= 2 || N * K <= FEW_TERMS)) return {FEW_ROWS, 0, 0, 0, 1, 0, 0.0};
+    Layout best{NONE, 0, 0, 1, 0, 0.0};
+    if (by_rows == 0 && M <= FEW && (M <= 2 || N * K <= FEW_TERMS)) return {FEW_ROWS, 0, 0, 1, 0, 0.0};
     for (int f = 0; f < FORMS; ++f) {
         const Form& form = forms[f];
         if (finish == GATED && form.fn % 2) continue;  // up and gate are half of a wave's columns each
         const int rows = 64 * form.fm, wide = 64 * form.fn, columns = finish == GATED ? wide / 2 : wide, slots = cus * form.a_cu;
-        const int64_t m_tiles = (M + rows - 1) / rows, n_tiles = (N + columns - 1) / columns, tiles = m_tiles * n_tiles;
+        const auto tiles_of = [&](int64_t m, int64_t n) { return (m + rows - 1) / rows * ((n + columns - 1) / columns); };
+        const int64_t tiles = tiles_of(M, N) + tiles_of(M2, N2);
         if (tiles >= 1 << 24) continue;
         const double full = form.step[by_rows], alone = form.alone[by_rows];
         const double fixed = form.start + out[finish][form.a_cu - 1] * rows * columns * form.a_cu / 20e3;
@@ -586,33 +606,35 @@ Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows) {
             if (s > 1 && (rest == 0 || part_steps < 2 || rest * s > 2 * slots)) break;  // parts for two rounds at most
             double us = rounds(whole, steps);
             if (rest) us += rounds(rest * s, part_steps) + 4.2 + (double)rest * s * rows * columns * 8.0 / 6.5e6;
-            if (best.form == NONE || us < best.us) best = {f, (int)m_tiles, (int)n_tiles, (int)whole, s, part_steps, us};
+            if (best.form == NONE || us < best.us) best = {f, (int)tiles, (int)whole, s, part_steps, us};
         }
     }
     return best;
 }
 
-template <typename T, int FM, int FN, int DEEP, bool A_ROWS, bool B_ROWS, Finish FINISH> int launch_tile(const Task& task, hipStream_t stream) {
+template <typename T, int FM, int FN, int DEEP, bool A_ROWS, bool B_ROWS, Finish FINISH> int launch_tile(Task task, hipStream_t stream) {
     constexpr auto kernel = product_kernel<T, FM, FN, DEEP, A_ROWS, B_ROWS, FINISH>;
     constexpr size_t bytes = (size_t)DEEP * 8192 * (FM + FN);
     static_assert(bytes >= 4 * 32 * (32 * FN + 4) * sizeof(float), "the turn of the results fits the ring");
     if (int status = ensure_dynamic_lds<kernel>(bytes)) return status;
-    const int rest = task.m_tiles * task.n_tiles - task.whole;
+    constexpr int ROWS = 64 * FM, WIDE = FINISH == GATED ? 32 * FN : 64 * FN;
+    task.m_tiles = (int)((task.M + ROWS - 1) / ROWS), task.n_tiles = (int)((task.N + WIDE - 1) / WIDE);
+    task.second.m_tiles = (int)((task.second.M + ROWS - 1) / ROWS), task.second.n_tiles = (int)((task.second.N + WIDE - 1) / WIDE);
+    const int rest = task.tiles - task.whole;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(task.whole + rest * task.parts)), dim3(NT), bytes, stream, task);
     if (rest) {
         const int eights = rest * 4 * FM * 32 * (FINISH == GATED ? 2 : 4) * FN;
-        hipLaunchKernelGGL((add_parts_kernel<T, FM, FN, FINISH>), dim3((unsigned)((eights + 255) / 256)), dim3(256), 0, stream, task);
+        hipLaunchKernelGGL((add_parts_kernel<T, FM, FN, FINISH, A_ROWS && B_ROWS>), dim3((unsigned)((eights + 255) / 256)), dim3(256), 0, stream, task);
     }
     LBI_HIP_CHECK(hipGetLastError());
     return LBI_OK;
 }
 
 // `partial`: l.bytes()
-template <typename T, bool A_ROWS, bool B_ROWS, Finish FINISH>
-int launch(const Layout& l, const void* a, const void* b, const void* bias, void* out, void* z, int64_t M, int64_t N, int64_t K, void* partial,
-           hipStream_t stream) {
+template <typename T, bool A_ROWS, bool B_ROWS, Finish FINISH> int launch(const Layout& l, Task task, void* partial, hipStream_t stream) {
     if (l.form == NONE) return fail(LBI_ERR_UNSUPPORTED, "lbi_gated_mlp: too many tiles");
-    const Task task{a, b, bias, out, z, M, N, K, static_cast<float*>(partial), l.m_tiles, l.n_tiles, l.whole, l.parts, l.part_steps};
+    task.partial = static_cast<float*>(partial);
+    task.tiles = l.tiles, task.whole = l.whole, task.parts = l.parts, task.part_steps = l.part_steps;
     if constexpr (!A_ROWS && !B_ROWS)
         if (l.form == FEW_ROWS) return launch_few<T, FINISH>(task, stream);
     int status = LBI_OK;
@@ -865,7 +887,7 @@ struct ForwardPlan {
 struct PullbackPlan {
     Padding pad;
     Pullback t;
-    Layout a, x, fc1, fc2;
+    Layout a, x, weights;
     size_t g_fc1, sums, partial;
     PullbackPlan(const Pullback& c, void* workspace) : pad{static_cast<char*>(workspace)}, t(c) {
         t.D = Padding::eights(c.D), t.hidden = Padding::eights(c.hidden), t.width = Padding::eights(c.width);
@@ -882,13 +904,12 @@ struct PullbackPlan {
         t.g_fc2_bias = pad.result(c.g_fc2_bias, 1, c.width, 1, t.width);
         a = layout_of(t.rows, t.hidden, t.width, UNGATED, 1);
         x = layout_of(t.rows, t.D, 2 * t.hidden, PLAIN, 1);
-        fc1 = layout_of(2 * t.hidden, t.D, t.rows, PLAIN, 2);
-        fc2 = layout_of(t.width, t.hidden, t.rows, PLAIN, 2);
+        weights = layout_of(2 * t.hidden, t.D, t.rows, PLAIN, 2, t.width, t.hidden);
         g_fc1 = pad.bytes;
         sums = g_fc1 + up((size_t)t.rows * 2 * t.hidden * 2);
         partial = sums + up((size_t)slabs_of(t.rows) * (2 * t.hidden + t.width) * sizeof(float));
     }
-    size_t bytes() const { return partial + up(std::max({a.bytes(), x.bytes(), fc1.bytes(), fc2.bytes()})); }
+    size_t bytes() const { return partial + up(std::max({a.bytes(), x.bytes(), weights.bytes()})); }
 };
 
 // Every tensor given: what a plan that only counts is told.
@@ -925,9 +946,9 @@ extern "C" int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* 
         using T = decltype(type);
         const Forward& t = p.t;
         void* partial = static_cast<char*>(workspace) + p.partial;
-        if (int s = launch<T, false, false, GATED>(p.fc1, t.x, t.fc1_weight, t.fc1_bias, t.down_input, t.fc1_output, rows, t.hidden, t.D, partial, on))
+        if (int s = launch<T, false, false, GATED>(p.fc1, {t.x, t.fc1_weight, t.fc1_bias, t.down_input, t.fc1_output, rows, t.hidden, t.D}, partial, on))
             return s;
-        return launch<T, false, false, PLAIN>(p.fc2, t.down_input, t.fc2_weight, t.fc2_bias, t.out, nullptr, rows, t.width, t.hidden, partial, on);
+        return launch<T, false, false, PLAIN>(p.fc2, {t.down_input, t.fc2_weight, t.fc2_bias, t.out, nullptr, rows, t.width, t.hidden}, partial, on);
     };
     if (int s = Padding::run(p.pad.in, on)) return s;
     if (int s = dtype == LBI_F16 ? run(_Float16{}) : run(bf16_raw{})) return s;
@@ -967,11 +988,13 @@ extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* f
         using T = decltype(type);
         const Pullback& t = p.t;
         void* z = const_cast<void*>(t.fc1_output);
-        if (int s = launch<T, false, true, UNGATED>(p.a, t.g_out, t.fc2_weight, nullptr, g_fc1, z, rows, t.hidden, t.width, partial, on)) return s;
-        if (int s = launch<T, false, true, PLAIN>(p.x, g_fc1, t.fc1_weight, nullptr, t.g_x, nullptr, rows, t.D, 2 * t.hidden, partial, on)) return s;
-        if (int s = launch<T, true, true, PLAIN>(p.fc1, g_fc1, t.x, nullptr, t.g_fc1_weight, nullptr, 2 * t.hidden, t.D, rows, partial, on)) return s;
-        if (int s = launch<T, true, true, PLAIN>(p.fc2, t.g_out, t.down_input, nullptr, t.g_fc2_weight, nullptr, t.width, t.hidden, rows, partial, on))
-            return s;
+        if (int s = launch<T, false, true, UNGATED>(p.a, {t.g_out, t.fc2_weight, nullptr, g_fc1, z, rows, t.hidden, t.width}, partial, on)) return s;
+        if (int s = launch<T, false, true, PLAIN>(p.x, {g_fc1, t.fc1_weight, nullptr, t.g_x, nullptr, rows, t.D, 2 * t.hidden}, partial, on)) return s;
+        // Both weights' gradients are sums over the rows: one list of tiles, with one last round (the whole call for one row of 768 / 2048: 33 -> 29 us, 16000
+        // of 256 / 1024 122 -> 112, 8192 of 768 / 2048 241 -> 230; 6007 of 2560 / 6912, whose products fill the chip alone, 1290 -> 1310).
+        Task weights{g_fc1, t.x, nullptr, t.g_fc1_weight, nullptr, 2 * t.hidden, t.D, rows};
+        weights.second = {t.g_out, t.down_input, t.g_fc2_weight, t.width, t.hidden};
+        if (int s = launch<T, true, true, PLAIN>(p.weights, weights, partial, on)) return s;
         return column_sums<T>({g_fc1, t.g_fc1_bias, sums, 2 * t.hidden, 0}, {t.g_out, t.g_fc2_bias, sums + slabs_of(rows) * 2 * t.hidden, t.width, 0}, rows, on);
     };
     if (int s = Padding::run(p.pad.in, on)) return s;

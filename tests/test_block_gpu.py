@@ -227,7 +227,7 @@ MLP_TILES = [(5632, 36, 3902, 154), (179, 2558, 2821, 87), (5886, 164, 2394, 26)
              (8245, 31, 151, 520), (1435, 172, 4013, 621), (1, 903, 2069, 34), (1, 1698, 1764, 1105), (1, 2100, 1922, 27), (2615, 21, 17, 2370),
              (1109, 17, 1982, 16), (8623, 411, 16, 69), (5548, 91, 16, 1411), (6510, 17, 23, 939), (1214, 22, 2444, 18), (8274, 697, 16, 20),
              (3889, 2182, 17, 18), (6409, 16, 965, 20), (8019, 28, 79, 1607), (6898, 29, 638, 513), (254, 1904, 4009, 653), (5, 1108, 18, 201),
-             (75, 1413, 16, 371), (67, 21, 729, 25), (5, 27, 1141, 18), (7711, 34, 527, 22)]
+             (75, 1413, 16, 371), (67, 21, 729, 25), (5, 27, 1141, 18), (7711, 34, 527, 22), (1, 164, 4011, 962), (78, 825, 3979, 2026)]
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
