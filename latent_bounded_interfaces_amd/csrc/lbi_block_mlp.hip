@@ -3,11 +3,14 @@
 //   forward    z = x W1^T + b1,  [u | g] = z,  a = u * g * sigmoid(g),  out = a W2^T + b2
 //   pullback   g_a = g_out W2;  g_u = g_a silu(g), g_g = g_a u silu'(g);  g_x = [g_u | g_g] W1;  g_W1 = [g_u | g_g]^T x;  g_W2 = g_out^T a
 //
-// All six products are one kernel, and the last two one launch: a workgroup of four waves owns a tile of results, 32 FM x 32 FN of them a wave, and takes 64 terms of
-// the sums a step through LDS, in a ring of two or three steps.  Operands arrive by buffer_load ... lds, whole 128-byte lines (what lies past the
-// end of an operand is zero, so ragged sizes take the same loop); one whose terms lie side by side is read in 16-byte pieces, one whose
-// terms are its rows through transposing reads.  The product is formed as C^T: a lane ends up with four neighbouring columns of one row.
-// Up and gate of one column meet in one lane, so the gate costs no pass of its own in either direction.
+// All six products are one kernel, and the last two one launch: a workgroup of four waves owns a tile of results, 32 FM x 32 FN of them a wave, and
+// takes 64 terms of the sums a step through LDS, in a ring of two or three steps.  Operands arrive by buffer_load ... lds, whole 128-byte lines
+// (what lies past the end of an operand is zero, so ragged sizes take the same loop); one whose terms lie side by side is read in 16-byte
+// pieces, one whose terms are its rows through transposing reads.  The product is formed as C^T: a lane ends up with four neighbouring columns
+// of one row.  Up and gate of one column meet in one lane, so the gate costs no pass of its own in either direction.
+//
+// Bound by the matrix units' issue in large calls (6007 rows, 4096 -> 2 x 11008 -> 4096 in bf16: 1.37 ms, 1.19 PFLOP/s), by starts, ends and results on
+// their way out in ordinary ones (8192 rows, 768 -> 2 x 2048 -> 768, fc1_output kept: 98 us, 0.79 PFLOP/s), by the weights' way through the chip in small ones.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -466,7 +469,8 @@ template <typename T, int FM, int FN, Finish FINISH, bool PAIR> __global__ __lau
 
 // Products of a few rows, both operands' terms side by side: a weight comes through once, and what counts is that all of the chip asks for it
 // at once.  KW waves share the sums of COLUMNS columns (GATED: pairs of them) of all rows, each lane 16 bytes of every 512 KW terms; lanes are
-// added by exchange, waves in order.  One token, 768 -> 2 x 2048 -> 768 in bf16: 4.8 and 2.3 us (64 x 128 tiles: 7.5 and 8.6).
+// added by exchange, waves in order.  One token, 768 -> 2 x 2048 -> 768 in bf16: 4.8 and 2.3 us (64 x 128 tiles: 7.5 and 8.6), from
+// memory 5.7 and 3.1.
 constexpr int FEW = 4, COLUMNS = 2;
 constexpr int64_t FEW_TERMS = 4 << 20;  // of a weight, from three rows on
 template <typename T, int ROWS, Finish FINISH, int KW> __global__ __launch_bounds__(256) void few_rows_kernel(Task task) {

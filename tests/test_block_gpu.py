@@ -403,7 +403,7 @@ def test_a_training_step_of_the_half(device):
     want = [out, stream, x.grad, residual.grad, total, *(g / (total + 1e-6) for g in parameters)]
     assert float(total) > 1
     for i, (a, b) in enumerate(zip(got, want)):
-        assert float((a.cpu().double() - b).norm() / b.norm()) <= 6 * 2.0 ** -8, i
+        assert float((a.cpu().double() - b.detach()).norm() / b.detach().norm()) <= 6 * 2.0 ** -8, i
 
 
 def test_captured_step_replays_with_new_inputs(device):
