@@ -53,7 +53,8 @@ def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight
     ``s`` in ``residual_dtype`` (that of ``residual`` by default, of ``hidden`` without one; of ``hidden`` or fp32).  ``scaled``:
     ``(y8, scales, s)`` instead, ``y8`` in ``torch.float8_e4m3fn`` and ``scales [...]`` in fp32, one a row, ``y = y8 * scales``:
     the row's largest magnitude over 448 (1 for a row of zeros).  Sums are fp32 and each result is rounded once: the norm is that of
-    the sum before its rounding to ``residual_dtype``."""
+    the sum before its rounding to ``residual_dtype``, and a ``residual`` of another type than that enters the sum as it is (in fp32, with
+    one more pass that rounds ``s``)."""
     if hidden.dim() < 1 or weight.shape != hidden.shape[-1:]:
         raise ValueError("residual_rmsnorm: hidden must be [..., D] and weight [D]")
     if residual is not None and residual.shape != hidden.shape:
@@ -64,9 +65,10 @@ def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight
     stream = residual_dtype or (branch if residual is None else residual.dtype)
     weight = _norm_types("residual_rmsnorm", branch, stream, weight).contiguous()
     hidden = hidden.contiguous()
+    held = stream if residual is None or residual.dtype == stream else torch.float32  # what the kernel reads and writes
     if residual is not None:
-        residual = (residual if residual.dtype == stream else residual.to(stream)).contiguous()
-    total = torch.empty_like(hidden, dtype=stream)
+        residual = residual.to(held).contiguous()
+    total = torch.empty_like(hidden, dtype=held)
     normed = torch.empty_like(hidden, dtype=torch.float8_e4m3fn) if scaled else torch.empty_like(hidden)
     scales = hidden.new_empty(hidden.shape[:-1], dtype=torch.float32) if scaled else None
     count, width = hidden.numel(), hidden.shape[-1]
@@ -75,10 +77,11 @@ def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight
             status = _lib.load().lbi_residual_rmsnorm(
                 hidden.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), normed.data_ptr(),
                 total.data_ptr(), None if scales is None else scales.data_ptr(), count // width, width, eps,
-                _lib.dtype_code(branch), _lib.dtype_code(stream), _lib.dtype_code(weight.dtype), _stream(hidden))
+                _lib.dtype_code(branch), _lib.dtype_code(held), _lib.dtype_code(weight.dtype), _stream(hidden))
         _lib.check(status, "lbi_residual_rmsnorm")
     elif scales is not None:
         scales.fill_(1.0)
+    total = total.to(stream)
     return (normed, scales, total) if scales is not None else (normed, total)
 
 
