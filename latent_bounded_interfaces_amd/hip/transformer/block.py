@@ -38,11 +38,11 @@ def _one_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) ->
 
 
 def _norm_types(what: str, branch: torch.dtype, stream: torch.dtype, weight: torch.Tensor) -> torch.Tensor:
-    """The weight in a type that the kernels take (the branch's or fp32), after a check of the other types."""
+    """The weight in a type that the kernels take (the branch's, or fp32 for any other), after a check of the other types."""
     _lib.dtype_code(branch)
     if stream not in (branch, torch.float32):
         raise ValueError(f"{what}: the residual stream must be in the dtype of the branch or fp32")
-    return weight if weight.dtype in (branch, torch.float32) else weight.to(branch)
+    return weight if weight.dtype in (branch, torch.float32) else weight.float()
 
 
 def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float, *,

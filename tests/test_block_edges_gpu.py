@@ -43,3 +43,21 @@ def test_norm_of_a_residual_past_the_streams_largest_number(device):
     normed, total = residual_rmsnorm(hidden.to(device), residual.to(device), weight.to(device), EPS, residual_dtype=F16)
     truth.assert_near(normed, truth.residual_rmsnorm(hidden, residual, weight, EPS, F16, F32)[0])
     assert bool(torch.isinf(total[0]).all()) and bool((total[1] == 6).all())
+
+
+@pytest.mark.parametrize("branch,weight_type", [(F16, BF16), (BF16, F16), (BF16, torch.float64), (F16, torch.float64)])
+def test_norm_of_a_weight_in_another_type(branch, weight_type, device):
+    """The weight is not rounded to the branch's type, whose largest number it may exceed."""
+    from latent_bounded_interfaces_amd.hip.transformer.block import residual_rmsnorm, residual_rmsnorm_pullback
+
+    gen = torch.Generator().manual_seed(8)
+    hidden, g = _randn(gen, 9, 130).to(branch), _randn(gen, 9, 130, std=0.1).to(branch)
+    weight = (1 + _randn(gen, 130, std=0.1)).to(F16).to(weight_type)
+    hidden[:, 0] = 2.0 ** -10
+    weight[0] = 60000.0 if weight_type == F16 else 80000.0
+    held = weight.float()  # what the kernels read
+    got = residual_rmsnorm(hidden.to(device), None, weight.to(device), EPS)
+    truth.assert_near(got[0], truth.residual_rmsnorm(hidden, None, held, EPS, branch, branch)[0])
+    got = residual_rmsnorm_pullback(g.to(device), hidden.to(device), weight.to(device), EPS)
+    for one, expected in zip(got, truth.residual_rmsnorm_pullback(g, hidden, held, EPS, None, branch, branch)):
+        truth.assert_near(one, expected)
