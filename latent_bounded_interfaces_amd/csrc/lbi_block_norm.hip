@@ -346,6 +346,7 @@ __global__ __launch_bounds__(COLUMNS * PARTS) void fold_kernel(const float* __re
 }
 
 constexpr int64_t MOST_COLUMNS = 1024 * 2 * PIECE, MOST_ROWS = (int64_t)1 << 31;
+constexpr int64_t MOST_THREADS = ((int64_t)1 << 32) - 1;  // of a launch
 
 // Slabs of the pullback, and the rows of one: four workgroups a CU of narrow rows, two of wide ones, whose shares of the weight's gradient
 // would be as many bytes as a twentieth of the rows themselves.
@@ -415,10 +416,18 @@ extern "C" int lbi_residual_rmsnorm(const void* hidden, const void* residual, co
             constexpr int NT = decltype(form)::NT, PIECES = decltype(form)::PIECES, COUNT = SIDE<NT>;
             const auto kernel = D % PIECE ? (scales ? norm_kernel<T, R, true, true, NT, PIECES> : norm_kernel<T, R, false, true, NT, PIECES>)
                                           : (scales ? norm_kernel<T, R, true, false, NT, PIECES> : norm_kernel<T, R, false, false, NT, PIECES>);
-            hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + COUNT - 1) / COUNT)), dim3((unsigned)(threads_of<NT, PIECES>(D) * COUNT)), 0, static_cast<hipStream_t>(stream),
-                               static_cast<const T*>(hidden), static_cast<const R*>(residual), weight, normed, static_cast<R*>(residual_out),
-                               scales, (long long)rows, (int)D, eps, (int)(weight_dtype == LBI_F32));
-            LBI_HIP_CHECK(hipGetLastError());
+            const int threads = threads_of<NT, PIECES>(D) * COUNT;
+            const int64_t most = (MOST_THREADS / threads) * COUNT;  // rows of a launch
+            for (int64_t first = 0; first < rows; first += most) {
+                const int64_t count = std::min(rows - first, most);
+                const auto from = [&](auto* p) { return p ? p + first * D : p; };
+                void* y = scales ? static_cast<void*>(from(static_cast<unsigned char*>(normed))) : static_cast<void*>(from(static_cast<T*>(normed)));
+                hipLaunchKernelGGL(kernel, dim3((unsigned)((count + COUNT - 1) / COUNT)), dim3((unsigned)threads), 0, static_cast<hipStream_t>(stream),
+                                   from(static_cast<const T*>(hidden)), from(static_cast<const R*>(residual)), weight, y,
+                                   from(static_cast<R*>(residual_out)), scales ? scales + first : nullptr, (long long)count, (int)D, eps,
+                                   (int)(weight_dtype == LBI_F32));
+                LBI_HIP_CHECK(hipGetLastError());
+            }
             return (int)LBI_OK;
         });
     });

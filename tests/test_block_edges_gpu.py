@@ -61,3 +61,20 @@ def test_norm_of_a_weight_in_another_type(branch, weight_type, device):
     got = residual_rmsnorm_pullback(g.to(device), hidden.to(device), weight.to(device), EPS)
     for one, expected in zip(got, truth.residual_rmsnorm_pullback(g, hidden, held, EPS, None, branch, branch)):
         truth.assert_near(one, expected)
+
+
+@pytest.mark.parametrize("scaled", [False, True])
+def test_norm_of_more_rows_than_a_launch_has_threads_for(scaled, device):
+    """Rows of up to 64 columns take eight threads each, and a launch has fewer than 2^32: 2^29 rows go in two.  A few rows again and again,
+    each time with the same results."""
+    from latent_bounded_interfaces_amd.hip.transformer.block import residual_rmsnorm
+
+    few = 97
+    rows = few * ((1 << 29) // few + 40)
+    gen = torch.Generator().manual_seed(11)
+    some, weight = _randn(gen, few, 1, std=0.01).to(BF16).to(device), torch.full((1,), 1.5, device=device, dtype=BF16)
+    want = residual_rmsnorm(some, some, weight, EPS, scaled=scaled)
+    hidden = some.repeat(rows // few, 1)
+    for a, b in zip(residual_rmsnorm(hidden, hidden, weight, EPS, scaled=scaled), want):
+        a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
+        assert bool((a.view(-1, few) == b.view(1, few)).all())
