@@ -67,7 +67,7 @@ def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight
     hidden = hidden.contiguous()
     held = stream if residual is None or residual.dtype == stream else torch.float32  # what the kernel reads and writes
     if residual is not None:
-        residual = residual.to(held).contiguous()
+        residual = (residual if residual.dtype == held else residual.to(held)).contiguous()
     total = torch.empty_like(hidden, dtype=held)
     normed = torch.empty_like(hidden, dtype=torch.float8_e4m3fn) if scaled else torch.empty_like(hidden)
     scales = hidden.new_empty(hidden.shape[:-1], dtype=torch.float32) if scaled else None
@@ -81,7 +81,8 @@ def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight
         _lib.check(status, "lbi_residual_rmsnorm")
     elif scales is not None:
         scales.fill_(1.0)
-    total = total.to(stream)
+    if held is not stream:
+        total = total.to(stream)
     return (normed, scales, total) if scales is not None else (normed, total)
 
 
