@@ -408,13 +408,13 @@ int lbi_matrix_norms(const void* mats, float* spectral, float* frobenius,
  *   hidden, normed [rows,D] in dtype; residual, residual_out [rows,D] in residual_dtype (dtype or fp32); weight [D] in weight_dtype (dtype
  *   or fp32).  residual_out = s, not written if NULL.  With scales [rows] (fp32) normed is e4m3, one byte an element: y divided by the
  *   row's scale max|y| / 448 (1 for a row of zeros, at least 2^-126 otherwise).
- *   residual_out may be residual, and hidden where the types are the same; normed may be hidden.
+ *   normed and residual_out may each be an input of their own type, but not the same one; other overlaps are refused.
  *
  * Pullback, from residual_out:
  *   i = rsqrt(mean(s^2) + eps), u = s i, p = g_normed * weight:   g_s = i (p - u mean(u p)) + g_residual_out (NULL = 0)
  *   g_hidden [rows,D] (dtype) and g_residual [rows,D] (residual_dtype) are both g_s, either may be NULL;
  *   g_weight [D] (fp32) = sum over rows of g_normed * u, in a fixed order.
- *   g_hidden may be g_normed, g_residual may be g_residual_out.
+ *   g_hidden and g_residual may each be an input of their own type and, where that is one type, the same tensor; other overlaps are refused.
  *
  * D up to 16384, fewer than 2^31 rows; tensors aligned to their elements.
  */

@@ -157,11 +157,11 @@ template <bool TAIL, typename T> __device__ __forceinline__ Eight load_weight(co
     return wide ? load8<TAIL>(static_cast<const float*>(weight) + c, left).wide() : load8<TAIL>(static_cast<const T*>(weight) + c, left).wide();
 }
 
-// NT threads a row (beyond 64: up to NT, the workgroup's), PIECES pieces a lane.  TAIL: D is no whole number of pieces.
+// NT threads a row (beyond 64: up to NT, the workgroup's), PIECES pieces a lane.  TAIL: D is no whole number of pieces.  Results may be inputs:
+// all of a row is read before any of it is written.
 template <typename T, typename R, bool SCALED, bool TAIL, int NT, int PIECES>
-__global__ __launch_bounds__(NT * SIDE<NT>) void norm_kernel(const T* __restrict__ hidden, const R* __restrict__ residual,
-                                                             const void* __restrict__ weight, void* __restrict__ normed,
-                                                             R* __restrict__ stream_out, float* __restrict__ scales, long long rows, int D,
+__global__ __launch_bounds__(NT * SIDE<NT>) void norm_kernel(const T* hidden, const R* residual, const void* __restrict__ weight,
+                                                             void* normed, R* stream_out, float* __restrict__ scales, long long rows, int D,
                                                              float eps, int weight_wide) {
     __shared__ float spare[2][NT <= 64 ? 1 : NT / 64];
     const int threads = NT <= 64 ? NT : (int)blockDim.x, t = threadIdx.x % threads;
@@ -232,11 +232,10 @@ __global__ __launch_bounds__(NT * SIDE<NT>) void norm_kernel(const T* __restrict
 
 // A workgroup takes the rows of one slab, NT threads a row, and leaves its share of the weight's gradient in `partials` [slabs, D].  The next
 // row is on its way while one is worked on; its loads stand in no branch, since the compiler waits for every load under way where branches meet
-// (past the end of a row or of the slab they fetch again what is there).  MORE: there is a g_stream.
+// (past the end of a row or of the slab they fetch again what is there, and nothing uses it).  MORE: there is a g_stream.  Results may be inputs here too.
 template <typename T, typename R, bool MORE, bool TAIL, int NT, int PIECES>
-__global__ __launch_bounds__(NT * SIDE<NT>) void norm_pullback_kernel(const T* __restrict__ g_normed, const R* __restrict__ stream,
-                                                                      const R* __restrict__ g_stream, const void* __restrict__ weight,
-                                                                      T* __restrict__ g_hidden, R* __restrict__ g_residual,
+__global__ __launch_bounds__(NT * SIDE<NT>) void norm_pullback_kernel(const T* g_normed, const R* stream, const R* g_stream,
+                                                                      const void* __restrict__ weight, T* g_hidden, R* g_residual,
                                                                       float* __restrict__ partials, long long rows, int D, float eps,
                                                                       int weight_wide, int slab) {
     extern __shared__ __align__(16) float lds[];  // SIDE > 1: [SIDE][D]
@@ -393,6 +392,15 @@ int check(const char* who, int64_t rows, int64_t D, int dtype, int stream, int w
 
 bool aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype_size(dtype)) == 0; }
 
+// A tensor of so many bytes; none if it is not given.
+struct Place {
+    uintptr_t at;
+    uint64_t bytes;
+    Place(const void* p, int64_t elements, size_t size) : at(reinterpret_cast<uintptr_t>(p)), bytes(p ? (uint64_t)elements * size : 0) {}
+    bool meets(const Place& o) const { return bytes && o.bytes && at < o.at + o.bytes && o.at < at + bytes; }
+    bool is(const Place& o) const { return at == o.at && bytes == o.bytes; }
+};
+
 }  // namespace
 }  // namespace block_norm
 }  // namespace lbi
@@ -409,6 +417,11 @@ extern "C" int lbi_residual_rmsnorm(const void* hidden, const void* residual, co
     if (!aligned(hidden, dtype) || (!scales && !aligned(normed, dtype)) || !aligned(residual, residual_dtype) || !aligned(weight, weight_dtype) ||
         !aligned(residual_out, residual_dtype) || !aligned(scales, LBI_F32))
         return fail(LBI_ERR_INVALID, "lbi_residual_rmsnorm: a tensor is not aligned to its elements");
+    const size_t size = dtype_size(dtype), of_stream = dtype_size(residual_dtype);
+    const Place y(normed, rows * D, scales ? 1 : size), s(residual_out, rows * D, of_stream);
+    for (const Place& in : {Place(hidden, rows * D, size), Place(residual, rows * D, of_stream)})
+        if ((y.meets(in) && !y.is(in)) || (s.meets(in) && !s.is(in)) || y.meets(s))
+            return fail(LBI_ERR_INVALID, "lbi_residual_rmsnorm: a result overlaps another tensor");
     return by_types(dtype, residual_dtype, [&](auto t, auto r) {
         using T = typename decltype(t)::type;
         using R = typename decltype(r)::type;
@@ -457,6 +470,11 @@ extern "C" int lbi_residual_rmsnorm_pullback(const void* g_normed, const void* r
         !aligned(weight, weight_dtype) || !aligned(g_hidden, dtype) || !aligned(g_residual, residual_dtype) || !aligned(g_weight, LBI_F32) ||
         !aligned(workspace, LBI_F32))
         return fail(LBI_ERR_INVALID, "lbi_residual_rmsnorm_pullback: a tensor is not aligned to its elements");
+    const size_t size = dtype_size(dtype), of_stream = dtype_size(residual_dtype);
+    const Place out(g_hidden, rows * D, size), more(g_residual, rows * D, of_stream);
+    for (const Place& in : {Place(g_normed, rows * D, size), Place(residual_out, rows * D, of_stream), Place(g_residual_out, rows * D, of_stream)})
+        if ((out.meets(in) && !out.is(in)) || (more.meets(in) && !more.is(in)) || (out.meets(more) && !out.is(more)))
+            return fail(LBI_ERR_INVALID, "lbi_residual_rmsnorm_pullback: a result overlaps another tensor");
     float* partials = static_cast<float*>(workspace);
     if (rows) {
         const int status = by_types(dtype, residual_dtype, [&](auto t, auto r) {

@@ -78,3 +78,46 @@ def test_norm_of_more_rows_than_a_launch_has_threads_for(scaled, device):
     for a, b in zip(residual_rmsnorm(hidden, hidden, weight, EPS, scaled=scaled), want):
         a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
         assert bool((a.view(-1, few) == b.view(1, few)).all())
+
+
+@pytest.mark.parametrize("dtype,stream", [(F32, F32), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("rows,dim", [(1, 5), (70, 64), (33, 100), (70, 768), (9, 1030), (5, 4100), (3, 12000), (5000, 200)])
+def test_norm_results_in_the_place_of_inputs(rows, dim, dtype, stream, device):
+    """What the C interface allows of results that are inputs: the bits of those that lie apart."""
+    from latent_bounded_interfaces_amd import _lib
+
+    lib, on = _lib.load(), torch.cuda.current_stream().cuda_stream
+    gen = torch.Generator().manual_seed(rows + dim)
+    h, g = (_randn(gen, rows, dim).to(dtype).to(device) for _ in range(2))
+    r, gr = (_randn(gen, rows, dim).to(stream).to(device) for _ in range(2))
+    w = torch.ones(dim, device=device, dtype=dtype)
+    codes = [_lib.dtype_code(t) for t in (dtype, stream, dtype)]
+    one = dtype == stream
+
+    def forward(hidden, residual, normed, out):
+        assert lib.lbi_residual_rmsnorm(hidden.data_ptr(), residual.data_ptr(), w.data_ptr(), normed.data_ptr(), out.data_ptr(), None, rows, dim, EPS,
+                                        *codes, on) == 0
+        return normed, out
+
+    want = forward(h, r, torch.empty_like(h), torch.empty_like(r))
+    for normed, out in (("h", None), (None, "r"), ("h", "r")) + ((("r", None), (None, "h"), ("r", "h")) if one else ()):
+        at = {"h": h.clone(), "r": r.clone()}
+        got = forward(at["h"], at["r"], at[normed] if normed else torch.empty_like(h), at[out] if out else torch.empty_like(r))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), (normed, out)
+
+    need = lib.lbi_residual_rmsnorm_pullback_workspace_bytes(rows, dim)
+    workspace = torch.empty(need, device=device, dtype=torch.uint8)
+
+    def pullback(g_normed, s, more, g_hidden, g_residual):
+        g_weight = torch.empty(dim, device=device)
+        assert lib.lbi_residual_rmsnorm_pullback(g_normed.data_ptr(), s.data_ptr(), more.data_ptr(), w.data_ptr(), g_hidden.data_ptr(),
+                                                 g_residual.data_ptr(), g_weight.data_ptr(), workspace.data_ptr(), need, rows, dim, EPS, *codes, on) == 0
+        return g_hidden, g_residual, g_weight
+
+    want = pullback(g, r, gr, torch.empty_like(h), torch.empty_like(r))
+    for hidden, residual in (("g", None), (None, "gr"), ("g", "gr"), (None, "r"), ("g", "r")) + ((("gr", "g"), ("r", "gr"), ("g", "g")) if one else ()):
+        at = {"g": g.clone(), "r": r.clone(), "gr": gr.clone()}
+        got = pullback(at["g"], at["r"], at["gr"], at[hidden] if hidden else torch.empty_like(h), at[residual] if residual else torch.empty_like(r))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), (hidden, residual)
