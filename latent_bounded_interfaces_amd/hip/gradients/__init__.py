@@ -24,6 +24,86 @@ def _flat(t: torch.Tensor) -> bool:
     return t.permute(order).is_contiguous()
 
 
+def _bytes(t: torch.Tensor) -> tuple[int, int]:
+    """First byte of ``t`` and the one behind its last."""
+    begin, size = t.data_ptr(), t.element_size()
+    return begin, begin + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _solvable(terms: list[tuple[int, int]], target: int, steps: list[int]) -> bool:
+    """Whether ``target`` is the sum of ``c * x`` over ``terms`` ``(c, most)``, c descending, each x a whole number of [0, most].  The largest c
+    leaves few x whose rest the others can make: strides of a tensor exceed what its inner dimensions span, as a rule.  ``steps`` counts
+    down; where they run out the answer is yes."""
+    rest = sum(c * most for c, most in terms)
+    if not 0 <= target <= rest:
+        return False
+    if target in (0, rest):
+        return True
+    (c, most), inner = terms[0], terms[1:]
+    rest -= c * most
+    for x in range(min(most, target // c), max(0, -((rest - target) // c)) - 1, -1):
+        steps[0] -= 1
+        if steps[0] < 0 or _solvable(inner, target - c * x, steps):
+            return True
+    return False
+
+
+_STEPS = 20_000  # of a search, some 10 ms
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether elements of ``a`` and ``b`` share a byte: a's address + strides * x + byte = b's likewise, b's indexes counted from the end."""
+    most: dict[int, int] = {}
+    for t in (a, b):
+        for c, n in [(s * t.element_size(), n) for s, n in zip(t.stride(), t.shape) if n > 1 and s] + [(1, t.element_size())]:
+            most[c] = most.get(c, 0) + n - 1
+    return _solvable(sorted(most.items(), reverse=True), _bytes(b)[1] - 1 - a.data_ptr(), [_STEPS])
+
+
+def _folded(t: torch.Tensor) -> bool:
+    """Whether two elements of ``t`` share their place."""
+    dims = sorted((s, n - 1) for s, n in zip(t.stride(), t.shape) if n > 1)
+    if not dims or t.numel() == 0:
+        return False
+    span = 0
+    for s, most in dims:
+        if s <= span:
+            break
+        span += s * most
+    else:
+        return False  # each stride exceeds what the dimensions inside it span
+    for k, (s, most) in enumerate(dims):
+        # differences of two indexes, here at least 1: s * d summed up is 0
+        if s == 0:
+            return True
+        terms = sorted([(c, 2 * m) for i, (c, m) in enumerate(dims) if i != k and c] + [(s, most - 1)], reverse=True)
+        if _solvable(terms, sum(c * m for i, (c, m) in enumerate(dims) if i != k) - s, [_STEPS]):
+            return True
+    return False
+
+
+def _check_apart(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], copied: set[int]) -> None:
+    """Raises where a result has a place twice, or shares one with another result or with a gradient that is not the same view.  For pairs with one of the
+    ``copied``, of which the native call sees only a copy: it looks at the others itself."""
+    places = []
+    for i, (g, out) in enumerate(zip(grads, outs)):
+        if out.numel() == 0:
+            continue
+        if i in copied and _folded(out):
+            raise ValueError("a result has elements that share their place")
+        places.append((*_bytes(out), True, i, out))
+        if not (out is g or (out.data_ptr() == g.data_ptr() and out.stride() == g.stride())):
+            places.append((*_bytes(g), False, i, g))
+    places.sort(key=lambda p: p[:2])
+    open_: list[tuple] = []  # those that reach past the place looked at
+    for p in places:
+        open_ = [q for q in open_ if q[1] > p[0]]
+        for q in open_:
+            if (p[2] or q[2]) and (p[3] in copied or q[3] in copied) and _meet(p[4], q[4]):
+                raise ValueError("a result overlaps another tensor")
+        open_.append(p)
+
+
 def _refuse(tensors: Sequence[torch.Tensor], what: str, index: int) -> None:
     """Raises for the first of ``tensors`` that the kernels do not take on the device ``index``."""
     for t in tensors:
@@ -72,7 +152,7 @@ def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None, ma
     if not isinstance(grads[0], torch.Tensor) or not grads[0].is_cuda:
         _refuse(grads[:1], "grads", 0)
     index = grads[0].get_device()
-    words, held, late = _plain_words(grads, outs, index), [], []
+    words, held, late, copied = _plain_words(grads, outs, index), [], [], set()
     for i, g in enumerate(grads if words is None else ()):
         to = out = None if outs is None else outs[i]
         _refuse([g], "grads", index)
@@ -84,6 +164,7 @@ def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None, ma
                 raise RuntimeError("clip_gradients writes tensors that require grad: call it under torch.no_grad()")
         if not _flat(g) or not (out is None or out is g or out.stride() == g.stride()):
             g = g.contiguous()
+            copied.add(i)
             if out is not None and (out is grads[i] or not out.is_contiguous()):
                 to = torch.empty_like(g)
                 late.append((out, to))
@@ -91,8 +172,8 @@ def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None, ma
         held.append((g.data_ptr(), 0 if to is None else to.data_ptr(), g.numel(), _lib.dtype_code(g.dtype), g, to))  # copies live until all is queued
     if words is None:
         words = [word for row in held for word in row[:4]]
-    if late and len({(o.data_ptr(), o.shape, o.stride()) for o, _ in late}) != len(late):
-        raise ValueError("a result overlaps another tensor")
+    if copied and outs is not None:
+        _check_apart(grads, outs, copied)
     count, device = len(grads), grads[0].device
     table = array.array("q", words)
     norm = grads[0].new_empty((), dtype=torch.float32)  # half the time of torch.empty
@@ -121,7 +202,7 @@ def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, *, out: Seque
     without ``out``.  Returns ``norm``, a scalar tensor of fp32 on the device: nothing here waits for it.
 
     ``out[i]`` has the shape and type of ``grads[i]`` and is ``grads[i]`` itself or overlaps no gradient and no other
-    result; the same gradient twice in the list counts twice and needs an ``out`` for each.  As
+    result, and no two of its elements are one; the same gradient twice in the list counts twice and needs an ``out`` for each.  As
     ``torch.nn.utils.clip_grad_norm_`` does: a norm that is not a number makes every result one, an infinite norm makes
     finite elements 0.  In place and with a norm below the limit, nothing is written."""
     grads = list(grads)

@@ -1,0 +1,58 @@
+"""Calls of the clipping beside those of its own tests, against 64 bits with bounds by arithmetic (oracle/mlp_half.py)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import mlp_half as truth
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _randn(seed, *shape, std=1.0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std
+
+
+def test_strided_results_that_share_memory_are_refused(device):
+    """Results that lie on each other or on another gradient in part, or twice on themselves: nothing is written."""
+    from latent_bounded_interfaces_amd.hip.gradients import clip_gradients
+
+    grads, outs = _randn(1, 4, 8).to(device), torch.zeros(4, 8, device=device)
+    alone, square = _randn(2, 7).to(device), _randn(3, 6, 6).to(device)
+    calls = [
+        ([grads[:, :3], grads[:, 3:6]], [outs[:, :3], outs[:, 2:5]]),
+        ([grads[:, :4], grads[:, 4:]], [grads[:, 1:5], outs[:, 4:]]),
+        ([grads[:, :4], grads[:, 4:]], [grads[:, 4:], grads[:, :4]]),
+        ([grads[:, :4], alone], [grads[:, 1:5], torch.empty_like(alone)]),
+        ([grads, alone], [outs[:, :1].expand(4, 8), torch.empty_like(alone)]),
+        ([alone, grads[:, :3], grads[0, :3]], [torch.empty_like(alone), outs[:, :3], outs[0, :3]]),
+        ([square, alone], [square.t(), torch.empty_like(alone)]),
+    ]
+    for got, into in calls:
+        before = [t.clone() for t in (grads, outs, alone, square)]
+        with pytest.raises((ValueError, RuntimeError), match="overlaps|share"):
+            clip_gradients(got, 0.5, out=into)
+        for a, b in zip((grads, outs, alone, square), before):
+            assert torch.equal(a, b)
+    spread = alone[:1].expand(5)
+    before = alone.clone()
+    with pytest.raises(ValueError, match="share"):
+        clip_gradients([alone[2:], spread], 0.5)
+    assert torch.equal(alone, before)
+
+
+def test_parts_of_one_storage(device):
+    """Results that lie between each other's elements, and some on their own gradients, are not refused."""
+    from latent_bounded_interfaces_amd.hip.gradients import clip_gradients
+
+    whole = _randn(4, 6, 12)
+    base, twin = whole.to(device), torch.zeros(6, 12, device=device)
+    cut = lambda t: [t[:, 0::3], t[:, 1::3], t[:2, 2::3], t[2:, 2::3]]
+    want_norm, want = truth.clip(cut(whole), 1.0)
+    truth.assert_near(clip_gradients(cut(base), 1.0, out=[*cut(base)[:2], *cut(twin)[2:]]), want_norm)
+    for got, one in zip([*cut(base)[:2], *cut(twin)[2:]], want):
+        truth.assert_near(got, one)
+    for got, one in zip(cut(base)[2:], cut(whole)[2:]):
+        assert torch.equal(got.cpu(), one)
