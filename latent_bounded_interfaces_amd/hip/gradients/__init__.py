@@ -185,6 +185,8 @@ def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None, ma
     _lib.check(status, "lbi_clip_gradients")
     for out, to in late:
         out.copy_(to)
+    if outs is not None:
+        torch.autograd.graph.increment_version(outs)  # autograd refuses a backward pass that saved what was there before
     return norm
 
 

@@ -56,3 +56,20 @@ def test_parts_of_one_storage(device):
         truth.assert_near(got, one)
     for got, one in zip(cut(base)[2:], cut(whole)[2:]):
         assert torch.equal(got.cpu(), one)
+
+
+@pytest.mark.parametrize("place", ["in place", "out", "strided"])
+def test_a_backward_pass_that_saved_what_clipping_wrote_is_refused(place, device):
+    from latent_bounded_interfaces_amd.hip.gradients import clip_gradients, gradient_norm
+
+    leaf = torch.ones(6, 5, device=device, requires_grad=True)
+    saved = _randn(5, 6, 5).to(device) if place != "strided" else _randn(5, 6, 9).to(device)[:, :5]
+    product = (leaf * saved).sum()
+    gradient_norm([saved])  # writes nothing
+    product.backward(retain_graph=True)
+    if place == "out":
+        clip_gradients([_randn(6, 6, 5).to(device)], 0.5, out=[saved])
+    else:
+        clip_gradients([saved], 0.5)
+    with pytest.raises(RuntimeError, match="inplace"):
+        product.backward()
