@@ -11,6 +11,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "liblbi_hip.so"
 
@@ -198,6 +199,18 @@ def check(status: int, what: str) -> None:
     if status != 0:
         message = load().lbi_last_error().decode("utf-8", "replace")
         raise LbiLibraryError(f"{what} failed (status {status}): {message}")
+
+
+def refuse_graph(what: str, *tensors) -> None:
+    """Raises where a derivative would be asked of a native call, which records none: a tensor (``None``: not given) that requires grad, with
+    grad mode on, or that carries a tangent of forward-mode differentiation."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} records no autograd graph, and a tensor requires grad: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} records no autograd graph, and a tensor carries a tangent")
 
 
 _SAME_DEVICE = contextlib.nullcontext()

@@ -12,6 +12,7 @@ import math
 from typing import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import _lib
 
@@ -130,13 +131,15 @@ def _plain_words(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | N
         words[2::4] = map(of.numel, grads)
         types = [g.dtype for g in grads]
         words[3::4] = [codes[t] for t in types]
+        if forward_ad._current_level >= 0 or torch.is_grad_enabled() and any([g.requires_grad for g in grads]):
+            return None
         if outs is None:
             return words
-        if torch.is_grad_enabled() and any([out.requires_grad for out in outs]):
-            return None
         if outs is grads:
             words[1::4] = words[0::4]
             return words
+        if torch.is_grad_enabled() and any([out.requires_grad for out in outs]):
+            return None
         if not all(map(of.is_contiguous, outs)) or set(map(of.get_device, outs)) != {index}:
             return None
         if [out.dtype for out in outs] != types or [out.shape for out in outs] != [g.shape for g in grads]:
@@ -162,6 +165,7 @@ def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None, ma
                 raise ValueError("out must have the shapes and types of the gradients")
             if out.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("clip_gradients writes tensors that require grad: call it under torch.no_grad()")
+        _lib.refuse_graph("gradient_norm" if outs is None else "clip_gradients", g, out)
         if not _flat(g) or not (out is None or out is g or out.stride() == g.stride()):
             g = g.contiguous()
             copied.add(i)
@@ -192,7 +196,8 @@ def _clip(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None, ma
 
 def gradient_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """The 2-norm over all elements of all ``grads`` (fp32, fp16, bf16, mixed), a scalar tensor of fp32 on their device.
-    Squares are added in 64 bits.  An empty list has the norm 0 (on the CPU)."""
+    Squares are added in 64 bits.  An empty list has the norm 0 (on the CPU).  No autograd graph is recorded: tensors that require grad, with
+    grad mode on, are refused."""
     grads = list(grads)
     if not grads:
         return torch.zeros(())
@@ -206,7 +211,8 @@ def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, *, out: Seque
     ``out[i]`` has the shape and type of ``grads[i]`` and is ``grads[i]`` itself or overlaps no gradient and no other
     result, and no two of its elements are one; the same gradient twice in the list counts twice and needs an ``out`` for each.  As
     ``torch.nn.utils.clip_grad_norm_`` does: a norm that is not a number makes every result one, an infinite norm makes
-    finite elements 0.  In place and with a norm below the limit, nothing is written."""
+    finite elements 0.  In place and with a norm below the limit, nothing is written.  No
+    autograd graph is recorded: tensors that require grad, with grad mode on, are refused."""
     grads = list(grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

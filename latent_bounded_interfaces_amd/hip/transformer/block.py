@@ -8,8 +8,9 @@ the caches of backends/transformer.py:172-188).  The forward functions return wh
 (``norm_input``, ``norm_output``, ``fc1_output``, ``down_input``); the pullbacks here are those of a single dense cotangent, parameter
 gradients included, where :mod:`.region` pulls a basis of cotangents back through a whole region.
 
-Like the rest of the package these are plain functions with explicit pullbacks and no autograd nodes: a forward function that is
-given a tensor that requires grad, with grad mode on, raises instead of returning a result that is cut off from the graph.
+Like the rest of the package these are plain functions with explicit pullbacks and no autograd nodes: forward function or pullback, one that
+is given a tensor (a parameter too) that requires grad, with grad mode on, or one with a tangent of forward-mode differentiation, raises
+instead of returning a result that is cut off from the graph.
 """
 from __future__ import annotations
 
@@ -19,12 +20,6 @@ from ... import _lib
 from .region import _require_cuda, _stream
 
 _PRODUCT_TYPES = (torch.float16, torch.bfloat16)
-
-
-def _no_graph(what: str, *tensors: torch.Tensor | None) -> None:
-    for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{what} records no autograd graph: call it under torch.no_grad(), with its pullback for the gradients")
 
 
 def _one_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
@@ -60,7 +55,7 @@ def residual_rmsnorm(hidden: torch.Tensor, residual: torch.Tensor | None, weight
     if residual is not None and residual.shape != hidden.shape:
         raise ValueError("residual_rmsnorm: residual must be shaped like hidden")
     _one_device("residual_rmsnorm", hidden, residual, weight)
-    _no_graph("residual_rmsnorm", hidden, residual, weight)
+    _lib.refuse_graph("residual_rmsnorm", hidden, residual, weight)
     branch = hidden.dtype
     stream = residual_dtype or (branch if residual is None else residual.dtype)
     weight = _norm_types("residual_rmsnorm", branch, stream, weight).contiguous()
@@ -99,6 +94,7 @@ def residual_rmsnorm_pullback(g_normed: torch.Tensor, residual_out: torch.Tensor
     if g_residual is not None and (g_residual.shape != g_normed.shape or g_residual.dtype != residual_out.dtype):
         raise ValueError("residual_rmsnorm_pullback: g_residual must have the shape and dtype of residual_out")
     _one_device("residual_rmsnorm_pullback", g_normed, residual_out, weight, g_residual)
+    _lib.refuse_graph("residual_rmsnorm_pullback", g_normed, residual_out, weight, g_residual)
     branch, stream = g_normed.dtype, residual_out.dtype
     weight = _norm_types("residual_rmsnorm_pullback", branch, stream, weight).contiguous()
     g_normed, residual_out = g_normed.contiguous(), residual_out.contiguous()
@@ -159,7 +155,7 @@ def gated_mlp(x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight: torch.Tenso
     if (fc1_bias is not None and fc1_bias.shape != (2 * hidden,)) or (fc2_bias is not None and fc2_bias.shape != (width,)):
         raise ValueError("gated_mlp: fc1_bias must be [2 * hidden] and fc2_bias [width]")
     _one_device("gated_mlp", x, fc1_weight, fc2_weight, fc1_bias, fc2_bias)
-    _no_graph("gated_mlp", x, fc1_weight, fc2_weight, fc1_bias, fc2_bias)
+    _lib.refuse_graph("gated_mlp", x, fc1_weight, fc2_weight, fc1_bias, fc2_bias)
     dtype, outer = x.dtype, x.shape[:-1]
     out, down = x.new_empty(*outer, width), x.new_empty(*outer, hidden)
     fc1_output = x.new_empty(*outer, 2 * hidden) if keep else None
@@ -192,6 +188,7 @@ def gated_mlp_vjp(g_out: torch.Tensor, x: torch.Tensor, fc1_output: torch.Tensor
         if t.shape != (*outer, extent) or t.dtype != dtype:
             raise ValueError(f"gated_mlp_vjp: {name} must be {(*outer, extent)} in the dtype of x")
     _one_device("gated_mlp_vjp", x, g_out, fc1_output, down_input, fc1_weight, fc2_weight)
+    _lib.refuse_graph("gated_mlp_vjp", x, g_out, fc1_output, down_input, fc1_weight, fc2_weight)
     if not rows:
         empty = [torch.zeros_like(x), x.new_zeros(fc1_weight.shape), x.new_zeros(fc2_weight.shape)]
         return tuple(empty + [x.new_zeros(2 * hidden), x.new_zeros(width)] if bias else empty)

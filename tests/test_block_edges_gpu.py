@@ -121,3 +121,40 @@ def test_norm_results_in_the_place_of_inputs(rows, dim, dtype, stream, device):
         got = pullback(at["g"], at["r"], at["gr"], at[hidden] if hidden else torch.empty_like(h), at[residual] if residual else torch.empty_like(r))
         for a, b in zip(got, want):
             assert torch.equal(a, b), (hidden, residual)
+
+
+def _half_calls(device):
+    """(name, call of a list of tensors, the tensors) of each function."""
+    from latent_bounded_interfaces_amd.hip.transformer.block import gated_mlp, gated_mlp_vjp, residual_rmsnorm, residual_rmsnorm_pullback
+
+    gen = torch.Generator().manual_seed(12)
+    rand = lambda *shape: _randn(gen, *shape).to(BF16).to(device)
+    norm = [rand(4, 16), rand(4, 16), rand(16)]
+    pullback = [*norm, rand(4, 16)]
+    mlp = [rand(4, 16), rand(48, 16), rand(8, 24), rand(48), rand(8)]
+    vjp = [rand(4, 8), rand(4, 16), rand(4, 48), rand(4, 24), rand(48, 16), rand(8, 24)]
+    return [("residual_rmsnorm", lambda t: residual_rmsnorm(*t, EPS), norm),
+            ("residual_rmsnorm_pullback", lambda t: residual_rmsnorm_pullback(*t[:3], EPS, g_residual=t[3]), pullback),
+            ("gated_mlp", lambda t: gated_mlp(*t), mlp), ("gated_mlp_vjp", lambda t: gated_mlp_vjp(*t), vjp)]
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")  # torch's own, where it first makes a tensor with a tangent
+def test_derivatives_that_would_be_lost_are_refused(device):
+    """Each tensor of each function in turn: one that requires grad, and one with a tangent."""
+    import torch.autograd.forward_ad as forward_ad
+
+    for name, call, tensors in _half_calls(device):
+        want = call(tensors)
+        want = want if isinstance(want, tuple) else (want,)
+        for i, t in enumerate(tensors):
+            leaf = [*tensors[:i], t.clone().requires_grad_(), *tensors[i + 1:]]
+            with pytest.raises(RuntimeError, match=f"{name} records no autograd graph"):
+                call(leaf)
+            with torch.no_grad():
+                got = call(leaf)
+            for a, b in zip(got if isinstance(got, tuple) else (got,), want):
+                assert torch.equal(a, b) and not a.requires_grad
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match=f"{name} records no autograd graph"):
+                call([*tensors[:i], forward_ad.make_dual(t, torch.ones_like(t)), *tensors[i + 1:]])
+        with forward_ad.dual_level():
+            call(tensors)  # no tangent among them

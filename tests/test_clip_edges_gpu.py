@@ -73,3 +73,29 @@ def test_a_backward_pass_that_saved_what_clipping_wrote_is_refused(place, device
         clip_gradients([saved], 0.5)
     with pytest.raises(RuntimeError, match="inplace"):
         product.backward()
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")  # torch's own, where it first makes a tensor with a tangent
+def test_derivatives_that_would_be_lost_are_refused(device):
+    import torch.autograd.forward_ad as forward_ad
+
+    from latent_bounded_interfaces_amd.hip.gradients import clip_gradients, gradient_norm
+
+    plain, other = _randn(7, 9).to(device), _randn(8, 3, 4).to(device)
+    for grads in ([plain.clone().requires_grad_(), other], [plain, other.clone().requires_grad_()], [plain, other.t().clone().requires_grad_().t()]):
+        outs = [torch.empty_like(g) for g in grads]
+        with pytest.raises(RuntimeError, match="gradient_norm records no autograd graph"):
+            gradient_norm(grads)
+        with pytest.raises(RuntimeError, match="clip_gradients records no autograd graph"):
+            clip_gradients(grads, 1.0, out=outs)
+        with pytest.raises(RuntimeError, match="require grad"):
+            clip_gradients(grads, 1.0)
+        with torch.no_grad():
+            assert torch.equal(gradient_norm(grads), clip_gradients(grads, 1.0, out=outs))
+    with forward_ad.dual_level():
+        dual = [plain, forward_ad.make_dual(other, torch.ones_like(other))]
+        for call in (lambda: gradient_norm(dual), lambda: clip_gradients(dual, 1.0, out=[torch.empty_like(plain), torch.empty_like(other)]),
+                     lambda: clip_gradients([plain], 1.0, out=[forward_ad.make_dual(plain.clone(), plain)]), lambda: clip_gradients(dual, 1.0)):
+            with pytest.raises(RuntimeError, match="records no autograd graph"):
+                call()
+        gradient_norm([plain, other])
