@@ -48,6 +48,7 @@ struct Task {
     const void *a, *b, *bias;  // A [M, K] or, by rows, [K, M]; B [N, K] or, by rows, [K, N]; GATED: B [2N, K]
     void *out, *z;             // GATED: z [M, 2N] written if given; UNGATED: z [M, 2N] read, out [M, 2N]
     long long M, N, K;
+    long long own;             // GATED, UNGATED: the first of N that are not padding; the next product sums over the others too, which must be 0
     int m_tiles, n_tiles;
     struct {  // both operands by rows: a second product over the same K, whose tiles follow those of the first
         const void *a, *b;
@@ -113,6 +114,13 @@ template <typename T, Finish FINISH> __device__ __forceinline__ Beside beside(co
     }
     return r;
 }
+// Zero where a column is padding.  The sums there are products with zeros, which an infinity on the other side makes NaN.
+__device__ __forceinline__ void drop_padding(const Task& task, long long col, Eight& x) {
+    if (col + 8 <= task.own) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (col + e >= task.own) x.v[e] = 0.0f;
+}
 // Eight columns of one row of the result, from their sums (GATED: up's and gate's).
 template <typename T, Finish FINISH>
 __device__ __forceinline__ void finish(const Task& task, long long row, long long col, const Eight& x, const Eight& y, const Beside& more) {
@@ -127,6 +135,7 @@ __device__ __forceinline__ void finish(const Task& task, long long row, long lon
         Eight act;
 #pragma unroll
         for (int e = 0; e < 8; ++e) act.v[e] = up.v[e] * (gate.v[e] * sigmoid(gate.v[e]));
+        drop_padding(task, col, act);
         store8(out + row * N + col, act);
         if (T* z = static_cast<T*>(task.z)) {
             store8(z + row * 2 * N + col, up);
@@ -140,6 +149,8 @@ __device__ __forceinline__ void finish(const Task& task, long long row, long lon
             g_up.v[e] = x.v[e] * (b.v[e] * open);
             g_gate.v[e] = x.v[e] * a.v[e] * (open * (1.0f + b.v[e] * (1.0f - open)));
         }
+        drop_padding(task, col, g_up);
+        drop_padding(task, col, g_gate);
         store8(out + row * 2 * N + col, g_up);
         store8(out + row * 2 * N + N + col, g_gate);
     }
@@ -533,7 +544,7 @@ template <typename T, int ROWS, Finish FINISH, int KW> __global__ __launch_bound
     if constexpr (FINISH == PLAIN) {
         store(out, total[0]);
     } else {
-        store(out, total[0] * (total[1] * sigmoid(total[1])));
+        store(out, col < task.own ? total[0] * (total[1] * sigmoid(total[1])) : 0.0f);
         if (T* z = static_cast<T*>(task.z)) {
             store(z + r * 2 * N + col, total[0]);
             store(z + r * 2 * N + N + col, total[1]);
@@ -950,7 +961,8 @@ extern "C" int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* 
         using T = decltype(type);
         const Forward& t = p.t;
         void* partial = static_cast<char*>(workspace) + p.partial;
-        if (int s = launch<T, false, false, GATED>(p.fc1, {t.x, t.fc1_weight, t.fc1_bias, t.down_input, t.fc1_output, rows, t.hidden, t.D}, partial, on))
+        if (int s = launch<T, false, false, GATED>(p.fc1, {t.x, t.fc1_weight, t.fc1_bias, t.down_input, t.fc1_output, rows, t.hidden, t.D, hidden}, partial,
+                                                     on))
             return s;
         return launch<T, false, false, PLAIN>(p.fc2, {t.down_input, t.fc2_weight, t.fc2_bias, t.out, nullptr, rows, t.width, t.hidden}, partial, on);
     };
@@ -992,7 +1004,7 @@ extern "C" int lbi_gated_mlp_vjp(const void* g_out, const void* x, const void* f
         using T = decltype(type);
         const Pullback& t = p.t;
         void* z = const_cast<void*>(t.fc1_output);
-        if (int s = launch<T, false, true, UNGATED>(p.a, {t.g_out, t.fc2_weight, nullptr, g_fc1, z, rows, t.hidden, t.width}, partial, on)) return s;
+        if (int s = launch<T, false, true, UNGATED>(p.a, {t.g_out, t.fc2_weight, nullptr, g_fc1, z, rows, t.hidden, t.width, hidden}, partial, on)) return s;
         if (int s = launch<T, false, true, PLAIN>(p.x, {g_fc1, t.fc1_weight, nullptr, t.g_x, nullptr, rows, t.D, 2 * t.hidden}, partial, on)) return s;
         // Both weights' gradients are sums over the rows: one list of tiles, with one last round (the whole call for one row of 768 / 2048: 33 -> 29 us, 16000
         // of 256 / 1024 122 -> 112, 8192 of 768 / 2048 241 -> 230; 6007 of 2560 / 6912, whose products fill the chip alone, 1290 -> 1310).

@@ -158,3 +158,39 @@ def test_derivatives_that_would_be_lost_are_refused(device):
                 call([*tensors[:i], forward_ad.make_dual(t, torch.ones_like(t)), *tensors[i + 1:]])
         with forward_ad.dual_level():
             call(tensors)  # no tangent among them
+
+
+#: (rows, D, hidden, width), hidden no multiple of 8: the products of few rows (sums of one, two and four waves), tiles, sums in parts
+PADDED = [(1, 8, 7, 8), (2, 1600, 13, 40), (3, 2500, 9, 24), (70, 64, 33, 40), (67, 2048, 13, 40), (600, 40, 521, 64)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,dim,hidden,width", PADDED)
+def test_mlp_infinities_next_to_padding(rows, dim, hidden, width, dtype, device):
+    """Columns that pad ``hidden`` take no part: a row with an infinity has the infinities and NaN that the formula gives it, its neighbours
+    are as without it."""
+    from latent_bounded_interfaces_amd.hip.transformer.block import gated_mlp, gated_mlp_vjp
+
+    gen = torch.Generator().manual_seed(hidden)
+    x, g_out = _randn(gen, rows, dim).to(dtype), _randn(gen, rows, width).to(dtype)
+    fc1, fc2 = (_randn(gen, 2 * hidden, dim).abs() + 0.5).to(dtype) / dim, (_randn(gen, width, hidden).abs() + 0.5).to(dtype) / hidden
+    fc2[width // 2:] *= -1
+    plain = gated_mlp(x.to(device), fc1.to(device), fc2.to(device), keep=True)
+    z, a = plain[1:]
+    grad = gated_mlp_vjp(g_out.to(device), x.to(device), z, a, fc1.to(device), fc2.to(device))[0]
+    bad_x, bad_g = x.clone(), g_out.clone()
+    bad_x[rows - 1, dim // 2], bad_g[rows - 1, 0] = float("inf"), float("inf")
+    # in 64 bits, for what is finite and what is not
+    up, gate = (bad_x.double() @ fc1.double().t()).chunk(2, -1)
+    want_out = (up * gate * torch.sigmoid(gate)) @ fc2.double().t()
+    up, gate = z.cpu().double().chunk(2, -1)
+    s, g_a = torch.sigmoid(gate), bad_g.double() @ fc2.double()
+    want_grad = torch.cat((g_a * gate * s, g_a * up * (s * (1 + gate * (1 - s)))), -1) @ fc1.double()
+    got_out = gated_mlp(bad_x.to(device), fc1.to(device), fc2.to(device))
+    got_grad = gated_mlp_vjp(bad_g.to(device), x.to(device), z, a, fc1.to(device), fc2.to(device))[0]
+    assert bool(torch.isinf(want_out[-1]).all())
+    for got, want, before in ((got_out, want_out, plain[0]), (got_grad, want_grad, grad)):
+        assert torch.equal(got[:-1], before[:-1])
+        last = got[-1].cpu().double()
+        assert torch.equal(torch.isnan(last), torch.isnan(want[-1])) and torch.equal(last[torch.isinf(want[-1])], want[-1][torch.isinf(want[-1])])
+        assert bool(torch.isfinite(last[torch.isfinite(want[-1])]).all())
