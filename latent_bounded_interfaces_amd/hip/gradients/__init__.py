@@ -119,6 +119,9 @@ def _refuse(tensors: Sequence[torch.Tensor], what: str, index: int) -> None:
             raise ValueError(f"{what} must be on one device")
 
 
+_DTYPE = torch.Tensor.dtype.__get__
+
+
 def _plain_words(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None, index: int) -> list[int] | None:
     """The kernels' table of a list whose tensors all lie as they take them (most lists: a tensor costs half a microsecond, in place
     a third); ``None`` for others, whatever it is about them."""
@@ -129,20 +132,18 @@ def _plain_words(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | N
         words = [0] * (4 * len(grads))  # lbi_gradient of include/lbi_hip.h: four words of 64 bits
         words[0::4] = map(of.data_ptr, grads)
         words[2::4] = map(of.numel, grads)
-        types = [g.dtype for g in grads]
-        words[3::4] = [codes[t] for t in types]
-        if forward_ad._current_level >= 0 or torch.is_grad_enabled() and any([g.requires_grad for g in grads]):
+        types = list(map(_DTYPE, grads))
+        words[3::4] = map(codes.__getitem__, types)
+        if forward_ad._current_level >= 0 or torch.is_grad_enabled() and torch._C._any_requires_grad(grads, () if outs is None or outs is grads else outs):
             return None
         if outs is None:
             return words
         if outs is grads:
             words[1::4] = words[0::4]
             return words
-        if torch.is_grad_enabled() and any([out.requires_grad for out in outs]):
-            return None
         if not all(map(of.is_contiguous, outs)) or set(map(of.get_device, outs)) != {index}:
             return None
-        if [out.dtype for out in outs] != types or [out.shape for out in outs] != [g.shape for g in grads]:
+        if list(map(_DTYPE, outs)) != types or not all(map(of.is_same_size, outs, grads)):
             return None
         words[1::4] = map(of.data_ptr, outs)
         return words
