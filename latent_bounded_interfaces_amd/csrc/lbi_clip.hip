@@ -25,6 +25,7 @@ using attn_mfma::Mma;
 
 constexpr int THREADS = 256, PIECE = 8, UNROLL = 4, CHUNK = THREADS * PIECE * UNROLL;
 constexpr int TABLE = 140, MOST_GROUPS = 1024;
+constexpr double SMALLEST_NORMAL = 1.1754943508222875e-38;  // of fp32
 
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -108,7 +109,14 @@ template <typename T> __device__ __forceinline__ double squares_of(const T* p, i
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-template <typename T> __device__ __forceinline__ void scale(const T* p, T* out, int count, float factor) {
+// times * 2^exponent: a factor below fp32's smallest normal number, which has few of its digits left there, is held in two, any other in `times`
+// alone.
+struct Factor {
+    float times;
+    int exponent;
+    __device__ __forceinline__ float operator()(float x) const { return ldexpf(x * times, exponent); }
+};
+template <typename T> __device__ __forceinline__ void scale(const T* p, T* out, int count, Factor factor) {
     if (count == CHUNK) {
         Eight x[UNROLL];
 #pragma unroll
@@ -116,7 +124,7 @@ template <typename T> __device__ __forceinline__ void scale(const T* p, T* out, 
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
 #pragma unroll
-            for (int e = 0; e < PIECE; ++e) x[u].v[e] *= factor;
+            for (int e = 0; e < PIECE; ++e) x[u].v[e] = factor(x[u].v[e]);
             store8(out + (u * THREADS + threadIdx.x) * PIECE, x[u]);
         }
     } else {
@@ -124,10 +132,10 @@ template <typename T> __device__ __forceinline__ void scale(const T* p, T* out, 
             if (i + PIECE <= count) {
                 Eight x = load8(p + i);
 #pragma unroll
-                for (int e = 0; e < PIECE; ++e) x.v[e] *= factor;
+                for (int e = 0; e < PIECE; ++e) x.v[e] = factor(x.v[e]);
                 store8(out + i, x);
             } else {
-                for (int e = i; e < count; ++e) store1(out + e, to_f32(p[e]) * factor);
+                for (int e = i; e < count; ++e) store1(out + e, factor(to_f32(p[e])));
             }
         }
     }
@@ -161,11 +169,12 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(Table table, const doubl
     double sum = 0.0;
     for (int i = threadIdx.x; i < n_sums; i += THREADS) sum += sums[i];
     const double norm = sqrt(over_group(sum, spare)), ratio = max_norm / (norm + 1e-6);
-    const float factor = (float)(ratio > 1.0 ? 1.0 : ratio);  // not a number stays one
+    Factor factor{(float)(ratio > 1.0 ? 1.0 : ratio), 0};  // not a number stays one
+    if (ratio < SMALLEST_NORMAL) factor.times = (float)frexp(ratio, &factor.exponent);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     for (unsigned chunk = blockIdx.x; chunk < table.chunks; chunk += gridDim.x) {
         const Piece p = piece_of(table, chunk);
-        if (!p.out || (p.in == p.out && factor == 1.0f)) continue;
+        if (!p.out || (p.in == p.out && factor.times == 1.0f)) continue;
         if (p.dtype == LBI_F32) scale(static_cast<const float*>(p.in) + p.at, static_cast<float*>(p.out) + p.at, p.count, factor);
         else if (p.dtype == LBI_F16) scale(static_cast<const _Float16*>(p.in) + p.at, static_cast<_Float16*>(p.out) + p.at, p.count, factor);
         else scale(static_cast<const bf16_raw*>(p.in) + p.at, static_cast<bf16_raw*>(p.out) + p.at, p.count, factor);

@@ -99,3 +99,20 @@ def test_derivatives_that_would_be_lost_are_refused(device):
             with pytest.raises(RuntimeError, match="records no autograd graph"):
                 call()
         gradient_norm([plain, other])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("max_norm,std", [(1.0, 3e37), (1e-3, 1e37), (1e-30, 1e9), (1e-38, 1e3), (0.0, 1.0), (2.0 ** -126, 0.25)])
+def test_factors_below_the_smallest_normal_number(max_norm, std, dtype, device):
+    """The factor's digits are not those that fp32 has left there."""
+    from latent_bounded_interfaces_amd.hip.gradients import clip_gradients
+
+    max_norm = float(torch.tensor(max_norm))  # as the call takes it
+    for count in (4001, 16):
+        grads = [_randn(9, count, std=std).to(dtype), _randn(10, 33, std=std)]
+        assert all(bool(torch.isfinite(g).all()) for g in grads)
+        _, want = truth.clip(grads, max_norm)
+        outs = [torch.empty_like(g, device=device) for g in grads]
+        clip_gradients([g.to(device) for g in grads], max_norm, out=outs)
+        for got, one in zip(outs, want):
+            truth.assert_near(got, one)
