@@ -19,6 +19,7 @@
 
 #include "lbi_attn_mfma.h"
 #include "lbi_attn_dkdv128.h"
+#include "lbi_block_mlp_layout.h"
 
 namespace lbi {
 namespace block_mlp {
@@ -31,16 +32,9 @@ using attn_mfma::tile_off;
 using attn_mfma::u32x2;
 using attn_mfma::u32x4;
 
-constexpr int STEP = 64, NT = 256;  // terms of a step, threads
+constexpr int NT = 256;  // threads
 constexpr unsigned PAST_END = 1u << 31;  // no operand's step reaches this far
 constexpr int PIECE = 1024;  // bytes that a wave's load brings: 8 rows of 64 terms, or 8 terms of 64 columns
-
-// What becomes of the sums.
-enum Finish {
-    PLAIN,   // out = C + bias
-    GATED,   // C is up and gate of one column: activation, and z where it is kept
-    UNGATED  // C is the activation's cotangent: that of z
-};
 
 template <int N> using Count = std::integral_constant<int, N>;
 
@@ -482,8 +476,7 @@ template <typename T, int FM, int FN, Finish FINISH, bool PAIR> __global__ __lau
 // at once.  KW waves share the sums of COLUMNS columns (GATED: pairs of them) of all rows, each lane 16 bytes of every 512 KW terms; lanes are
 // added by exchange, waves in order.  One token, 768 -> 2 x 2048 -> 768 in bf16: 4.8 and 2.3 us (64 x 128 tiles: 7.5 and 8.6), from
 // memory 5.7 and 3.1.
-constexpr int FEW = 4, COLUMNS = 2;
-constexpr int64_t FEW_TERMS = 4 << 20;  // of a weight, from three rows on
+constexpr int COLUMNS = 2;
 template <typename T, int ROWS, Finish FINISH, int KW> __global__ __launch_bounds__(256) void few_rows_kernel(Task task) {
     constexpr int HALVES = FINISH == GATED ? 2 : 1;
     __shared__ float sums[4][HALVES][COLUMNS][ROWS];
@@ -566,65 +559,6 @@ template <typename T, Finish FINISH> int launch_few(const Task& task, hipStream_
     if (task.M <= 1) return with_rows(Count<1>{});
     if (task.M <= 2) return with_rows(Count<2>{});
     return with_rows(Count<4>{});
-}
-
-// How a product is laid out: the tile, and into how many parts the sums of those tiles are cut that do not fill the chip once more.
-constexpr int NONE = -1, FORMS = 7, FEW_ROWS = FORMS;
-// A tile's fragments, the steps of its ring, how many workgroups of it LDS lets share a CU, and what it takes there, in us (see layout_of).  Where
-// there is one workgroup a CU a ring of three is the better one (8192 x 768 x 4096 in tiles of 128 x 192: 64 -> 51 us).
-struct Form {
-    int fm, fn, deep, a_cu;
-    double step[3], alone[3], start;
-};
-constexpr Form forms[FORMS] = {
-    {4, 4, 2, 1, {1.33, 1.33, 1.56}, {1.32, 1.28, 1.82}, 2.8}, {3, 2, 2, 2, {1.10, 1.11, 1.11}, {0.59, 0.64, 0.62}, 1.9},
-    {3, 2, 3, 1, {0.60, 0.64, 0.57}, {0.49, 0.54, 0.51}, 2.2}, {2, 3, 3, 1, {0.60, 0.69, 0.64}, {0.52, 0.54, 0.57}, 2.2},
-    {2, 2, 2, 2, {0.86, 0.89, 0.93}, {0.49, 0.48, 0.62}, 2.0}, {2, 2, 3, 1, {0.48, 0.44, 0.39}, {0.42, 0.36, 0.47}, 2.2},
-    {1, 2, 3, 2, {0.55, 0.59, 0.54}, {0.31, 0.27, 0.32}, 2.8}};
-struct Layout {
-    int form;
-    int tiles, whole, parts, part_steps;
-    double us;
-    size_t bytes() const {
-        return parts > 1 ? (size_t)(tiles - whole) * parts * (64 * forms[form].fm) * (64 * forms[form].fn) * sizeof(float) : 0;
-    }
-};
-
-// By what a call takes, in us: for each round of workgroups over the chip its steps, its start and the results on their way out (20 GB/s a CU, all
-// finishing together; less of it shows where two share a CU); for parts a second launch and their sums out and back.  The constants are fitted to
-// 430 products of 73 blocks (1 ... 16384 rows, widths 128 ... 11264), each in up to 60 layouts: what is chosen took 1.007 times the best on
-// average, 1.19 at most.  A step of 256 x 256 takes 1.3 ... 1.6 us; of 192 x 128 two on a CU 1.1, one 0.6; of 128 x 128 0.9 and 0.4 ... 0.5; of
-// 64 x 128 0.55 and 0.3.
-// M2, N2: of a second product that is laid out together with the first.
-Layout layout_of(int64_t M, int64_t N, int64_t K, Finish finish, int by_rows, int64_t M2 = 0, int64_t N2 = 0) {
-    constexpr double out[3][2] = {{2.2, 1.7}, {4.4, 3.5}, {5.6, 2.6}};  // bytes of a result that show
-    const int cus = device_compute_units(), steps = (int)((K + STEP - 1) / STEP);
-    Layout best{NONE, 0, 0, 1, 0, 0.0};
-    if (by_rows == 0 && M <= FEW && (M <= 2 || N * K <= FEW_TERMS)) return {FEW_ROWS, 0, 0, 1, 0, 0.0};
-    for (int f = 0; f < FORMS; ++f) {
-        const Form& form = forms[f];
-        if (finish == GATED && form.fn % 2) continue;  // up and gate are half of a wave's columns each
-        const int rows = 64 * form.fm, wide = 64 * form.fn, columns = finish == GATED ? wide / 2 : wide, slots = cus * form.a_cu;
-        const auto tiles_of = [&](int64_t m, int64_t n) { return (m + rows - 1) / rows * ((n + columns - 1) / columns); };
-        const int64_t tiles = tiles_of(M, N) + tiles_of(M2, N2);
-        if (tiles >= 1 << 24) continue;
-        const double full = form.step[by_rows], alone = form.alone[by_rows];
-        const double fixed = form.start + out[finish][form.a_cu - 1] * rows * columns * form.a_cu / 20e3;
-        const auto rounds = [&](int64_t items, int of) {
-            const int deep = (int)((items % slots + cus - 1) / cus);  // workgroups that share a CU in the last round
-            return (double)(items / slots) * (of * full + fixed) + (deep ? of * (deep == 1 ? alone : full) + fixed : 0.0);
-        };
-        for (int s : {1, 2, 3, 4, 5, 6, 8, 12, 16}) {
-            const int part_steps = (steps + s - 1) / s, parts = (steps + part_steps - 1) / part_steps;
-            if (parts != s) continue;
-            const int64_t whole = s == 1 ? tiles : tiles / slots * slots, rest = tiles - whole;
-            if (s > 1 && (rest == 0 || part_steps < 2 || rest * s > 2 * slots)) break;  // parts for two rounds at most
-            double us = rounds(whole, steps);
-            if (rest) us += rounds(rest * s, part_steps) + 4.2 + (double)rest * s * rows * columns * 8.0 / 6.5e6;
-            if (best.form == NONE || us < best.us) best = {f, (int)tiles, (int)whole, s, part_steps, us};
-        }
-    }
-    return best;
 }
 
 template <typename T, int FM, int FN, int DEEP, bool A_ROWS, bool B_ROWS, Finish FINISH> int launch_tile(Task task, hipStream_t stream) {
@@ -884,6 +818,7 @@ struct ForwardPlan {
     Layout fc1, fc2;
     size_t partial;
     ForwardPlan(const Forward& c, void* workspace) : pad{static_cast<char*>(workspace)}, t(c) {
+        const int cus = device_compute_units();
         t.D = Padding::eights(c.D), t.hidden = Padding::eights(c.hidden), t.width = Padding::eights(c.width);
         t.x = pad.operand(c.x, c.rows, c.D, c.rows, t.D);
         t.fc1_weight = pad.operand(c.fc1_weight, c.hidden, c.D, t.hidden, t.D, 2);
@@ -893,8 +828,8 @@ struct ForwardPlan {
         t.fc1_output = pad.result_side_by_side(c.fc1_output, c.rows, c.hidden, t.hidden);
         t.down_input = pad.result(c.down_input, c.rows, c.hidden, c.rows, t.hidden);
         t.out = pad.result(c.out, c.rows, c.width, c.rows, t.width);
-        fc1 = layout_of(t.rows, t.hidden, t.D, GATED, 0);
-        fc2 = layout_of(t.rows, t.width, t.hidden, PLAIN, 0);
+        fc1 = layout_of(cus, t.rows, t.hidden, t.D, GATED, 0);
+        fc2 = layout_of(cus, t.rows, t.width, t.hidden, PLAIN, 0);
         partial = pad.bytes;
     }
     size_t bytes() const { return partial + up(std::max(fc1.bytes(), fc2.bytes())); }
@@ -905,6 +840,7 @@ struct PullbackPlan {
     Layout a, x, weights;
     size_t g_fc1, sums, partial;
     PullbackPlan(const Pullback& c, void* workspace) : pad{static_cast<char*>(workspace)}, t(c) {
+        const int cus = device_compute_units();
         t.D = Padding::eights(c.D), t.hidden = Padding::eights(c.hidden), t.width = Padding::eights(c.width);
         t.g_out = pad.operand(c.g_out, c.rows, c.width, c.rows, t.width);
         t.x = pad.operand(c.x, c.rows, c.D, c.rows, t.D);
@@ -917,9 +853,9 @@ struct PullbackPlan {
         t.g_fc2_weight = pad.result(c.g_fc2_weight, c.width, c.hidden, t.width, t.hidden);
         t.g_fc1_bias = pad.result(c.g_fc1_bias, 1, c.hidden, 1, t.hidden, 2);
         t.g_fc2_bias = pad.result(c.g_fc2_bias, 1, c.width, 1, t.width);
-        a = layout_of(t.rows, t.hidden, t.width, UNGATED, 1);
-        x = layout_of(t.rows, t.D, 2 * t.hidden, PLAIN, 1);
-        weights = layout_of(2 * t.hidden, t.D, t.rows, PLAIN, 2, t.width, t.hidden);
+        a = layout_of(cus, t.rows, t.hidden, t.width, UNGATED, 1);
+        x = layout_of(cus, t.rows, t.D, 2 * t.hidden, PLAIN, 1);
+        weights = layout_of(cus, 2 * t.hidden, t.D, t.rows, PLAIN, 2, t.width, t.hidden);
         g_fc1 = pad.bytes;
         sums = g_fc1 + up((size_t)t.rows * 2 * t.hidden * 2);
         partial = sums + up((size_t)slabs_of(t.rows) * (2 * t.hidden + t.width) * sizeof(float));
