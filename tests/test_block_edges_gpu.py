@@ -194,3 +194,31 @@ def test_mlp_infinities_next_to_padding(rows, dim, hidden, width, dtype, device)
         last = got[-1].cpu().double()
         assert torch.equal(torch.isnan(last), torch.isnan(want[-1])) and torch.equal(last[torch.isinf(want[-1])], want[-1][torch.isinf(want[-1])])
         assert bool(torch.isfinite(last[torch.isfinite(want[-1])]).all())
+
+
+def test_the_region_pullback_reads_what_the_forward_functions_return(device):
+    """A region's cache with its MLP halves as these functions compute them, from the modules' own parameters.  Beside the reference's modules, which round
+    the normalised value before its weight, the activation before its product: at most eight half steps of bf16 a layer between what is read, and
+    pullbacks whose derivative in it is of order one."""
+    from latent_bounded_interfaces_amd.hip.transformer.block import gated_mlp, residual_rmsnorm
+    from latent_bounded_interfaces_amd.hip.transformer.region import region_input_pullback_basis, region_parameter_vjp
+    from oracle import transformer_region as oreg
+
+    layers, dim = 2, 96
+    backend = oreg.make_backend(dim=dim, n_heads=4, n_kv_heads=2, hidden=136, layers=layers, d_conv=4, dtype=BF16, seed=3).to(device)
+    gen = torch.Generator().manual_seed(14)
+    basis = _randn(gen, 2, 3, 40, dim).to(BF16).to(device)
+    with torch.no_grad():
+        out, cache = backend.forward_region(region_input=_randn(gen, 2, 40, dim).to(BF16).to(device), region_index=0)
+        want = [region_input_pullback_basis(backend, cache, basis), *region_parameter_vjp(backend, cache, basis[:, 0]).items()]
+        for block, layer in zip(backend.backbone.blocks, cache.layer_caches):
+            half = layer.mlp
+            half.norm_output, half.norm_input = residual_rmsnorm(layer.attention.out_proj_output, layer.attention.norm_input.float(), block.norm2.weight,
+                                                                 block.norm2.eps)
+            down, half.fc1_output, half.down_input = gated_mlp(half.norm_output, block.mlp.fc1.weight, block.mlp.fc2.weight, keep=True)
+            assert float((down - half.down_output).float().norm() / down.float().norm()) <= 8 * 2.0 ** -8
+        got = [region_input_pullback_basis(backend, cache, basis), *region_parameter_vjp(backend, cache, basis[:, 0]).items()]
+    assert len(got) == len(want) > 10
+    for a, b in zip(got, want):
+        a, b, name = (a, b, "input") if torch.is_tensor(a) else (a[1], b[1], a[0])
+        assert float((a - b).float().norm() / b.float().norm()) <= layers * 8 * 2.0 ** -8, name

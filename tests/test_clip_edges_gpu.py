@@ -116,3 +116,23 @@ def test_factors_below_the_smallest_normal_number(max_norm, std, dtype, device):
         clip_gradients([g.to(device) for g in grads], max_norm, out=outs)
         for got, one in zip(outs, want):
             truth.assert_near(got, one)
+
+
+@pytest.mark.parametrize("max_norm", [2.0, 1e6])
+def test_in_place_results_of_every_layout(max_norm, device):
+    """Tensors off the vector grid, transposed, strided, of no and of one element, clipped where they are; what lies beside them is left as it was."""
+    from latent_bounded_interfaces_amd.hip.gradients import clip_gradients
+
+    flat, base, wide = _randn(11, 50_009).to(BF16), _randn(12, 64, 96), _randn(13, 40, 50).to(F16)
+    parts = lambda f, b, w: [f[1:20_002], f[20_002:50_004], b[:, :60].t(), w[:, 3:20], f[50_004:50_004], f[50_006:50_007], w[5, 30:41]]
+    on = [t.to(device) for t in (flat, base, wide)]
+    want_norm, want = truth.clip(parts(flat, base, wide), max_norm)
+    truth.assert_near(clip_gradients(parts(*on), max_norm), want_norm)
+    for got, one in zip(parts(*on), want):
+        truth.assert_near(got, one)
+    for now, before in zip(on, (flat, base, wide)):
+        kept = now.cpu()
+        for part, old in zip(parts(kept, base, wide) if now is on[0] else parts(flat, kept, wide) if now is on[1] else parts(flat, base, kept),
+                             parts(flat, base, wide)):
+            part.copy_(old)
+        assert torch.equal(kept, before)
