@@ -438,8 +438,8 @@ int lbi_residual_rmsnorm_pullback(const void* g_normed, const void* residual_out
  *   g_x [rows,D], g_fc1_weight, g_fc2_weight as the weights, g_fc1_bias [2 hidden] and g_fc2_bias [width] unless NULL.
  *   The cotangent of fc1_output is rounded once, where it is stored between the products.
  *
- * 16-bit types; tensors 16-byte aligned, workspace 256-byte.  Widths that are no multiples of 8 run on copies padded with zeros, in the
- * workspace.  rows up to 2^23, widths up to 2^20; at least one row for the pullback.
+ * 16-bit types; tensors 16-byte aligned, workspace 256-byte; results and workspace overlap no other tensor.  Widths that are no multiples of 8
+ * run on copies padded with zeros, in the workspace.  rows up to 2^23, widths up to 2^20; at least one row for the pullback.
  */
 size_t lbi_gated_mlp_workspace_bytes(int64_t rows, int64_t D, int64_t hidden, int64_t width);
 int lbi_gated_mlp(const void* x, const void* fc1_weight, const void* fc1_bias, const void* fc2_weight, const void* fc2_bias,

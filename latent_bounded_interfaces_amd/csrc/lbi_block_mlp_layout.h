@@ -42,10 +42,11 @@ struct Layout {
 };
 
 // By what a call takes, in us: for each round of workgroups over the chip its steps, its start and the results on their way out (20 GB/s a CU, all
-// finishing together; less of it shows where two share a CU); for parts a second launch and their sums out and back.  The constants are fitted to
-// 430 products of 73 blocks (1 ... 16384 rows, widths 128 ... 11264), each in up to 60 layouts: what is chosen took 1.007 times the best on
-// average, 1.19 at most.  A step of 256 x 256 takes 1.3 ... 1.6 us; of 192 x 128 two on a CU 1.1, one 0.6; of 128 x 128 0.9 and 0.4 ... 0.5; of
-// 64 x 128 0.55 and 0.3.
+// finishing together; less of it shows where two share a CU); for parts a second launch and their sums out and back (of the gated product's two
+// sums a column one; the fit counted both).  The constants were fitted to 438 products of 73 blocks (1 ... 16384 rows, widths 128 ... 11264), each in
+// up to 60 layouts, the weights' gradients one by one; what is chosen of them took 1.013 times the best on average, 1.36 at most (540 rows,
+// 1920 -> 2 x 640, gated).  A step of 256 x 256 takes 1.3 ... 1.6 us; of 192 x 128 two on a CU 1.1, one 0.6; of 128 x 128 0.9 and 0.4 ... 0.5;
+// of 64 x 128 0.55 and 0.3.
 // cus: compute units; by_rows: operands whose terms are their rows.  M2, N2: of a second product that is laid out together with the first.
 inline Layout layout_of(int cus, int64_t M, int64_t N, int64_t K, Finish finish, int by_rows, int64_t M2 = 0, int64_t N2 = 0) {
     constexpr double out[3][2] = {{2.2, 1.7}, {4.4, 3.5}, {5.6, 2.6}};  // bytes of a result that show

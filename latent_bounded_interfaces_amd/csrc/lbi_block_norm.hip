@@ -357,11 +357,11 @@ int slab_rows(int64_t rows, int64_t D) {
 int slab_count(int64_t rows, int64_t D) { return (int)((rows + slab_rows(rows, D) - 1) / slab_rows(rows, D)); }
 
 template <int NT_, int PIECES_> struct Form { static constexpr int NT = NT_, PIECES = PIECES_; };
-// What holds a row of D columns in registers.
 // Threads of a row: as few waves as hold it where that is more than one.
 template <int NT, int PIECES> int threads_of(int64_t D) {
     return NT <= 64 ? NT : (int)((D + 64 * PIECE * PIECES - 1) / (64 * PIECE * PIECES)) * 64;
 }
+// What holds a row of D columns in registers.
 template <bool PULLBACK, typename F> int by_width(int64_t D, F&& launch) {
     if (D <= 64) return launch(Form<8, 1>{});
     if (D <= 128) return launch(Form<16, 1>{});

@@ -6,7 +6,7 @@
 // Squares are formed and added in 64 bits: no gradient of fp32 overflows or vanishes in them, and the norm does not depend on how the chunks
 // fall (fp32 sums of eight would be no faster).  Chunks go to workgroups in a fixed order and sums are added in a fixed order: reruns are bit-identical.
 //
-// Bound by memory: 162 M elements of bf16 are read twice, which the caches cannot hold, and written once, 980 MB in 200 us, the rate of a
+// Bound by memory: 162 M elements of bf16 are read twice, which the caches cannot hold, and written once, 980 MB in 194 us, the rate of a
 // large copy.  A call of a few small tensors is two launches, 4 + 5 us.
 #include <hip/hip_runtime.h>
 
