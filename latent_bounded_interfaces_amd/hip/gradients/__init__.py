@@ -31,6 +31,19 @@ def _bytes(t: torch.Tensor) -> tuple[int, int]:
     return begin, begin + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
+def _column(t: torch.Tensor) -> tuple[int, int, int]:
+    """``(pitch, begin, end)``: the largest stride in bytes, and where within it all bytes of ``t`` lie, if they do not reach around its end
+    (0 for the pitch otherwise, and without a stride)."""
+    size = t.element_size()
+    dims = [(s * size, n - 1) for s, n in zip(t.stride(), t.shape) if n > 1]
+    pitch = max(dims, default=(0, 0))[0]
+    if not pitch:
+        return 0, 0, 0
+    begin = t.data_ptr() % pitch
+    end = begin + size + sum(s * most for s, most in dims if s < pitch)
+    return (pitch, begin, end) if end <= pitch else (0, 0, 0)
+
+
 def _solvable(terms: list[tuple[int, int]], target: int, steps: list[int]) -> bool:
     """Whether ``target`` is the sum of ``c * x`` over ``terms`` ``(c, most)``, c descending, each x a whole number of [0, most].  The largest c
     leaves few x whose rest the others can make: strides of a tensor exceed what its inner dimensions span, as a rule.  ``steps`` counts
@@ -92,14 +105,17 @@ def _check_apart(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], co
             continue
         if i in copied and _folded(out):
             raise ValueError("a result has elements that share their place")
-        places.append((*_bytes(out), True, i, out))
+        places.append((*_bytes(out), True, i, out, _column(out)))
         if not (out is g or (out.data_ptr() == g.data_ptr() and out.stride() == g.stride())):
-            places.append((*_bytes(g), False, i, g))
+            places.append((*_bytes(g), False, i, g, _column(g)))
     places.sort(key=lambda p: p[:2])
     open_: list[tuple] = []  # those that reach past the place looked at
     for p in places:
         open_ = [q for q in open_ if q[1] > p[0]]
+        pitch, begin, end = p[5]
         for q in open_:
+            if pitch and q[5][0] == pitch and (q[5][2] <= begin or end <= q[5][1]):
+                continue  # columns of one matrix, next to each other: the many pairs of a list that there may be
             if (p[2] or q[2]) and (p[3] in copied or q[3] in copied) and _meet(p[4], q[4]):
                 raise ValueError("a result overlaps another tensor")
         open_.append(p)
