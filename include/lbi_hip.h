@@ -472,6 +472,100 @@ size_t lbi_clip_gradients_workspace_bytes(int64_t n);
 int lbi_clip_gradients(const lbi_gradient* gradients, int64_t n, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/*
+ * Rotary positions.  The packed projection qkv [B,T,(H + 2 Hkv) D] (strides of sequence and token in elements, as given; the heads dense) into
+ * q [B,H,T,D] and k [B,Hkv,T,D], contiguous, the first R elements of each head turned by the angle of its position; the values stay where they are.
+ *
+ *   pair i of R / 2:  (x1, x2) -> (x1 cos - x2 sin, x1 sin + x2 cos),   elements (i, i + R/2), or (2 i, 2 i + 1) if interleaved
+ *   cos, sin [table,R/2] fp32; positions [B,T] (int32, or int64 if positions_wide; NULL: 0 ... T-1, which needs table >= T) choose their rows.  A
+ *   position outside the table turns the R elements into NaN.
+ *
+ * Pullback: dq [B,P,H,T,D], dk and dv [B,P,kv_heads,T,D], contiguous, into g_qkv [B,P,T,(H + 2 Hkv) D]: turned back; with kv_heads = H those of the
+ * heads that share a key or value are added up in fp32 first (kv_heads = Hkv: as they are).  What lbi_attn_qkv_pullback does for whole heads, kv_heads = H and
+ * positions 0 ... T-1.  All dtypes; results overlap no other tensor.
+ */
+int lbi_rotary(const void* qkv, const float* cos, const float* sin, const void* positions, void* q, void* k, int64_t B, int64_t T, int64_t H,
+               int64_t Hkv, int64_t D, int64_t R, int64_t table, int64_t stride_b, int64_t stride_t, int positions_wide, int interleaved, int dtype,
+               void* stream);
+int lbi_rotary_pullback(const void* dq, const void* dk, const void* dv, const float* cos, const float* sin, const void* positions, void* g_qkv,
+                        int64_t B, int64_t P, int64_t T, int64_t H, int64_t Hkv, int64_t kv_heads, int64_t D, int64_t R, int64_t table,
+                        int positions_wide, int interleaved, int dtype, void* stream);
+
+/*
+ * The norms behind a block's branch and in front of the next one, with the branch's gate and the residual's scale:
+ *
+ *   u = branch * rsqrt(mean(branch^2) + eps) * post_weight;   s = residual_scale * residual + gate * u;   y = s * rsqrt(mean(s^2) + eps) * weight
+ *   branch, normed [rows,D] in dtype; residual, residual_out = s [rows,D] in residual_dtype (dtype or fp32); weights [D] in dtype or fp32; gate in
+ *   dtype: [rows / per_gate, D], a row for each per_gate rows, or with per_gate = 0 [rows,D]; NULL: 1.
+ *   normed and residual_out may each be an input of their own type, but not the same one; other overlaps are refused.
+ *
+ * Pullback, from branch and residual_out:
+ *   g_s as in lbi_residual_rmsnorm_pullback;  g_residual = residual_scale g_s;  g_gate = g_s u (each row, in dtype, with per_gate = 0; otherwise fp32
+ *   [rows / per_gate, D], summed over a gate's rows);  g_branch, g_post_weight and g_weight (fp32) as the formulas say.  All are written; only g_residual_out and
+ *   gate (with g_gate) may be NULL.  Results overlap no other tensor; sums in a fixed order.
+ *
+ * D up to 16384, fewer than 2^31 rows; tensors aligned to their elements.
+ */
+int lbi_gated_residual_rmsnorm(const void* branch, const void* residual, const void* gate, const void* post_weight, const void* weight, void* normed,
+                               void* residual_out, int64_t rows, int64_t D, int64_t per_gate, float eps, float residual_scale, int dtype,
+                               int residual_dtype, int post_weight_dtype, int weight_dtype, void* stream);
+size_t lbi_gated_residual_rmsnorm_pullback_workspace_bytes(int64_t rows, int64_t D, int64_t per_gate);
+int lbi_gated_residual_rmsnorm_pullback(const void* g_normed, const void* branch, const void* residual_out, const void* g_residual_out,
+                                        const void* gate, const void* post_weight, const void* weight, void* g_branch, void* g_residual, void* g_gate,
+                                        float* g_post_weight, float* g_weight, void* workspace, size_t workspace_bytes, int64_t rows, int64_t D,
+                                        int64_t per_gate, float eps, float residual_scale, int dtype, int residual_dtype, int post_weight_dtype,
+                                        int weight_dtype, void* stream);
+
+/*
+ * Linear attention with a decay for each head (no softmax): over a sequence, for q, k [..,Dk] and v [..,Dv],
+ *
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t,   S [Dk,Dv] in fp32, S_{-1} = state (NULL = 0)
+ *
+ * q [B,H,T,Dk], k [B,Hkv,T,Dk], v [B,Hkv,T,Dv], out [B,H,T,Dv] in a 16-bit dtype, any strides of sequence, head and token (in elements,
+ * as given), the last dimension dense; Hkv divides H, neighbouring heads share.  log_decay [H] fp32 on the device, 0 or less (-inf: no memory).
+ * lengths [B] (int32, or int64 if lengths_wide; NULL: T each, clamped to 0 ... T): tokens that count; what lies behind them in q, k, v and g_out
+ * is not read, and the results' rows there are zero.  state, state_out [B,H,Dk,Dv] contiguous; state_out (NULL: not wanted) is S after the last
+ * token that counts.
+ *
+ * Pullback for P cotangents g_out [B,P,H,T,Dv] (strides given) of out and g_state [B,P,H,Dk,Dv] (NULL = 0) of state_out:
+ *   dq, dk [B,P,H,T,Dk] and dv [B,P,H,T,Dv], contiguous, those of shared heads one for each query head (lbi_rotary_pullback adds them up), and
+ *   d_state [B,P,H,Dk,Dv], the cotangent of state (NULL: not wanted).  log_decay is a constant.
+ *
+ * Products on the 16-bit matrix cores, sums in fp32.  Rounded to 16 bits in between: the decayed scores and a copy of the state, each as an operand
+ * (in fp16 brought into range by powers of two).  The state itself is fp32; the decayed values that it adds up have 24 significant bits (22 in fp16) in calls
+ * with state_out or d_state, 16 otherwise.  A value that is not finite reaches every row of its aligned 64 tokens, earlier ones too.
+ * Dk, Dv up to 128; 3 B P H up to 65535; scale finite and not 0.  Results overlap no other tensor.  Reruns are bit-identical.
+ */
+typedef struct lbi_linear_attention_call {
+    int64_t B, P, H, Hkv, T, Dk, Dv;
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const float *log_decay, *state;
+    const void* lengths;
+    void* out;
+    int64_t out_stride[3];
+    float* state_out;
+    const void* g_out;
+    int64_t g_out_stride[4];
+    const float* g_state;
+    void *dq, *dk, *dv;
+    float* d_state;
+    float scale;
+    int dtype, lengths_wide;
+} lbi_linear_attention_call;
+
+size_t lbi_linear_attention_workspace_bytes(const lbi_linear_attention_call* call);
+int lbi_linear_attention(const lbi_linear_attention_call* call, void* workspace, size_t workspace_bytes, void* stream);
+size_t lbi_linear_attention_pullback_workspace_bytes(const lbi_linear_attention_call* call);
+int lbi_linear_attention_pullback(const lbi_linear_attention_call* call, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One token of each sequence: q [B,H,Dk], k [B,Hkv,Dk], v [B,Hkv,Dv], out [B,H,Dv] contiguous in dtype (fp32 too), state [B,H,Dk,Dv] fp32
+ * contiguous, read and written in place.  active [B] (a byte each, NULL: all): a sequence whose byte is 0 keeps its state and gets a row of zeros.
+ */
+int lbi_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, float* state, const unsigned char* active,
+                              void* out, int64_t B, int64_t H, int64_t Hkv, int64_t Dk, int64_t Dv, float scale, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,7 +17,7 @@ LIB_PATH = Path(__file__).resolve().parent / "liblbi_hip.so"
 
 LBI_F32, LBI_F16, LBI_BF16 = 0, 1, 2
 ATTN_STATIC_SCRATCH_BYTES = 32 << 20  # LBI_ATTN_STATIC_SCRATCH_BYTES of include/lbi_hip.h
-ABI_VERSION = 12
+ABI_VERSION = 13
 LBI_SCAN_EXACT_SUFFIX = 1  # lbi_scan_flags of include/lbi_hip.h
 
 _DTYPE_CODES = {torch.float32: LBI_F32, torch.float16: LBI_F16, torch.bfloat16: LBI_BF16}
@@ -37,6 +37,20 @@ class RegionLayer(_c.Structure):
             "conv_weight", "fc1_output", "norm2_input", "norm1_input", "q", "k", "v", "rope_cos", "rope_sin", "g_input",
             "g_input_branch", "down_input", "norm2_output", "out_input", "norm1_output", "grad_fc2", "grad_fc1", "grad_out",
             "grad_in", "grad_norm2", "grad_norm1", "grad_conv")]
+    )
+
+
+class LinearAttentionCall(_c.Structure):
+    """``lbi_linear_attention_call`` of include/lbi_hip.h."""
+
+    _fields_ = (
+        [(name, _c.c_int64) for name in ("B", "P", "H", "Hkv", "T", "Dk", "Dv")]
+        + [(name, _c.c_void_p) for name in ("q", "k", "v")]
+        + [(name, _c.c_int64 * 3) for name in ("q_stride", "k_stride", "v_stride")]
+        + [(name, _c.c_void_p) for name in ("log_decay", "state", "lengths", "out")]
+        + [("out_stride", _c.c_int64 * 3), ("state_out", _c.c_void_p), ("g_out", _c.c_void_p), ("g_out_stride", _c.c_int64 * 4)]
+        + [(name, _c.c_void_p) for name in ("g_state", "dq", "dk", "dv", "d_state")]
+        + [("scale", _c.c_float), ("dtype", _c.c_int), ("lengths_wide", _c.c_int)]
     )
 
 
@@ -138,6 +152,31 @@ SYMBOLS = {
     "lbi_gated_mlp_vjp": (
         _c.c_int,
         [_c.c_void_p] * 12 + [_c.c_size_t] + [_c.c_int64] * 4 + [_c.c_int, _c.c_void_p],
+    ),
+    "lbi_rotary": (
+        _c.c_int,
+        [_c.c_void_p] * 6 + [_c.c_int64] * 9 + [_c.c_int] * 3 + [_c.c_void_p],
+    ),
+    "lbi_rotary_pullback": (
+        _c.c_int,
+        [_c.c_void_p] * 7 + [_c.c_int64] * 9 + [_c.c_int] * 3 + [_c.c_void_p],
+    ),
+    "lbi_gated_residual_rmsnorm": (
+        _c.c_int,
+        [_c.c_void_p] * 7 + [_c.c_int64] * 3 + [_c.c_float] * 2 + [_c.c_int] * 4 + [_c.c_void_p],
+    ),
+    "lbi_gated_residual_rmsnorm_pullback_workspace_bytes": (_c.c_size_t, [_c.c_int64] * 3),
+    "lbi_gated_residual_rmsnorm_pullback": (
+        _c.c_int,
+        [_c.c_void_p] * 13 + [_c.c_size_t] + [_c.c_int64] * 3 + [_c.c_float] * 2 + [_c.c_int] * 4 + [_c.c_void_p],
+    ),
+    "lbi_linear_attention_workspace_bytes": (_c.c_size_t, [_c.POINTER(LinearAttentionCall)]),
+    "lbi_linear_attention": (_c.c_int, [_c.POINTER(LinearAttentionCall), _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "lbi_linear_attention_pullback_workspace_bytes": (_c.c_size_t, [_c.POINTER(LinearAttentionCall)]),
+    "lbi_linear_attention_pullback": (_c.c_int, [_c.POINTER(LinearAttentionCall), _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "lbi_linear_attention_step": (
+        _c.c_int,
+        [_c.c_void_p] * 7 + [_c.c_int64] * 5 + [_c.c_float, _c.c_int, _c.c_void_p],
     ),
     "lbi_clip_gradients_workspace_bytes": (_c.c_size_t, [_c.c_int64]),
     "lbi_clip_gradients": (

@@ -17,7 +17,9 @@ LIB_PATH = PKG_DIR / "liblbi_hip.so"
 SOURCES = ("lbi_common.hip", "lbi_scan.hip", "lbi_scan_narrow.hip", "lbi_scan_narrow_f32.hip", "lbi_scan_narrow_f16.hip",
            "lbi_scan_narrow_bf16.hip", "lbi_attn.hip", "lbi_attn_f32.hip", "lbi_attn_f32_f16.hip",
            "lbi_attn_f32_bf16.hip", "lbi_region.hip", "lbi_product.hip", "lbi_gradient.hip", "lbi_region_layer.hip", "lbi_norms.hip", "lbi_param_grads.hip",
-           "lbi_block_norm.hip", "lbi_block_mlp.hip", "lbi_clip.hip")
+           "lbi_block_norm.hip", "lbi_block_mlp.hip", "lbi_clip.hip", "lbi_block_gated_norm.hip", "lbi_block_gated_norm_f32.hip",
+           "lbi_block_gated_norm_f16.hip", "lbi_block_gated_norm_bf16.hip", "lbi_rotary.hip", "lbi_linear_attn.hip",
+           "lbi_linear_attn_f16.hip", "lbi_linear_attn_bf16.hip")
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -34,7 +36,9 @@ HIPCC_FLAGS = [
 # unroll puts them into scratch memory.
 SOURCE_FLAGS = {src: ["-Werror=pass-failed"] for src in ("lbi_region.hip", "lbi_product.hip", "lbi_attn_f32.hip", "lbi_attn_f32_f16.hip",
                                                           "lbi_attn_f32_bf16.hip", "lbi_scan.hip", "lbi_scan_narrow_f32.hip", "lbi_scan_narrow_f16.hip", "lbi_scan_narrow_bf16.hip",
-                                                          "lbi_block_norm.hip", "lbi_block_mlp.hip", "lbi_clip.hip")}
+                                                          "lbi_block_norm.hip", "lbi_block_mlp.hip", "lbi_clip.hip", "lbi_block_gated_norm_f32.hip",
+                                                          "lbi_block_gated_norm_f16.hip", "lbi_block_gated_norm_bf16.hip", "lbi_rotary.hip", "lbi_linear_attn.hip",
+                                                          "lbi_linear_attn_f16.hip", "lbi_linear_attn_bf16.hip")}
 
 
 def _hipcc() -> str:

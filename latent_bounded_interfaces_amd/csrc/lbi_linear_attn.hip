@@ -1,0 +1,272 @@
+// Linear attention with a decay for each head: the C entries, and the kernel for single tokens.
+//
+//   prompts    S_t = l S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t          lbi_linear_attention (lbi_linear_attn_kernel.h)
+//   pullback   of the same for P cotangents of out, from q, k and v          lbi_linear_attention_pullback
+//   tokens     one step of it for each sequence, the state in place          lbi_linear_attention_step
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "lbi_linear_attn.h"
+
+namespace lbi {
+namespace linear_attn {
+
+int run_bf16(const Call& call, bool exact_last, hipStream_t stream);
+int run_f16(const Call& call, hipStream_t stream);
+
+namespace {
+
+constexpr int64_t MOST_UNITS = 65535;  // of a launch's second dimension
+
+int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
+    return dtype == LBI_F16 ? run_f16(call, stream) : run_bf16(call, exact_last, stream);
+}
+
+// Segments that a chain is cut into, so many tokens each: none while the chains alone fill the chip.
+int segments_of(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
+    const int64_t chunks = (T + CHUNK - 1) / CHUNK, room = (int64_t)device_compute_units() * (Da > 64 && Dc > 64 ? 2 : 3);
+    if (units * 2 > room || chunks < 4) return 1;
+    const int64_t wanted = std::min(room / units, chunks / 2), of = (chunks + wanted - 1) / wanted;
+    return (int)((chunks + of - 1) / of);
+}
+size_t states_bytes(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
+    const int segments = segments_of(units, T, Da, Dc);
+    return segments > 1 ? (size_t)units * segments * Da * Dc * sizeof(float) : 0;
+}
+void cut(Call& call, float* workspace) {
+    const int64_t chunks = (call.T + CHUNK - 1) / CHUNK;
+    call.segments = segments_of((int64_t)call.chains * call.B * call.P * call.H, call.T, call.chain[0].Da, call.chain[0].Dc);
+    call.segment = (int)((chunks + call.segments - 1) / call.segments) * CHUNK;
+    call.segment_states = workspace;
+}
+
+bool any_null(std::initializer_list<const void*> pointers) {
+    return std::any_of(pointers.begin(), pointers.end(), [](const void* p) { return !p; });
+}
+bool off(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+int check(const char* who, const lbi_linear_attention_call* call, bool pullback) {
+    if (!call) return fail(LBI_ERR_INVALID, "%s: null pointer", who);
+    const auto& c = *call;
+    if (c.B < 0 || c.H < 1 || c.Hkv < 1 || c.T < 0 || c.Dk < 1 || c.Dv < 1 || (pullback && c.P < 0))
+        return fail(LBI_ERR_INVALID, "%s: bad size (B=%lld H=%lld Hkv=%lld T=%lld Dk=%lld Dv=%lld)", who, (long long)c.B, (long long)c.H,
+                    (long long)c.Hkv, (long long)c.T, (long long)c.Dk, (long long)c.Dv);
+    if (c.H % c.Hkv) return fail(LBI_ERR_INVALID, "%s: H=%lld not a multiple of Hkv=%lld", who, (long long)c.H, (long long)c.Hkv);
+    if (c.dtype != LBI_F16 && c.dtype != LBI_BF16) return fail(dtype_size(c.dtype) ? LBI_ERR_UNSUPPORTED : LBI_ERR_INVALID, "%s: bad dtype %d", who, c.dtype);
+    if (c.Dk > MOST_DIM || c.Dv > MOST_DIM) return fail(LBI_ERR_UNSUPPORTED, "%s: head dims of up to %d", who, MOST_DIM);
+    const int64_t basis = pullback ? std::max<int64_t>(c.P, 1) : 1;
+    if (c.T >= (int64_t)1 << 30 || c.B >= (int64_t)1 << 20 || c.H >= (int64_t)1 << 16 || basis >= (int64_t)1 << 16 ||
+        MOST_CHAINS * c.B * c.H * basis > MOST_UNITS)
+        return fail(LBI_ERR_UNSUPPORTED, "%s: too many sequences, heads and directions, or too many tokens", who);
+    if (!std::isfinite(c.scale) || c.scale == 0.0f) return fail(LBI_ERR_INVALID, "%s: scale must be finite and not zero", who);
+    return LBI_OK;
+}
+
+int check_workspace(const char* who, size_t need, const void* workspace, size_t bytes) {
+    if (need && (!workspace || bytes < need)) return fail(LBI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, bytes);
+    if (need && off(workspace, 4)) return fail(LBI_ERR_INVALID, "%s: a tensor is not aligned to its elements", who);
+    return LBI_OK;
+}
+
+View shared(const void* p, const int64_t* stride, int64_t group) { return View{p, stride[0], 0, stride[1], stride[2], (int)group}; }
+// contiguous [B, P, H, T, width]
+View dense(const void* p, const lbi_linear_attention_call& c, int64_t width) {
+    return View{p, c.P * c.H * c.T * width, c.H * c.T * width, c.T * width, width, 1};
+}
+Call base(const lbi_linear_attention_call& c, int64_t basis) {
+    Call call{};
+    call.log_decay = c.log_decay;
+    call.lengths = c.lengths;
+    call.lengths_wide = c.lengths_wide != 0;
+    call.B = (int)c.B, call.P = (int)basis, call.H = (int)c.H, call.T = (int)c.T;
+    return call;
+}
+
+// One token of each head: a workgroup takes COLS columns of a head's state, VEC neighbouring ones a thread, and as many rows side by side as it
+// has threads left.  Bound by memory: the state is read and written once; all of a thread's share is asked for before any of it is used.
+template <typename T, int COLS, int VEC, int ROUNDS>
+__global__ __launch_bounds__(256) void step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+                                                   const float* __restrict__ log_decay, float* state, const unsigned char* __restrict__ active,
+                                                   T* __restrict__ out, int H, int group, int Dk, int Dv, float scale) {
+    constexpr int LANES = COLS / VEC, SIDE = 256 / LANES;
+    typedef float vec __attribute__((ext_vector_type(VEC), aligned(4 * VEC)));
+    __shared__ float sums[SIDE][COLS];
+    const int bh = blockIdx.x, h = bh % H, b = bh / H, col = (int)blockIdx.y * COLS + threadIdx.x % LANES * VEC, row0 = threadIdx.x / LANES;
+    const int64_t kv = (int64_t)b * (H / group) + h / group;
+    float* s = state + (int64_t)bh * Dk * Dv;
+    const bool on = !active || active[b];
+    float part[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) part[e] = 0.0f;
+    if (on && col < Dv) {
+        vec x[ROUNDS];
+        float kk[ROUNDS], qq[ROUNDS], vv[VEC];
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) {
+            const int row = row0 + i * SIDE, from = row < Dk ? row : 0;
+            x[i] = *reinterpret_cast<const vec*>(s + from * Dv + col);
+            kk[i] = to_f32(k[kv * Dk + from]);
+            qq[i] = to_f32(q[(int64_t)bh * Dk + from]);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) vv[e] = to_f32(v[kv * Dv + col + e]);
+        const float l = log_decay[h], fade = expm1f(l);
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) {
+            const int row = row0 + i * SIDE;
+            if (row >= Dk) continue;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                // x + x (l - 1): a decay near 1 is not rounded, which over many tokens would add up
+                x[i][e] = fmaf(kk[i], vv[e], fmaf(x[i][e], fade, x[i][e]));
+                part[e] = fmaf(qq[i], x[i][e], part[e]);
+            }
+            *reinterpret_cast<vec*>(s + row * Dv + col) = x[i];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sums[row0][threadIdx.x % LANES * VEC + e] = part[e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < COLS; c += 256) {
+        const int to = (int)blockIdx.y * COLS + c;
+        if (to >= Dv) continue;
+        float sum = sums[0][c];
+#pragma unroll
+        for (int r = 1; r < SIDE; ++r) sum += sums[r][c];
+        sum *= scale;
+        T* o = out + (int64_t)bh * Dv + to;
+        if constexpr (std::is_same_v<T, bf16_raw>) o->bits = f32_to_bf16_bits(sum);
+        else *o = (T)sum;
+    }
+}
+
+template <typename T, int COLS, int VEC>
+int launch_step(const void* q, const void* k, const void* v, const float* log_decay, float* state, const unsigned char* active, void* out, int64_t B,
+                int64_t H, int64_t Hkv, int64_t Dk, int64_t Dv, float scale, hipStream_t stream) {
+    constexpr int SIDE = 256 / (COLS / VEC);
+    const auto kernel = Dk <= 64 ? step_kernel<T, COLS, VEC, (64 + SIDE - 1) / SIDE> : step_kernel<T, COLS, VEC, (128 + SIDE - 1) / SIDE>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(B * H), (unsigned)((Dv + COLS - 1) / COLS)), dim3(256), 0, stream, static_cast<const T*>(q),
+                       static_cast<const T*>(k), static_cast<const T*>(v), log_decay, state, active, static_cast<T*>(out), (int)H, (int)(H / Hkv), (int)Dk,
+                       (int)Dv, scale);
+    LBI_HIP_CHECK(hipGetLastError());
+    return LBI_OK;
+}
+
+}  // namespace
+}  // namespace linear_attn
+}  // namespace lbi
+
+extern "C" size_t lbi_linear_attention_workspace_bytes(const lbi_linear_attention_call* c) {
+    using namespace lbi::linear_attn;
+    if (check("lbi_linear_attention_workspace_bytes", c, false)) return 0;
+    if (!c->B || !c->T) return 0;
+    return states_bytes(c->B * c->H, c->T, c->Dk, c->Dv);
+}
+
+extern "C" int lbi_linear_attention(const lbi_linear_attention_call* c, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace lbi;
+    using namespace lbi::linear_attn;
+    clear_error();
+    if (int bad = check("lbi_linear_attention", c, false)) return bad;
+    if (!c->B) return LBI_OK;
+    if (any_null({c->log_decay}) || (c->T && any_null({c->q, c->k, c->v, c->out}))) return fail(LBI_ERR_INVALID, "lbi_linear_attention: null pointer");
+    if (off(c->q, 2) || off(c->k, 2) || off(c->v, 2) || off(c->out, 2) || off(c->state, 4) || off(c->state_out, 4) || off(c->log_decay, 4) ||
+        off(c->lengths, c->lengths_wide ? 8 : 4))
+        return fail(LBI_ERR_INVALID, "lbi_linear_attention: a tensor is not aligned to its elements");
+    if (int bad = check_workspace("lbi_linear_attention", lbi_linear_attention_workspace_bytes(c), workspace, workspace_bytes)) return bad;
+    clear_error();
+    Call call = base(*c, 1);
+    call.chains = 1;
+    Chain& ch = call.chain[0];
+    ch.a = shared(c->q, c->q_stride, 1);
+    ch.b = shared(c->k, c->k_stride, c->H / c->Hkv);
+    ch.c = shared(c->v, c->v_stride, c->H / c->Hkv);
+    ch.out = shared(c->out, c->out_stride, 1);
+    const auto states = [&](const float* p) { return States{const_cast<float*>(p), c->H * c->Dk * c->Dv, 0, c->Dk * c->Dv, c->Dv, 1}; };
+    ch.first = states(c->state), ch.last = states(c->state_out);
+    ch.first_scale = ch.last_scale = 1.0f;
+    ch.scale = c->scale;
+    ch.Da = (int)c->Dk, ch.Dc = (int)c->Dv, ch.reverse = 0, ch.shift = 0;
+    cut(call, static_cast<float*>(workspace));
+    return run(call, c->dtype, c->state_out != nullptr, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t lbi_linear_attention_pullback_workspace_bytes(const lbi_linear_attention_call* c) {
+    using namespace lbi::linear_attn;
+    if (check("lbi_linear_attention_pullback_workspace_bytes", c, true)) return 0;
+    if (!c->B || !c->T || !c->P) return 0;
+    const int64_t units = c->B * c->P * c->H;
+    if (c->Dk == c->Dv) return states_bytes(3 * units, c->T, c->Dk, c->Dv);
+    return std::max(states_bytes(2 * units, c->T, c->Dv, c->Dk), states_bytes(units, c->T, c->Dk, c->Dv));
+}
+
+extern "C" int lbi_linear_attention_pullback(const lbi_linear_attention_call* c, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace lbi;
+    using namespace lbi::linear_attn;
+    clear_error();
+    if (int bad = check("lbi_linear_attention_pullback", c, true)) return bad;
+    if (!c->B || !c->P) return LBI_OK;
+    if (any_null({c->log_decay}) || (c->T && any_null({c->q, c->k, c->v, c->g_out, c->dq, c->dk, c->dv})))
+        return fail(LBI_ERR_INVALID, "lbi_linear_attention_pullback: null pointer");
+    if (off(c->q, 2) || off(c->k, 2) || off(c->v, 2) || off(c->g_out, 2) || off(c->dq, 2) || off(c->dk, 2) || off(c->dv, 2) || off(c->state, 4) ||
+        off(c->g_state, 4) || off(c->d_state, 4) || off(c->log_decay, 4) || off(c->lengths, c->lengths_wide ? 8 : 4))
+        return fail(LBI_ERR_INVALID, "lbi_linear_attention_pullback: a tensor is not aligned to its elements");
+    if (int bad = check_workspace("lbi_linear_attention_pullback", lbi_linear_attention_pullback_workspace_bytes(c), workspace, workspace_bytes)) return bad;
+    clear_error();
+    const int64_t group = c->H / c->Hkv, of_state = c->Dk * c->Dv;
+    const View q = shared(c->q, c->q_stride, 1), k = shared(c->k, c->k_stride, group), v = shared(c->v, c->v_stride, group);
+    const View gv = View{c->g_out, c->g_out_stride[0], c->g_out_stride[1], c->g_out_stride[2], c->g_out_stride[3], 1};
+    // of the forward's first state, one for all directions, and of the cotangents of the last and the first
+    const States none{}, first{const_cast<float*>(c->state), c->H * of_state, 0, of_state, 1, c->Dv};
+    const auto cotangent = [&](const float* p, bool turned) {
+        return States{const_cast<float*>(p), c->P * c->H * of_state, c->H * of_state, of_state, turned ? 1 : c->Dv, turned ? c->Dv : 1};
+    };
+    Call call = base(*c, c->P);
+    const int dk = (int)c->Dk, dv = (int)c->Dv;
+    const float s = c->scale;
+    const Chain of_q{gv, v, k, dense(c->dq, *c, dk), first, none, 1.0f, 1.0f, s, dv, dk, 0, 0};
+    const Chain of_k{v, gv, q, dense(c->dk, *c, dk), cotangent(c->g_state, true), none, 1.0f / s, s, s, dv, dk, 1, 1};
+    const Chain of_v{k, q, gv, dense(c->dv, *c, dv), cotangent(c->g_state, false), cotangent(c->d_state, false), 1.0f / s, s, s, dk, dv, 1, 1};
+    const bool exact = c->d_state != nullptr;
+    const auto go = [&](std::initializer_list<Chain> chains) {
+        call.chains = 0;
+        for (const Chain& ch : chains) call.chain[call.chains++] = ch;
+        cut(call, static_cast<float*>(workspace));
+        return run(call, c->dtype, exact, static_cast<hipStream_t>(stream));
+    };
+    if (dk == dv) return go({of_q, of_k, of_v});
+    if (int bad = go({of_q, of_k})) return bad;
+    return go({of_v});
+}
+
+extern "C" int lbi_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, float* state, const unsigned char* active,
+                                         void* out, int64_t B, int64_t H, int64_t Hkv, int64_t Dk, int64_t Dv, float scale, int dtype, void* stream) {
+    using namespace lbi;
+    using namespace lbi::linear_attn;
+    clear_error();
+    if (B < 0 || H < 1 || Hkv < 1 || Dk < 1 || Dv < 1)
+        return fail(LBI_ERR_INVALID, "lbi_linear_attention_step: bad size (B=%lld H=%lld Hkv=%lld Dk=%lld Dv=%lld)", (long long)B, (long long)H,
+                    (long long)Hkv, (long long)Dk, (long long)Dv);
+    if (H % Hkv) return fail(LBI_ERR_INVALID, "lbi_linear_attention_step: H=%lld not a multiple of Hkv=%lld", (long long)H, (long long)Hkv);
+    const size_t size = dtype_size(dtype);
+    if (!size) return fail(LBI_ERR_INVALID, "lbi_linear_attention_step: bad dtype %d", dtype);
+    if (Dk > MOST_DIM || Dv > MOST_DIM) return fail(LBI_ERR_UNSUPPORTED, "lbi_linear_attention_step: head dims of up to %d", MOST_DIM);
+    if (B >= (int64_t)1 << 24 || H >= (int64_t)1 << 16 || B * H >= (int64_t)1 << 24)
+        return fail(LBI_ERR_UNSUPPORTED, "lbi_linear_attention_step: too many sequences and heads");
+    if (!B) return LBI_OK;
+    if (any_null({q, k, v, log_decay, state, out})) return fail(LBI_ERR_INVALID, "lbi_linear_attention_step: null pointer");
+    if (off(q, size) || off(k, size) || off(v, size) || off(out, size) || off(state, 4) || off(log_decay, 4))
+        return fail(LBI_ERR_INVALID, "lbi_linear_attention_step: a tensor is not aligned to its elements");
+    const bool in_fours = Dv % 4 == 0 && !off(state, 16), few = B * H * 2 < device_compute_units();
+    const auto go = [&](auto t) {
+        using T = decltype(t);
+        const auto with = [&](auto launch) { return launch(q, k, v, log_decay, state, active, out, B, H, Hkv, Dk, Dv, scale, static_cast<hipStream_t>(stream)); };
+        if (!in_fours) return with(launch_step<T, 64, 1>);
+        if (few) return with(launch_step<T, 16, 4>);
+        return Dv > 64 ? with(launch_step<T, 128, 4>) : with(launch_step<T, 64, 4>);
+    };
+    if (dtype == LBI_F32) return go(float{});
+    return dtype == LBI_F16 ? go(_Float16{}) : go(bf16_raw{});
+}

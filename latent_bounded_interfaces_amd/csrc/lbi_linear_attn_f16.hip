@@ -1,0 +1,10 @@
+// Linear attention over chunks, fp16 storage.
+#include "lbi_linear_attn_launch.h"
+
+namespace lbi {
+namespace linear_attn {
+
+int run_f16(const Call& call, hipStream_t stream) { return by_pieces<_Float16, 2>(call, stream); }
+
+}  // namespace linear_attn
+}  // namespace lbi

@@ -1,0 +1,236 @@
+// Rotary positions: a packed projection's queries and keys turned into heads, and back.
+//
+//   forward    (x1, x2) -> (x1 cos - x2 sin, x1 sin + x2 cos) for each pair of the first R elements of a head, the others as they are
+//   pullback   the same with -sin, after the heads that share a key or value are added up, into the packed projection's cotangent
+//
+// A pair is (c, c + R/2), or (2 c, 2 c + 1) if interleaved.  cos and sin are tables of fp32 over positions; a position past their end turns to
+// NaN.  Arithmetic is fp32, each result is rounded once.
+//
+// Bound by memory: every element is read and written once, in 16-byte pieces where all rows allow it (an element each otherwise), a thread to
+// a piece or to a pair of them; the tables come from the caches, once a thread.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "lbi_common.h"
+
+namespace lbi {
+namespace rotary {
+namespace {
+
+constexpr int64_t MOST_THREADS = ((int64_t)1 << 32) - 256;  // of a launch
+
+template <typename T, int N> struct Piece;
+template <int N> struct Piece<float, N> { typedef float type __attribute__((ext_vector_type(N), aligned(4 * N))); };
+template <int N> struct Piece<_Float16, N> { typedef _Float16 type __attribute__((ext_vector_type(N), aligned(2 * N))); };
+template <int N> struct Piece<bf16_raw, N> { typedef unsigned short type __attribute__((ext_vector_type(N), aligned(2 * N))); };
+
+template <typename T> __device__ __forceinline__ float widen(T x) { return (float)x; }
+template <> __device__ __forceinline__ float widen(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
+template <typename T> __device__ __forceinline__ auto narrow(float x) {
+    if constexpr (std::is_same_v<T, bf16_raw>) return f32_to_bf16_bits(x);
+    else return (T)x;
+}
+
+struct Call {
+    const void *q, *k, *v;  // forward: the packed projection in q; pullback: [B, P, heads, T, D]
+    void *out, *out_k;      // forward: [B, H, T, D] and [B, Hkv, T, D]; pullback: [B, P, T, (H + 2 Hkv) D]
+    const float *cos, *sin;  // [table, R / 2]
+    const void* positions;   // [B, T], NULL: 0, 1, ...; 8 bytes each if positions_wide
+    int64_t stride_b, stride_t;  // of the packed projection
+    int64_t table, first, units;
+    int positions_wide, P, T, H, Hkv, shared, D, R, interleaved;  // shared: heads of k and v that are added up
+};
+
+__device__ __forceinline__ int64_t row_of_table(const Call& c, int64_t b, int64_t t) {
+    int64_t at = t;
+    if (c.positions) at = c.positions_wide ? static_cast<const int64_t*>(c.positions)[b * c.T + t] : (int64_t)static_cast<const int*>(c.positions)[b * c.T + t];
+    return at >= 0 && at < c.table ? at : -1;
+}
+
+// N elements from `p` on, `shared` times `apart` elements apart, added up.
+template <typename T, int N> __device__ __forceinline__ void load(const T* p, int shared, int64_t apart, float* x) {
+    typedef typename Piece<T, N>::type piece;
+    const piece own = *reinterpret_cast<const piece*>(p);
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = widen(own[e]);
+    for (int s = 1; s < shared; ++s) {
+        const piece more = *reinterpret_cast<const piece*>(p + s * apart);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] += widen(more[e]);
+    }
+}
+template <typename T, int N> __device__ __forceinline__ void store(T* p, const float* x) {
+    typedef typename Piece<T, N>::type piece;
+    piece own;
+#pragma unroll
+    for (int e = 0; e < N; ++e) own[e] = narrow<T>(x[e]);
+    *reinterpret_cast<piece*>(p) = own;
+}
+
+// A unit is a place of a head of a row: half layout, pairs of pieces of the turned part, then the pieces of the rest; interleaved, the pieces in order.
+template <typename T, int N, bool BACK> __global__ __launch_bounds__(256) void rotary_kernel(Call c) {
+    const int64_t id = c.first + (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= c.units) return;
+    const int turned = c.interleaved ? c.R / N : c.R / 2 / N, places = turned + (c.D - c.R) / N;  // of a head
+    const int heads = c.H + (BACK ? 2 : 1) * c.Hkv;
+    int place = (int)(id % places);
+    const int64_t rest = id / places;
+    const int head = (int)(rest % heads);
+    const int64_t row = rest / heads;  // of [B, P, T]
+    const int t = (int)(row % c.T);
+    const int64_t bp = row / c.T, b = BACK ? bp / c.P : bp;
+    const bool is_q = head < c.H, is_v = head >= c.H + c.Hkv;
+    const int own = is_q ? head : is_v ? head - c.H - c.Hkv : head - c.H;
+    const int shared = BACK && !is_q ? c.shared : 1;
+    const int64_t apart = (int64_t)c.T * c.D;  // from one head to the next
+
+    const T* from;
+    T* to;
+    if constexpr (BACK) {
+        const int count = is_q ? c.H : c.Hkv * c.shared;
+        from = static_cast<const T*>(is_q ? c.q : is_v ? c.v : c.k) + ((bp * count + own * shared) * c.T + t) * c.D;
+        to = static_cast<T*>(c.out) + (row * heads + head) * c.D;
+    } else {
+        from = static_cast<const T*>(c.q) + b * c.stride_b + t * c.stride_t + (int64_t)head * c.D;
+        to = static_cast<T*>(is_q ? c.out : c.out_k) + ((b * (is_q ? c.H : c.Hkv) + own) * c.T + t) * c.D;
+    }
+    float x[N], y[N];
+    if (place >= turned) {
+        const int at = c.R + (place - turned) * N;
+        load<T, N>(from + at, shared, apart, x);
+        store<T, N>(to + at, x);
+        return;
+    }
+    const int64_t line = is_v ? 0 : row_of_table(c, b, t);
+    const float nan = __builtin_nanf("");
+    if (c.interleaved) {
+        if constexpr (N % 2 == 0) {
+            load<T, N>(from + place * N, shared, apart, x);
+            if (!is_v) {
+                const float *cs = c.cos + line * (c.R / 2) + place * (N / 2), *sn = c.sin + line * (c.R / 2) + place * (N / 2);
+#pragma unroll
+                for (int e = 0; e < N / 2; ++e) {
+                    const float co = line < 0 ? nan : cs[e], si = line < 0 ? nan : BACK ? -sn[e] : sn[e];
+                    y[2 * e] = x[2 * e] * co - x[2 * e + 1] * si;
+                    y[2 * e + 1] = x[2 * e] * si + x[2 * e + 1] * co;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) y[e] = x[e];
+            }
+            store<T, N>(to + place * N, y);
+        } else {  // one element: its pair's other one is next to it
+            const int at = place, other = at ^ 1;
+            load<T, 1>(from + at, shared, apart, x);
+            if (!is_v) {
+                load<T, 1>(from + other, shared, apart, y);
+                const float co = line < 0 ? nan : c.cos[line * (c.R / 2) + at / 2];
+                float si = line < 0 ? nan : c.sin[line * (c.R / 2) + at / 2];
+                if ((at & 1) == 0) si = -si;
+                if (BACK) si = -si;
+                x[0] = x[0] * co + y[0] * si;
+            }
+            store<T, 1>(to + at, x);
+        }
+        return;
+    }
+    const int at = place * N, half = c.R / 2;
+    load<T, N>(from + at, shared, apart, x);
+    load<T, N>(from + at + half, shared, apart, y);
+    if (!is_v) {
+        const float *cs = c.cos + line * half + at, *sn = c.sin + line * half + at;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float co = line < 0 ? nan : cs[e], si = line < 0 ? nan : BACK ? -sn[e] : sn[e];
+            const float a = x[e], o = y[e];
+            x[e] = a * co - o * si;
+            y[e] = a * si + o * co;
+        }
+    }
+    store<T, N>(to + at, x);
+    store<T, N>(to + at + half, y);
+}
+
+bool off(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+template <typename T, int N, bool BACK> int launch(Call c, int64_t rows, hipStream_t stream) {
+    const int turned = c.interleaved ? c.R / N : c.R / 2 / N;
+    c.units = rows * (c.H + (BACK ? 2 : 1) * c.Hkv) * (turned + (c.D - c.R) / N);
+    for (c.first = 0; c.first < c.units; c.first += MOST_THREADS) {
+        const int64_t count = std::min(c.units - c.first, MOST_THREADS);
+        hipLaunchKernelGGL((rotary_kernel<T, N, BACK>), dim3((unsigned)((count + 255) / 256)), dim3(256), 0, stream, c);
+        LBI_HIP_CHECK(hipGetLastError());
+    }
+    return LBI_OK;
+}
+
+template <typename T, bool BACK> int by_pieces(const Call& c, int64_t rows, hipStream_t stream) {
+    constexpr int N = 16 / sizeof(T);
+    const bool whole = c.D % N == 0 && (c.interleaved ? c.R : c.R / 2) % N == 0 && !off(c.q, 16) && !off(c.k, 16) && !off(c.v, 16) && !off(c.out, 16) &&
+                       !off(c.out_k, 16) && c.stride_b % N == 0 && c.stride_t % N == 0;
+    return whole ? launch<T, N, BACK>(c, rows, stream) : launch<T, 1, BACK>(c, rows, stream);
+}
+template <bool BACK> int by_type(const Call& c, int64_t rows, int dtype, hipStream_t stream) {
+    if (dtype == LBI_F32) return by_pieces<float, BACK>(c, rows, stream);
+    return dtype == LBI_F16 ? by_pieces<_Float16, BACK>(c, rows, stream) : by_pieces<bf16_raw, BACK>(c, rows, stream);
+}
+
+int check(const char* who, int64_t B, int64_t P, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t R, int64_t table, const void* positions, int dtype) {
+    if (B < 0 || P < 0 || T < 0 || H < 1 || Hkv < 1 || D < 1 || R < 0 || R > D || table < 0)
+        return fail(LBI_ERR_INVALID, "%s: bad size (B=%lld P=%lld T=%lld H=%lld Hkv=%lld D=%lld R=%lld table=%lld)", who, (long long)B, (long long)P,
+                    (long long)T, (long long)H, (long long)Hkv, (long long)D, (long long)R, (long long)table);
+    if (H % Hkv) return fail(LBI_ERR_INVALID, "%s: H=%lld not a multiple of Hkv=%lld", who, (long long)H, (long long)Hkv);
+    if (R % 2) return fail(LBI_ERR_INVALID, "%s: rotary embedding needs an even part of a head, got %lld", who, (long long)R);
+    if (!dtype_size(dtype)) return fail(LBI_ERR_INVALID, "%s: bad dtype %d", who, dtype);
+    if (!positions && table < T) return fail(LBI_ERR_INVALID, "%s: tables of %lld positions for %lld tokens", who, (long long)table, (long long)T);
+    if (D > (int64_t)1 << 16 || H > (int64_t)1 << 16 || T >= (int64_t)1 << 31 || P >= (int64_t)1 << 31 || B >= (int64_t)1 << 31 ||
+        B * P >= (int64_t)1 << 31 || B * P * T >= (int64_t)1 << 40)
+        return fail(LBI_ERR_UNSUPPORTED, "%s: too many elements", who);
+    return LBI_OK;
+}
+
+}  // namespace
+}  // namespace rotary
+}  // namespace lbi
+
+extern "C" int lbi_rotary(const void* qkv, const float* cos, const float* sin, const void* positions, void* q, void* k, int64_t B, int64_t T, int64_t H,
+                          int64_t Hkv, int64_t D, int64_t R, int64_t table, int64_t stride_b, int64_t stride_t, int positions_wide, int interleaved,
+                          int dtype, void* stream) {
+    using namespace lbi;
+    using namespace lbi::rotary;
+    clear_error();
+    if (int bad = check("lbi_rotary", B, 1, T, H, Hkv, D, R, table, positions, dtype)) return bad;
+    if (!B || !T) return LBI_OK;
+    if (!qkv || !q || !k || (R && table && (!cos || !sin))) return fail(LBI_ERR_INVALID, "lbi_rotary: null pointer");
+    const size_t size = dtype_size(dtype);
+    if (off(qkv, size) || off(q, size) || off(k, size) || off(cos, 4) || off(sin, 4) || off(positions, positions_wide ? 8 : 4))
+        return fail(LBI_ERR_INVALID, "lbi_rotary: a tensor is not aligned to its elements");
+    Call c{};
+    c.q = qkv, c.out = q, c.out_k = k, c.cos = cos, c.sin = sin, c.positions = positions;
+    c.stride_b = stride_b, c.stride_t = stride_t, c.table = table, c.positions_wide = positions_wide != 0;
+    c.P = 1, c.T = (int)T, c.H = (int)H, c.Hkv = (int)Hkv, c.shared = 1, c.D = (int)D, c.R = (int)R, c.interleaved = interleaved != 0;
+    return by_type<false>(c, B * T, dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int lbi_rotary_pullback(const void* dq, const void* dk, const void* dv, const float* cos, const float* sin, const void* positions, void* g_qkv,
+                                   int64_t B, int64_t P, int64_t T, int64_t H, int64_t Hkv, int64_t kv_heads, int64_t D, int64_t R, int64_t table,
+                                   int positions_wide, int interleaved, int dtype, void* stream) {
+    using namespace lbi;
+    using namespace lbi::rotary;
+    clear_error();
+    if (int bad = check("lbi_rotary_pullback", B, P, T, H, Hkv, D, R, table, positions, dtype)) return bad;
+    if (kv_heads != H && kv_heads != Hkv)
+        return fail(LBI_ERR_INVALID, "lbi_rotary_pullback: dk and dv of %lld heads, neither H=%lld nor Hkv=%lld", (long long)kv_heads, (long long)H, (long long)Hkv);
+    if (!B || !P || !T) return LBI_OK;
+    if (!dq || !dk || !dv || !g_qkv || (R && table && (!cos || !sin))) return fail(LBI_ERR_INVALID, "lbi_rotary_pullback: null pointer");
+    const size_t size = dtype_size(dtype);
+    if (off(dq, size) || off(dk, size) || off(dv, size) || off(g_qkv, size) || off(cos, 4) || off(sin, 4) || off(positions, positions_wide ? 8 : 4))
+        return fail(LBI_ERR_INVALID, "lbi_rotary_pullback: a tensor is not aligned to its elements");
+    Call c{};
+    c.q = dq, c.k = dk, c.v = dv, c.out = g_qkv, c.cos = cos, c.sin = sin, c.positions = positions;
+    c.table = table, c.positions_wide = positions_wide != 0;
+    c.P = (int)P, c.T = (int)T, c.H = (int)H, c.Hkv = (int)Hkv, c.shared = (int)(kv_heads / Hkv), c.D = (int)D, c.R = (int)R, c.interleaved = interleaved != 0;
+    return by_type<true>(c, B * P * T, dtype, static_cast<hipStream_t>(stream));
+}

@@ -119,6 +119,102 @@ def residual_rmsnorm_pullback(g_normed: torch.Tensor, residual_out: torch.Tensor
     return g_hidden, g_stream, g_weight
 
 
+def _rows_of_gate(what: str, gate: torch.Tensor | None, branch: torch.Tensor) -> int:
+    """Rows of ``branch [..., D]`` for each row of the gate; 0: each has its own."""
+    if gate is None:
+        return 0
+    if gate.dtype != branch.dtype:
+        raise ValueError(f"{what}: gate must be in the dtype of the branch")
+    if gate.shape == branch.shape and gate.dim() > 1:
+        return 0
+    if gate.shape == branch.shape[-1:]:
+        return max(branch.numel() // max(branch.shape[-1], 1), 1)
+    if gate.dim() == branch.dim() > 2 and gate.shape[0] == branch.shape[0] and gate.shape[-1] == branch.shape[-1] \
+            and all(extent == 1 for extent in gate.shape[1:-1]):
+        return max(branch[:1].numel() // max(branch.shape[-1], 1), 1)
+    raise ValueError(f"{what}: gate must be [D], [B, 1, ..., D] or shaped like the branch")
+
+
+def gated_residual_rmsnorm(branch: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor, weight: torch.Tensor, eps: float, *,
+                           gate: torch.Tensor | None = None, residual_scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """A branch's way into the residual stream, and the next norm, in one pass: ``u = rmsnorm(branch) * post_weight``,
+    ``s = residual_scale * residual + gate * u`` and ``y = rmsnorm(s) * weight`` over the last dimension.
+
+    ``branch, residual [..., D]``, weights ``[D]``; ``gate`` in the dtype of ``branch``: ``[D]`` (each channel's), ``[B, 1, ..., D]`` (each sequence's) or
+    ``[..., D]`` (each position's; a branch without leading dimensions has the first only).  Returns ``(y, s)`` in the dtypes of ``branch`` and of
+    ``residual`` (that of ``branch`` or fp32).  Sums are fp32 and each result is rounded once."""
+    what = "gated_residual_rmsnorm"
+    if branch.dim() < 1 or residual.shape != branch.shape or post_weight.shape != branch.shape[-1:] or weight.shape != branch.shape[-1:]:
+        raise ValueError(f"{what}: branch and residual must be [..., D] and the weights [D]")
+    per_gate = _rows_of_gate(what, gate, branch)
+    _one_device(what, branch, residual, post_weight, weight, gate)
+    _lib.refuse_graph(what, branch, residual, post_weight, weight, gate)
+    stream = residual.dtype
+    post_weight = _norm_types(what, branch.dtype, stream, post_weight).contiguous()
+    weight = _norm_types(what, branch.dtype, stream, weight).contiguous()
+    branch, residual = branch.contiguous(), residual.contiguous()
+    gate = None if gate is None else gate.contiguous()
+    normed, total = torch.empty_like(branch), torch.empty_like(residual)
+    count, width = branch.numel(), branch.shape[-1]
+    if count:
+        with _lib.device_guard(branch.device):
+            status = _lib.load().lbi_gated_residual_rmsnorm(
+                branch.data_ptr(), residual.data_ptr(), None if gate is None else gate.data_ptr(), post_weight.data_ptr(), weight.data_ptr(),
+                normed.data_ptr(), total.data_ptr(), count // width, width, per_gate, float(eps), float(residual_scale), _lib.dtype_code(branch.dtype),
+                _lib.dtype_code(stream), _lib.dtype_code(post_weight.dtype), _lib.dtype_code(weight.dtype), _stream(branch))
+        _lib.check(status, "lbi_gated_residual_rmsnorm")
+    return normed, total
+
+
+def gated_residual_rmsnorm_pullback(
+        g_normed: torch.Tensor, branch: torch.Tensor, residual_out: torch.Tensor, post_weight: torch.Tensor, weight: torch.Tensor, eps: float, *,
+        gate: torch.Tensor | None = None, residual_scale: float = 1.0, g_residual: torch.Tensor | None = None
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor, torch.Tensor]:
+    """The cotangents of :func:`gated_residual_rmsnorm` from ``g_normed`` (of its ``y``) and ``g_residual`` (of its ``s``; ``None``: zero), at the
+    ``branch`` that it was given and the ``residual_out`` that it returned as ``s``.
+
+    Returns ``(g_branch, g_residual_in, g_gate, g_post_weight, g_weight)``: in the dtypes of ``branch`` and ``residual_out``, the gate's shaped like it
+    (in its dtype for a gate of each position; otherwise summed over the rows that it gates, in fp32; ``None`` without one), and the weights' in fp32
+    ``[D]``, summed over all rows.  Sums run in a fixed order."""
+    what = "gated_residual_rmsnorm_pullback"
+    if branch.dim() < 1 or g_normed.shape != branch.shape or residual_out.shape != branch.shape or post_weight.shape != branch.shape[-1:] \
+            or weight.shape != branch.shape[-1:]:
+        raise ValueError(f"{what}: g_normed, branch and residual_out must be [..., D] and the weights [D]")
+    if g_normed.dtype != branch.dtype:
+        raise ValueError(f"{what}: g_normed must be in the dtype of branch")
+    if g_residual is not None and (g_residual.shape != branch.shape or g_residual.dtype != residual_out.dtype):
+        raise ValueError(f"{what}: g_residual must have the shape and dtype of residual_out")
+    per_gate = _rows_of_gate(what, gate, branch)
+    _one_device(what, g_normed, branch, residual_out, post_weight, weight, gate, g_residual)
+    _lib.refuse_graph(what, g_normed, branch, residual_out, post_weight, weight, gate, g_residual)
+    stream = residual_out.dtype
+    post_weight = _norm_types(what, branch.dtype, stream, post_weight).contiguous()
+    weight = _norm_types(what, branch.dtype, stream, weight).contiguous()
+    g_normed, branch, residual_out = g_normed.contiguous(), branch.contiguous(), residual_out.contiguous()
+    gate = None if gate is None else gate.contiguous()
+    g_residual = None if g_residual is None else g_residual.contiguous()
+    g_branch, g_stream = torch.empty_like(branch), torch.empty_like(residual_out)
+    g_gate = None if gate is None else torch.empty_like(gate, dtype=torch.float32 if per_gate else None)
+    count, width = branch.numel(), int(branch.shape[-1])
+    if not count:
+        zeros = branch.new_zeros(2, width, dtype=torch.float32)
+        return g_branch, g_stream, None if g_gate is None else g_gate.zero_(), zeros[0], zeros[1]
+    g_post_weight, g_weight = (branch.new_empty(width, dtype=torch.float32) for _ in range(2))
+    rows = count // width
+    lib = _lib.load()
+    with _lib.device_guard(branch.device):
+        need = lib.lbi_gated_residual_rmsnorm_pullback_workspace_bytes(rows, width, per_gate)
+        workspace = branch.new_empty(need, dtype=torch.uint8)
+        status = lib.lbi_gated_residual_rmsnorm_pullback(
+            g_normed.data_ptr(), branch.data_ptr(), residual_out.data_ptr(), None if g_residual is None else g_residual.data_ptr(),
+            None if gate is None else gate.data_ptr(), post_weight.data_ptr(), weight.data_ptr(), g_branch.data_ptr(), g_stream.data_ptr(),
+            None if g_gate is None else g_gate.data_ptr(), g_post_weight.data_ptr(), g_weight.data_ptr(), workspace.data_ptr(), need, rows, width,
+            per_gate, float(eps), float(residual_scale), _lib.dtype_code(branch.dtype), _lib.dtype_code(stream),
+            _lib.dtype_code(post_weight.dtype), _lib.dtype_code(weight.dtype), _stream(branch))
+    _lib.check(status, "lbi_gated_residual_rmsnorm_pullback")
+    return g_branch, g_stream, g_gate, g_post_weight, g_weight
+
+
 def _check_mlp(what: str, x: torch.Tensor, fc1_weight: torch.Tensor, fc2_weight: torch.Tensor) -> tuple[int, int, int, int]:
     """``(rows, D, hidden, width)``."""
     if x.dtype not in _PRODUCT_TYPES:
@@ -208,4 +304,4 @@ def gated_mlp_vjp(g_out: torch.Tensor, x: torch.Tensor, fc1_output: torch.Tensor
     return (g_x, g_fc1, g_fc2, g_fc1_bias, g_fc2_bias) if bias else (g_x, g_fc1, g_fc2)
 
 
-__all__ = ["gated_mlp", "gated_mlp_vjp", "residual_rmsnorm", "residual_rmsnorm_pullback"]
+__all__ = ["gated_mlp", "gated_mlp_vjp", "gated_residual_rmsnorm", "gated_residual_rmsnorm_pullback", "residual_rmsnorm", "residual_rmsnorm_pullback"]
