@@ -45,10 +45,11 @@ struct Call {
     Chain chain[MOST_CHAINS];
     const float* log_decay;  // [H]
     const void* lengths;     // [B], NULL: T; 8 bytes each if lengths_wide
-    float* segment_states;   // [units / segments, segments, Da, Dc] in front of each segment
+    float* segment_states;   // [chains, B, P, H, segments - 1, Da, Dc]
     int chains, lengths_wide;
     int B, P, H, T;
     int segments, segment;  // tokens of one, a multiple of CHUNK
+    int joined;             // a launch of its own makes the states behind the segments of what these add
 };
 
 }  // namespace linear_attn

@@ -24,22 +24,22 @@ int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
     return dtype == LBI_F16 ? run_f16(call, stream) : run_bf16(call, exact_last, stream);
 }
 
-// Segments that a chain is cut into, so many tokens each: none while the chains alone fill the chip.
+// Segments that a chain is cut into: none while the chains alone fill the chip.
 int segments_of(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
-    const int64_t chunks = (T + CHUNK - 1) / CHUNK, room = (int64_t)device_compute_units() * (Da > 64 && Dc > 64 ? 2 : 3);
+    const int64_t chunks = (T + CHUNK - 1) / CHUNK, room = (int64_t)device_compute_units() * (Dc > 64 ? 1 : 2);
     if (units * 2 > room || chunks < 4) return 1;
     const int64_t wanted = std::min(room / units, chunks / 2), of = (chunks + wanted - 1) / wanted;
     return (int)((chunks + of - 1) / of);
 }
 size_t states_bytes(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
-    const int segments = segments_of(units, T, Da, Dc);
-    return segments > 1 ? (size_t)units * segments * Da * Dc * sizeof(float) : 0;
+    return (size_t)units * (segments_of(units, T, Da, Dc) - 1) * Da * Dc * sizeof(float);
 }
 void cut(Call& call, float* workspace) {
     const int64_t chunks = (call.T + CHUNK - 1) / CHUNK;
     call.segments = segments_of((int64_t)call.chains * call.B * call.P * call.H, call.T, call.chain[0].Da, call.chain[0].Dc);
     call.segment = (int)((chunks + call.segments - 1) / call.segments) * CHUNK;
     call.segment_states = workspace;
+    call.joined = call.segments > 8;
 }
 
 bool any_null(std::initializer_list<const void*> pointers) {

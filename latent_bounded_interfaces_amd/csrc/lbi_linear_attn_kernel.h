@@ -1,19 +1,24 @@
 // The kernels of linear attention over chunks (lbi_linear_attn.h has the mathematics).
 //
-// A workgroup takes the chunks of one segment of one chain one after the other; its four waves hold a quarter of the state's columns each, in
-// fp32 and in registers for the whole segment, and never exchange it: the accumulators of X, packed, are the operand of the next readout.
-//   1  wave w: pairs of tokens i = 16 w ... 16 w + 15 with all j <= i, times l^(i-j), rounded to 16 bits into LDS
-//   2  every wave: out^T of its columns = X^T a^T, times l^(i+1), plus c^T pairs^T
-//   3  every wave: X = l^64 X + b^T (l^(63-j) c), the decayed c in planes of 16 bits whose sum has 16 (22 in half precision) significant bits
-// The next chunk's tiles are on their way in registers meanwhile.
+// A workgroup takes the chunks of one segment of one chain one after the other.  Each of its waves holds 16 columns of the state, in fp32 and in
+// registers for the whole segment, and never exchanges them: the accumulators of X, packed, are the operand of the next readout.
+//   1  waves 0 ... 3: the scores of 16 tokens i each with all j <= i, times l^(i-j), rounded to 16 bits into LDS
+//   2  every wave: out^T of its columns = X^T a^T, times l^(i+1), plus c^T scores^T
+//   3  every wave: X = l^64 X + b^T (l^(63-j) c), the decayed c in planes of 16 bits that add up to 16 or 24 significant bits (22 in half precision)
+// The next chunk's tiles are on their way into the other half of the LDS meanwhile, past the registers.
 #pragma once
 
 #include "lbi_linear_attn.h"
+#include "lbi_scan_planes.h"
 
 namespace lbi {
 namespace linear_attn {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr unsigned NOWHERE = 0x80000000u;  // an offset past the end of every buffer
+
+// Everything that this wave has in LDS is there, for all waves; transfers from and to memory stay under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <typename T> struct Mma16;
 template <> struct Mma16<bf16_raw> {
@@ -52,36 +57,45 @@ __device__ __forceinline__ float rate_of(const Call& call, int h) {
     return l < -1e30f ? -1e30f : l;
 }
 
-// Tile of 64 tokens x W elements: rows of 16-byte pieces, DIM / 8 of them, from tensors whose rows start on any element (!VEC: and whose
-// widths are any).
-template <typename T, int DIM, bool VEC> struct Tile {
-    static constexpr int PIECES = DIM / 8, N = CHUNK * PIECES / 256;
-    u32x4 regs[N];
-    // local tokens first ... first + 63; what is at or past `end` and columns past `dim` are zero
-    __device__ __forceinline__ void fetch(const T* base, int64_t st, bool reverse, int n, int first, int end, int dim) {
-        const T* from = base + (reverse ? (int64_t)(n - first - CHUNK) : (int64_t)first) * st;
+// A tile of 64 tokens, rows of DIM 16-bit elements in LDS (16-byte pieces, swizzled as in lbi_attn_mfma.h).  VEC: by transfers of 16 bytes past the
+// registers, zeros past the end of a row and behind the last token; otherwise, rows that start on any element, an element at a time.
+template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
+    static constexpr int PIECES = DIM / 8, N = CHUNK * PIECES / THREADS;
+    const T* base;
+    int64_t st;
+    int dim;
+    unsigned full[N];  // offsets of this lane's pieces from the first token in memory of a whole chunk
+    __device__ __forceinline__ unsigned piece_of(int u, int count, bool reverse) const {
+        const int id = u * THREADS + (int)threadIdx.x, r = id / PIECES, slot = id % PIECES;
+        const int chunk = tile_off<DIM>(r, slot) / 16 % PIECES;  // the swizzle is its own inverse
+        const int64_t at = (int64_t)(reverse ? count - 1 - r : r) * st + chunk * 8;
+        return r < count && chunk * 8 < dim ? (unsigned)(at * 2) : NOWHERE;
+    }
+    __device__ __forceinline__ Tile(const T* base_, int64_t st_, int dim_, bool reverse) : base(base_), st(st_), dim(dim_) {
+        if constexpr (VEC)
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int id = threadIdx.x + 256 * u, r = id / PIECES, c = id % PIECES * 8;
-            const T* p = from + (int64_t)(reverse ? CHUNK - 1 - r : r) * st + c;
-            regs[u] = u32x4{0, 0, 0, 0};
-            if (first + r < end && c < dim) {
-                if constexpr (VEC) {
-                    regs[u] = *reinterpret_cast<const u32x4*>(p);
-                } else {
-                    const unsigned short* raw = reinterpret_cast<const unsigned short*>(p);
+            for (int u = 0; u < N; ++u) full[u] = piece_of(u, CHUNK, reverse);
+    }
+    // local tokens first ... first + count - 1 of the n that count
+    __device__ __forceinline__ void bring(char* tile, unsigned tile_at, bool reverse, int n, int first, int count) const {
+        const T* from = base + (int64_t)(reverse ? n - first - count : first) * st;
+        if constexpr (VEC) {
+            const auto source = scan_planes::rows(from, 0x7fffffffu);
+            const unsigned to = tile_at + (threadIdx.x >> 6) * 1024;
+#pragma unroll
+            for (int u = 0; u < N; ++u) scan_planes::dma16(source, count == CHUNK ? full[u] : piece_of(u, count, reverse), 0, to + u * THREADS * 16);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int id = u * THREADS + (int)threadIdx.x, r = id / PIECES, c = id % PIECES * 8;
+                const unsigned short* raw = reinterpret_cast<const unsigned short*>(from + (int64_t)(reverse ? count - 1 - r : r) * st + c);
+                u32x4 words = {0, 0, 0, 0};
+                if (r < count)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        regs[u][e] = (c + 2 * e < dim ? raw[2 * e] : 0u) | (c + 2 * e + 1 < dim ? (unsigned)raw[2 * e + 1] << 16 : 0u);
-                }
+                        words[e] = (c + 2 * e < dim ? raw[2 * e] : 0u) | (c + 2 * e + 1 < dim ? (unsigned)raw[2 * e + 1] << 16 : 0u);
+                *reinterpret_cast<u32x4*>(tile + tile_off<DIM>(r, c / 8)) = words;
             }
-        }
-    }
-    __device__ __forceinline__ void commit(char* tile) const {
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int id = threadIdx.x + 256 * u;
-            *reinterpret_cast<u32x4*>(tile + tile_off<DIM>(id / PIECES, id % PIECES)) = regs[u];
         }
     }
 };
@@ -123,276 +137,235 @@ __device__ __forceinline__ bool unit_of(const Call& call, int segments, Unit& u)
     return true;
 }
 
-// OUT false: only the state that a segment leaves behind, from zero, into the slot of the next one.
+template <int DA, int DC, bool OUT> constexpr int stage_bytes() { return CHUNK * 2 * ((OUT ? 2 : 1) * DA + DC); }
+template <int DA, int DC, bool OUT> constexpr int lds_bytes() { return 2 * stage_bytes<DA, DC, OUT>() + (OUT ? CHUNK * CHUNK * 2 : 0); }
+
+// OUT false: only the state that a segment leaves behind, from zero, into its slot.
 template <typename T, int DA, int DC, bool VEC, bool OUT, int PLANES>
-__global__ __launch_bounds__(256, 2) void chunk_kernel(Call call) {
+__global__ __launch_bounds__(4 * DC, 2) void chunk_kernel(Call call) {
     constexpr bool HALF = std::is_same_v<T, _Float16>;
-    constexpr int KS = DA / 32, MT = DA / 16, NT = DC / 64;  // steps and tiles of the state: rows, this wave's columns
-    __shared__ __align__(16) char lds[(OUT ? CHUNK * DA * 2 : 0) + CHUNK * DA * 2 + CHUNK * DC * 2 + (OUT ? CHUNK * CHUNK * 2 : 0)];
-    __shared__ float pair_up[4];
-    char* const tb = lds;
-    char* const tc = tb + CHUNK * DA * 2;
-    char* const ta = tc + CHUNK * DC * 2;
-    char* const tp = ta + CHUNK * DA * 2;
+    constexpr int THREADS = 4 * DC, KS = DA / 32, MT = DA / 16, STAGE = stage_bytes<DA, DC, OUT>();
+    extern __shared__ __align__(16) char lds[];  // two of: b, c, a; then the scores
+    __shared__ float score_up[4];
+    char* const tp = lds + 2 * STAGE;
     Unit u;
     if (!unit_of(call, OUT ? call.segments : call.segments - 1, u)) return;
     const Chain& ch = call.chain[u.chain];
-    const int n = length_of(call, u.b), w = threadIdx.x >> 6, m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const int n = length_of(call, u.b), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
     const int begin = u.segment * call.segment, end = begin + call.segment < n ? begin + call.segment : n;  // of the tokens that count
-    const int stop = OUT ? (begin + call.segment < call.T ? begin + call.segment : call.T) : end;           // of the rows written
     auto at = [&](const View& v) { return static_cast<const T*>(v.p) + u.b * v.sb + u.p * v.sp + (u.h / v.group) * v.sh; };
-    const T *a = OUT ? at(ch.a) : nullptr, *b = at(ch.b), *c = at(ch.c);
     const bool reverse = ch.reverse != 0;
     const float rate = rate_of(call, u.h), rate2 = rate * LOG2E;
-    const int shift = ch.shift, Da = ch.Da, Dc = ch.Dc;
-    const int col0 = w * (DC / 4);
+    const int shift = ch.shift, Da = ch.Da, Dc = ch.Dc, col = 16 * w + m;
 
-    float pair[4][4], read[4], keep[2][8];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int apart = 16 * w + m - (16 * t + 4 * g + r);
-            pair[t][r] = apart < 0 ? 0.0f : exp2f(rate2 * (float)apart);
-        }
-        read[t] = exp2f(rate2 * (float)(16 * t + m + 1 - shift));
-    }
-    auto weigh = [&](int count) {  // of a chunk of `count` tokens
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int left = count - 1 - (32 * ks + 8 * g + e);
-                keep[ks][e] = exp2f(rate2 * (float)((left < 0 ? 0 : left) + shift));
-            }
+    const Tile<T, DA, THREADS, VEC> a(OUT ? at(ch.a) : nullptr, ch.a.st, Da, reverse), b(at(ch.b), ch.b.st, Da, reverse);
+    const Tile<T, DC, THREADS, VEC> c(at(ch.c), ch.c.st, Dc, reverse);
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
+    auto bring = [&](int stage, int from) {
+        const int count = end - from < CHUNK ? end - from : CHUNK, to = stage * STAGE;
+        b.bring(lds + to, lds0 + to, reverse, n, from, count);
+        c.bring(lds + to + CHUNK * 2 * DA, lds0 + to + CHUNK * 2 * DA, reverse, n, from, count);
+        if constexpr (OUT) a.bring(lds + to + CHUNK * 2 * (DA + DC), lds0 + to + CHUNK * 2 * (DA + DC), reverse, n, from, count);
     };
-    weigh(CHUNK);
+    if (begin < end) bring(0, begin);
+
+    // l to the power of tokens apart, as products of l^0 ... l^31 of this lane's place and of l^16, l^32, l^48
+    const float l16 = exp2f(rate2 * 16.0f), l32 = exp2f(rate2 * 32.0f), l48 = exp2f(rate2 * 48.0f);
+    const float read0 = exp2f(rate2 * (float)(m + 1 - shift));
+    float near[4], far[4], keep[8];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int apart = m - 4 * g - r;
+        near[r] = exp2f(rate2 * (float)(apart < 0 ? 0 : apart));
+        far[r] = exp2f(rate2 * (float)(16 + apart));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) keep[e] = exp2f(rate2 * (float)(31 - 8 * g - e + shift));
     float fade = expm1f(rate * (float)CHUNK);  // X + X (l^64 - 1) keeps what rounding l^64 near 1 would add up over many chunks
 
-    f32x4 x[MT][NT];
-    const float* first = OUT ? (call.segments > 1 ? call.segment_states : ch.first.p) : nullptr;
-    if (OUT && first) {
-        int64_t sr = Dc, sc = 1;
-        float factor = 1.0f;
-        if (call.segments > 1) {
-            first += ((int64_t)u.number * call.segments + u.segment) * Da * Dc;
-        } else {
-            first += u.b * ch.first.sb + u.p * ch.first.sp + u.h * ch.first.sh;
-            sr = ch.first.sr, sc = ch.first.sc, factor = ch.first_scale;
-        }
+    f32x4 x[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto each = [&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * i + 4 * g + r, col = col0 + 16 * j + m;
-                    x[i][j][r] = row < Da && col < Dc ? first[row * sr + col * sc] * factor : 0.0f;
-                }
-    } else {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) x[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    if constexpr (OUT) {  // pairs of later tokens stay zero
-        for (int i = threadIdx.x; i < CHUNK * CHUNK * 2 / 16; i += 256) reinterpret_cast<u32x4*>(tp)[i] = u32x4{0, 0, 0, 0};
-    }
-
-    Tile<T, DA, VEC> na, nb;
-    Tile<T, DC, VEC> nc;
-    auto bring = [&](int from) {
-        if constexpr (OUT) na.fetch(a, ch.a.st, reverse, n, from, end, Da);
-        nb.fetch(b, ch.b.st, reverse, n, from, end, Da);
-        nc.fetch(c, ch.c.st, reverse, n, from, end, Dc);
+            for (int r = 0; r < 4; ++r)
+                if (16 * i + 4 * g + r < Da && col < Dc) x[i][r] = f(x[i][r], 16 * i + 4 * g + r);
     };
-    if (begin < end) bring(begin);
-    for (int from = begin; from < end; from += CHUNK) {
-        __syncthreads();  // everyone is done with the tiles
-        if constexpr (OUT) na.commit(ta);
-        nb.commit(tb);
-        nc.commit(tc);
-        __syncthreads();
-        if (from + CHUNK < end) bring(from + CHUNK);
+    if constexpr (OUT) {
+        const float* slots = call.segment_states + (int64_t)u.number * (call.segments - 1) * Da * Dc;
+        if (ch.first.p && (u.segment == 0 || !call.joined)) {
+            const float* first = ch.first.p + u.b * ch.first.sb + u.p * ch.first.sp + u.h * ch.first.sh + col * ch.first.sc;
+            each([&](float, int row) __attribute__((always_inline)) { return first[row * ch.first.sr] * ch.first_scale; });
+        }
+        for (int s = call.joined ? u.segment - 1 : 0; s >= 0 && s < u.segment; ++s) {  // what the segments before add, the first one first
+            int tokens = n - s * call.segment;
+            tokens = tokens < 0 ? 0 : tokens > call.segment ? call.segment : tokens;
+            const float left = call.joined ? -1.0f : expm1f(rate * (float)tokens);
+            const float* slot = slots + (int64_t)s * Da * Dc + col;
+            each([&](float v, int row) __attribute__((always_inline)) { return fmaf(v, left, v) + slot[row * Dc]; });
+        }
+        // scores of later tokens stay zero
+        for (int i = threadIdx.x; i < CHUNK * CHUNK * 2 / 16; i += THREADS) reinterpret_cast<u32x4*>(tp)[i] = u32x4{0, 0, 0, 0};
+    }
+    scan_planes::wait_vm<0>();
+
+    int stage = 0;
+    for (int from = begin; from < end; from += CHUNK, stage ^= 1) {
+        lds_barrier();  // this chunk's tiles are there, and everyone is done with the ones before
+        if (from + CHUNK < end) bring(stage ^ 1, from + CHUNK);
+        const char *tb = lds + stage * STAGE, *tc = tb + CHUNK * 2 * DA, *ta = tc + CHUNK * 2 * DC;
         const int count = end - from < CHUNK ? end - from : CHUNK;
 
-        f32x4 acc[OUT ? NT : 1][4];
-        float bring_up = 1.0f;
+        f32x4 acc[4];
         if constexpr (OUT) {
-            f32x4 s[4];
+            if (w < 4) {
+                f32x4 s[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int t = 0; t < 4; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 mine = nat<DA>(ta, 16 * w + m, 4 * ks + g);
+                for (int ks = 0; ks < KS; ++ks) {
+                    const u32x4 mine = nat<DA>(ta, 16 * w + m, 4 * ks + g);
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    if (t <= w) s[t] = Mma16<T>::mma(nat<DA>(tb, 16 * t + m, 4 * ks + g), mine, s[t]);
-            }
-            float down = 1.0f;
-            if constexpr (HALF) {
+                    for (int t = 0; t < 4; ++t)
+                        if (t <= w) s[t] = Mma16<T>::mma(nat<DA>(tb, 16 * t + m, 4 * ks + g), mine, s[t]);
+                }
                 float most = 0.0f;
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(s[t][r] * pair[t][r]));
-                const Pow2 by = into_range(over_wave_max(most));
-                down = by.down;
-                if ((threadIdx.x & 63) == 0) pair_up[w] = by.up;
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t <= w) {
-                    float v[4];
+                for (int t = 0; t < 4; ++t) {
+                    const float more = w - t == 2 ? l16 : w - t == 3 ? l32 : 1.0f;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        v[r] = 16 * w + m < 16 * t + 4 * g + r ? 0.0f : s[t][r] * pair[t][r];
-                        if constexpr (HALF) v[r] *= down;
+                        s[t][r] = t < w ? s[t][r] * (far[r] * more) : t == w && m >= 4 * g + r ? s[t][r] * near[r] : 0.0f;
+                        if constexpr (HALF) most = fmaxf(most, fabsf(s[t][r]));
                     }
-                    *reinterpret_cast<u32x2*>(tp + tile_off<CHUNK>(16 * w + m, 2 * t + (g >> 1)) + 8 * (g & 1)) =
-                        u32x2{Mma<T>::pack2(v[0], v[1]), Mma<T>::pack2(v[2], v[3])};
                 }
+                if constexpr (HALF) {
+                    const Pow2 by = into_range(over_wave_max(most));
+                    if ((threadIdx.x & 63) == 0) score_up[w] = by.up;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) s[t] *= by.down;
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    if (t <= w)
+                        *reinterpret_cast<u32x2*>(tp + tile_off<CHUNK>(16 * w + m, 2 * t + (g >> 1)) + 8 * (g & 1)) =
+                            u32x2{Mma<T>::pack2(s[t][0], s[t][1]), Mma<T>::pack2(s[t][2], s[t][3])};
+            }
             // what the state in front of the chunk gives
+            Pow2 state_by = {1.0f, 1.0f};
             if constexpr (HALF) {
                 float most = 0.0f;
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(x[i][j][r]));
-                const Pow2 by = into_range(over_wave_max(most));
-                down = by.down;
-                bring_up = by.up;
+                    for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(x[i][r]));
+                state_by = into_range(over_wave_max(most));
             }
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) acc[j][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                u32x4 state[NT];
+                const f32x4 lo = x[2 * ks] * state_by.down, hi = x[2 * ks + 1] * state_by.down;
+                const u32x4 state = {Mma<T>::pack2(lo[0], lo[1]), Mma<T>::pack2(lo[2], lo[3]), Mma<T>::pack2(hi[0], hi[1]), Mma<T>::pack2(hi[2], hi[3])};
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const f32x4 lo = x[2 * ks][j] * down, hi = x[2 * ks + 1][j] * down;
-                    state[j] = u32x4{Mma<T>::pack2(lo[0], lo[1]), Mma<T>::pack2(lo[2], lo[3]), Mma<T>::pack2(hi[0], hi[1]), Mma<T>::pack2(hi[2], hi[3])};
-                }
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const u32x4 mine = split<DA>(ta, 16 * t + m, ks, g);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(state[j], mine, acc[j][t]);
-                }
+                for (int t = 0; t < 4; ++t) acc[t] = Mma16<T>::mma(state, split<DA>(ta, 16 * t + m, ks, g), acc[t]);
             }
-            __syncthreads();  // the pairs are there
+            lds_barrier();  // the scores are there
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                float by = read[t];
-                if constexpr (HALF) by *= bring_up / pair_up[t];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j][t] *= by;
+                float by = read0 * (t == 0 ? 1.0f : t == 1 ? l16 : t == 2 ? l32 : l48);
+                if constexpr (HALF) by *= state_by.up / score_up[t];
+                acc[t] *= by;
             }
         }
 
-        // the chunk's c: as it is for the pairs, decayed for the state
-        if (count < CHUNK) {
-            weigh(count);
-            fade = expm1f(rate * (float)count);
-        }
+        // the chunk's c: as it is for the scores, decayed for the state
+        if (count < CHUNK) fade = expm1f(rate * (float)count);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[i][j][r] = fmaf(x[i][j][r], fade, x[i][j][r]);
+            for (int r = 0; r < 4; ++r) x[i][r] = fmaf(x[i][r], fade, x[i][r]);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            u32x4 plane[PLANES][NT];
+            if (count < CHUNK)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const u32x4 raw = turned<DC>(tc, 32 * ks + 8 * g, col0 + 16 * j);
-                if constexpr (OUT)
+                for (int e = 0; e < 8; ++e) {
+                    const int left = count - 1 - (32 * ks + 8 * g + e);
+                    keep[e] = exp2f(rate2 * (float)((left < 0 ? 0 : left) + shift));
+                }
+            const float more = ks == 0 && count == CHUNK ? l32 : 1.0f;
+            const u32x4 raw = turned<DC>(tc, 32 * ks + 8 * g, 16 * w);
+            if constexpr (OUT)
 #pragma unroll
-                    for (int t = 2 * ks; t < 4; ++t) acc[j][t] = Mma16<T>::mma(raw, nat<CHUNK>(tp, 16 * t + m, 4 * ks + g), acc[j][t]);
+                for (int t = 2 * ks; t < 4; ++t) acc[t] = Mma16<T>::mma(raw, nat<CHUNK>(tp, 16 * t + m, 4 * ks + g), acc[t]);
+            u32x4 plane[PLANES];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float lo = Mma<T>::lo(raw[e]) * keep[ks][2 * e], hi = Mma<T>::hi(raw[e]) * keep[ks][2 * e + 1];
+            for (int e = 0; e < 4; ++e) {
+                float lo = Mma<T>::lo(raw[e]) * (keep[2 * e] * more), hi = Mma<T>::hi(raw[e]) * (keep[2 * e + 1] * more);
 #pragma unroll
-                    for (int q = 0; q < PLANES; ++q) {
-                        const unsigned word = Mma<T>::pack2(lo, hi);
-                        plane[q][j][e] = word;
-                        lo -= Mma<T>::lo(word), hi -= Mma<T>::hi(word);
-                    }
+                for (int q = 0; q < PLANES; ++q) {
+                    const unsigned word = Mma<T>::pack2(lo, hi);
+                    plane[q][e] = word;
+                    lo -= Mma<T>::lo(word), hi -= Mma<T>::hi(word);
                 }
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const u32x4 bt = turned<DA>(tb, 32 * ks + 8 * g, 16 * i);
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int q = PLANES - 1; q >= 0; --q) x[i][j] = Mma16<T>::mma(bt, plane[q][j], x[i][j]);
+                for (int q = PLANES - 1; q >= 0; --q) x[i] = Mma16<T>::mma(bt, plane[q], x[i]);
             }
         }
 
         if constexpr (OUT) {
-            T* out = const_cast<T*>(at(ch.out));
+            T* const out = const_cast<T*>(at(ch.out)) + (int64_t)(reverse ? n - from - count : from) * ch.out.st;
+            const auto to = scan_planes::rows(out, 0x7fffffffu);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const int i = from + 16 * t + m;
+                const int i = 16 * t + m, row = reverse ? count - 1 - i : i, first = 16 * w + 4 * g;
                 float by = ch.scale;
-                if constexpr (HALF) by *= pair_up[t];
-                if (i < end) {
-                    T* row = out + (int64_t)(reverse ? n - 1 - i : i) * ch.out.st;
+                if constexpr (HALF) by *= score_up[t];
+                const u32x2 words = {Mma<T>::pack2(acc[t][0] * by, acc[t][1] * by), Mma<T>::pack2(acc[t][2] * by, acc[t][3] * by)};
+                if constexpr (VEC) {  // each wave has the same number of stores under way, whatever there is to store
+                    __builtin_amdgcn_raw_buffer_store_b64(words, to, i < count && first < Dc ? (unsigned)(((int64_t)row * ch.out.st + first) * 2) : NOWHERE, 0, 0);
+                } else if (i < count) {
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const int col = col0 + 16 * j + 4 * g;
-                        const u32x2 words = {Mma<T>::pack2(acc[j][t][0] * by, acc[j][t][1] * by), Mma<T>::pack2(acc[j][t][2] * by, acc[j][t][3] * by)};
-                        if constexpr (VEC) {
-                            if (col < Dc) *reinterpret_cast<u32x2*>(row + col) = words;
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (col + r < Dc) reinterpret_cast<unsigned short*>(row)[col + r] = (unsigned short)(words[r / 2] >> (16 * (r % 2)));
-                        }
-                    }
+                    for (int r = 0; r < 4; ++r)
+                        if (first + r < Dc) reinterpret_cast<unsigned short*>(out + row * ch.out.st)[first + r] = (unsigned short)(words[r / 2] >> (16 * (r % 2)));
                 }
             }
         }
+        scan_planes::wait_vm<OUT && VEC ? 4 : 0>();  // the next tiles; this chunk's stores may still be under way
     }
     if constexpr (OUT) {  // rows behind the sequence
         T* out = const_cast<T*>(at(ch.out));
-        const int past = begin > n ? begin : n;
-        for (int64_t i = (int64_t)past * Dc + threadIdx.x; i < (int64_t)stop * Dc; i += 256)
+        const int stop = begin + call.segment < call.T ? begin + call.segment : call.T, past = begin > n ? begin : n;
+        for (int64_t i = (int64_t)past * Dc + threadIdx.x; i < (int64_t)stop * Dc; i += THREADS)
             reinterpret_cast<unsigned short*>(out)[i / Dc * ch.out.st + i % Dc] = 0;
     }
-    float* last = nullptr;
-    int64_t sr = Dc, sc = 1;
-    float factor = 1.0f;
     if constexpr (OUT) {
         if (ch.last.p && u.segment == call.segments - 1) {
-            last = ch.last.p + u.b * ch.last.sb + u.p * ch.last.sp + u.h * ch.last.sh;
-            sr = ch.last.sr, sc = ch.last.sc, factor = ch.last_scale;
+            float* last = ch.last.p + u.b * ch.last.sb + u.p * ch.last.sp + u.h * ch.last.sh + col * ch.last.sc;
+            each([&](float v, int row) __attribute__((always_inline)) {
+                last[row * ch.last.sr] = v * ch.last_scale;
+                return v;
+            });
         }
     } else {
-        last = call.segment_states + ((int64_t)u.number * call.segments + u.segment + 1) * Da * Dc;
-    }
-    if (last) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * i + 4 * g + r, col = col0 + 16 * j + m;
-                    if (row < Da && col < Dc) last[row * sr + col * sc] = x[i][j][r] * factor;
-                }
+        float* slot = call.segment_states + ((int64_t)u.number * (call.segments - 1) + u.segment) * Da * Dc + col;
+        each([&](float v, int row) __attribute__((always_inline)) {
+            slot[row * Dc] = v;
+            return v;
+        });
     }
 }
 
-// Slot s + 1 of each unit holds what segment s adds; with the first state in slot 0 they become the states in front of the segments.
+// Slot s of each unit holds what segment s adds; they become the states behind the segments.  BATCH slots are asked for at once.
 template <typename T> __global__ __launch_bounds__(256) void join_kernel(Call call) {
-    const int of_chain = call.B * call.P * call.H;
+    constexpr int BATCH = 8;
+    const int of_chain = call.B * call.P * call.H, slots = call.segments - 1;
     int id = (int)blockIdx.y;
     const int number = id;
     const Chain& ch = call.chain[id / of_chain];
@@ -401,16 +374,22 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(Call ca
     const int e = (int)(blockIdx.x * 256 + threadIdx.x), count = ch.Da * ch.Dc;
     if (e >= count) return;
     const int n = length_of(call, b);
-    const float rate = rate_of(call, h);
-    float* slot = call.segment_states + (int64_t)number * call.segments * count + e;
+    const float rate = rate_of(call, h), whole = expm1f(rate * (float)call.segment);
+    float* slot = call.segment_states + (int64_t)number * slots * count + e;
     float x = 0.0f;
     if (ch.first.p) x = ch.first.p[b * ch.first.sb + p * ch.first.sp + h * ch.first.sh + e / ch.Dc * ch.first.sr + e % ch.Dc * ch.first.sc] * ch.first_scale;
-    for (int s = 0; s < call.segments; ++s) {
-        const float more = s + 1 < call.segments ? slot[(int64_t)(s + 1) * count] : 0.0f;
-        slot[(int64_t)s * count] = x;
-        int tokens = n - s * call.segment;
-        tokens = tokens < 0 ? 0 : tokens > call.segment ? call.segment : tokens;
-        x = fmaf(x, expm1f(rate * (float)tokens), x) + more;
+    for (int from = 0; from < slots; from += BATCH) {
+        float more[BATCH];
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) more[s] = slot[(int64_t)(from + s < slots ? from + s : slots - 1) * count];
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) {
+            if (from + s >= slots) break;
+            const int left = n - (from + s) * call.segment;
+            const float fade = left >= call.segment ? whole : expm1f(rate * (float)(left < 0 ? 0 : left));
+            x = fmaf(x, fade, x) + more[s];
+            slot[(int64_t)(from + s) * count] = x;
+        }
     }
 }
 

@@ -6,20 +6,28 @@
 namespace lbi {
 namespace linear_attn {
 
+template <typename T, int DA, int DC, bool VEC, bool OUT, int PLANES>
+int launch_chunks(const Call& call, int64_t workgroups, hipStream_t stream) {
+    constexpr auto kernel = chunk_kernel<T, DA, DC, VEC, OUT, PLANES>;
+    constexpr size_t bytes = lds_bytes<DA, DC, OUT>();
+    if (int rc = ensure_dynamic_lds<kernel>(bytes)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((workgroups + 7) / 8 * 8)), dim3(4 * DC), bytes, stream, call);
+    LBI_HIP_CHECK(hipGetLastError());
+    return LBI_OK;
+}
+
 template <typename T, int DA, int DC, bool VEC, int PLANES>
 int launch(const Call& call, hipStream_t stream) {
     const int64_t units = (int64_t)call.chains * call.B * call.P * call.H;
-    const auto grid = [](int64_t workgroups) { return dim3((unsigned)((workgroups + 7) / 8 * 8)); };
     if (call.segments > 1) {
-        hipLaunchKernelGGL((chunk_kernel<T, DA, DC, VEC, false, PLANES>), grid(units * (call.segments - 1)), dim3(256), 0, stream, call);
-        LBI_HIP_CHECK(hipGetLastError());
-        const int elements = call.chain[0].Da * call.chain[0].Dc;
-        hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)((elements + 255) / 256), (unsigned)units), dim3(256), 0, stream, call);
-        LBI_HIP_CHECK(hipGetLastError());
+        if (int rc = launch_chunks<T, DA, DC, VEC, false, PLANES>(call, units * (call.segments - 1), stream)) return rc;
+        if (call.joined) {
+            const int elements = call.chain[0].Da * call.chain[0].Dc;
+            hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)((elements + 255) / 256), (unsigned)units), dim3(256), 0, stream, call);
+            LBI_HIP_CHECK(hipGetLastError());
+        }
     }
-    hipLaunchKernelGGL((chunk_kernel<T, DA, DC, VEC, true, PLANES>), grid(units * call.segments), dim3(256), 0, stream, call);
-    LBI_HIP_CHECK(hipGetLastError());
-    return LBI_OK;
+    return launch_chunks<T, DA, DC, VEC, true, PLANES>(call, units * call.segments, stream);
 }
 
 template <typename T, bool VEC, int PLANES> int by_dims(const Call& call, hipStream_t stream) {
@@ -28,13 +36,16 @@ template <typename T, bool VEC, int PLANES> int by_dims(const Call& call, hipStr
     return wide_c ? launch<T, 64, 128, VEC, PLANES>(call, stream) : launch<T, 64, 64, VEC, PLANES>(call, stream);
 }
 
+// Offsets within a chunk are 32 bits.
+constexpr int64_t MOST_STRIDE = (int64_t)1 << 23;
+
 // Whether rows can be taken in whole 16-byte pieces.
 inline bool in_pieces(const Call& call) {
     for (int i = 0; i < call.chains; ++i) {
         const Chain& ch = call.chain[i];
         if (ch.Da % 8 || ch.Dc % 8) return false;
         for (const View* v : {&ch.a, &ch.b, &ch.c, &ch.out})
-            if (reinterpret_cast<uintptr_t>(v->p) % 16 || v->sb % 8 || v->sp % 8 || v->sh % 8 || v->st % 8) return false;
+            if (reinterpret_cast<uintptr_t>(v->p) % 16 || v->sb % 8 || v->sp % 8 || v->sh % 8 || v->st % 8 || v->st < 0 || v->st >= MOST_STRIDE) return false;
     }
     return true;
 }
