@@ -83,7 +83,11 @@ template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
             const auto source = scan_planes::rows(from, 0x7fffffffu);
             const unsigned to = tile_at + (threadIdx.x >> 6) * 1024;
 #pragma unroll
-            for (int u = 0; u < N; ++u) scan_planes::dma16(source, count == CHUNK ? full[u] : piece_of(u, count, reverse), 0, to + u * THREADS * 16);
+            for (int u = 0; u < N; ++u) {
+                unsigned from_at = full[u];
+                if (__builtin_expect(count < CHUNK, 0)) from_at = piece_of(u, count, reverse);
+                scan_planes::dma16(source, from_at, 0, to + u * THREADS * 16);
+            }
         } else {
 #pragma unroll
             for (int u = 0; u < N; ++u) {
@@ -186,39 +190,50 @@ __global__ __launch_bounds__(4 * DC, 2) void chunk_kernel(Call call) {
     f32x4 x[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto each = [&](auto&& f) __attribute__((always_inline)) {
+    // This wave's columns of a state in memory, strides in elements: all asked for before any is waited for, zeros past the dimensions.
+    auto place = [&](int i, int r, unsigned sr, unsigned sc) __attribute__((always_inline)) {
+        const int row = 16 * i + 4 * g + r;
+        return row < Da && col < Dc ? 4 * (row * sr + col * sc) : NOWHERE;
+    };
+    auto state_at = [&](const float* p, unsigned sr, unsigned sc, auto&& use) __attribute__((always_inline)) {
+        const auto from = scan_planes::rows(p, 0x7fffffffu);
+        float v[MT][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (16 * i + 4 * g + r < Da && col < Dc) x[i][r] = f(x[i][r], 16 * i + 4 * g + r);
+            for (int r = 0; r < 4; ++r) v[i][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, place(i, r, sr, sc), 0, 0));
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[i][r] = use(x[i][r], v[i][r]);
     };
     if constexpr (OUT) {
-        const float* slots = call.segment_states + (int64_t)u.number * (call.segments - 1) * Da * Dc;
         if (ch.first.p && (u.segment == 0 || !call.joined)) {
-            const float* first = ch.first.p + u.b * ch.first.sb + u.p * ch.first.sp + u.h * ch.first.sh + col * ch.first.sc;
-            each([&](float, int row) __attribute__((always_inline)) { return first[row * ch.first.sr] * ch.first_scale; });
+            const float scale = ch.first_scale;
+            state_at(ch.first.p + u.b * ch.first.sb + u.p * ch.first.sp + u.h * ch.first.sh, (unsigned)ch.first.sr, (unsigned)ch.first.sc,
+                     [&](float, float v) __attribute__((always_inline)) { return v * scale; });
         }
+        const float* slots = call.segment_states + (int64_t)u.number * (call.segments - 1) * Da * Dc;
         for (int s = call.joined ? u.segment - 1 : 0; s >= 0 && s < u.segment; ++s) {  // what the segments before add, the first one first
             int tokens = n - s * call.segment;
             tokens = tokens < 0 ? 0 : tokens > call.segment ? call.segment : tokens;
             const float left = call.joined ? -1.0f : expm1f(rate * (float)tokens);
-            const float* slot = slots + (int64_t)s * Da * Dc + col;
-            each([&](float v, int row) __attribute__((always_inline)) { return fmaf(v, left, v) + slot[row * Dc]; });
+            state_at(slots + (int64_t)s * Da * Dc, (unsigned)Dc, 1, [&](float x_, float v) __attribute__((always_inline)) { return fmaf(x_, left, x_) + v; });
         }
-        // scores of later tokens stay zero
-        for (int i = threadIdx.x; i < CHUNK * CHUNK * 2 / 16; i += THREADS) reinterpret_cast<u32x4*>(tp)[i] = u32x4{0, 0, 0, 0};
     }
     scan_planes::wait_vm<0>();
 
-    int stage = 0;
-    for (int from = begin; from < end; from += CHUNK, stage ^= 1) {
+    const unsigned out_at = (unsigned)(((int64_t)(reverse ? 15 - m : m) * ch.out.st + 16 * w + 4 * g) * 2), out_tile = (unsigned)(32 * ch.out.st);
+    int stage = 0, from = begin;
+    auto chunk = [&](auto whole_tag) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(whole_tag)::value;  // 64 tokens
         lds_barrier();  // this chunk's tiles are there, and everyone is done with the ones before
-        if (from + CHUNK < end) bring(stage ^ 1, from + CHUNK);
+        if (WHOLE && from + CHUNK < end) bring(stage ^ 1, from + CHUNK);
         const char *tb = lds + stage * STAGE, *tc = tb + CHUNK * 2 * DA, *ta = tc + CHUNK * 2 * DC;
-        const int count = end - from < CHUNK ? end - from : CHUNK;
+        const int count = WHOLE ? CHUNK : end - from;
 
         f32x4 acc[4];
+        Pow2 state_by = {1.0f, 1.0f};
         if constexpr (OUT) {
             if (w < 4) {
                 f32x4 s[4];
@@ -228,8 +243,7 @@ __global__ __launch_bounds__(4 * DC, 2) void chunk_kernel(Call call) {
                 for (int ks = 0; ks < KS; ++ks) {
                     const u32x4 mine = nat<DA>(ta, 16 * w + m, 4 * ks + g);
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        if (t <= w) s[t] = Mma16<T>::mma(nat<DA>(tb, 16 * t + m, 4 * ks + g), mine, s[t]);
+                    for (int t = 0; t < 4; ++t) s[t] = Mma16<T>::mma(nat<DA>(tb, 16 * t + m, 4 * ks + g), mine, s[t]);
                 }
                 float most = 0.0f;
 #pragma unroll
@@ -249,12 +263,10 @@ __global__ __launch_bounds__(4 * DC, 2) void chunk_kernel(Call call) {
                 }
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
-                    if (t <= w)
-                        *reinterpret_cast<u32x2*>(tp + tile_off<CHUNK>(16 * w + m, 2 * t + (g >> 1)) + 8 * (g & 1)) =
-                            u32x2{Mma<T>::pack2(s[t][0], s[t][1]), Mma<T>::pack2(s[t][2], s[t][3])};
+                    *reinterpret_cast<u32x2*>(tp + tile_off<CHUNK>(16 * w + m, 2 * t + (g >> 1)) + 8 * (g & 1)) =
+                        u32x2{Mma<T>::pack2(s[t][0], s[t][1]), Mma<T>::pack2(s[t][2], s[t][3])};
             }
             // what the state in front of the chunk gives
-            Pow2 state_by = {1.0f, 1.0f};
             if constexpr (HALF) {
                 float most = 0.0f;
 #pragma unroll
@@ -272,38 +284,28 @@ __global__ __launch_bounds__(4 * DC, 2) void chunk_kernel(Call call) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) acc[t] = Mma16<T>::mma(state, split<DA>(ta, 16 * t + m, ks, g), acc[t]);
             }
-            lds_barrier();  // the scores are there
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                float by = read0 * (t == 0 ? 1.0f : t == 1 ? l16 : t == 2 ? l32 : l48);
-                if constexpr (HALF) by *= state_by.up / score_up[t];
-                acc[t] *= by;
-            }
         }
 
-        // the chunk's c: as it is for the scores, decayed for the state
-        if (count < CHUNK) fade = expm1f(rate * (float)count);
+        u32x4 raws[2];  // the chunk's c: as it is for the scores, decayed for the state
+        if constexpr (!WHOLE) fade = expm1f(rate * (float)count);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[i][r] = fmaf(x[i][r], fade, x[i][r]);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            if (count < CHUNK)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int left = count - 1 - (32 * ks + 8 * g + e);
-                    keep[e] = exp2f(rate2 * (float)((left < 0 ? 0 : left) + shift));
-                }
-            const float more = ks == 0 && count == CHUNK ? l32 : 1.0f;
             const u32x4 raw = turned<DC>(tc, 32 * ks + 8 * g, 16 * w);
-            if constexpr (OUT)
+            if constexpr (OUT) raws[ks] = raw;
+            float left[8];
 #pragma unroll
-                for (int t = 2 * ks; t < 4; ++t) acc[t] = Mma16<T>::mma(raw, nat<CHUNK>(tp, 16 * t + m, 4 * ks + g), acc[t]);
+            for (int e = 0; e < 8; ++e) {
+                const int tokens = count - 1 - (32 * ks + 8 * g + e);
+                left[e] = !WHOLE ? exp2f(rate2 * (float)((tokens < 0 ? 0 : tokens) + shift)) : ks == 0 ? keep[e] * l32 : keep[e];
+            }
             u32x4 plane[PLANES];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float lo = Mma<T>::lo(raw[e]) * (keep[2 * e] * more), hi = Mma<T>::hi(raw[e]) * (keep[2 * e + 1] * more);
+                float lo = Mma<T>::lo(raw[e]) * left[2 * e], hi = Mma<T>::hi(raw[e]) * left[2 * e + 1];
 #pragma unroll
                 for (int q = 0; q < PLANES; ++q) {
                     const unsigned word = Mma<T>::pack2(lo, hi);
@@ -320,6 +322,17 @@ __global__ __launch_bounds__(4 * DC, 2) void chunk_kernel(Call call) {
         }
 
         if constexpr (OUT) {
+            lds_barrier();  // the scores are there
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                float by = read0 * (t == 0 ? 1.0f : t == 1 ? l16 : t == 2 ? l32 : l48);
+                if constexpr (HALF) by *= state_by.up / score_up[t];
+                acc[t] *= by;
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int t = 2 * ks; t < 4; ++t) acc[t] = Mma16<T>::mma(raws[ks], nat<CHUNK>(tp, 16 * t + m, 4 * ks + g), acc[t]);
             T* const out = const_cast<T*>(at(ch.out)) + (int64_t)(reverse ? n - from - count : from) * ch.out.st;
             const auto to = scan_planes::rows(out, 0x7fffffffu);
 #pragma unroll
@@ -328,7 +341,9 @@ __global__ __launch_bounds__(4 * DC, 2) void chunk_kernel(Call call) {
                 float by = ch.scale;
                 if constexpr (HALF) by *= score_up[t];
                 const u32x2 words = {Mma<T>::pack2(acc[t][0] * by, acc[t][1] * by), Mma<T>::pack2(acc[t][2] * by, acc[t][3] * by)};
-                if constexpr (VEC) {  // each wave has the same number of stores under way, whatever there is to store
+                if constexpr (VEC && WHOLE) {  // each wave has the same number of stores under way, whatever there is to store
+                    __builtin_amdgcn_raw_buffer_store_b64(words, to, first < Dc ? out_at : NOWHERE, out_tile * (reverse ? 3 - t : t), 0);
+                } else if constexpr (VEC) {
                     __builtin_amdgcn_raw_buffer_store_b64(words, to, i < count && first < Dc ? (unsigned)(((int64_t)row * ch.out.st + first) * 2) : NOWHERE, 0, 0);
                 } else if (i < count) {
 #pragma unroll
@@ -338,27 +353,30 @@ __global__ __launch_bounds__(4 * DC, 2) void chunk_kernel(Call call) {
             }
         }
         scan_planes::wait_vm<OUT && VEC ? 4 : 0>();  // the next tiles; this chunk's stores may still be under way
-    }
+    };
+    for (; from + CHUNK <= end; from += CHUNK, stage ^= 1) chunk(std::true_type{});
+    if (from < end) chunk(std::false_type{});
     if constexpr (OUT) {  // rows behind the sequence
         T* out = const_cast<T*>(at(ch.out));
         const int stop = begin + call.segment < call.T ? begin + call.segment : call.T, past = begin > n ? begin : n;
         for (int64_t i = (int64_t)past * Dc + threadIdx.x; i < (int64_t)stop * Dc; i += THREADS)
             reinterpret_cast<unsigned short*>(out)[i / Dc * ch.out.st + i % Dc] = 0;
     }
+    auto leave = [&](float* p, unsigned sr, unsigned sc, float scale) __attribute__((always_inline)) {
+        const auto to = scan_planes::rows(p, 0x7fffffffu);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float v = x[i][r] * scale;
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), to, place(i, r, sr, sc), 0, 0);
+            }
+    };
     if constexpr (OUT) {
-        if (ch.last.p && u.segment == call.segments - 1) {
-            float* last = ch.last.p + u.b * ch.last.sb + u.p * ch.last.sp + u.h * ch.last.sh + col * ch.last.sc;
-            each([&](float v, int row) __attribute__((always_inline)) {
-                last[row * ch.last.sr] = v * ch.last_scale;
-                return v;
-            });
-        }
+        if (ch.last.p && u.segment == call.segments - 1)
+            leave(ch.last.p + u.b * ch.last.sb + u.p * ch.last.sp + u.h * ch.last.sh, (unsigned)ch.last.sr, (unsigned)ch.last.sc, ch.last_scale);
     } else {
-        float* slot = call.segment_states + ((int64_t)u.number * (call.segments - 1) + u.segment) * Da * Dc + col;
-        each([&](float v, int row) __attribute__((always_inline)) {
-            slot[row * Dc] = v;
-            return v;
-        });
+        leave(call.segment_states + ((int64_t)u.number * (call.segments - 1) + u.segment) * Da * Dc, (unsigned)Dc, 1, 1.0f);
     }
 }
 
