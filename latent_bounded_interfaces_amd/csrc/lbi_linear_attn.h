@@ -16,7 +16,6 @@ namespace lbi {
 namespace linear_attn {
 
 using attn_mfma::Mma;
-using attn_mfma::tile_off;
 using attn_mfma::u32x2;
 using attn_mfma::u32x4;
 

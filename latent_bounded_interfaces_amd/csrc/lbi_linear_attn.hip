@@ -26,7 +26,7 @@ int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
 
 // Segments that a chain is cut into: none while the chains alone fill the chip.
 int segments_of(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
-    const int64_t chunks = (T + CHUNK - 1) / CHUNK, room = (int64_t)device_compute_units() * (Dc > 64 ? 1 : 2);
+    const int64_t chunks = (T + CHUNK - 1) / CHUNK, room = (int64_t)device_compute_units() * (Dc > 64 || Da > 64 ? 2 : 3);
     if (units * 2 > room || chunks < 4) return 1;
     const int64_t wanted = std::min(room / units, chunks / 2), of = (chunks + wanted - 1) / wanted;
     return (int)((chunks + of - 1) / of);

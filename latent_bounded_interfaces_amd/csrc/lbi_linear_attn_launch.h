@@ -11,7 +11,7 @@ int launch_chunks(const Call& call, int64_t workgroups, hipStream_t stream) {
     constexpr auto kernel = chunk_kernel<T, DA, DC, VEC, OUT, PLANES>;
     constexpr size_t bytes = lds_bytes<DA, DC, OUT>();
     if (int rc = ensure_dynamic_lds<kernel>(bytes)) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((workgroups + 7) / 8 * 8)), dim3(4 * DC), bytes, stream, call);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((workgroups + 7) / 8 * 8)), dim3(256), bytes, stream, call);
     LBI_HIP_CHECK(hipGetLastError());
     return LBI_OK;
 }
