@@ -70,35 +70,36 @@ __device__ __forceinline__ float rate_of(const Call& call, int h) {
 // registers, zeros past the end of a row and behind the last token; otherwise, rows that start on any element, an element at a time.
 template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
     static constexpr int PIECES = DIM / 8, N = CHUNK * PIECES / THREADS;
-    const T* base;
+    const T* next;  // where the chunk that is brought next lies in memory (reverse: as if it were whole)
     int64_t st;
     int dim;
-    unsigned full[N];  // offsets of this lane's pieces from the first token in memory of a whole chunk
+    unsigned whole[N];  // offsets of this lane's pieces of a whole chunk
     __device__ __forceinline__ unsigned piece_of(int u, int count, bool reverse) const {
         const int id = u * THREADS + (int)threadIdx.x, r = id / PIECES, slot = id % PIECES;
         const int chunk = tile_off<DIM>(r, slot) / 16 % PIECES;  // the swizzle is its own inverse
-        const int64_t at = (int64_t)(reverse ? count - 1 - r : r) * st + chunk * 8;
-        return r < count && chunk * 8 < dim ? (unsigned)(at * 2) : NOWHERE;
+        const unsigned at = (unsigned)((reverse ? count - 1 - r : r) * (int)st + chunk * 8) * 2;
+        return r < count && chunk * 8 < dim ? at : NOWHERE;
     }
-    __device__ __forceinline__ Tile(const T* base_, int64_t st_, int dim_, bool reverse) : base(base_), st(st_), dim(dim_) {
+    __device__ __forceinline__ Tile(const T* base, int64_t st_, int dim_, bool reverse, int64_t chunk_at) : next(base + chunk_at * st_), st(st_), dim(dim_) {
         if constexpr (VEC)
 #pragma unroll
-            for (int u = 0; u < N; ++u) full[u] = piece_of(u, CHUNK, reverse);
+            for (int u = 0; u < N; ++u) whole[u] = piece_of(u, CHUNK, reverse);
     }
-    // The `count` tokens from `chunk` on (reverse: of a chunk that would begin there); `wave`: threadIdx.x / 64.
-    __device__ __forceinline__ void bring(char* tile, unsigned tile_at, bool reverse, const T* chunk, int count, int wave) const {
-        const T* from = chunk;
-        if (reverse && count < CHUNK) from += (CHUNK - count) * st;
+    // The next `count` tokens; `wave`: threadIdx.x / 64.
+    __device__ __forceinline__ void bring(char* tile, unsigned tile_at, bool reverse, int count, int wave) {
         if constexpr (VEC) {
-            const auto source = scan_planes::rows(from, 0x7fffffffu);
             const unsigned to = tile_at + wave * 1024;
+            if (__builtin_expect(count == CHUNK, 1)) {
+                const auto source = scan_planes::rows(next, 0x7fffffffu);
 #pragma unroll
-            for (int u = 0; u < N; ++u) {
-                unsigned from_at = full[u];
-                if (__builtin_expect(count < CHUNK, 0)) from_at = piece_of(u, count, reverse);
-                scan_planes::dma16(source, from_at, 0, to + u * THREADS * 16);
+                for (int u = 0; u < N; ++u) scan_planes::dma16(source, whole[u], 0, to + u * THREADS * 16);
+            } else {
+                const auto source = scan_planes::rows(next + (reverse ? (CHUNK - count) * st : 0), 0x7fffffffu);
+#pragma unroll
+                for (int u = 0; u < N; ++u) scan_planes::dma16(source, piece_of(u, count, reverse), 0, to + u * THREADS * 16);
             }
         } else {
+            const T* const from = next + (reverse ? (CHUNK - count) * st : 0);
 #pragma unroll
             for (int u = 0; u < N; ++u) {
                 const int id = u * THREADS + (int)threadIdx.x, r = id / PIECES, c = id % PIECES * 8;
@@ -111,6 +112,7 @@ template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
                 *reinterpret_cast<u32x4*>(tile + tile_off<DIM>(r, c / 8)) = words;
             }
         }
+        next += reverse ? -CHUNK * st : CHUNK * st;
     }
 };
 
@@ -128,7 +130,8 @@ template <int DIM> struct Places {
     }
     // row 16 t + m, elements 32 ks + 4 g ... + 3 and 16 further: the order in which accumulators hold the rows of two tiles
     __device__ __forceinline__ u32x4 split(lds_ptr tile, int t, int ks) const {
-        typedef __attribute__((address_space(3))) const u32x2* half;
+        // (volatile: two rows' halves in one instruction would have to be taken apart again)
+        typedef __attribute__((address_space(3))) const volatile u32x2* half;
         const u32x2 lo = *(half)(tile + (split_ ^ (ks << 6)) + t * 32 * DIM), hi = *(half)(tile + (split_ ^ (ks << 6) ^ 32) + t * 32 * DIM);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
@@ -147,14 +150,16 @@ __device__ __forceinline__ bool unit_of(const Call& call, int segments, Unit& u)
     const int total = call.chains * call.B * call.P * call.H * segments, per = (int)(gridDim.x >> 3);
     int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
     if (id >= total) return false;
-    u.chain = id % call.chains;
-    id /= call.chains;
-    u.segment = id % segments;
-    id /= segments;
-    u.p = id % call.P;
-    id /= call.P;
-    u.h = id % call.H;
-    u.b = id / call.H;
+    const auto digit = [&](int base) __attribute__((always_inline)) {  // (in scalar registers, and so is all that is read by it)
+        const int rest = __builtin_amdgcn_readfirstlane(id / base), of = id - rest * base;
+        id = rest;
+        return of;
+    };
+    u.chain = digit(call.chains);
+    u.segment = digit(segments);
+    u.p = digit(call.P);
+    u.h = digit(call.H);
+    u.b = id;
     u.number = ((u.chain * call.B + u.b) * call.P + u.p) * call.H + u.h;
     return true;
 }
@@ -180,30 +185,27 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     const float rate = rate_of(call, u.h), rate2 = rate * LOG2E;
     const int shift = ch.shift, Da = ch.Da, Dc = ch.Dc, col0 = w * (DC / 4);
 
-    const Tile<T, DA, 256, VEC> a(OUT ? at(ch.a) : nullptr, ch.a.st, Da, reverse), b(at(ch.b), ch.b.st, Da, reverse);
-    const Tile<T, DC, 256, VEC> c(at(ch.c), ch.c.st, Dc, reverse);
+    const int64_t chunk_at = reverse ? (int64_t)n - begin - CHUNK : begin;
+    Tile<T, DA, 256, VEC> a(OUT ? at(ch.a) : nullptr, ch.a.st, Da, reverse, chunk_at), b(at(ch.b), ch.b.st, Da, reverse, chunk_at);
+    Tile<T, DC, 256, VEC> c(at(ch.c), ch.c.st, Dc, reverse, chunk_at);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
-    // where a whole chunk lies in memory, for the one that is brought next
-    const int64_t chunk_at = reverse ? (int64_t)n - begin - CHUNK : begin, step = reverse ? -CHUNK : CHUNK;
-    const T *next_a = a.base + chunk_at * a.st, *next_b = b.base + chunk_at * b.st, *next_c = c.base + chunk_at * c.st;
     auto bring = [&](int stage, int from) __attribute__((always_inline)) {
         const int count = end - from < CHUNK ? end - from : CHUNK, to = stage * STAGE;
-        b.bring(lds + to, lds0 + to, reverse, next_b, count, w);
-        c.bring(lds + to + CHUNK * 2 * DA, lds0 + to + CHUNK * 2 * DA, reverse, next_c, count, w);
-        if constexpr (OUT) a.bring(lds + to + CHUNK * 2 * (DA + DC), lds0 + to + CHUNK * 2 * (DA + DC), reverse, next_a, count, w);
-        next_a += step * a.st, next_b += step * b.st, next_c += step * c.st;
+        b.bring(lds + to, lds0 + to, reverse, count, w);
+        c.bring(lds + to + CHUNK * 2 * DA, lds0 + to + CHUNK * 2 * DA, reverse, count, w);
+        if constexpr (OUT) a.bring(lds + to + CHUNK * 2 * (DA + DC), lds0 + to + CHUNK * 2 * (DA + DC), reverse, count, w);
     };
     if (begin < end) bring(0, begin);
 
-    // l to the power of tokens apart, as products of l^0 ... l^31 of this lane's place and of l^16, l^32, l^48
+    // l to the power of tokens apart (and the result's scale), as products of l^0 ... l^31 of this lane's place and of l^16, l^32, l^48
     const float l16 = exp2f(rate2 * 16.0f), l32 = exp2f(rate2 * 32.0f), l48 = exp2f(rate2 * 48.0f);
-    const float read0 = exp2f(rate2 * (float)(m + 1 - shift));
+    const float read0 = exp2f(rate2 * (float)(m + 1 - shift)) * ch.scale;
     float near[4], far[4], keep[8];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int apart = m - 4 * g - r;
-        near[r] = exp2f(rate2 * (float)(apart < 0 ? 0 : apart));
-        far[r] = exp2f(rate2 * (float)(16 + apart));
+        near[r] = exp2f(rate2 * (float)(apart < 0 ? 0 : apart)) * ch.scale;
+        far[r] = exp2f(rate2 * (float)(16 + apart)) * ch.scale;
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) keep[e] = exp2f(rate2 * (float)(31 - 8 * g - e + shift));
@@ -219,24 +221,25 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 for (int r = 0; r < 4; ++r) f(i, j, r);
     };
     each([&](int i, int j, int r) __attribute__((always_inline)) { x[i][j][r] = 0.0f; });
-    // This wave's columns of a state in memory, strides in elements: f(row tile, column tile, register, lane's offset, its tile's offset) in bytes, no
-    // place for what lies past the dimensions.  Full tiles share one lane offset.
-    const bool full = Da == DA && Dc == DC;
+    // This wave's columns of a state in memory, strides in elements: f(row tile, column tile, register, offset in bytes), no place for what lies past
+    // the dimensions.
     auto of_state = [&](unsigned sr, unsigned sc, auto&& f) __attribute__((always_inline)) {
-        const unsigned lane = 4 * (4 * g * sr + (col0 + m) * sc);
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int j = 0; j < NT; ++j) {
+            unsigned at_row = col0 + 16 * j + m < Dc ? 4 * (4 * g * sr + (col0 + 16 * j + m) * sc) : NOWHERE;
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int i = 0; i < MT; ++i) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    f(i, j, r, full || (16 * i + 4 * g + r < Da && col0 + 16 * j + m < Dc) ? lane : NOWHERE, 4 * ((16 * i + r) * sr + 16 * j * sc));
+                for (int r = 0; r < 4; ++r) f(i, j, r, 16 * i + 4 * g + r < Da ? at_row + 4 * r * sr : NOWHERE);
+                at_row += 64 * sr;
+            }
+        }
     };
     auto state_at = [&](const float* p, unsigned sr, unsigned sc, auto&& use) __attribute__((always_inline)) {
         const auto from = scan_planes::rows(p, 0x7fffffffu);
         float v[MT][NT][4];  // all asked for before any is waited for
-        of_state(sr, sc, [&](int i, int j, int r, unsigned lane, unsigned tile) __attribute__((always_inline)) {
-            v[i][j][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, lane, tile, 0));
+        of_state(sr, sc, [&](int i, int j, int r, unsigned place) __attribute__((always_inline)) {
+            v[i][j][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, place, 0, 0));
         });
         each([&](int i, int j, int r) __attribute__((always_inline)) { x[i][j][r] = use(x[i][j][r], v[i][j][r]); });
     };
@@ -256,8 +259,11 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     }
     scan_planes::wait_vm<0>();
 
-    const unsigned out_at = (unsigned)(((int64_t)(reverse ? 15 - m : m) * ch.out.st + col0 + 4 * g) * 2), out_tile = (unsigned)(32 * ch.out.st);
-    T* next_out = OUT ? const_cast<T*>(at(ch.out)) + chunk_at * ch.out.st : nullptr;
+    const int64_t out_st = ch.out.st;
+    T* next_out = OUT ? const_cast<T*>(at(ch.out)) + chunk_at * out_st : nullptr;
+    unsigned out_at[4];  // of a whole chunk's rows
+#pragma unroll
+    for (int t = 0; t < 4; ++t) out_at[t] = (unsigned)((reverse ? CHUNK - 1 - 16 * t - m : 16 * t + m) * (int)out_st + col0 + 4 * g) * 2;
     Places<DA> in_a(m, g);  // and in b's
     Places<DC> in_c(m, g);
     Places<CHUNK> in_p(m, g);
@@ -286,12 +292,19 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             float most = 0.0f;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const float more = w - t == 2 ? l16 : w - t == 3 ? l32 : 1.0f;
+                if (t < w) {
+                    const float more = w - t == 2 ? l16 : w - t == 3 ? l32 : 1.0f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[t][r] = t < w ? s[t][r] * (far[r] * more) : t == w && m >= 4 * g + r ? s[t][r] * near[r] : 0.0f;
-                    if constexpr (HALF) most = fmaxf(most, fabsf(s[t][r]));
+                    for (int r = 0; r < 4; ++r) s[t][r] *= far[r] * more;
+                } else if (t == w) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][r] = m >= 4 * g + r ? s[t][r] * near[r] : 0.0f;
+                } else {
+                    s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
+                if constexpr (HALF)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(s[t][r]));
             }
             if constexpr (HALF) {
                 const Pow2 by = into_range(over_wave_max(most));
@@ -371,6 +384,12 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 
         if constexpr (OUT) {
             lds_barrier();  // the scores are there, and everyone is done with the tiles
+            u32x4 scores[2][4];  // (read before the next tiles are asked for, which they would wait behind)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int t = 2 * ks; t < 4; ++t) scores[ks][t] = in_p.nat(tp, t, ks);
+            LBI_PHASE_FENCE();
             if (WHOLE && from + CHUNK < end) bring(0, from + CHUNK);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -382,31 +401,28 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int t = 2 * ks; t < 4; ++t) {
-                    const u32x4 scores = in_p.nat(tp, t, ks);
+                for (int t = 2 * ks; t < 4; ++t)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(raw[ks][j], scores, acc[j][t]);
-                }
-            T* const out = next_out + (WHOLE || !reverse ? 0 : (CHUNK - count) * ch.out.st);
-            next_out += step * ch.out.st;
+                    for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(raw[ks][j], scores[ks][t], acc[j][t]);
+            T* const out = next_out + (WHOLE || !reverse ? 0 : (CHUNK - count) * out_st);
+            next_out += reverse ? -CHUNK * out_st : CHUNK * out_st;
             const auto to = scan_planes::rows(out, 0x7fffffffu);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 const int i = 16 * t + m, row = reverse ? count - 1 - i : i;
-                float by = ch.scale;
-                if constexpr (HALF) by *= score_up[t];
+                const float by = HALF ? score_up[t] : 1.0f;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const int first = col0 + 16 * j + 4 * g;
                     const u32x2 words = {Mma<T>::pack2(acc[j][t][0] * by, acc[j][t][1] * by), Mma<T>::pack2(acc[j][t][2] * by, acc[j][t][3] * by)};
                     if constexpr (VEC && WHOLE) {  // each wave has the same number of stores under way, whatever there is to store
-                        __builtin_amdgcn_raw_buffer_store_b64(words, to, first < Dc ? out_at + 32 * j : NOWHERE, out_tile * (reverse ? 3 - t : t), 0);
+                        __builtin_amdgcn_raw_buffer_store_b64(words, to, first < Dc ? out_at[t] + 32 * j : NOWHERE, 0, 0);
                     } else if constexpr (VEC) {
-                        __builtin_amdgcn_raw_buffer_store_b64(words, to, i < count && first < Dc ? (unsigned)(((int64_t)row * ch.out.st + first) * 2) : NOWHERE, 0, 0);
+                        __builtin_amdgcn_raw_buffer_store_b64(words, to, i < count && first < Dc ? (unsigned)(row * (int)out_st + first) * 2 : NOWHERE, 0, 0);
                     } else if (i < count) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (first + r < Dc) reinterpret_cast<unsigned short*>(out + row * ch.out.st)[first + r] = (unsigned short)(words[r / 2] >> (16 * (r % 2)));
+                            if (first + r < Dc) reinterpret_cast<unsigned short*>(out + row * out_st)[first + r] = (unsigned short)(words[r / 2] >> (16 * (r % 2)));
                     }
                 }
             }
@@ -424,9 +440,9 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     }
     auto leave = [&](float* p, unsigned sr, unsigned sc, float scale) __attribute__((always_inline)) {
         const auto to = scan_planes::rows(p, 0x7fffffffu);
-        of_state(sr, sc, [&](int i, int j, int r, unsigned lane, unsigned tile) __attribute__((always_inline)) {
+        of_state(sr, sc, [&](int i, int j, int r, unsigned place) __attribute__((always_inline)) {
             const float v = x[i][j][r] * scale;
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), to, lane, tile, 0);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), to, place, 0, 0);
         });
     };
     if constexpr (OUT) {
