@@ -73,7 +73,7 @@ template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
     const T* next;  // where the chunk that is brought next lies in memory (reverse: as if it were whole)
     int64_t st;
     int dim;
-    unsigned whole[N];  // offsets of this lane's pieces of a whole chunk
+    unsigned whole;  // offset of this lane's first piece (reverse: its last) of a whole chunk; the others lie so many whole rows further, in the same columns
     __device__ __forceinline__ unsigned piece_of(int u, int count, bool reverse) const {
         const int id = u * THREADS + (int)threadIdx.x, r = id / PIECES, slot = id % PIECES;
         const int chunk = tile_off<DIM>(r, slot) / 16 % PIECES;  // the swizzle is its own inverse
@@ -81,9 +81,8 @@ template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
         return r < count && chunk * 8 < dim ? at : NOWHERE;
     }
     __device__ __forceinline__ Tile(const T* base, int64_t st_, int dim_, bool reverse, int64_t chunk_at) : next(base + chunk_at * st_), st(st_), dim(dim_) {
-        if constexpr (VEC)
-#pragma unroll
-            for (int u = 0; u < N; ++u) whole[u] = piece_of(u, CHUNK, reverse);
+        static_assert(THREADS / PIECES % 16 == 0, "the swizzle repeats after 16 rows");
+        whole = VEC ? piece_of(reverse ? N - 1 : 0, CHUNK, reverse) : 0;
     }
     // The next `count` tokens; `wave`: threadIdx.x / 64.
     __device__ __forceinline__ void bring(char* tile, unsigned tile_at, bool reverse, int count, int wave) {
@@ -92,7 +91,8 @@ template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
             if (__builtin_expect(count == CHUNK, 1)) {
                 const auto source = scan_planes::rows(next, 0x7fffffffu);
 #pragma unroll
-                for (int u = 0; u < N; ++u) scan_planes::dma16(source, whole[u], 0, to + u * THREADS * 16);
+                for (int u = 0; u < N; ++u)
+                    scan_planes::dma16(source, whole, (unsigned)((reverse ? N - 1 - u : u) * (THREADS / PIECES) * (int)st * 2), to + u * THREADS * 16);
             } else {
                 const auto source = scan_planes::rows(next + (reverse ? (CHUNK - count) * st : 0), 0x7fffffffu);
 #pragma unroll
@@ -197,16 +197,18 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     };
     if (begin < end) bring(0, begin);
 
-    // l to the power of tokens apart (and the result's scale), as products of l^0 ... l^31 of this lane's place and of l^16, l^32, l^48
+    // l to the power of tokens apart (and the result's scale): of this lane's scores, 0 for later tokens, of its readouts and of its rows of c
     const float l16 = exp2f(rate2 * 16.0f), l32 = exp2f(rate2 * 32.0f), l48 = exp2f(rate2 * 48.0f);
     const float read0 = exp2f(rate2 * (float)(m + 1 - shift)) * ch.scale;
-    float near[4], far[4], keep[8];
+    float apart[OUT ? 4 : 1][4], keep[8];
+    if constexpr (OUT)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int apart = m - 4 * g - r;
-        near[r] = exp2f(rate2 * (float)(apart < 0 ? 0 : apart)) * ch.scale;
-        far[r] = exp2f(rate2 * (float)(16 + apart)) * ch.scale;
-    }
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int tokens = 16 * (w - t) + m - 4 * g - r;
+                apart[t][r] = tokens < 0 ? 0.0f : exp2f(rate2 * (float)tokens) * ch.scale;
+            }
 #pragma unroll
     for (int e = 0; e < 8; ++e) keep[e] = exp2f(rate2 * (float)(31 - 8 * g - e + shift));
     float fade = expm1f(rate * (float)CHUNK);  // X + X (l^64 - 1) keeps what rounding l^64 near 1 would add up over many chunks
@@ -261,9 +263,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 
     const int64_t out_st = ch.out.st;
     T* next_out = OUT ? const_cast<T*>(at(ch.out)) + chunk_at * out_st : nullptr;
-    unsigned out_at[4];  // of a whole chunk's rows
-#pragma unroll
-    for (int t = 0; t < 4; ++t) out_at[t] = (unsigned)((reverse ? CHUNK - 1 - 16 * t - m : 16 * t + m) * (int)out_st + col0 + 4 * g) * 2;
+    const unsigned out_at = (unsigned)((reverse ? 15 - m : m) * (int)out_st + col0 + 4 * g) * 2;  // in sixteen rows of a whole chunk
     Places<DA> in_a(m, g);  // and in b's
     Places<DC> in_c(m, g);
     Places<CHUNK> in_p(m, g);
@@ -275,6 +275,35 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         in_a.here(), in_c.here(), in_p.here();
         const int count = WHOLE ? CHUNK : end - from;
         if (!OUT && WHOLE && from + CHUNK < end) bring(stage ^ 1, from + CHUNK);
+
+        // What a wave issues between its products runs beside them: each stretch below, between fences, holds the vector work of a later one.
+        u32x4 raw[2][NT];  // the chunk's c: as it is for the scores, decayed for the state
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) raw[ks][j] = in_c.turned(tc, ks, col0 + 16 * j);
+        u32x4 plane[2][PLANES][NT];
+        // words e of the decayed c of step ks, column tile j
+        auto decay = [&](int ks, int j, int e) __attribute__((always_inline)) {
+            auto left = [&](int at_e) __attribute__((always_inline)) {
+                const int tokens = count - 1 - (32 * ks + 8 * g + at_e);
+                return !WHOLE ? exp2f(rate2 * (float)((tokens < 0 ? 0 : tokens) + shift)) : ks == 0 ? keep[at_e] * l32 : keep[at_e];
+            };
+            float lo = Mma<T>::lo(raw[ks][j][e]) * left(2 * e), hi = Mma<T>::hi(raw[ks][j][e]) * left(2 * e + 1);
+#pragma unroll
+            for (int q = 0; q < PLANES; ++q) {
+                const unsigned word = Mma<T>::pack2(lo, hi);
+                plane[ks][q][j][e] = word;
+                lo -= Mma<T>::lo(word), hi -= Mma<T>::hi(word);
+            }
+        };
+        if constexpr (!WHOLE) fade = expm1f(rate * (float)count);
+        auto move_on = [&](int i) __attribute__((always_inline)) {  // rows 16 i ... of the state, past the chunk's tokens
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[i][j][r] = fmaf(x[i][j][r], fade, x[i][j][r]);
+        };
 
         f32x4 acc[NT][4];
         Pow2 state_by = {1.0f, 1.0f};
@@ -288,24 +317,35 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
                 for (int t = 0; t < 4; ++t) s[t] = Mma16<T>::mma(in_a.nat(tb, t, ks), mine, s[t]);
             }
+            if constexpr (HALF) {
+                float of_state = 0.0f;
+                each([&](int i, int j, int r) __attribute__((always_inline)) { of_state = fmaxf(of_state, fabsf(x[i][j][r])); });
+                state_by = into_range(over_wave_max(of_state));
+            }
+            u32x4 state[2][NT];  // this step's rows of the state as an operand, and the next one's
+            auto pack = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const f32x4 lo = x[2 * ks][j] * state_by.down, hi = x[2 * ks + 1][j] * state_by.down;
+                    state[ks & 1][j] = u32x4{Mma<T>::pack2(lo[0], lo[1]), Mma<T>::pack2(lo[2], lo[3]), Mma<T>::pack2(hi[0], hi[1]), Mma<T>::pack2(hi[2], hi[3])};
+                }
+                move_on(2 * ks);
+                move_on(2 * ks + 1);
+            };
+            pack(0);
+            u32x4 tokens[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) tokens[t] = in_a.split(ta, t, 0);
             LBI_PHASE_FENCE();
+            // the scores, rounded, beside the readout's first step
             float most = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if (t < w) {
-                    const float more = w - t == 2 ? l16 : w - t == 3 ? l32 : 1.0f;
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][r] *= far[r] * more;
-                } else if (t == w) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][r] = m >= 4 * g + r ? s[t][r] * near[r] : 0.0f;
-                } else {
-                    s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int r = 0; r < 4; ++r) {
+                    s[t][r] = m - 4 * g >= 16 * (t - w) + r ? s[t][r] * apart[t][r] : 0.0f;
+                    if constexpr (HALF) most = fmaxf(most, fabsf(s[t][r]));
                 }
-                if constexpr (HALF)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(s[t][r]));
-            }
             if constexpr (HALF) {
                 const Pow2 by = into_range(over_wave_max(most));
                 if ((threadIdx.x & 63) == 0) score_up[w] = by.up;
@@ -316,70 +356,68 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             for (int t = 0; t < 4; ++t)
                 *(__attribute__((address_space(3))) u32x2*)(tp + (in_p.split_ ^ (t << 5)) + w * 32 * CHUNK) =
                     u32x2{Mma<T>::pack2(s[t][0], s[t][1]), Mma<T>::pack2(s[t][2], s[t][3])};
-            LBI_PHASE_FENCE();
-            // what the state in front of the chunk gives
-            if constexpr (HALF) {
-                most = 0.0f;
-                each([&](int i, int j, int r) __attribute__((always_inline)) { most = fmaxf(most, fabsf(x[i][j][r])); });
-                state_by = into_range(over_wave_max(most));
-            }
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) acc[j][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                u32x4 state[NT];
+                constexpr int EARLY = NT == 1 ? 4 : 2;  // tokens' tiles that are read a step ahead: what the registers hold
+                u32x4 more[EARLY];
+                if (ks > 0)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const f32x4 lo = x[2 * ks][j] * state_by.down, hi = x[2 * ks + 1][j] * state_by.down;
-                    state[j] = u32x4{Mma<T>::pack2(lo[0], lo[1]), Mma<T>::pack2(lo[2], lo[3]), Mma<T>::pack2(hi[0], hi[1]), Mma<T>::pack2(hi[2], hi[3])};
-                }
+                    for (int t = EARLY; t < 4; ++t) tokens[t] = in_a.split(ta, t, ks);
+                if (ks + 1 < KS)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const u32x4 tokens = in_a.split(ta, t, ks);
+                    for (int t = 0; t < EARLY; ++t) more[t] = in_a.split(ta, t, ks + 1);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(state[j], tokens, acc[j][t]);
-                }
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(state[ks & 1][j], tokens[t], acc[j][t]);
+                if (ks + 1 < KS) pack(ks + 1);
+#pragma unroll
+                for (int p = ks * 4 * NT / KS; p < (ks + 1) * 4 * NT / KS; ++p) decay(0, p / 4, p % 4);
+                if constexpr (WHOLE && !HALF)
+#pragma unroll
+                    for (int i = 0; i < 4 * NT; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                    }
+                LBI_PHASE_FENCE();
+                if (ks + 1 < KS)
+#pragma unroll
+                    for (int t = 0; t < EARLY; ++t) tokens[t] = more[t];
             }
+        } else {
+#pragma unroll
+            for (int p = 0; p < 4 * NT; ++p) decay(0, p / 4, p % 4);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) move_on(i);
         }
 
-        LBI_PHASE_FENCE();
-        u32x4 raw[2][NT];  // the chunk's c: as it is for the scores, decayed for the state
-        if constexpr (!WHOLE) fade = expm1f(rate * (float)count);
-        each([&](int i, int j, int r) __attribute__((always_inline)) { x[i][j][r] = fmaf(x[i][j][r], fade, x[i][j][r]); });
+        u32x4 rows = in_a.turned(tb, 0, 0);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            u32x4 plane[PLANES][NT];
-            float left[8];
+        for (int step = 0; step < 2 * MT; ++step) {
+            const int ks = step / MT, i = step % MT;
+            u32x4 more;
+            if (step + 1 < 2 * MT) more = in_a.turned(tb, (step + 1) / MT, 16 * ((step + 1) % MT));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int tokens = count - 1 - (32 * ks + 8 * g + e);
-                left[e] = !WHOLE ? exp2f(rate2 * (float)((tokens < 0 ? 0 : tokens) + shift)) : ks == 0 ? keep[e] * l32 : keep[e];
-            }
+            for (int q = PLANES - 1; q >= 0; --q)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                raw[ks][j] = in_c.turned(tc, ks, col0 + 16 * j);
+                for (int j = 0; j < NT; ++j) x[i][j] = Mma16<T>::mma(rows, plane[ks][q][j], x[i][j]);
+            if (ks == 0)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float lo = Mma<T>::lo(raw[ks][j][e]) * left[2 * e], hi = Mma<T>::hi(raw[ks][j][e]) * left[2 * e + 1];
+                for (int p = i * 4 * NT / MT; p < (i + 1) * 4 * NT / MT; ++p) decay(1, p / 4, p % 4);
+            if constexpr (WHOLE)
 #pragma unroll
-                    for (int q = 0; q < PLANES; ++q) {
-                        const unsigned word = Mma<T>::pack2(lo, hi);
-                        plane[q][j][e] = word;
-                        lo -= Mma<T>::lo(word), hi -= Mma<T>::hi(word);
-                    }
+                for (int n_ = 0; n_ < PLANES * NT; ++n_) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const u32x4 bt = in_a.turned(tb, ks, 16 * i);
-#pragma unroll
-                for (int q = PLANES - 1; q >= 0; --q)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) x[i][j] = Mma16<T>::mma(bt, plane[q][j], x[i][j]);
-            }
             LBI_PHASE_FENCE();
+            rows = more;
         }
 
         if constexpr (OUT) {
@@ -416,7 +454,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                     const int first = col0 + 16 * j + 4 * g;
                     const u32x2 words = {Mma<T>::pack2(acc[j][t][0] * by, acc[j][t][1] * by), Mma<T>::pack2(acc[j][t][2] * by, acc[j][t][3] * by)};
                     if constexpr (VEC && WHOLE) {  // each wave has the same number of stores under way, whatever there is to store
-                        __builtin_amdgcn_raw_buffer_store_b64(words, to, first < Dc ? out_at[t] + 32 * j : NOWHERE, 0, 0);
+                        __builtin_amdgcn_raw_buffer_store_b64(words, to, first < Dc ? out_at + 32 * j : NOWHERE, (unsigned)((reverse ? 3 - t : t) * 32 * (int)out_st), 0);
                     } else if constexpr (VEC) {
                         __builtin_amdgcn_raw_buffer_store_b64(words, to, i < count && first < Dc ? (unsigned)(row * (int)out_st + first) * 2 : NOWHERE, 0, 0);
                     } else if (i < count) {
