@@ -482,7 +482,7 @@ int lbi_clip_gradients(const lbi_gradient* gradients, int64_t n, float max_norm,
  *
  * Pullback: dq [B,P,H,T,D], dk and dv [B,P,kv_heads,T,D], contiguous, into g_qkv [B,P,T,(H + 2 Hkv) D]: turned back; with kv_heads = H those of the
  * heads that share a key or value are added up in fp32 first (kv_heads = Hkv: as they are).  What lbi_attn_qkv_pullback does for whole heads, kv_heads = H and
- * positions 0 ... T-1.  All dtypes; results overlap no other tensor.
+ * positions 0 ... T-1.  All dtypes; fewer than 2^30 tokens; results overlap no other tensor.
  */
 int lbi_rotary(const void* qkv, const float* cos, const float* sin, const void* positions, void* q, void* k, int64_t B, int64_t T, int64_t H,
                int64_t Hkv, int64_t D, int64_t R, int64_t table, int64_t stride_b, int64_t stride_t, int positions_wide, int interleaved, int dtype,

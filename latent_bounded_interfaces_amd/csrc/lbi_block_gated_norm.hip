@@ -142,10 +142,10 @@ extern "C" int lbi_gated_residual_rmsnorm_pullback(const void* g_normed, const v
     }
     // one launch for all sums, in so many more as there are gates past what a launch numbers
     const int64_t outs = 2 + (summed && rows ? plan.gates : 0);
-    const bool wide = D >= 4096;  // enough columns to fill the chip in whole lines
+    const bool wide = D >= 1024;  // enough columns to fill the chip in whole lines
     for (int64_t first = 0; first < outs; first += 65535) {
-        const auto fold = wide ? gated_fold_kernel<32, 32> : gated_fold_kernel<16, 64>;
-        hipLaunchKernelGGL(fold, dim3((unsigned)((D + (wide ? 31 : 15)) / (wide ? 32 : 16)), (unsigned)std::min<int64_t>(outs - first, 65535)), dim3(1024),
+        const auto fold = wide ? gated_fold_kernel<64, 16> : gated_fold_kernel<16, 64>;
+        hipLaunchKernelGGL(fold, dim3((unsigned)((D + (wide ? 63 : 15)) / (wide ? 64 : 16)), (unsigned)std::min<int64_t>(outs - first, 65535)), dim3(1024),
                            0, s, partials, g_post_weight, g_weight, static_cast<float*>(g_gate), first, slabs, plan.slabs_per_gate, (int)D);
         LBI_HIP_CHECK(hipGetLastError());
     }

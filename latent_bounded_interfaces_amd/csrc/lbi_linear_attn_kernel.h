@@ -116,14 +116,13 @@ template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
     }
 };
 
-// Places of a lane in a tile, from which all that it reads lie an exclusive or of constants (pieces) and a constant (rows) away.  Kept from being moved
-// out of the loop over chunks, where each would take a register.
+// Places of a lane in a tile, from which all that it reads lie an exclusive or of constants (pieces) and a constant (rows) away.
 typedef __attribute__((address_space(3))) char* lds_ptr;
 template <int DIM> struct Places {
-    unsigned nat_, split_, turned_;
+    unsigned nat_, split_, turned_, halved_;
     __device__ __forceinline__ Places(int m, int g)
-        : nat_(tile_off<DIM>(m, g)), split_(tile_off<DIM>(m, g >> 1) + 8 * (g & 1)), turned_(tile_off<DIM>(8 * g + (m >> 2), (m & 3) >> 1) + ((m & 1) << 3)) {}
-    __device__ __forceinline__ void here() { asm volatile("" : "+v"(nat_), "+v"(split_), "+v"(turned_)); }
+        : nat_(tile_off<DIM>(m, g)), split_(tile_off<DIM>(m, g >> 1) + 8 * (g & 1)), turned_(tile_off<DIM>(8 * g + (m >> 2), (m & 3) >> 1) + ((m & 1) << 3)),
+          halved_(tile_off<DIM>(8 * g + (m >> 2), m & 3)) {}
     // row 16 t + m, elements 32 ks + 8 g ... + 7
     __device__ __forceinline__ u32x4 nat(lds_ptr tile, int t, int ks) const {
         return *(__attribute__((address_space(3))) const u32x4*)(tile + (nat_ ^ (ks << 6)) + t * 32 * DIM);
@@ -135,11 +134,12 @@ template <int DIM> struct Places {
         const u32x2 lo = *(half)(tile + (split_ ^ (ks << 6)) + t * 32 * DIM), hi = *(half)(tile + (split_ ^ (ks << 6) ^ 32) + t * 32 * DIM);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
-    // column `col` + m (a multiple of 16), rows 32 ks + 8 g ... + 7
-    __device__ __forceinline__ u32x4 turned(lds_ptr tile, int ks, int col) const {
-        typedef __attribute__((address_space(3))) attn_mfma::s16x4* half;
-        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((half)(tile + (turned_ ^ (col << 1)) + ks * 64 * DIM)));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((half)(tile + (turned_ ^ (col << 1) ^ 32) + ks * 64 * DIM + 8 * DIM)));
+    // column `col` + m (a multiple of 16), rows 32 ks + 8 g ... + 7; of HALVES 2, column `col` + 8 (m / 4) + 4 half + m % 4 of 32
+    template <int HALVES = 1> __device__ __forceinline__ u32x4 turned(lds_ptr tile, int ks, int col, int half = 0) const {
+        typedef __attribute__((address_space(3))) attn_mfma::s16x4* four;
+        const unsigned at = (HALVES == 1 ? turned_ : halved_) ^ (col << 1);
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((four)(tile + at + 8 * half + ks * 64 * DIM)));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((four)(tile + (at ^ 32) + 8 * half + ks * 64 * DIM + 8 * DIM)));
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
 };
@@ -228,7 +228,8 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     auto of_state = [&](unsigned sr, unsigned sc, auto&& f) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            unsigned at_row = col0 + 16 * j + m < Dc ? 4 * (4 * g * sr + (col0 + 16 * j + m) * sc) : NOWHERE;
+            const int col = col0 + (NT == 1 ? m : 8 * (m >> 2) + 4 * j + (m & 3));
+            unsigned at_row = col < Dc ? 4 * (4 * g * sr + col * sc) : NOWHERE;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
 #pragma unroll
@@ -263,7 +264,8 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 
     const int64_t out_st = ch.out.st;
     T* next_out = OUT ? const_cast<T*>(at(ch.out)) + chunk_at * out_st : nullptr;
-    const unsigned out_at = (unsigned)((reverse ? 15 - m : m) * (int)out_st + col0 + 4 * g) * 2;  // in sixteen rows of a whole chunk
+    const int first_col = col0 + 4 * NT * g;  // of the 4 NT neighbouring ones that this lane has of a row
+    const unsigned out_at = (unsigned)((reverse ? 15 - m : m) * (int)out_st + first_col) * 2;  // in sixteen rows of a whole chunk
     Places<DA> in_a(m, g);  // and in b's
     Places<DC> in_c(m, g);
     Places<CHUNK> in_p(m, g);
@@ -272,7 +274,8 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         constexpr bool WHOLE = decltype(whole_tag)::value;  // 64 tokens
         lds_barrier();  // this chunk's tiles are there
         const lds_ptr tb = (lds_ptr)lds + stage * STAGE, tc = tb + CHUNK * 2 * DA, ta = tc + CHUNK * 2 * DC, tp = (lds_ptr)lds + STAGE;
-        in_a.here(), in_c.here(), in_p.here();
+        // (what is made of them stays in this loop: in front of it, each would take a register)
+        asm volatile("" : "+v"(in_a.nat_), "+v"(in_a.split_), "+v"(in_a.turned_), "+v"(in_p.nat_), "+v"(in_p.split_), "+v"(NT == 1 ? in_c.turned_ : in_c.halved_));
         const int count = WHOLE ? CHUNK : end - from;
         if (!OUT && WHOLE && from + CHUNK < end) bring(stage ^ 1, from + CHUNK);
 
@@ -281,7 +284,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) raw[ks][j] = in_c.turned(tc, ks, col0 + 16 * j);
+            for (int j = 0; j < NT; ++j) raw[ks][j] = in_c.template turned<NT>(tc, ks, col0, j);
         u32x4 plane[2][PLANES][NT];
         // words e of the decayed c of step ks, column tile j
         auto decay = [&](int ks, int j, int e) __attribute__((always_inline)) {
@@ -449,23 +452,26 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             for (int t = 0; t < 4; ++t) {
                 const int i = 16 * t + m, row = reverse ? count - 1 - i : i;
                 const float by = HALF ? score_up[t] : 1.0f;
+                unsigned words[2 * NT];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const int first = col0 + 16 * j + 4 * g;
-                    const u32x2 words = {Mma<T>::pack2(acc[j][t][0] * by, acc[j][t][1] * by), Mma<T>::pack2(acc[j][t][2] * by, acc[j][t][3] * by)};
-                    if constexpr (VEC && WHOLE) {  // each wave has the same number of stores under way, whatever there is to store
-                        __builtin_amdgcn_raw_buffer_store_b64(words, to, first < Dc ? out_at + 32 * j : NOWHERE, (unsigned)((reverse ? 3 - t : t) * 32 * (int)out_st), 0);
-                    } else if constexpr (VEC) {
-                        __builtin_amdgcn_raw_buffer_store_b64(words, to, i < count && first < Dc ? (unsigned)(row * (int)out_st + first) * 2 : NOWHERE, 0, 0);
-                    } else if (i < count) {
+                    words[2 * j] = Mma<T>::pack2(acc[j][t][0] * by, acc[j][t][1] * by);
+                    words[2 * j + 1] = Mma<T>::pack2(acc[j][t][2] * by, acc[j][t][3] * by);
+                }
+                if constexpr (VEC) {  // each wave has the same number of stores under way, whatever there is to store
+                    const unsigned place = WHOLE ? (first_col < Dc ? out_at : NOWHERE)
+                                                 : (i < count && first_col < Dc ? (unsigned)(row * (int)out_st + first_col) * 2 : NOWHERE);
+                    const unsigned tile = WHOLE ? (unsigned)((reverse ? 3 - t : t) * 32 * (int)out_st) : 0;
+                    if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b64(u32x2{words[0], words[1]}, to, place, tile, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b128(u32x4{words[0], words[1], words[2], words[3]}, to, place, tile, 0);
+                } else if (i < count) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (first + r < Dc) reinterpret_cast<unsigned short*>(out + row * out_st)[first + r] = (unsigned short)(words[r / 2] >> (16 * (r % 2)));
-                    }
+                    for (int r = 0; r < 4 * NT; ++r)
+                        if (first_col + r < Dc) reinterpret_cast<unsigned short*>(out + row * out_st)[first_col + r] = (unsigned short)(words[r / 2] >> (16 * (r % 2)));
                 }
             }
         }
-        scan_planes::wait_vm<OUT && VEC ? 4 * NT : 0>();  // the next tiles; this chunk's stores may still be under way
+        scan_planes::wait_vm<OUT && VEC ? 4 : 0>();  // the next tiles; this chunk's stores may still be under way
         if (!OUT) stage ^= 1;
     };
     for (; from + CHUNK <= end; from += CHUNK) chunk(std::true_type{});

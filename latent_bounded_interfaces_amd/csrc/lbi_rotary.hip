@@ -19,7 +19,17 @@ namespace lbi {
 namespace rotary {
 namespace {
 
-constexpr int64_t MOST_THREADS = ((int64_t)1 << 32) - 256;  // of a launch
+constexpr int64_t MOST_UNITS = (int64_t)1 << 31;  // of a launch: what the divisions below take
+
+// n / d for n < 2^31 by a multiplication: a thread moves a piece or two, next to which the processor's own divisions count.
+struct Divisor {
+    unsigned d, factor, shift;
+    Divisor(unsigned d_ = 1) : d(d_), factor(0), shift(0) {
+        while (((uint64_t)1 << shift) < d) ++shift;
+        factor = (unsigned)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ unsigned of(unsigned n) const { return (__umulhi(n, factor) + n) >> shift; }
+};
 
 template <typename T, int N> struct Piece;
 template <int N> struct Piece<float, N> { typedef float type __attribute__((ext_vector_type(N), aligned(4 * N))); };
@@ -39,7 +49,10 @@ struct Call {
     const float *cos, *sin;  // [table, R / 2]
     const void* positions;   // [B, T], NULL: 0, 1, ...; 8 bytes each if positions_wide
     int64_t stride_b, stride_t;  // of the packed projection
-    int64_t table, first, units;
+    int64_t table, first_row;
+    unsigned units;  // of this launch
+    Divisor places, heads, by_t, by_p;
+    unsigned first_bp, first_t;  // of the launch's first row
     int positions_wide, P, T, H, Hkv, shared, D, R, interleaved;  // shared: heads of k and v that are added up
 };
 
@@ -49,17 +62,27 @@ __device__ __forceinline__ int64_t row_of_table(const Call& c, int64_t b, int64_
     return at >= 0 && at < c.table ? at : -1;
 }
 
-// N elements from `p` on, `shared` times `apart` elements apart, added up.
+// N elements from `p` on, `shared` times `apart` elements apart, added up; four are asked for at once.
 template <typename T, int N> __device__ __forceinline__ void load(const T* p, int shared, int64_t apart, float* x) {
     typedef typename Piece<T, N>::type piece;
-    const piece own = *reinterpret_cast<const piece*>(p);
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = 0.0f;
+    for (int s = 0; s < shared; s += 4) {
+        piece own[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (s + k < shared) own[k] = *reinterpret_cast<const piece*>(p + (s + k) * apart);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (s + k < shared)
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[e] += widen(own[k][e]);
+    }
+}
+template <typename T, int N> __device__ __forceinline__ void load(const T* p, float* x) {
+    const typename Piece<T, N>::type own = *reinterpret_cast<const typename Piece<T, N>::type*>(p);
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = widen(own[e]);
-    for (int s = 1; s < shared; ++s) {
-        const piece more = *reinterpret_cast<const piece*>(p + s * apart);
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] += widen(more[e]);
-    }
 }
 template <typename T, int N> __device__ __forceinline__ void store(T* p, const float* x) {
     typedef typename Piece<T, N>::type piece;
@@ -71,20 +94,26 @@ template <typename T, int N> __device__ __forceinline__ void store(T* p, const f
 
 // A unit is a place of a head of a row: half layout, pairs of pieces of the turned part, then the pieces of the rest; interleaved, the pieces in order.
 template <typename T, int N, bool BACK> __global__ __launch_bounds__(256) void rotary_kernel(Call c) {
-    const int64_t id = c.first + (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const unsigned id = blockIdx.x * 256 + threadIdx.x;
     if (id >= c.units) return;
-    const int turned = c.interleaved ? c.R / N : c.R / 2 / N, places = turned + (c.D - c.R) / N;  // of a head
+    const int turned = c.interleaved ? c.R / N : c.R / 2 / N;  // places of a head's turned part
     const int heads = c.H + (BACK ? 2 : 1) * c.Hkv;
-    int place = (int)(id % places);
-    const int64_t rest = id / places;
-    const int head = (int)(rest % heads);
-    const int64_t row = rest / heads;  // of [B, P, T]
-    const int t = (int)(row % c.T);
-    const int64_t bp = row / c.T, b = BACK ? bp / c.P : bp;
+    const unsigned rest = c.places.of(id), row_here = c.heads.of(rest);
+    const int place = (int)(id - rest * c.places.d), head = (int)(rest - row_here * c.heads.d);
+    const int64_t row = c.first_row + row_here;  // of [B, P, T]
+    const unsigned tokens = c.first_t + row_here, bp_here = c.by_t.of(tokens);
+    const int t = (int)(tokens - bp_here * c.by_t.d);
+    const int64_t bp = c.first_bp + bp_here, b = BACK ? c.by_p.of((unsigned)bp) : bp;
     const bool is_q = head < c.H, is_v = head >= c.H + c.Hkv;
     const int own = is_q ? head : is_v ? head - c.H - c.Hkv : head - c.H;
-    const int shared = BACK && !is_q ? c.shared : 1;
-    const int64_t apart = (int64_t)c.T * c.D;  // from one head to the next
+    const int shared = is_q ? 1 : c.shared;
+    const auto bring = [&](auto count, const T* p, float* x) __attribute__((always_inline)) {
+        constexpr int COUNT = decltype(count)::value;
+        if (!BACK || shared == 1) load<T, COUNT>(p, x);
+        else load<T, COUNT>(p, shared, (int64_t)c.T * c.D, x);
+    };
+    using Pieces = std::integral_constant<int, N>;
+    using One = std::integral_constant<int, 1>;
 
     const T* from;
     T* to;
@@ -99,7 +128,7 @@ template <typename T, int N, bool BACK> __global__ __launch_bounds__(256) void r
     float x[N], y[N];
     if (place >= turned) {
         const int at = c.R + (place - turned) * N;
-        load<T, N>(from + at, shared, apart, x);
+        bring(Pieces{}, from + at, x);
         store<T, N>(to + at, x);
         return;
     }
@@ -107,7 +136,7 @@ template <typename T, int N, bool BACK> __global__ __launch_bounds__(256) void r
     const float nan = __builtin_nanf("");
     if (c.interleaved) {
         if constexpr (N % 2 == 0) {
-            load<T, N>(from + place * N, shared, apart, x);
+            bring(Pieces{}, from + place * N, x);
             if (!is_v) {
                 const float *cs = c.cos + line * (c.R / 2) + place * (N / 2), *sn = c.sin + line * (c.R / 2) + place * (N / 2);
 #pragma unroll
@@ -123,9 +152,9 @@ template <typename T, int N, bool BACK> __global__ __launch_bounds__(256) void r
             store<T, N>(to + place * N, y);
         } else {  // one element: its pair's other one is next to it
             const int at = place, other = at ^ 1;
-            load<T, 1>(from + at, shared, apart, x);
+            bring(One{}, from + at, x);
             if (!is_v) {
-                load<T, 1>(from + other, shared, apart, y);
+                bring(One{}, from + other, y);
                 const float co = line < 0 ? nan : c.cos[line * (c.R / 2) + at / 2];
                 float si = line < 0 ? nan : c.sin[line * (c.R / 2) + at / 2];
                 if ((at & 1) == 0) si = -si;
@@ -137,8 +166,8 @@ template <typename T, int N, bool BACK> __global__ __launch_bounds__(256) void r
         return;
     }
     const int at = place * N, half = c.R / 2;
-    load<T, N>(from + at, shared, apart, x);
-    load<T, N>(from + at + half, shared, apart, y);
+    bring(Pieces{}, from + at, x);
+    bring(Pieces{}, from + at + half, y);
     if (!is_v) {
         const float *cs = c.cos + line * half + at, *sn = c.sin + line * half + at;
 #pragma unroll
@@ -156,10 +185,14 @@ template <typename T, int N, bool BACK> __global__ __launch_bounds__(256) void r
 bool off(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
 template <typename T, int N, bool BACK> int launch(Call c, int64_t rows, hipStream_t stream) {
-    const int turned = c.interleaved ? c.R / N : c.R / 2 / N;
-    c.units = rows * (c.H + (BACK ? 2 : 1) * c.Hkv) * (turned + (c.D - c.R) / N);
-    for (c.first = 0; c.first < c.units; c.first += MOST_THREADS) {
-        const int64_t count = std::min(c.units - c.first, MOST_THREADS);
+    const int64_t places = (c.interleaved ? c.R / N : c.R / 2 / N) + (c.D - c.R) / N, heads = c.H + (BACK ? 2 : 1) * c.Hkv;
+    if (places * heads >= MOST_UNITS) return fail(LBI_ERR_UNSUPPORTED, "rotary positions: too many elements of a token");
+    c.places = Divisor((unsigned)places), c.heads = Divisor((unsigned)heads), c.by_t = Divisor((unsigned)c.T), c.by_p = Divisor((unsigned)c.P);
+    const int64_t most = std::min((MOST_UNITS - 1) / (places * heads), MOST_UNITS / 2);  // rows of a launch
+    for (int64_t first = 0; first < rows; first += most) {
+        const int64_t count = std::min(rows - first, most) * places * heads;
+        c.first_row = first, c.first_bp = (unsigned)(first / c.T), c.first_t = (unsigned)(first % c.T);
+        c.units = (unsigned)count;
         hipLaunchKernelGGL((rotary_kernel<T, N, BACK>), dim3((unsigned)((count + 255) / 256)), dim3(256), 0, stream, c);
         LBI_HIP_CHECK(hipGetLastError());
     }
@@ -185,7 +218,7 @@ int check(const char* who, int64_t B, int64_t P, int64_t T, int64_t H, int64_t H
     if (R % 2) return fail(LBI_ERR_INVALID, "%s: rotary embedding needs an even part of a head, got %lld", who, (long long)R);
     if (!dtype_size(dtype)) return fail(LBI_ERR_INVALID, "%s: bad dtype %d", who, dtype);
     if (!positions && table < T) return fail(LBI_ERR_INVALID, "%s: tables of %lld positions for %lld tokens", who, (long long)table, (long long)T);
-    if (D > (int64_t)1 << 16 || H > (int64_t)1 << 16 || T >= (int64_t)1 << 31 || P >= (int64_t)1 << 31 || B >= (int64_t)1 << 31 ||
+    if (D > (int64_t)1 << 16 || H > (int64_t)1 << 16 || T >= (int64_t)1 << 30 || P >= (int64_t)1 << 31 || B >= (int64_t)1 << 31 ||
         B * P >= (int64_t)1 << 31 || B * P * T >= (int64_t)1 << 40)
         return fail(LBI_ERR_UNSUPPORTED, "%s: too many elements", who);
     return LBI_OK;

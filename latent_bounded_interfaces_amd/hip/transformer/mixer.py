@@ -81,7 +81,7 @@ def _check_positions(what: str, positions: torch.Tensor | None, bsz: int, seqlen
         raise ValueError(f"{what}: positions must be int32 or int64")
     if positions.shape not in ((seqlen,), (bsz, seqlen)):
         raise ValueError(f"{what}: positions must be [T] or [B, T]")
-    return positions.expand(bsz, seqlen).contiguous()
+    return (positions if positions.dim() == 2 else positions.expand(bsz, seqlen)).contiguous()
 
 
 def rotary_heads(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, n_heads: int, n_kv_heads: int, interleaved: bool = False,
@@ -106,12 +106,13 @@ def rotary_heads(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, n_h
     _lib.refuse_graph(what, qkv, cos, sin)
     qkv = _dense_rows(qkv)
     q, k = qkv.new_empty(bsz, n_heads, seqlen, head_dim), qkv.new_empty(bsz, n_kv_heads, seqlen, head_dim)
-    v = qkv[..., (n_heads + n_kv_heads) * head_dim:].unflatten(-1, (n_kv_heads, head_dim)).transpose(1, 2)
+    step_b, step_t, _ = qkv.stride()
+    v = qkv.as_strided((bsz, n_kv_heads, seqlen, head_dim), (step_b, head_dim, step_t, 1), qkv.storage_offset() + (n_heads + n_kv_heads) * head_dim)
     if q.numel():
         with _lib.device_guard(qkv.device):
             status = _lib.load().lbi_rotary(
                 qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), None if positions is None else positions.data_ptr(), q.data_ptr(), k.data_ptr(),
-                bsz, seqlen, n_heads, n_kv_heads, head_dim, 2 * cos.shape[1], cos.shape[0], qkv.stride(0), qkv.stride(1),
+                bsz, seqlen, n_heads, n_kv_heads, head_dim, 2 * cos.shape[1], cos.shape[0], step_b, step_t,
                 int(positions is not None and positions.dtype == torch.int64), int(bool(interleaved)), dtype, _stream(qkv))
         _lib.check(status, "lbi_rotary")
     return q, k, v

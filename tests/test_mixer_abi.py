@@ -31,7 +31,7 @@ def test_rotary_statuses():
         assert call(Hkv=3)[0] == -1 and b"multiple" in call(Hkv=3)[1]
         assert call(R=3)[0] == -1 and b"even" in call(R=3)[1]
         assert call(dtype=7)[0] == -1 and call(table=2)[0] == -1 and b"tables" in call(table=2)[1]
-        for bad in (dict(D=1 << 17), dict(B=1 << 31), dict(T=1 << 31, table=1 << 31), dict(B=1 << 20, T=1 << 20, table=1 << 20)):
+        for bad in (dict(D=1 << 17), dict(B=1 << 31), dict(T=1 << 30, table=1 << 30), dict(B=1 << 20, T=1 << 20, table=1 << 20)):
             assert call(**bad)[0] == -2, bad
         for name in ("cos", "sin", "q", "k"):
             assert call(**{name: None})[0] == -1 and b"null" in call(**{name: None})[1], name
