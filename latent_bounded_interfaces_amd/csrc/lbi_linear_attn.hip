@@ -24,22 +24,26 @@ int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
     return dtype == LBI_F16 ? run_f16(call, stream) : run_bf16(call, exact_last, stream);
 }
 
-// Segments that a chain is cut into: none while the chains alone fill the chip.
-int segments_of(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
-    const int64_t chunks = (T + CHUNK - 1) / CHUNK, room = (int64_t)device_compute_units() * (Dc > 64 || Da > 64 ? 2 : 3);
-    if (units * 2 > room || chunks < 4) return 1;
-    const int64_t wanted = std::min(room / units, chunks / 2), of = (chunks + wanted - 1) / wanted;
+// Segments that a chain is cut into: none where the chains alone give a workgroup to half the CUs, as many as make two for each otherwise.  us, with 1 / 2 / 4 /
+// 8 / 16 / 32 segments: 64 chains of 4096 tokens of 128 223 / 176 / 123 / 117 / 156 / 199, 12 of 8192 of 64 176 / 140 / 79 / 48 / 35 / 33, 8 of 2999
+// of 80 and 112 162 / 118 / 67 / 44 / 35 / 33, 96 of 1024 of 64 30 / 30 / 28 / 29 / 43; 192 of 2048 of 128 109 / 110 / 122 / 146, 288 of 1024 of 64 39 /
+// 42 / 45 / 58.
+int segments_of(int64_t units, int64_t T) {
+    const int64_t chunks = (T + CHUNK - 1) / CHUNK, cus = device_compute_units();
+    if (2 * units >= cus || chunks < 4) return 1;
+    const int64_t wanted = std::min(2 * cus / units, chunks / 2), of = (chunks + wanted - 1) / wanted;
     return (int)((chunks + of - 1) / of);
 }
 size_t states_bytes(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
-    return (size_t)units * (segments_of(units, T, Da, Dc) - 1) * Da * Dc * sizeof(float);
+    return (size_t)units * (segments_of(units, T) - 1) * Da * Dc * sizeof(float);
 }
 void cut(Call& call, float* workspace) {
     const int64_t chunks = (call.T + CHUNK - 1) / CHUNK;
-    call.segments = segments_of((int64_t)call.chains * call.B * call.P * call.H, call.T, call.chain[0].Da, call.chain[0].Dc);
+    call.segments = segments_of((int64_t)call.chains * call.B * call.P * call.H, call.T);
     call.segment = (int)((chunks + call.segments - 1) / call.segments) * CHUNK;
     call.segment_states = workspace;
-    call.joined = call.segments > 8;
+    // a workgroup adds up to fourteen segments' states by itself (us, by itself / by a launch: 11 segments 42 / 42, 79 / 80, 16 71 / 70, 38 / 35, 32 91 / 73)
+    call.joined = call.segments > 15;
 }
 
 bool any_null(std::initializer_list<const void*> pointers) {

@@ -477,10 +477,17 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     for (; from + CHUNK <= end; from += CHUNK) chunk(std::true_type{});
     if (from < end) chunk(std::false_type{});
     if constexpr (OUT) {  // rows behind the sequence
-        T* out = const_cast<T*>(at(ch.out));
+        T* const out = const_cast<T*>(at(ch.out));
         const int stop = begin + call.segment < call.T ? begin + call.segment : call.T, past = begin > n ? begin : n;
-        for (int64_t i = (int64_t)past * Dc + threadIdx.x; i < (int64_t)stop * Dc; i += 256)
-            reinterpret_cast<unsigned short*>(out)[i / Dc * ch.out.st + i % Dc] = 0;
+        const int c8 = (int)threadIdx.x % (DC / 8) * 8;
+        for (int i = past + (int)threadIdx.x / (DC / 8); i < stop; i += 256 / (DC / 8)) {
+            T* const row = out + i * out_st + c8;
+            if (VEC && c8 < Dc) *reinterpret_cast<u32x4*>(row) = u32x4{0, 0, 0, 0};
+            if constexpr (!VEC)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c8 + e < Dc) reinterpret_cast<unsigned short*>(row)[e] = 0;
+        }
     }
     auto leave = [&](float* p, unsigned sr, unsigned sc, float scale) __attribute__((always_inline)) {
         const auto to = scan_planes::rows(p, 0x7fffffffu);
