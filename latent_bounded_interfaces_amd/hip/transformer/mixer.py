@@ -13,7 +13,6 @@ grad mode on, or one with a tangent of forward-mode differentiation, raises.  No
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -152,20 +151,21 @@ def rotary_heads_pullback(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, 
 
 
 def _check_attention(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float, tokens: int) -> None:
-    """Shapes ``[B, H, (T,) D]`` of ``2 + tokens`` dimensions before the last, types and what no kernel takes."""
-    if q.dim() != 3 + tokens or k.dim() != q.dim() or v.dim() != q.dim() or k.shape[-1] != q.shape[-1] or v.shape[:-1] != k.shape[:-1] \
-            or k.shape[0] != q.shape[0] or (tokens and k.shape[2] != q.shape[2]):
+    """Shapes ``[B, H, (T,) D]`` (``tokens``: with ``T``), types and what no kernel takes."""
+    of_q, of_k, of_v = q.shape, k.shape, v.shape
+    if len(of_q) != 3 + tokens or len(of_k) != len(of_q) or of_v[:-1] != of_k[:-1] or of_k[0] != of_q[0] or of_k[2:] != of_q[2:]:
         raise ValueError(f"{what}: q must be [B, H, {'T, ' * tokens}Dk], k [B, Hkv, {'T, ' * tokens}Dk] and v [B, Hkv, {'T, ' * tokens}Dv]")
-    heads, kv_heads = q.shape[1], k.shape[1]
+    heads, kv_heads = of_q[1], of_k[1]
     if not heads or not kv_heads or heads % kv_heads:
         raise ValueError(f"{what}: the heads of q must be a multiple of those of k and v")
-    if not q.shape[-1] or not v.shape[-1]:
+    if not of_q[-1] or not of_v[-1]:
         raise ValueError(f"{what}: head dimensions must not be 0")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         raise ValueError(f"{what}: q, k and v must have one dtype")
     if log_decay.shape != (heads,) or log_decay.dtype != torch.float32:
         raise ValueError(f"{what}: log_decay must be [H] in fp32")
-    if not math.isfinite(scale) or scale == 0:
+    if scale == 0 or not math.isfinite(scale):
         raise ValueError(f"{what}: scale must be finite and not zero")
 
 
@@ -185,16 +185,23 @@ def _check_lengths(what: str, lengths: torch.Tensor | None, bsz: int) -> torch.T
     return lengths.contiguous()
 
 
-def _pointer(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+def _pointer(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _call(q, k, v, log_decay, scale, state, lengths, **more) -> _lib.LinearAttentionCall:
+_NO_STRIDES = (0, 0, 0, 0)
+
+
+def _call(q, k, v, log_decay, scale, state, lengths, *, basis=1, out=None, state_out=None, g_out=None, g_state=None, grads=(None, None, None),
+          d_state=None) -> bytes:
+    """``lbi_linear_attention_call`` of include/lbi_hip.h, as bytes."""
     bsz, heads, seqlen, dk = q.shape
-    return _lib.LinearAttentionCall(
-        B=bsz, H=heads, Hkv=k.shape[1], T=seqlen, Dk=dk, Dv=v.shape[-1], q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=q.stride()[:3],
-        k_stride=k.stride()[:3], v_stride=v.stride()[:3], log_decay=log_decay.data_ptr(), state=_pointer(state), lengths=_pointer(lengths),
-        lengths_wide=int(lengths is not None and lengths.dtype == torch.int64), scale=float(scale), dtype=_lib.dtype_code(q.dtype), **more)
+    _, kv_heads, _, dv = v.shape
+    return _lib.pack_linear_attention_call(
+        bsz, basis, heads, kv_heads, seqlen, dk, dv, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+        log_decay.data_ptr(), _pointer(state), _pointer(lengths), _pointer(out), *(_NO_STRIDES[:3] if out is None else out.stride()[:3]),
+        _pointer(state_out), _pointer(g_out), *(_NO_STRIDES if g_out is None else g_out.stride()[:4]), _pointer(g_state), _pointer(grads[0]),
+        _pointer(grads[1]), _pointer(grads[2]), _pointer(d_state), scale, _lib.dtype_code(q.dtype), lengths is not None and lengths.dtype == torch.int64)
 
 
 def _attention_types(what: str, q: torch.Tensor) -> None:
@@ -225,14 +232,14 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     _one_device(what, q, k, v, log_decay, state, lengths)
     _lib.refuse_graph(what, q, k, v, log_decay, state)
     q, k, v, log_decay = _dense_rows(q), _dense_rows(k), _dense_rows(v), log_decay.contiguous()
-    out = q.new_empty(bsz, seqlen, heads, dv).transpose(1, 2)
+    out = q.new_empty_strided((bsz, heads, seqlen, dv), (seqlen * heads * dv, dv, heads * dv, 1))
     state_out = q.new_empty(bsz, heads, dk, dv, dtype=torch.float32) if return_state else None
     lib = _lib.load()
     with _lib.device_guard(q.device):
-        call = _call(q, k, v, log_decay, scale, state, lengths, out=out.data_ptr(), out_stride=out.stride()[:3], state_out=_pointer(state_out))
-        need = lib.lbi_linear_attention_workspace_bytes(ctypes.byref(call))
+        call = _call(q, k, v, log_decay, scale, state, lengths, out=out, state_out=state_out)
+        need = lib.lbi_linear_attention_workspace_bytes(call)
         workspace = q.new_empty(need, dtype=torch.uint8) if need else None
-        status = lib.lbi_linear_attention(ctypes.byref(call), _pointer(workspace), need, _stream(q))
+        status = lib.lbi_linear_attention(call, _pointer(workspace), need, _stream(q))
     _lib.check(status, "lbi_linear_attention")
     return out, state_out
 
@@ -296,11 +303,10 @@ def linear_attention_input_pullback_basis(
     d_state = None if state is None else q.new_empty(bsz, basis, heads, dk, dv, dtype=torch.float32)
     lib = _lib.load()
     with _lib.device_guard(q.device):
-        call = _call(q, k, v, log_decay, scale, state, lengths, P=basis, g_out=g.data_ptr(), g_out_stride=g.stride()[:4], g_state=_pointer(g_state),
-                     dq=grads[0].data_ptr(), dk=grads[1].data_ptr(), dv=grads[2].data_ptr(), d_state=_pointer(d_state))
-        need = lib.lbi_linear_attention_pullback_workspace_bytes(ctypes.byref(call))
+        call = _call(q, k, v, log_decay, scale, state, lengths, basis=basis, g_out=g, g_state=g_state, grads=grads, d_state=d_state)
+        need = lib.lbi_linear_attention_pullback_workspace_bytes(call)
         workspace = q.new_empty(need, dtype=torch.uint8) if need else None
-        status = lib.lbi_linear_attention_pullback(ctypes.byref(call), _pointer(workspace), need, _stream(q))
+        status = lib.lbi_linear_attention_pullback(call, _pointer(workspace), need, _stream(q))
     _lib.check(status, "lbi_linear_attention_pullback")
     return (*grads, d_state)
 
