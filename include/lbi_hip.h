@@ -534,7 +534,7 @@ int lbi_gated_residual_rmsnorm_pullback(const void* g_normed, const void* branch
  * Products on the 16-bit matrix cores, sums in fp32.  Rounded to 16 bits in between: the decayed scores and a copy of the state, each as an operand
  * (in fp16 brought into range by powers of two).  The state itself is fp32; the decayed values that it adds up have 24 significant bits (22 in fp16) in calls
  * with state_out or d_state, 16 otherwise.  A value that is not finite reaches every row of its aligned 64 tokens, earlier ones too.
- * Dk, Dv up to 128; 3 B P H up to 65535; scale finite and not 0.  Results overlap no other tensor.  Reruns are bit-identical.
+ * Dk, Dv up to 128; T below 2^30, 3 B P H up to 2^28; scale finite and not 0.  Results overlap no other tensor.  Reruns are bit-identical.
  */
 typedef struct lbi_linear_attention_call {
     int64_t B, P, H, Hkv, T, Dk, Dv;

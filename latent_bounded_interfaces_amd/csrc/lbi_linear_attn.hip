@@ -18,7 +18,7 @@ int run_f16(const Call& call, hipStream_t stream);
 
 namespace {
 
-constexpr int64_t MOST_UNITS = 65535;  // of a launch's second dimension
+constexpr int64_t MOST_UNITS = (int64_t)1 << 28;  // chains of a call: a workgroup each, or a few of a hundred and less
 
 int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
     return dtype == LBI_F16 ? run_f16(call, stream) : run_bf16(call, exact_last, stream);
@@ -61,7 +61,7 @@ int check(const char* who, const lbi_linear_attention_call* call, bool pullback)
     if (c.dtype != LBI_F16 && c.dtype != LBI_BF16) return fail(dtype_size(c.dtype) ? LBI_ERR_UNSUPPORTED : LBI_ERR_INVALID, "%s: bad dtype %d", who, c.dtype);
     if (c.Dk > MOST_DIM || c.Dv > MOST_DIM) return fail(LBI_ERR_UNSUPPORTED, "%s: head dims of up to %d", who, MOST_DIM);
     const int64_t basis = pullback ? std::max<int64_t>(c.P, 1) : 1;
-    if (c.T >= (int64_t)1 << 30 || c.B >= (int64_t)1 << 20 || c.H >= (int64_t)1 << 16 || basis >= (int64_t)1 << 16 ||
+    if (c.T >= (int64_t)1 << 30 || c.B >= (int64_t)1 << 20 || c.H >= (int64_t)1 << 16 || basis >= (int64_t)1 << 20 ||
         MOST_CHAINS * c.B * c.H * basis > MOST_UNITS)
         return fail(LBI_ERR_UNSUPPORTED, "%s: too many sequences, heads and directions, or too many tokens", who);
     if (!std::isfinite(c.scale) || c.scale == 0.0f) return fail(LBI_ERR_INVALID, "%s: scale must be finite and not zero", who);

@@ -42,11 +42,11 @@ template <> struct Mma16<_Float16> {
 };
 
 // The power of two that brings values of up to `most` below 2^14, as (down, up): half precision ends at 65504, and the sums of linear
-// attention, which no softmax bounds, do not.
+// attention, which no softmax bounds, do not.  At most 2^60 down: what rounds off then is below 2^-85, and the quotient of two of them stays finite.
 struct Pow2 { float down, up; };
 __device__ __forceinline__ Pow2 into_range(float most) {
     int e = (int)(__float_as_uint(most) >> 23) - 127 - 13;
-    e = e < -100 ? -100 : e > 100 ? 0 : e;  // infinities and NaN as they are
+    e = e < -60 ? -60 : e > 100 ? 0 : e;  // infinities and NaN as they are
     return Pow2{__uint_as_float((unsigned)(127 - e) << 23), __uint_as_float((unsigned)(127 + e) << 23)};
 }
 __device__ __forceinline__ float over_wave_max(float x) {

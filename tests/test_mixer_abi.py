@@ -105,7 +105,7 @@ def test_linear_attention_statuses():
         for bad in (dict(B=-1), dict(H=0), dict(Hkv=0), dict(T=-1), dict(Dk=0), dict(Dv=0)):
             assert run(entry, **bad)[0] == -1 and b"bad size" in run(entry, **bad)[1], bad
         assert run(entry, Hkv=3)[0] == -1 and run(entry, dtype=F32)[0] == -2 and run(entry, dtype=9)[0] == -1
-        for bad in (dict(Dk=129), dict(Dv=129), dict(T=1 << 30), dict(B=1 << 14)):
+        for bad in (dict(Dk=129), dict(Dv=129), dict(T=1 << 30), dict(B=1 << 20), dict(B=1 << 19, H=512, Hkv=2)):
             assert run(entry, **bad)[0] == -2, bad
         for bad in (0.0, math.nan, math.inf):
             assert run(entry, scale=bad)[0] == -1 and b"scale" in run(entry, scale=bad)[1]
@@ -120,7 +120,7 @@ def test_linear_attention_statuses():
         assert getattr(lib, entry + "_workspace_bytes")(ctypes.byref(_call(B=1, T=8192, Dk=200))) == 0
     assert run("lbi_linear_attention", out=None)[0] == -1 and run("lbi_linear_attention", state_out=257)[0] == -1
     pull = "lbi_linear_attention_pullback"
-    assert run(pull, P=0) == (0, b"") and run(pull, P=-1)[0] == -1 and run(pull, P=1 << 14)[0] == -2
+    assert run(pull, P=0) == (0, b"") and run(pull, P=-1)[0] == -1 and run(pull, P=1 << 20)[0] == -2
     for name in ("g_out", "dq", "dk", "dv"):
         assert run(pull, **{name: None})[0] == -1 and run(pull, **{name: 257})[0] == -1, name
     assert run(pull, g_state=258)[0] == -1 and run(pull, d_state=258)[0] == -1

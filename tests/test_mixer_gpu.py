@@ -131,6 +131,47 @@ def test_half_precision_past_its_largest_number(device):
     check_forward(q, k, v, log_decay, None, None, 1e-6, out, final)
 
 
+def test_half_precision_scores_of_nothing_beside_a_large_state(device):
+    """Keys of zero in whole tiles, a state of 2^20 in front of them and queries of hundreds: neither's scale is the other's."""
+    gen = torch.Generator().manual_seed(21)
+    q, k, v, log_decay, first = inputs(gen, 1, 2, 2, 150, 64, 64, F16, state=True)
+    k[:, :, :100] = 0
+    q, first = q * 100, first * 2.0 ** 20
+    out, final = linear_attention(*on(device, q, k, v, log_decay), scale=1e-7, state=first.to(device))
+    check_forward(q, k, v, log_decay, first, None, 1e-7, out, final)
+
+
+def test_offsets_past_32_bits(device):
+    gen = torch.Generator().manual_seed(22)
+    q, k, v, log_decay, _ = on(device, *inputs(gen, 1, 2, 2, 70, 64, 64, BF16))
+    want = linear_attention(q, k, v, log_decay, scale=0.125) + linear_attention_input_pullback_basis(q, k, v, q[:, None], log_decay, scale=0.125)[:3]
+    for strides in ((0, (1 << 31) + 64, 64, 1), (0, 64, (1 << 25) + 8, 1)):  # heads, then tokens, far apart
+        far = torch.empty(1 + sum((n - 1) * s for n, s in zip((1, 2, 70, 64), strides)), dtype=BF16, device=device)
+        views = [far.as_strided((1, 2, 70, 64), strides)]
+        for i, t in enumerate((q, k, v)):
+            views[0].copy_(t)
+            args = [q, k, v]
+            args[i] = views[0]
+            got = linear_attention(*args, log_decay, scale=0.125) + linear_attention_input_pullback_basis(*args, q[:, None], log_decay, scale=0.125)[:3]
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (strides, i)
+        del far, views
+
+
+def test_one_cotangent_for_all_tokens_and_many_directions(device):
+    gen = torch.Generator().manual_seed(23)
+    q, k, v, log_decay, _ = on(device, *inputs(gen, 2, 2, 1, 80, 64, 32, BF16))
+    g = rand(gen, 2, 3, 2, 1, 32).to(device).expand(-1, -1, -1, 80, -1)
+    for a, b in zip(linear_attention_input_pullback_basis(q, k, v, g, log_decay, scale=0.125)[:3],
+                    linear_attention_input_pullback_basis(q, k, v, g.contiguous(), log_decay, scale=0.125)[:3]):
+        assert torch.equal(a, b)
+    # more chains than a launch numbers in its second dimension
+    q, k, v, log_decay, _ = on(device, *inputs(gen, 1, 2, 2, 3, 8, 8, BF16))
+    g = rand(gen, 1, 12000, 2, 3, 8).to(device)
+    got = linear_attention_input_pullback_basis(q, k, v, g, log_decay, scale=0.5)
+    some = linear_attention_input_pullback_basis(q, k, v, g[:, 11990:], log_decay, scale=0.5)
+    assert all(torch.equal(a[:, 11990:], b) for a, b in zip(got[:3], some[:3]))
+
+
 def test_strides(device):
     gen = torch.Generator().manual_seed(8)
     packed = rand(gen, 2, 150, (4 + 2 * 2) * 64).to(device)
