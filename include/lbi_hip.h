@@ -533,7 +533,8 @@ int lbi_gated_residual_rmsnorm_pullback(const void* g_normed, const void* branch
  *
  * Products on the 16-bit matrix cores, sums in fp32.  Rounded to 16 bits in between: the decayed scores and a copy of the state, each as an operand
  * (in fp16 brought into range by powers of two).  The state itself is fp32; the decayed values that it adds up have 24 significant bits (22 in fp16) in calls
- * with state_out or d_state, 16 otherwise.  A value that is not finite reaches every row of its aligned 64 tokens, earlier ones too.
+ * with state_out or d_state, 16 otherwise.  A value that is not finite reaches every row of its 64 tokens (of a multiple of 64 and the 63 behind it, for
+ * dk and dv counted back from a sequence's last token), earlier ones too.
  * Dk, Dv up to 128; T below 2^30, 3 B P H up to 2^28; scale finite and not 0.  Results overlap no other tensor.  Reruns are bit-identical.
  */
 typedef struct lbi_linear_attention_call {
@@ -562,6 +563,7 @@ int lbi_linear_attention_pullback(const lbi_linear_attention_call* call, void* w
 /*
  * One token of each sequence: q [B,H,Dk], k [B,Hkv,Dk], v [B,Hkv,Dv], out [B,H,Dv] contiguous in dtype (fp32 too), state [B,H,Dk,Dv] fp32
  * contiguous, read and written in place.  active [B] (a byte each, NULL: all): a sequence whose byte is 0 keeps its state and gets a row of zeros.
+ * state and out overlap no other tensor and not each other.
  */
 int lbi_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, float* state, const unsigned char* active,
                               void* out, int64_t B, int64_t H, int64_t Hkv, int64_t Dk, int64_t Dv, float scale, int dtype, void* stream);

@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "lbi_linear_attn.h"
 
@@ -263,6 +264,15 @@ extern "C" int lbi_linear_attention_step(const void* q, const void* k, const voi
     if (any_null({q, k, v, log_decay, state, out})) return fail(LBI_ERR_INVALID, "lbi_linear_attention_step: null pointer");
     if (off(q, size) || off(k, size) || off(v, size) || off(out, size) || off(state, 4) || off(log_decay, 4))
         return fail(LBI_ERR_INVALID, "lbi_linear_attention_step: a tensor is not aligned to its elements");
+    const int64_t heads = B * H, kv_heads = B * Hkv;
+    const std::pair<const void*, uint64_t> places[] = {{state, heads * Dk * Dv * 4}, {out, heads * Dv * size}, {q, heads * Dk * size}, {k, kv_heads * Dk * size},
+                                                       {v, kv_heads * Dv * size},    {log_decay, H * 4},        {active, B}};
+    for (int w = 0; w < 2; ++w)  // what is written: state and out, which other workgroups of a head read beside
+        for (int o = w + 1; o < 7; ++o) {
+            const uintptr_t here = reinterpret_cast<uintptr_t>(places[w].first), there = reinterpret_cast<uintptr_t>(places[o].first);
+            if (there && here < there + places[o].second && there < here + places[w].second)
+                return fail(LBI_ERR_INVALID, "lbi_linear_attention_step: a result overlaps another tensor");
+        }
     const bool in_fours = Dv % 4 == 0 && !off(state, 16), few = B * H * 2 < device_compute_units();
     const auto go = [&](auto t) {
         using T = decltype(t);

@@ -221,7 +221,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     Returns ``(out, S)``: ``out [B, H, T, Dv]`` in the dtype of ``q``, laid out as ``[B, T, H, Dv]`` (what an output projection reads, without a copy), and
     the state ``[B, H, Dk, Dv]`` in fp32 after each sequence's last token, for :func:`linear_attention_step` or the next piece of the context (``None``
     unless ``return_state``).  Sums are fp32; the decayed scores and a copy of the state are rounded to the dtype as operands.  A value that is
-    not finite reaches the rows of its 64 tokens (those from a multiple of 64 on), earlier ones among them."""
+    not finite reaches the rows of its 64 tokens (those from a multiple of 64 on; in the pullback's ``dk`` and ``dv`` counted back from the last token),
+    earlier ones among them."""
     what = "linear_attention"
     _check_attention(what, q, k, v, log_decay, scale, 1)
     _attention_types(what, q)
@@ -247,7 +248,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, *, scale: float,
                           active: torch.Tensor | None = None) -> torch.Tensor:
     """One token of each sequence through :func:`linear_attention`: ``q [B, H, Dk]``, ``k [B, Hkv, Dk]``, ``v [B, Hkv, Dv]`` in fp32, fp16 or bf16, and
-    ``state [B, H, Dk, Dv]``, fp32 and contiguous, which is updated in place.  ``active [B]`` (bool): sequences that have no token keep their state
+    ``state [B, H, Dk, Dv]``, fp32 and contiguous, which is updated in place and shares memory with none of them.  ``active [B]`` (bool): sequences that have no token keep their state
     and get zeros.  Returns ``out [B, H, Dv]``; arithmetic is fp32."""
     what = "linear_attention_step"
     _check_attention(what, q, k, v, log_decay, scale, 0)

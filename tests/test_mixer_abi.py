@@ -240,3 +240,22 @@ def test_rotary_tables():
                 dict(original_length=5, ramp=(2.0, 1.0)), dict(magnitude=math.nan)):
         with pytest.raises(ValueError, match="rotary_tables"):
             mixer.rotary_tables(**{**dict(length=4, rotary_dim=8, device="cpu"), **bad})
+
+
+def test_a_step_refuses_a_state_that_shares_memory():
+    lib = _lib.load()
+    bsz, heads, shared, dim = 2, 4, 2, 64
+    sizes = dict(state=bsz * heads * dim * dim * 4, out=bsz * heads * dim * 2, q=bsz * heads * dim * 2, k=bsz * shared * dim * 2,
+                 v=bsz * shared * dim * 2, log_decay=heads * 4, active=bsz)
+    place, at = {}, 1 << 20
+    for name, size in sizes.items():
+        place[name], at = at, at + (size + 255) // 256 * 256
+    for written in ("state", "out"):
+        for other in sizes:
+            if other == written:
+                continue
+            for shift in (0, sizes[written] - 4, 4 - sizes[other] if sizes[other] >= 8 else 0):  # from the start, over the end, over the start
+                p = {**place, other: (1 << 30) + shift, written: 1 << 30}
+                status = lib.lbi_linear_attention_step(*(ctypes.c_void_p(p[n]) for n in ("q", "k", "v", "log_decay", "state", "active", "out")), bsz, heads,
+                                                       shared, dim, dim, 1.0, BF16, None)
+                assert status == -1 and b"overlaps" in lib.lbi_last_error(), (written, other, shift)
