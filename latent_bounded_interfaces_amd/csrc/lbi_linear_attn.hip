@@ -25,14 +25,15 @@ int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
     return dtype == LBI_F16 ? run_f16(call, stream) : run_bf16(call, exact_last, stream);
 }
 
-// Segments that a chain is cut into: none where the chains alone give a workgroup to half the CUs, as many as make two for each otherwise.  us, with 1 / 2 / 4 /
-// 8 / 16 / 32 segments: 64 chains of 4096 tokens of 128 223 / 176 / 123 / 117 / 156 / 199, 12 of 8192 of 64 176 / 140 / 79 / 48 / 35 / 33, 8 of 2999
-// of 80 and 112 162 / 118 / 67 / 44 / 35 / 33, 96 of 1024 of 64 30 / 30 / 28 / 29 / 43; 192 of 2048 of 128 109 / 110 / 122 / 146, 288 of 1024 of 64 39 /
-// 42 / 45 / 58.
+// Segments that a chain is cut into: as many as give a workgroup to each CU, since one alone on a CU takes a chunk in about 0.6 of the time of two that
+// share it, and the states in front of the segments are a pass over b and c and a join on top.  Two segments pay for that from 32 chunks on only.
+// us, with 1 / 2 / 3 / 4 / 8 / 16 / 32 segments: 64 chains of 4096 tokens of 128 173 / 153 / 123 / 106 / 118 / 154 / 201, 16 of 8192 of 128 327 / 266 / 183 / 142 /
+// 88 / 64 / 72, 12 of 8192 of 64 163 / 133 / 95 / 74 / 47 / 33 / 33; with 1 / 2 / 3 / 4: 80 of 2048 of 128 89 / 81 / 66 / 73, 96 of 4096 of 64 90 / 81 / 79 / 73,
+// of 1024 of 128 48 / 51 / 54 / 54; 128 of 4096 of 128 182 / 179 / 179 / 182; 192 of 2048 of 128 118 / 147 / 153 / 154.
 int segments_of(int64_t units, int64_t T) {
-    const int64_t chunks = (T + CHUNK - 1) / CHUNK, cus = device_compute_units();
-    if (2 * units >= cus || chunks < 4) return 1;
-    const int64_t wanted = std::min(2 * cus / units, chunks / 2), of = (chunks + wanted - 1) / wanted;
+    const int64_t chunks = (T + CHUNK - 1) / CHUNK, each = device_compute_units() / std::max<int64_t>(units, 1);
+    if (each < 2 || chunks < (each == 2 ? 32 : 4)) return 1;
+    const int64_t wanted = std::min(each, chunks / 2), of = (chunks + wanted - 1) / wanted;
     return (int)((chunks + of - 1) / of);
 }
 size_t states_bytes(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
@@ -43,7 +44,8 @@ void cut(Call& call, float* workspace) {
     call.segments = segments_of((int64_t)call.chains * call.B * call.P * call.H, call.T);
     call.segment = (int)((chunks + call.segments - 1) / call.segments) * CHUNK;
     call.segment_states = workspace;
-    // a workgroup adds up to fourteen segments' states by itself (us, by itself / by a launch: 11 segments 42 / 42, 79 / 80, 16 71 / 70, 38 / 35, 32 91 / 73)
+    // A workgroup adds up to fourteen segments' states by itself: a launch costs what it saves there (us, by itself / by a launch: 11 segments 42 / 42 and
+    // 79 / 80, 16 71 / 70 and 38 / 35, 32 91 / 73).
     call.joined = call.segments > 15;
 }
 

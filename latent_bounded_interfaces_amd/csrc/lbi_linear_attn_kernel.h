@@ -164,16 +164,16 @@ __device__ __forceinline__ bool unit_of(const Call& call, int segments, Unit& u)
     return true;
 }
 
-template <int DA, int DC, bool OUT> constexpr int stage_bytes() { return CHUNK * 2 * ((OUT ? 2 : 1) * DA + DC); }
-// One stage where the next tiles come in behind the barrier, two where there is none.
-template <int DA, int DC, bool OUT> constexpr int lds_bytes() { return (OUT ? 1 : 2) * stage_bytes<DA, DC, OUT>() + (OUT ? CHUNK * CHUNK * 2 : 0); }
+// Two tiles of b; of c one and a's and the scores, or two of c where only the state is wanted.
+template <int DA, int DC, bool OUT> constexpr int lds_bytes() { return CHUNK * 2 * (OUT ? 3 * DA + DC + CHUNK : 2 * (DA + DC)); }
 
 // OUT false: only the state that a segment leaves behind, from zero, into its slot.
 template <typename T, int DA, int DC, bool VEC, bool OUT, int PLANES>
 __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chunk_kernel(Call call) {
     constexpr bool HALF = std::is_same_v<T, _Float16>;
-    constexpr int KS = DA / 32, MT = DA / 16, NT = DC / 64, STAGE = stage_bytes<DA, DC, OUT>();  // steps and tiles of the state: rows, this wave's columns
-    extern __shared__ __align__(16) char lds[];  // stages of b, c, a; then the scores
+    constexpr int KS = DA / 32, MT = DA / 16, NT = DC / 64;  // steps and tiles of the state: rows, this wave's columns
+    constexpr int TILE_A = CHUNK * 2 * DA, TILE_C = CHUNK * 2 * DC, AT_C = 2 * TILE_A, AT_A = AT_C + TILE_C, AT_P = AT_A + TILE_A;
+    extern __shared__ __align__(16) char lds[];  // b, b, c, a, the scores; b, b, c, c
     __shared__ float score_up[4];
     Unit u;
     if (!unit_of(call, OUT ? call.segments : call.segments - 1, u)) return;
@@ -189,13 +189,18 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     Tile<T, DA, 256, VEC> a(OUT ? at(ch.a) : nullptr, ch.a.st, Da, reverse, chunk_at), b(at(ch.b), ch.b.st, Da, reverse, chunk_at);
     Tile<T, DC, 256, VEC> c(at(ch.c), ch.c.st, Dc, reverse, chunk_at);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
-    auto bring = [&](int stage, int from) __attribute__((always_inline)) {
-        const int count = end - from < CHUNK ? end - from : CHUNK, to = stage * STAGE;
-        b.bring(lds + to, lds0 + to, reverse, count, w);
-        c.bring(lds + to + CHUNK * 2 * DA, lds0 + to + CHUNK * 2 * DA, reverse, count, w);
-        if constexpr (OUT) a.bring(lds + to + CHUNK * 2 * (DA + DC), lds0 + to + CHUNK * 2 * (DA + DC), reverse, count, w);
+    auto bring_b = [&](int stage, int from) __attribute__((always_inline)) {
+        b.bring(lds + stage * TILE_A, lds0 + stage * TILE_A, reverse, end - from < CHUNK ? end - from : CHUNK, w);
     };
-    if (begin < end) bring(0, begin);
+    auto bring_rest = [&](int stage, int from) __attribute__((always_inline)) {
+        const int count = end - from < CHUNK ? end - from : CHUNK, to = AT_C + (OUT ? 0 : stage * TILE_C);
+        c.bring(lds + to, lds0 + to, reverse, count, w);
+        if constexpr (OUT) a.bring(lds + AT_A, lds0 + AT_A, reverse, count, w);
+    };
+    if (begin < end) {
+        bring_b(0, begin);
+        bring_rest(0, begin);
+    }
 
     // l to the power of tokens apart (and the result's scale): of this lane's scores, 0 for later tokens, of its readouts and of its rows of c
     const float l16 = exp2f(rate2 * 16.0f), l32 = exp2f(rate2 * 32.0f), l48 = exp2f(rate2 * 48.0f);
@@ -273,11 +278,15 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     auto chunk = [&](auto whole_tag) __attribute__((always_inline)) {
         constexpr bool WHOLE = decltype(whole_tag)::value;  // 64 tokens
         lds_barrier();  // this chunk's tiles are there
-        const lds_ptr tb = (lds_ptr)lds + stage * STAGE, tc = tb + CHUNK * 2 * DA, ta = tc + CHUNK * 2 * DC, tp = (lds_ptr)lds + STAGE;
+        const lds_ptr tb = (lds_ptr)lds + stage * TILE_A, tc = (lds_ptr)lds + AT_C + (OUT ? 0 : stage * TILE_C), ta = (lds_ptr)lds + AT_A, tp = (lds_ptr)lds + AT_P;
         // (what is made of them stays in this loop: in front of it, each would take a register)
         asm volatile("" : "+v"(in_a.nat_), "+v"(in_a.split_), "+v"(in_a.turned_), "+v"(in_p.nat_), "+v"(in_p.split_), "+v"(NT == 1 ? in_c.turned_ : in_c.halved_));
         const int count = WHOLE ? CHUNK : end - from;
-        if (!OUT && WHOLE && from + CHUNK < end) bring(stage ^ 1, from + CHUNK);
+        const bool more_tokens = WHOLE && from + CHUNK < end;
+        if (more_tokens) {
+            bring_b(stage ^ 1, from + CHUNK);
+            if (!OUT) bring_rest(stage ^ 1, from + CHUNK);
+        }
 
         // What a wave issues between its products runs beside them: each stretch below, between fences, holds the vector work of a later one.
         u32x4 raw[2][NT];  // the chunk's c: as it is for the scores, decayed for the state
@@ -399,39 +408,39 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             for (int i = 0; i < MT; ++i) move_on(i);
         }
 
-        u32x4 rows = in_a.turned(tb, 0, 0);
+        T* const out = OUT ? next_out + (WHOLE || !reverse ? 0 : (CHUNK - count) * out_st) : nullptr;
+        const auto to = scan_planes::rows(out, 0x7fffffffu);
+        auto store = [&](int t) __attribute__((always_inline)) {  // sixteen rows
+            const int i = 16 * t + m, row = reverse ? count - 1 - i : i;
+            const float by = HALF ? score_up[t] : 1.0f;
+            unsigned words[2 * NT];
 #pragma unroll
-        for (int step = 0; step < 2 * MT; ++step) {
-            const int ks = step / MT, i = step % MT;
-            u32x4 more;
-            if (step + 1 < 2 * MT) more = in_a.turned(tb, (step + 1) / MT, 16 * ((step + 1) % MT));
+            for (int j = 0; j < NT; ++j) {
+                words[2 * j] = Mma<T>::pack2(acc[j][t][0] * by, acc[j][t][1] * by);
+                words[2 * j + 1] = Mma<T>::pack2(acc[j][t][2] * by, acc[j][t][3] * by);
+            }
+            if constexpr (VEC) {  // each wave has the same number of stores under way, whatever there is to store
+                const unsigned place = WHOLE ? (first_col < Dc ? out_at : NOWHERE)
+                                             : (i < count && first_col < Dc ? (unsigned)(row * (int)out_st + first_col) * 2 : NOWHERE);
+                const unsigned tile = WHOLE ? (unsigned)((reverse ? 3 - t : t) * 32 * (int)out_st) : 0;
+                if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b64(u32x2{words[0], words[1]}, to, place, tile, 0);
+                else __builtin_amdgcn_raw_buffer_store_b128(u32x4{words[0], words[1], words[2], words[3]}, to, place, tile, 0);
+            } else if (i < count) {
 #pragma unroll
-            for (int q = PLANES - 1; q >= 0; --q)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) x[i][j] = Mma16<T>::mma(rows, plane[ks][q][j], x[i][j]);
-            if (ks == 0)
-#pragma unroll
-                for (int p = i * 4 * NT / MT; p < (i + 1) * 4 * NT / MT; ++p) decay(1, p / 4, p % 4);
-            if constexpr (WHOLE)
-#pragma unroll
-                for (int n_ = 0; n_ < PLANES * NT; ++n_) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-                }
-            LBI_PHASE_FENCE();
-            rows = more;
-        }
-
+                for (int r = 0; r < 4 * NT; ++r)
+                    if (first_col + r < Dc) reinterpret_cast<unsigned short*>(out + row * out_st)[first_col + r] = (unsigned short)(words[r / 2] >> (16 * (r % 2)));
+            }
+        };
         if constexpr (OUT) {
-            lds_barrier();  // the scores are there, and everyone is done with the tiles
+            next_out += reverse ? -CHUNK * out_st : CHUNK * out_st;
+            lds_barrier();  // the scores are there, and everyone is done with a and c
             u32x4 scores[2][4];  // (read before the next tiles are asked for, which they would wait behind)
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int t = 2 * ks; t < 4; ++t) scores[ks][t] = in_p.nat(tp, t, ks);
             LBI_PHASE_FENCE();
-            if (WHOLE && from + CHUNK < end) bring(0, from + CHUNK);
+            if (more_tokens) bring_rest(0, from + CHUNK);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 float by = read0 * (t == 0 ? 1.0f : t == 1 ? l16 : t == 2 ? l32 : l48);
@@ -445,34 +454,37 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 for (int t = 2 * ks; t < 4; ++t)
 #pragma unroll
                     for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(raw[ks][j], scores[ks][t], acc[j][t]);
-            T* const out = next_out + (WHOLE || !reverse ? 0 : (CHUNK - count) * out_st);
-            next_out += reverse ? -CHUNK * out_st : CHUNK * out_st;
-            const auto to = scan_planes::rows(out, 0x7fffffffu);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int i = 16 * t + m, row = reverse ? count - 1 - i : i;
-                const float by = HALF ? score_up[t] : 1.0f;
-                unsigned words[2 * NT];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    words[2 * j] = Mma<T>::pack2(acc[j][t][0] * by, acc[j][t][1] * by);
-                    words[2 * j + 1] = Mma<T>::pack2(acc[j][t][2] * by, acc[j][t][3] * by);
-                }
-                if constexpr (VEC) {  // each wave has the same number of stores under way, whatever there is to store
-                    const unsigned place = WHOLE ? (first_col < Dc ? out_at : NOWHERE)
-                                                 : (i < count && first_col < Dc ? (unsigned)(row * (int)out_st + first_col) * 2 : NOWHERE);
-                    const unsigned tile = WHOLE ? (unsigned)((reverse ? 3 - t : t) * 32 * (int)out_st) : 0;
-                    if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b64(u32x2{words[0], words[1]}, to, place, tile, 0);
-                    else __builtin_amdgcn_raw_buffer_store_b128(u32x4{words[0], words[1], words[2], words[3]}, to, place, tile, 0);
-                } else if (i < count) {
-#pragma unroll
-                    for (int r = 0; r < 4 * NT; ++r)
-                        if (first_col + r < Dc) reinterpret_cast<unsigned short*>(out + row * out_st)[first_col + r] = (unsigned short)(words[r / 2] >> (16 * (r % 2)));
-                }
-            }
+            LBI_PHASE_FENCE();
         }
+
+        u32x4 rows = in_a.turned(tb, 0, 0);
+#pragma unroll
+        for (int step = 0; step < 2 * MT; ++step) {
+            const int ks = step / MT, i = step % MT;
+            u32x4 more;
+            if (step + 1 < 2 * MT) more = in_a.turned(tb, (step + 1) / MT, 16 * ((step + 1) % MT));
+#pragma unroll
+            for (int q = PLANES - 1; q >= 0; --q)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) x[i][j] = Mma16<T>::mma(rows, plane[ks][q][j], x[i][j]);
+            if (ks == 0)
+#pragma unroll
+                for (int p = i * 4 * NT / MT; p < (i + 1) * 4 * NT / MT; ++p) decay(1, p / 4, p % 4);
+            if constexpr (OUT)
+                if (ks == 1 && i < 4) store(i);
+            if constexpr (WHOLE)
+#pragma unroll
+                for (int n_ = 0; n_ < PLANES * NT; ++n_) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                }
+            LBI_PHASE_FENCE();
+            rows = more;
+        }
+
         scan_planes::wait_vm<OUT && VEC ? 4 : 0>();  // the next tiles; this chunk's stores may still be under way
-        if (!OUT) stage ^= 1;
+        stage ^= 1;
     };
     for (; from + CHUNK <= end; from += CHUNK) chunk(std::true_type{});
     if (from < end) chunk(std::false_type{});
