@@ -39,7 +39,9 @@ Plan plan_of(int64_t rows, int64_t D, int64_t per_gate) {
     Plan p;
     p.per_gate = summed ? per_gate : std::max<int64_t>(rows, 1);
     p.gates = summed ? rows / per_gate : 1;
-    const int64_t slabs = D <= 1024 ? 1024 : 512, least = D <= 512 ? 2048 / D : 1;
+    // One slab a CU for short sums over narrow rows and for the widest rows, two otherwise (us, one / two, bf16 with a gate for each of 5 sequences: 5015 rows of
+    // 768 20 / 22, 40000 94 / 88, 1000 12 / 17; 5015 of 2048 44 / 33, of 4096 62 / 58, of 8192 117 / 123; four take 22 to 40 % longer, but 40000 x 1024).
+    const int64_t cus = device_compute_units(), slabs = D > 4096 || (D <= 1024 && rows <= 16384) ? cus : 2 * cus, least = D <= 512 ? 2048 / D : 1;
     p.slab = (int)std::min<int64_t>(std::max<int64_t>((rows + slabs - 1) / slabs, least), p.per_gate);
     p.slabs_per_gate = (int)((p.per_gate + p.slab - 1) / p.slab);
     return p;
@@ -142,7 +144,9 @@ extern "C" int lbi_gated_residual_rmsnorm_pullback(const void* g_normed, const v
     }
     // one launch for all sums, in so many more as there are gates past what a launch numbers
     const int64_t outs = 2 + (summed && rows ? plan.gates : 0);
-    const bool wide = D >= 1024;  // enough columns to fill the chip in whole lines
+    // Enough columns to fill the chip in whole lines (us of a pullback of 5015 rows, 16 / 64 columns: 768 wide 29.7 / 29.8, 2048 35 / 33, 8192 179 / 167; of 64 of
+    // 1024 10.1 / 10.6).
+    const bool wide = D > 1024;
     for (int64_t first = 0; first < outs; first += 65535) {
         const auto fold = wide ? gated_fold_kernel<64, 16> : gated_fold_kernel<16, 64>;
         hipLaunchKernelGGL(fold, dim3((unsigned)((D + (wide ? 63 : 15)) / (wide ? 64 : 16)), (unsigned)std::min<int64_t>(outs - first, 65535)), dim3(1024),

@@ -103,7 +103,7 @@ template <int COUNT, int NT> __device__ __forceinline__ void sums(float (&x)[COU
 
 enum Gate { SHARED, EACH };  // SHARED: by the rows of a slab; none at all is one of ones whose gradient nobody wants
 
-// A workgroup takes the rows of one slab, which lies within the rows of one gate, as norm_pullback_kernel does.
+// A workgroup takes the rows of one slab, which lies within the rows of one gate, SIDE of them at a time, and keeps the sums over them in registers.
 template <typename T, typename R, int GATE, bool MORE, bool TAIL, int NT, int PIECES>
 __global__ __launch_bounds__(NT * SIDE<NT>) void gated_norm_pullback_kernel(const T* g_normed, const T* branch, const R* stream, const R* g_stream,
                                                                             const T* __restrict__ gate, const void* __restrict__ post_weight,
@@ -249,15 +249,18 @@ __global__ __launch_bounds__(NT * SIDE<NT>) void gated_norm_pullback_kernel(cons
         if (gate) leave(of_gate, partials.gate);
 }
 
-// Threads and pieces that hold a row of D columns; of the pullback, whose rows are six tensors and three sums, few enough a lane for the
-// registers of as many waves.
+// Threads and pieces that hold a row of D columns; the pullback, whose rows are six tensors and three sums, in as few waves as have the registers for the next
+// row too (us, 5015 rows of bf16: of 2048 256 threads of one piece 33 and of two 37, 1024 of one 44; of 4096 256 of two 58, 512 of one 68; of 8192 512 of two 122,
+// 1024 of one 167; of 1000 rows of 768 64 of two 12, 256 of one 14).
 template <bool PULLBACK, typename F> int by_row(int64_t D, F&& launch) {
     if (D <= 128) return launch(Form<16, 1>{});
     if (D <= 512) return launch(Form<64, 1>{});
     if (D <= 1024) return launch(Form<64, 2>{});
-    if (PULLBACK && D <= 2048) return launch(Form<PULLBACK ? 256 : 512, PULLBACK ? 1 : 2>{});
-    if (PULLBACK && D <= 4096) return launch(Form<512, PULLBACK ? 1 : 2>{});
-    if (D <= 8192) return launch(Form<PULLBACK ? 1024 : 512, PULLBACK ? 1 : 2>{});
+    if constexpr (PULLBACK) {
+        if (D <= 2048) return launch(Form<256, 1>{});
+        if (D <= 4096) return launch(Form<256, 2>{});
+    }
+    if (D <= 8192) return launch(Form<512, 2>{});
     return launch(Form<1024, 2>{});
 }
 
