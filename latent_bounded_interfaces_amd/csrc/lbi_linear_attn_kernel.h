@@ -4,8 +4,17 @@
 // fp32 and in registers for the whole segment, and never exchanges them: the accumulators of X, packed, are the operand of the next readout.
 //   1  wave w: the scores of tokens i = 16 w ... 16 w + 15 with all j <= i, times l^(i-j), rounded to 16 bits into LDS
 //   2  every wave: X^T a^T of its columns, the readout of the state in front of the chunk
-//   3  every wave: X = l^64 X + b^T (l^(63-j) c), the decayed c in planes of 16 bits that add up to 16 or 24 significant bits (22 in half precision)
-//   4  behind a barrier: out^T = l^(i+1) readout + c^T scores^T, from registers and the scores alone, while the next chunk's tiles come in
+//   3  behind a barrier: out^T = l^(i+1) readout + c^T scores^T, from registers and the scores alone
+//   4  every wave: X = l^64 X + b^T (l^(63-j) c), the decayed c in planes of 16 bits that add up to 16 or 24 significant bits (22 in half precision), while
+//      the results go out
+// b has two tiles in LDS and the next chunk's comes in from the start of this one; a and c have one, which is free behind 2's barrier.  72 KB for heads of
+// 128, so that two workgroups share a CU, whose vector work then runs beside the other's products.
+//
+// Bound by memory in long calls that fill the chip: 512 chains of 4096 tokens of 128 457 us, 4.7 TB/s, 1024 of 2048 of 64 235 us, 4.6 TB/s, of the 4.9 that a copy
+// reaches.  The pullback of 4 directions for 4 x 16 heads of 4096 of 128, three chains each, takes 470 to 510 us (1.24 GB, 2.5 TB/s): 768 workgroups are one and a
+// half rounds of the 512 that fit, and of a chunk's 124 products and 400 vector instructions a wave about three quarters run beside nothing else.  All
+// tiles asked for behind the last barrier, as long as the results took, had it at 541 us; a second tile of c instead of b's gained with one workgroup a CU
+// and lost with two; eight waves of 16 columns, priorities of waves, results past the caches (4 to 40 % slower) did not pay.
 #pragma once
 
 #include "lbi_linear_attn.h"
@@ -66,8 +75,13 @@ __device__ __forceinline__ float rate_of(const Call& call, int h) {
     return l < -1e30f ? -1e30f : l;
 }
 
+// So many 16-bit elements that start on any of them: the memory takes such pieces as a whole, too.
+template <int N> struct Any { typedef unsigned short type __attribute__((ext_vector_type(N), aligned(2))); };
+template <int N> using Anywhere = typename Any<N>::type;
+
 // A tile of 64 tokens, rows of DIM 16-bit elements in LDS (16-byte pieces, swizzled as in lbi_attn_mfma.h).  VEC: by transfers of 16 bytes past the
-// registers, zeros past the end of a row and behind the last token; otherwise, rows that start on any element, an element at a time.
+// registers, zeros past the end of a row and behind the last token; otherwise, rows that start on any element, by loads of the same size where they
+// are whole.
 template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
     static constexpr int PIECES = DIM / 8, N = CHUNK * PIECES / THREADS;
     const T* next;  // where the chunk that is brought next lies in memory (reverse: as if it were whole)
@@ -105,7 +119,8 @@ template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
                 const int id = u * THREADS + (int)threadIdx.x, r = id / PIECES, c = id % PIECES * 8;
                 const unsigned short* raw = reinterpret_cast<const unsigned short*>(from + (int64_t)(reverse ? count - 1 - r : r) * st + c);
                 u32x4 words = {0, 0, 0, 0};
-                if (r < count)
+                if (r < count && c + 8 <= dim) words = __builtin_bit_cast(u32x4, *reinterpret_cast<const Anywhere<8>*>(raw));
+                else if (r < count)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         words[e] = (c + 2 * e < dim ? raw[2 * e] : 0u) | (c + 2 * e + 1 < dim ? (unsigned)raw[2 * e + 1] << 16 : 0u);
@@ -425,6 +440,12 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 const unsigned tile = WHOLE ? (unsigned)((reverse ? 3 - t : t) * 32 * (int)out_st) : 0;
                 if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b64(u32x2{words[0], words[1]}, to, place, tile, 0);
                 else __builtin_amdgcn_raw_buffer_store_b128(u32x4{words[0], words[1], words[2], words[3]}, to, place, tile, 0);
+            } else if (i < count && first_col + 4 * NT <= Dc) {
+                typedef unsigned whole __attribute__((ext_vector_type(2 * NT)));
+                whole all;
+#pragma unroll
+                for (int e = 0; e < 2 * NT; ++e) all[e] = words[e];
+                *reinterpret_cast<Anywhere<4 * NT>*>(out + row * out_st + first_col) = __builtin_bit_cast(Anywhere<4 * NT>, all);
             } else if (i < count) {
 #pragma unroll
                 for (int r = 0; r < 4 * NT; ++r)

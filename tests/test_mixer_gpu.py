@@ -377,6 +377,35 @@ def test_rotary_of_strided_projections(device):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("shift", (1, 2, 5))
+def test_tensors_that_start_on_any_element(device, shift, dtype):
+    gen = torch.Generator().manual_seed(23)
+
+    def shifted(t):
+        room = torch.empty(t.numel() + shift, dtype=t.dtype, device=device)
+        room[shift:].copy_(t.flatten())
+        return room[shift:].view(t.shape)
+
+    cos, sin = rotary_tables(70, 64, device=device)
+    qkv, dq = rand(gen, 2, 70, 4 * 64, dtype=dtype).to(device), rand(gen, 2, 3, 2, 70, 64, dtype=dtype).to(device)
+    for interleaved in (False, True):
+        for a, b in zip(rotary_heads(shifted(qkv), cos, sin, n_heads=2, n_kv_heads=1, interleaved=interleaved),
+                        rotary_heads(qkv, cos, sin, n_heads=2, n_kv_heads=1, interleaved=interleaved)):
+            assert torch.equal(a, b)
+        assert torch.equal(rotary_heads_pullback(shifted(dq), dq, shifted(dq), cos, sin, n_kv_heads=1, interleaved=interleaved),
+                           rotary_heads_pullback(dq, dq, dq, cos, sin, n_kv_heads=1, interleaved=interleaved))
+    if dtype == torch.float32:
+        return
+    q, g = dq[:, 0], dq
+    log_decay = torch.tensor([-0.5, -0.01], device=device)
+    for a, b in zip(linear_attention(shifted(q), q, shifted(q), log_decay, scale=0.125), linear_attention(q, q, q, log_decay, scale=0.125)):
+        assert torch.equal(a, b)
+    for a, b in zip(linear_attention_input_pullback_basis(shifted(q), q, q, shifted(g), log_decay, scale=0.125)[:3],
+                    linear_attention_input_pullback_basis(q, q, q, g, log_decay, scale=0.125)[:3]):
+        assert torch.equal(a, b)
+
+
 def _layer(gen, bsz, seqlen, heads, kv_heads, dim, dtype):
     qkv = rand(gen, bsz, seqlen, (heads + 2 * kv_heads) * dim, dtype=dtype)
     cos, sin = rotary_tables(2048, dim // 2, base=500.0, device="cpu", factor=4.0, original_length=512)
