@@ -11,9 +11,9 @@
 // 128, so that two workgroups share a CU, whose vector work then runs beside the other's products.
 //
 // Bound by memory in long calls that fill the chip: 512 chains of 4096 tokens of 128 457 us, 4.7 TB/s, 1024 of 2048 of 64 235 us, 4.6 TB/s, of the 4.9 that a copy
-// reaches.  The pullback of 4 directions for 4 x 16 heads of 4096 of 128, three chains each, takes 470 to 510 us (1.24 GB, 2.5 TB/s): 768 workgroups are one and a
-// half rounds of the 512 that fit, and of a chunk's 124 products and 400 vector instructions a wave about three quarters run beside nothing else.  All
-// tiles asked for behind the last barrier, as long as the results took, had it at 541 us; a second tile of c instead of b's gained with one workgroup a CU
+// reaches.  The pullback of 4 directions for 4 x 16 heads of 4096 of 128, three chains each, takes 470 to 505 us (1.28 GB, 2.6 TB/s): 768 workgroups are one and a
+// half rounds of the 512 that fit, and a chunk's 124 products and 400 vector instructions a wave take 159 and 129 us of the SIMDs in all.  All tiles
+// asked for behind the last barrier had it at 541 us; a second tile of c instead of b's gained with one workgroup a CU
 // and lost with two; eight waves of 16 columns, priorities of waves, results past the caches (4 to 40 % slower) did not pay.
 #pragma once
 

@@ -207,3 +207,10 @@ def test_captured_and_replayed(device):
         torch.cuda.synchronize()
         for got, want in zip(results, run(b, r)):
             assert torch.equal(got, want), turn
+
+
+@pytest.mark.parametrize("shape, kind", [((3, 500, 770), "sequence"), ((3, 500, 768), "channel"), ((3, 400, 2056), "sequence"), ((2, 500, 2500), None),
+                                         ((1, 600, 4104), "channel"), ((2, 300, 8191), "position"), ((1, 300, 9000), "sequence")])
+@pytest.mark.parametrize("types", [(BF16, F32, BF16), (F16, F16, F16), (F32, F32, F32)])
+def test_several_rows_for_each_workgroup(device, shape, types, kind):
+    test_forward_and_pullback(device, shape, types, kind)
