@@ -44,11 +44,14 @@ struct Call {
     Chain chain[MOST_CHAINS];
     const float* log_decay;  // [H]
     const void* lengths;     // [B], NULL: T; 8 bytes each if lengths_wide
-    float* segment_states;   // [chains, B, P, H, segments - 1, Da, Dc]
+    float* segment_states;   // [chains, B, P, H, slots, Da, Dc]
     int chains, lengths_wide;
     int B, P, H, T;
     int segments, segment;  // tokens of one, a multiple of CHUNK
-    int joined;             // a launch of its own makes the states behind the segments of what these add
+    int halved, half;       // each segment's state comes in two slots, of so many tokens (a multiple of CHUNK) and of the rest
+    int joined;             // a launch of its own makes the states behind the segments of what these add; never with halves
+    __host__ __device__ int slots() const { return (segments - 1) << halved; }
+    __host__ __device__ int slot_at(int s) const { return (s >> halved) * segment + (s & halved) * half; }  // the first token of slot s
 };
 
 }  // namespace linear_attn

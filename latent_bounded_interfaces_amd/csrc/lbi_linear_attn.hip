@@ -30,23 +30,28 @@ int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
 // us, with 1 / 2 / 3 / 4 / 8 / 16 / 32 segments: 64 chains of 4096 tokens of 128 173 / 153 / 123 / 106 / 118 / 154 / 201, 16 of 8192 of 128 327 / 266 / 183 / 142 /
 // 88 / 64 / 72, 12 of 8192 of 64 163 / 133 / 95 / 74 / 47 / 33 / 33; with 1 / 2 / 3 / 4: 80 of 2048 of 128 89 / 81 / 66 / 73, 96 of 4096 of 64 90 / 81 / 79 / 73,
 // of 1024 of 128 48 / 51 / 54 / 54; 128 of 4096 of 128 182 / 179 / 179 / 182; 192 of 2048 of 128 118 / 147 / 153 / 154.
-int segments_of(int64_t units, int64_t T) {
-    const int64_t chunks = (T + CHUNK - 1) / CHUNK, each = device_compute_units() / std::max<int64_t>(units, 1);
-    if (each < 2 || chunks < (each == 2 ? 32 : 4)) return 1;
-    const int64_t wanted = std::min(each, chunks / 2), of = (chunks + wanted - 1) / wanted;
-    return (int)((chunks + of - 1) / of);
+void cut(Call& call, int64_t units, int64_t T) {
+    const int64_t chunks = (T + CHUNK - 1) / CHUNK, cus = device_compute_units(), each = cus / std::max<int64_t>(units, 1);
+    const int64_t wanted = each < 2 || chunks < (each == 2 ? 32 : 4) ? 1 : std::min(each, chunks / 2);
+    const int64_t of = std::max<int64_t>((chunks + wanted - 1) / wanted, 1);
+    call.segments = std::max((int)((chunks + of - 1) / of), 1);
+    call.segment = (int)of * CHUNK;
+    // The states' pass takes half a segment a workgroup where that, too, gives each CU one at most, which is with two segments (us, whole / half: 96 chains of 4096 of
+    // 128 147 / 132, of 64 79 / 69, 128 of 4096 of 128 171 / 163); more workgroups than CUs lose (80 of 4096 of 128 117 / 121, 16 of 8192 of 128 64 / 72).
+    call.halved = of >= 4 && 2 * units * (call.segments - 1) <= cus;
+    call.half = (int)((of + 1) / 2) * CHUNK;
 }
 size_t states_bytes(int64_t units, int64_t T, int64_t Da, int64_t Dc) {
-    return (size_t)units * (segments_of(units, T) - 1) * Da * Dc * sizeof(float);
+    Call call{};
+    cut(call, units, T);
+    return (size_t)units * call.slots() * Da * Dc * sizeof(float);
 }
 void cut(Call& call, float* workspace) {
-    const int64_t chunks = (call.T + CHUNK - 1) / CHUNK;
-    call.segments = segments_of((int64_t)call.chains * call.B * call.P * call.H, call.T);
-    call.segment = (int)((chunks + call.segments - 1) / call.segments) * CHUNK;
+    cut(call, (int64_t)call.chains * call.B * call.P * call.H, call.T);
     call.segment_states = workspace;
-    // A workgroup adds up to fourteen segments' states by itself: a launch costs what it saves there (us, by itself / by a launch: 11 segments 42 / 42 and
+    // A workgroup adds up to fourteen slots by itself: a launch costs what it saves there (us, by itself / by a launch: 11 segments 42 / 42 and
     // 79 / 80, 16 71 / 70 and 38 / 35, 32 91 / 73).
-    call.joined = call.segments > 15;
+    call.joined = !call.halved && call.slots() > 14;
 }
 
 bool any_null(std::initializer_list<const void*> pointers) {

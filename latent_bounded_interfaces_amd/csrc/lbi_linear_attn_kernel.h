@@ -182,7 +182,7 @@ __device__ __forceinline__ bool unit_of(const Call& call, int segments, Unit& u)
 // Two tiles of b; of c one and a's and the scores, or two of c where only the state is wanted.
 template <int DA, int DC, bool OUT> constexpr int lds_bytes() { return CHUNK * 2 * (OUT ? 3 * DA + DC + CHUNK : 2 * (DA + DC)); }
 
-// OUT false: only the state that a segment leaves behind, from zero, into its slot.
+// OUT false: only the state that a segment, or half of one, leaves behind, from zero, into its slot.
 template <typename T, int DA, int DC, bool VEC, bool OUT, int PLANES>
 __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chunk_kernel(Call call) {
     constexpr bool HALF = std::is_same_v<T, _Float16>;
@@ -191,10 +191,11 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     extern __shared__ __align__(16) char lds[];  // b, b, c, a, the scores; b, b, c, c
     __shared__ float score_up[4];
     Unit u;
-    if (!unit_of(call, OUT ? call.segments : call.segments - 1, u)) return;
+    if (!unit_of(call, OUT ? call.segments : call.slots(), u)) return;
     const Chain& ch = call.chain[u.chain];
     const int n = length_of(call, u.b), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-    const int begin = u.segment * call.segment, end = begin + call.segment < n ? begin + call.segment : n;  // of the tokens that count
+    const int begin = OUT ? u.segment * call.segment : call.slot_at(u.segment), stop = OUT ? begin + call.segment : call.slot_at(u.segment + 1);
+    const int end = stop < n ? stop : n;  // of the tokens that count
     auto at = [&](const View& v) { return static_cast<const T*>(v.p) + u.b * v.sb + u.p * v.sp + (u.h / v.group) * v.sh; };
     const bool reverse = ch.reverse != 0;
     const float rate = rate_of(call, u.h), rate2 = rate * LOG2E;
@@ -272,10 +273,12 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             state_at(ch.first.p + u.b * ch.first.sb + u.p * ch.first.sp + u.h * ch.first.sh, (unsigned)ch.first.sr, (unsigned)ch.first.sc,
                      [&](float, float v) __attribute__((always_inline)) { return v * scale; });
         }
-        const float* slots = call.segment_states + (int64_t)u.number * (call.segments - 1) * Da * Dc;
-        for (int s = call.joined ? u.segment - 1 : 0; s >= 0 && s < u.segment; ++s) {  // what the segments before add, the first one first
-            int tokens = n - s * call.segment;
-            tokens = tokens < 0 ? 0 : tokens > call.segment ? call.segment : tokens;
+        const float* slots = call.segment_states + (int64_t)u.number * call.slots() * Da * Dc;
+        const int before = u.segment << call.halved;
+        for (int s = call.joined ? before - 1 : 0; s >= 0 && s < before; ++s) {  // what the slots before add, the first one first
+            const int from = call.slot_at(s), most = call.slot_at(s + 1) - from;
+            int tokens = n - from;
+            tokens = tokens < 0 ? 0 : tokens > most ? most : tokens;
             const float left = call.joined ? -1.0f : expm1f(rate * (float)tokens);
             state_at(slots + (int64_t)s * Da * Dc, (unsigned)Dc, 1, [&](float x_, float v) __attribute__((always_inline)) { return fmaf(x_, left, x_) + v; });
         }
@@ -511,9 +514,9 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     if (from < end) chunk(std::false_type{});
     if constexpr (OUT) {  // rows behind the sequence
         T* const out = const_cast<T*>(at(ch.out));
-        const int stop = begin + call.segment < call.T ? begin + call.segment : call.T, past = begin > n ? begin : n;
+        const int last = stop < call.T ? stop : call.T, past = begin > n ? begin : n;
         const int c8 = (int)threadIdx.x % (DC / 8) * 8;
-        for (int i = past + (int)threadIdx.x / (DC / 8); i < stop; i += 256 / (DC / 8)) {
+        for (int i = past + (int)threadIdx.x / (DC / 8); i < last; i += 256 / (DC / 8)) {
             T* const row = out + i * out_st + c8;
             if (VEC && c8 < Dc) *reinterpret_cast<u32x4*>(row) = u32x4{0, 0, 0, 0};
             if constexpr (!VEC)
@@ -533,14 +536,14 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         if (ch.last.p && u.segment == call.segments - 1)
             leave(ch.last.p + u.b * ch.last.sb + u.p * ch.last.sp + u.h * ch.last.sh, (unsigned)ch.last.sr, (unsigned)ch.last.sc, ch.last_scale);
     } else {
-        leave(call.segment_states + ((int64_t)u.number * (call.segments - 1) + u.segment) * Da * Dc, (unsigned)Dc, 1, 1.0f);
+        leave(call.segment_states + ((int64_t)u.number * call.slots() + u.segment) * Da * Dc, (unsigned)Dc, 1, 1.0f);
     }
 }
 
 // Slot s of each unit holds what segment s adds; they become the states behind the segments.  BATCH slots are asked for at once.
 template <typename T> __global__ __launch_bounds__(256) void join_kernel(Call call) {
     constexpr int BATCH = 8;
-    const int of_chain = call.B * call.P * call.H, slots = call.segments - 1;
+    const int of_chain = call.B * call.P * call.H, slots = call.slots();
     int id = (int)blockIdx.y;
     const int number = id;
     const Chain& ch = call.chain[id / of_chain];

@@ -20,7 +20,7 @@ template <typename T, int DA, int DC, bool VEC, int PLANES>
 int launch(const Call& call, hipStream_t stream) {
     const int64_t units = (int64_t)call.chains * call.B * call.P * call.H;
     if (call.segments > 1) {
-        if (int rc = launch_chunks<T, DA, DC, VEC, false, PLANES>(call, units * (call.segments - 1), stream)) return rc;
+        if (int rc = launch_chunks<T, DA, DC, VEC, false, PLANES>(call, units * call.slots(), stream)) return rc;
         if (call.joined) {
             const int elements = call.chain[0].Da * call.chain[0].Dc;
             hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)((elements + 255) / 256), (unsigned)units), dim3(256), 0, stream, call);

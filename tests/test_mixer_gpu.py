@@ -300,6 +300,34 @@ def test_pullback_with_lengths(device, dtype):
             assert (t[n, :, :, int(lengths[n]):] == 0).all()
 
 
+# chains that are cut in two, whose states come in halves; in three; and in so many that a launch joins their states
+@pytest.mark.parametrize("bsz, heads, seqlen", [(4, 24, 2100), (5, 16, 1500), (5, 1, 2500)])
+def test_long_sequences_of_some_length_in_many_chains(device, bsz, heads, seqlen):
+    gen = torch.Generator().manual_seed(29)
+    lengths = torch.tensor([0, 1100, seqlen, 40, 700][:bsz])
+    q, k, v, log_decay, first = inputs(gen, bsz, heads, heads, seqlen, 32, 24, BF16, state=True)
+    for n in range(bsz):
+        k[n, :, int(lengths[n]):] = math.nan
+    out, final = linear_attention(*on(device, q, k, v, log_decay), scale=0.3, state=first.to(device), lengths=lengths.to(device))
+    check_forward(q, k, v, log_decay, first, lengths, 0.3, out, final)
+    for n in range(bsz):
+        assert (out[n, :, int(lengths[n]):] == 0).all()
+
+
+@pytest.mark.parametrize("bsz, heads, seqlen", [(4, 8, 2100), (3, 1, 2500)])
+def test_pullback_of_long_sequences_of_some_length(device, bsz, heads, seqlen):
+    gen = torch.Generator().manual_seed(30)
+    lengths = torch.tensor([0, 1100, seqlen, 40][4 - bsz:])
+    q, k, v, log_decay, first = inputs(gen, bsz, heads, heads, seqlen, 16, 16, BF16, state=True)
+    g, g_state = rand(gen, bsz, 1, heads, seqlen, 16, dtype=BF16), rand(gen, bsz, 1, heads, 16, 16, dtype=F32)
+    for n in range(bsz):
+        q[n, :, int(lengths[n]):] = math.nan
+        g[n, :, :, int(lengths[n]):] = math.inf
+    got = linear_attention_input_pullback_basis(*on(device, q, k, v, g, log_decay), scale=0.2, state=first.to(device), g_state=g_state.to(device),
+                                                lengths=lengths.to(device))
+    check_pullback(q, k, v, g, log_decay, 0.2, first, g_state, lengths, got)
+
+
 @pytest.mark.parametrize("seqlen", [0, 3])
 @pytest.mark.parametrize("bsz", [0, 2])
 def test_nothing_to_do(device, bsz, seqlen):
