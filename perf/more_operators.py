@@ -331,7 +331,7 @@ def _norms_backward(s):
     pulled = opened * post
     g_branch = inv * (pulled - unit * (unit * pulled).mean(dim=-1, keepdim=True))
     grads = [g_branch.to(dtype), (s["residual_scale"] * total).to(stream)]
-    if s["gate"] is not None and s["gate"].shape == s["branch"].shape:
+    if s["case"]["gate"] == "position":
         grads.append((total * unit * post).to(dtype))
     elif s["case"]["gate"] == "sequence":
         grads.append((total * unit * post).sum(dim=1, keepdim=True))
