@@ -5,8 +5,10 @@
 //   1  wave w: the scores of tokens i = 16 w ... 16 w + 15 with all j <= i, times l^(i-j), rounded to 16 bits into LDS
 //   2  every wave: X^T a^T of its columns, the readout of the state in front of the chunk
 //   3  behind a barrier: out^T = l^(i+1) readout + c^T scores^T, from registers and the scores alone
-//   4  every wave: X = l^64 X + b^T (l^(63-j) c), the decayed c in planes of 16 bits that add up to 16 or 24 significant bits (22 in half precision), while
-//      the results go out
+//   4  every wave: X = l^64 X + b^T (l^(63-j) c), the decayed c in planes of 16 bits that add up to 16 or 24 significant bits, while
+//      the results go out.  In half precision, whose numbers end at 2^-24, a column's decayed c are brought into range by a power of two of their own: 22 bits of
+//      values down to 2^-16 of the column's largest, 2^-38 of that below.  Their sum over the chunk comes in that power and joins X with it taken out (without:
+//      0.002 ... 0.005 of an fp32 state of values of 1e-5; with: us, 512 chains of 4096 tokens of 128 471 -> 483, split ones 105 -> 116).
 // b has two tiles in LDS and the next chunk's comes in from the start of this one; a and c have one, which is free behind 2's barrier.  72 KB for heads of
 // 128, so that two workgroups share a CU, whose vector work then runs beside the other's products.
 //
@@ -50,18 +52,28 @@ template <> struct Mma16<_Float16> {
     }
 };
 
-// The power of two that brings values of up to `most` below 2^14, as (down, up): half precision ends at 65504, and the sums of linear
+// The power of two that brings values of up to `most` below 2^14: half precision ends at 65504, and the sums of linear
 // attention, which no softmax bounds, do not.  At most 2^60 down: what rounds off then is below 2^-85, and the quotient of two of them stays finite.
-struct Pow2 { float down, up; };
+struct Pow2 {
+    int e;
+    __device__ __forceinline__ float down() const { return __uint_as_float((unsigned)(127 - e) << 23); }
+    __device__ __forceinline__ float up() const { return __uint_as_float((unsigned)(127 + e) << 23); }
+};
 __device__ __forceinline__ Pow2 into_range(float most) {
     int e = (int)(__float_as_uint(most) >> 23) - 127 - 13;
     e = e < -60 ? -60 : e > 100 ? 0 : e;  // infinities and NaN as they are
-    return Pow2{__uint_as_float((unsigned)(127 - e) << 23), __uint_as_float((unsigned)(127 + e) << 23)};
+    return Pow2{e};
 }
 __device__ __forceinline__ float over_wave_max(float x) {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
     return x;
+}
+
+// Over the lanes that hold one column of an operand's tokens or of a state.
+__device__ __forceinline__ float over_rows_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
 }
 
 __device__ __forceinline__ int length_of(const Call& call, int b) {
@@ -313,13 +325,29 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
             for (int j = 0; j < NT; ++j) raw[ks][j] = in_c.template turned<NT>(tc, ks, col0, j);
         u32x4 plane[2][PLANES][NT];
+        auto left = [&](int ks, int at_e) __attribute__((always_inline)) {
+            const int tokens = count - 1 - (32 * ks + 8 * g + at_e);
+            return !WHOLE ? exp2f(rate2 * (float)((tokens < 0 ? 0 : tokens) + shift)) : ks == 0 ? keep[at_e] * l32 : keep[at_e];
+        };
+        Pow2 decayed_by[NT];  // half precision: of this lane's columns
+        auto decayed_into_range = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                float most = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const unsigned word = raw[ks][j][e / 2];
+                        most = fmaxf(most, fabsf((e % 2 ? Mma<T>::hi(word) : Mma<T>::lo(word)) * left(ks, e)));
+                    }
+                decayed_by[j] = into_range(over_rows_max(most));
+            }
+        };
         // words e of the decayed c of step ks, column tile j
         auto decay = [&](int ks, int j, int e) __attribute__((always_inline)) {
-            auto left = [&](int at_e) __attribute__((always_inline)) {
-                const int tokens = count - 1 - (32 * ks + 8 * g + at_e);
-                return !WHOLE ? exp2f(rate2 * (float)((tokens < 0 ? 0 : tokens) + shift)) : ks == 0 ? keep[at_e] * l32 : keep[at_e];
-            };
-            float lo = Mma<T>::lo(raw[ks][j][e]) * left(2 * e), hi = Mma<T>::hi(raw[ks][j][e]) * left(2 * e + 1);
+            float lo = Mma<T>::lo(raw[ks][j][e]) * left(ks, 2 * e), hi = Mma<T>::hi(raw[ks][j][e]) * left(ks, 2 * e + 1);
+            if constexpr (HALF) lo *= decayed_by[j].down(), hi *= decayed_by[j].down();
 #pragma unroll
             for (int q = 0; q < PLANES; ++q) {
                 const unsigned word = Mma<T>::pack2(lo, hi);
@@ -336,7 +364,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         };
 
         f32x4 acc[NT][4];
-        Pow2 state_by = {1.0f, 1.0f};
+        Pow2 state_by = {0};
         if constexpr (OUT) {
             f32x4 s[4];
 #pragma unroll
@@ -356,7 +384,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             auto pack = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const f32x4 lo = x[2 * ks][j] * state_by.down, hi = x[2 * ks + 1][j] * state_by.down;
+                    const f32x4 lo = x[2 * ks][j] * state_by.down(), hi = x[2 * ks + 1][j] * state_by.down();
                     state[ks & 1][j] = u32x4{Mma<T>::pack2(lo[0], lo[1]), Mma<T>::pack2(lo[2], lo[3]), Mma<T>::pack2(hi[0], hi[1]), Mma<T>::pack2(hi[2], hi[3])};
                 }
                 move_on(2 * ks);
@@ -378,14 +406,19 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 }
             if constexpr (HALF) {
                 const Pow2 by = into_range(over_wave_max(most));
-                if ((threadIdx.x & 63) == 0) score_up[w] = by.up;
+                if ((threadIdx.x & 63) == 0) score_up[w] = by.up();
 #pragma unroll
-                for (int t = 0; t < 4; ++t) s[t] *= by.down;
+                for (int t = 0; t < 4; ++t) s[t] *= by.down();
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t)
                 *(__attribute__((address_space(3))) u32x2*)(tp + (in_p.split_ ^ (t << 5)) + w * 32 * CHUNK) =
                     u32x2{Mma<T>::pack2(s[t][0], s[t][1]), Mma<T>::pack2(s[t][2], s[t][3])};
+            if constexpr (HALF) {
+                if constexpr (!VEC) LBI_PHASE_FENCE();
+                decayed_into_range();
+                if constexpr (!VEC) LBI_PHASE_FENCE();
+            }
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -420,8 +453,9 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                     for (int t = 0; t < EARLY; ++t) tokens[t] = more[t];
             }
         } else {
+            if constexpr (HALF) decayed_into_range();
 #pragma unroll
-            for (int p = 0; p < 4 * NT; ++p) decay(0, p / 4, p % 4);
+            for (int p = 0; p < (HALF ? 8 : 4) * NT; ++p) decay(p / (4 * NT), p / 4 % NT, p % 4);
 #pragma unroll
             for (int i = 0; i < MT; ++i) move_on(i);
         }
@@ -468,7 +502,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 float by = read0 * (t == 0 ? 1.0f : t == 1 ? l16 : t == 2 ? l32 : l48);
-                if constexpr (HALF) by *= state_by.up / score_up[t];
+                if constexpr (HALF) by *= state_by.up() / score_up[t];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[j][t] *= by;
             }
@@ -478,20 +512,40 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 for (int t = 2 * ks; t < 4; ++t)
 #pragma unroll
                     for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(raw[ks][j], scores[ks][t], acc[j][t]);
+            if constexpr (HALF) {
+                if constexpr (!VEC) LBI_PHASE_FENCE();
+#pragma unroll
+                for (int p = 0; p < 4 * NT; ++p) decay(1, p / 4, p % 4);
+            }
             LBI_PHASE_FENCE();
         }
 
+        // In half precision the sum of a chunk comes in the power of two of its decayed values: both steps of a row tile, then onto the state.
+        const auto step_of = [](int step) __attribute__((always_inline)) { return HALF ? step % 2 : step / MT; };
+        const auto tile_of = [](int step) __attribute__((always_inline)) { return HALF ? step / 2 : step % MT; };
         u32x4 rows = in_a.turned(tb, 0, 0);
+        f32x4 added[HALF ? NT : 1];
 #pragma unroll
         for (int step = 0; step < 2 * MT; ++step) {
-            const int ks = step / MT, i = step % MT;
+            const int ks = step_of(step), i = tile_of(step);
             u32x4 more;
-            if (step + 1 < 2 * MT) more = in_a.turned(tb, (step + 1) / MT, 16 * ((step + 1) % MT));
+            if (step + 1 < 2 * MT) more = in_a.turned(tb, step_of(step + 1), 16 * tile_of(step + 1));
+            if (HALF && ks == 0)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) added[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int q = PLANES - 1; q >= 0; --q)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) x[i][j] = Mma16<T>::mma(rows, plane[ks][q][j], x[i][j]);
-            if (ks == 0)
+                for (int j = 0; j < NT; ++j) {
+                    f32x4& sum = HALF ? added[j] : x[i][j];
+                    sum = Mma16<T>::mma(rows, plane[ks][q][j], sum);
+                }
+            if (HALF && ks == 1)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[i][j][r] = fmaf(added[j][r], decayed_by[j].up(), x[i][j][r]);
+            if (!HALF && ks == 0)
 #pragma unroll
                 for (int p = i * 4 * NT / MT; p < (i + 1) * 4 * NT / MT; ++p) decay(1, p / 4, p % 4);
             if constexpr (OUT)
