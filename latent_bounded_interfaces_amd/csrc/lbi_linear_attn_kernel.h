@@ -53,16 +53,16 @@ template <> struct Mma16<_Float16> {
 };
 
 // The power of two that brings values of up to `most` below 2^14: half precision ends at 65504, and the sums of linear
-// attention, which no softmax bounds, do not.  At most 2^60 down: what rounds off then is below 2^-85, and the quotient of two of them stays finite.
+// attention, which no softmax bounds, do not.  Values below the power `least` lose digits; every finite one is taken.
 struct Pow2 {
     int e;
     __device__ __forceinline__ float down() const { return __uint_as_float((unsigned)(127 - e) << 23); }
     __device__ __forceinline__ float up() const { return __uint_as_float((unsigned)(127 + e) << 23); }
 };
-__device__ __forceinline__ Pow2 into_range(float most) {
-    int e = (int)(__float_as_uint(most) >> 23) - 127 - 13;
-    e = e < -60 ? -60 : e > 100 ? 0 : e;  // infinities and NaN as they are
-    return Pow2{e};
+constexpr int LEAST = -100;
+__device__ __forceinline__ Pow2 into_range(float most, int least = LEAST) {
+    const int e = (int)(__float_as_uint(most) >> 23) - 127 - 13;
+    return Pow2{e < least ? least : e > 114 ? 0 : e};  // infinities and NaN as they are
 }
 __device__ __forceinline__ float over_wave_max(float x) {
 #pragma unroll
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     constexpr int KS = DA / 32, MT = DA / 16, NT = DC / 64;  // steps and tiles of the state: rows, this wave's columns
     constexpr int TILE_A = CHUNK * 2 * DA, TILE_C = CHUNK * 2 * DC, AT_C = 2 * TILE_A, AT_A = AT_C + TILE_C, AT_P = AT_A + TILE_A;
     extern __shared__ __align__(16) char lds[];  // b, b, c, a, the scores; b, b, c, c
-    __shared__ float score_up[4];
+    __shared__ int score_by[4];  // half precision: exponents
     Unit u;
     if (!unit_of(call, OUT ? call.segments : call.slots(), u)) return;
     const Chain& ch = call.chain[u.chain];
@@ -244,6 +244,8 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             }
 #pragma unroll
     for (int e = 0; e < 8; ++e) keep[e] = exp2f(rate2 * (float)(31 - 8 * g - e + shift));
+    // half precision: the least power of scores whose inverse times the scale is a number (only a scale of 2^26 and more raises it)
+    const int by_scale = (int)(__float_as_uint(ch.scale) >> 23 & 255) - 126 - 126, least_score = by_scale > LEAST ? by_scale : LEAST;
     float fade = expm1f(rate * (float)CHUNK);  // X + X (l^64 - 1) keeps what rounding l^64 near 1 would add up over many chunks
 
     f32x4 x[MT][NT];
@@ -405,8 +407,8 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                     if constexpr (HALF) most = fmaxf(most, fabsf(s[t][r]));
                 }
             if constexpr (HALF) {
-                const Pow2 by = into_range(over_wave_max(most));
-                if ((threadIdx.x & 63) == 0) score_up[w] = by.up();
+                const Pow2 by = into_range(over_wave_max(most), least_score);
+                if ((threadIdx.x & 63) == 0) score_by[w] = by.e;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) s[t] *= by.down();
             }
@@ -452,6 +454,11 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
                     for (int t = 0; t < EARLY; ++t) tokens[t] = more[t];
             }
+            if constexpr (HALF)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[j][t] *= state_by.up();
         } else {
             if constexpr (HALF) decayed_into_range();
 #pragma unroll
@@ -464,7 +471,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         const auto to = scan_planes::rows(out, 0x7fffffffu);
         auto store = [&](int t) __attribute__((always_inline)) {  // sixteen rows
             const int i = 16 * t + m, row = reverse ? count - 1 - i : i;
-            const float by = HALF ? score_up[t] : 1.0f;
+            const float by = HALF ? Pow2{score_by[t]}.up() : 1.0f;
             unsigned words[2 * NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -502,7 +509,9 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 float by = read0 * (t == 0 ? 1.0f : t == 1 ? l16 : t == 2 ? l32 : l48);
-                if constexpr (HALF) by *= state_by.up() / score_up[t];
+                // Into the scores' power, which what reads the state out has room for (least_score).  A readout that is past fp32 then would be past half
+                // precision as a result: scores of so small a power add less than 2^-64 to it.
+                if constexpr (HALF) by *= Pow2{score_by[t]}.down();
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[j][t] *= by;
             }

@@ -55,3 +55,30 @@ def test_cotangents_of_states_of_small_values(device, shape, basis, of_q, of_g):
         a, b = q.double() * decay[..., None] * scale, g[:, p].double()
         want, sizes = a.mT @ b, a.abs().mT @ b.abs()
         base.close(d_state[:, p], want, (2.0 ** -20 + count * STEP32) * sizes + scale * summed(q.double(), b), "d_state")
+
+
+@pytest.mark.parametrize("power", [60, 82, 100, 113, 120])
+@pytest.mark.parametrize("keys", [0.0, 2.0 ** -20, 1.0])
+def test_large_states_over_tiles_of_small_scores(device, power, keys):
+    """States of 2^power, and queries, keys or both of zero in whole tiles: what is zero stays so, what is finite too."""
+    gen = torch.Generator().manual_seed(42)
+    q, k, v, log_decay, first = base.inputs(gen, 1, 2, 2, 200, 64, 96, F16, state=True)
+    scale, first = 2.0 ** -power, first * 2.0 ** power
+    k[:, :, :130] *= keys
+    q[:, :, 64:128] = 0
+    q[:, :, 140] = 0
+    out, final = linear_attention(*base.on(device, q, k, v, log_decay), scale=scale, state=first.to(device))
+    base.check_forward(q, k, v, log_decay, first, None, scale, out, final)
+    assert (out[:, :, 64:128] == 0).all() and (out[:, :, 140] == 0).all()
+
+
+@pytest.mark.parametrize("power", [30, 84, 110])
+def test_cotangents_of_states_under_a_small_scale(device, power):
+    """The chains of dk and dv begin with the state's cotangent over the scale."""
+    gen = torch.Generator().manual_seed(43)
+    q, k, v, log_decay, first = base.inputs(gen, 1, 2, 2, 150, 64, 64, F16, state=True)
+    q[:, :, :70] = 0
+    g, g_state = base.rand(gen, 1, 1, 2, 150, 64, dtype=F16), base.rand(gen, 1, 1, 2, 64, 64, dtype=F32)
+    scale = 2.0 ** -power
+    got = linear_attention_input_pullback_basis(*base.on(device, q, k, v, g, log_decay), scale=scale, state=first.to(device), g_state=g_state.to(device))
+    base.check_pullback(q, k, v, g, log_decay, scale, first, g_state, None, got)
