@@ -6,9 +6,12 @@
 //   2  every wave: X^T a^T of its columns, the readout of the state in front of the chunk
 //   3  behind a barrier: out^T = l^(i+1) readout + c^T scores^T, from registers and the scores alone
 //   4  every wave: X = l^64 X + b^T (l^(63-j) c), the decayed c in planes of 16 bits that add up to 16 or 24 significant bits, while
-//      the results go out.  In half precision, whose numbers end at 2^-24, a column's decayed c are brought into range by a power of two of their own: 22 bits of
-//      values down to 2^-16 of the column's largest, 2^-38 of that below.  Their sum over the chunk comes in that power and joins X with it taken out (without:
-//      0.002 ... 0.005 of an fp32 state of values of 1e-5; with: us, 512 chains of 4096 tokens of 128 471 -> 483, split ones 105 -> 116).
+//      the results go out
+// Half precision ends at 65504 and 2^-24, so its operands are brought into range by powers of two: a query's scores, a column's copy of the state, and
+// a column's decayed c (22 bits of those down to 2^-16 of the column's largest, 2^-38 of that below), each by its own.  The chunk's sum comes in the last one's
+// power and joins X with it taken out, a readout goes from the second's into the first's.  Without, an fp32 state of values of 1e-5 was off by 0.002 to 0.005 and
+// a column of 2^-39 of its neighbour was lost (us, without / with: 512 chains of 4096 tokens of 128 474 / 483, split ones 105 / 115, a basis of 4 587 / 622).
+// Below 2^-38 of the largest of its sum an operand is lost all the same.
 // b has two tiles in LDS and the next chunk's comes in from the start of this one; a and c have one, which is free behind 2's barrier.  72 KB for heads of
 // 128, so that two workgroups share a CU, whose vector work then runs beside the other's products.
 //
@@ -64,13 +67,7 @@ __device__ __forceinline__ Pow2 into_range(float most, int least = LEAST) {
     const int e = (int)(__float_as_uint(most) >> 23) - 127 - 13;
     return Pow2{e < least ? least : e > 114 ? 0 : e};  // infinities and NaN as they are
 }
-__device__ __forceinline__ float over_wave_max(float x) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
-    return x;
-}
-
-// Over the lanes that hold one column of an operand's tokens or of a state.
+// Over the lanes that hold one column of a state, of an operand's tokens, or one query's scores.
 __device__ __forceinline__ float over_rows_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16, 64));
     return fmaxf(x, __shfl_xor(x, 32, 64));
@@ -201,7 +198,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     constexpr int KS = DA / 32, MT = DA / 16, NT = DC / 64;  // steps and tiles of the state: rows, this wave's columns
     constexpr int TILE_A = CHUNK * 2 * DA, TILE_C = CHUNK * 2 * DC, AT_C = 2 * TILE_A, AT_A = AT_C + TILE_C, AT_P = AT_A + TILE_A;
     extern __shared__ __align__(16) char lds[];  // b, b, c, a, the scores; b, b, c, c
-    __shared__ int score_by[4];  // half precision: exponents
+    __shared__ int score_by[HALF ? CHUNK : 1];  // exponents, a query each
     Unit u;
     if (!unit_of(call, OUT ? call.segments : call.slots(), u)) return;
     const Chain& ch = call.chain[u.chain];
@@ -366,7 +363,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         };
 
         f32x4 acc[NT][4];
-        Pow2 state_by = {0};
+        Pow2 state_by[NT];  // half precision: of this lane's columns
         if constexpr (OUT) {
             f32x4 s[4];
 #pragma unroll
@@ -378,15 +375,22 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 for (int t = 0; t < 4; ++t) s[t] = Mma16<T>::mma(in_a.nat(tb, t, ks), mine, s[t]);
             }
             if constexpr (HALF) {
-                float of_state = 0.0f;
-                each([&](int i, int j, int r) __attribute__((always_inline)) { of_state = fmaxf(of_state, fabsf(x[i][j][r])); });
-                state_by = into_range(over_wave_max(of_state));
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float of_state = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) of_state = fmaxf(of_state, fabsf(x[i][j][r]));
+                    state_by[j] = into_range(over_rows_max(of_state));
+                }
             }
             u32x4 state[2][NT];  // this step's rows of the state as an operand, and the next one's
             auto pack = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const f32x4 lo = x[2 * ks][j] * state_by.down(), hi = x[2 * ks + 1][j] * state_by.down();
+                    const float by = HALF ? state_by[j].down() : 1.0f;
+                    const f32x4 lo = x[2 * ks][j] * by, hi = x[2 * ks + 1][j] * by;
                     state[ks & 1][j] = u32x4{Mma<T>::pack2(lo[0], lo[1]), Mma<T>::pack2(lo[2], lo[3]), Mma<T>::pack2(hi[0], hi[1]), Mma<T>::pack2(hi[2], hi[3])};
                 }
                 move_on(2 * ks);
@@ -407,8 +411,8 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                     if constexpr (HALF) most = fmaxf(most, fabsf(s[t][r]));
                 }
             if constexpr (HALF) {
-                const Pow2 by = into_range(over_wave_max(most), least_score);
-                if ((threadIdx.x & 63) == 0) score_by[w] = by.e;
+                const Pow2 by = into_range(over_rows_max(most), least_score);
+                if (g == 0) score_by[16 * w + m] = by.e;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) s[t] *= by.down();
             }
@@ -417,9 +421,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 *(__attribute__((address_space(3))) u32x2*)(tp + (in_p.split_ ^ (t << 5)) + w * 32 * CHUNK) =
                     u32x2{Mma<T>::pack2(s[t][0], s[t][1]), Mma<T>::pack2(s[t][2], s[t][3])};
             if constexpr (HALF) {
-                if constexpr (!VEC) LBI_PHASE_FENCE();
                 decayed_into_range();
-                if constexpr (!VEC) LBI_PHASE_FENCE();
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j)
@@ -458,7 +460,11 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) acc[j][t] *= state_by.up();
+                    for (int r = 0; r < 4; ++r) {
+                        const float up = Pow2{__shfl(state_by[j].e, 4 * g + r, 64)}.up();  // the state's columns are rows here
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) acc[j][t][r] *= up;
+                    }
         } else {
             if constexpr (HALF) decayed_into_range();
 #pragma unroll
@@ -471,7 +477,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         const auto to = scan_planes::rows(out, 0x7fffffffu);
         auto store = [&](int t) __attribute__((always_inline)) {  // sixteen rows
             const int i = 16 * t + m, row = reverse ? count - 1 - i : i;
-            const float by = HALF ? Pow2{score_by[t]}.up() : 1.0f;
+            const float by = HALF ? Pow2{score_by[16 * t + m]}.up() : 1.0f;
             unsigned words[2 * NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -511,7 +517,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 float by = read0 * (t == 0 ? 1.0f : t == 1 ? l16 : t == 2 ? l32 : l48);
                 // Into the scores' power, which what reads the state out has room for (least_score).  A readout that is past fp32 then would be past half
                 // precision as a result: scores of so small a power add less than 2^-64 to it.
-                if constexpr (HALF) by *= Pow2{score_by[t]}.down();
+                if constexpr (HALF) by *= Pow2{score_by[16 * t + m]}.down();
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[j][t] *= by;
             }

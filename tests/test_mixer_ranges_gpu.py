@@ -82,3 +82,53 @@ def test_cotangents_of_states_under_a_small_scale(device, power):
     scale = 2.0 ** -power
     got = linear_attention_input_pullback_basis(*base.on(device, q, k, v, g, log_decay), scale=scale, state=first.to(device), g_state=g_state.to(device))
     base.check_pullback(q, k, v, g, log_decay, scale, first, g_state, None, got)
+
+
+@pytest.mark.parametrize("dv", [64, 128])
+def test_columns_of_a_state_do_not_share_a_range(device, dv):
+    """Every third column 2^50 times as large, in rows that no query reads."""
+    gen = torch.Generator().manual_seed(44)
+    q, k, v, log_decay, first = base.inputs(gen, 1, 2, 2, 90, 64, dv, F16, state=True)
+    q[..., :32] = 0
+    first[:, :, 32:, ::3] = 0
+    first[:, :, :32, ::3] *= 2.0 ** 50
+    out, final = linear_attention(*base.on(device, q, k, v, log_decay), scale=0.125, state=first.to(device))
+    small = torch.arange(dv) % 3 != 0
+    base.check_forward(q, k, v[..., small], log_decay, first[..., small], None, 0.125, out[..., small], final[..., small])
+    # A large column's own rows do share one: its copy is scaled so that its largest element, which rows that no query reads hold, is 2^13 at least, and ends at 2^-24.
+    # Half a step there is 2^-38 of the largest in each row that is read, on top of what the smaller columns are held to.
+    want, sizes = (oracle.linear_attention(*(f(t.double()) for t in (q, k, v[..., ~small])), log_decay, scale=0.125, state=f(first[..., ~small].double()))[0]
+                   for f in (lambda t: t, torch.abs))
+    lost = 2.0 ** -38 * 0.125 * q.double().abs().sum(-1, keepdim=True) * first[..., ~small].double().abs().amax(-2)[:, :, None]
+    u = base.half_step(F16)
+    # (decayed scores and the copy's own rounding: half a step of each against their magnitudes; the weights and sums: fp32 steps)
+    base.close(out[..., ~small], want, u * (want.abs() + sizes) * (1 + 4 * u) + (2.0 ** -21 + (90 + dv + 16) * STEP32) * sizes + lost + 2.0 ** -24 * (1 + 0.125 * dv),
+               "large columns")
+
+
+def test_queries_do_not_share_a_range(device):
+    """Every second query's scores are 2^41 times as large, with tokens whose values are zero."""
+    gen = torch.Generator().manual_seed(45)
+    q, k, v, log_decay, _ = base.inputs(gen, 1, 2, 2, 150, 64, 64, F16)
+    for t in (q, k):
+        t[:, :, ::2, 1:] = 0
+        t[:, :, ::2, 0] = 1000
+        t[:, :, 1::2, 0] = 0
+        t[:, :, 1::2] *= 2.0 ** -12
+    v[:, :, ::2] = 0
+    v[:, :, 1::2] *= 2.0 ** 13
+    out, final = linear_attention(*base.on(device, q, k, v, log_decay), scale=1.0)
+    base.check_forward(q, k, v, log_decay, None, None, 1.0, out, final)
+    assert (out[:, :, ::2] == 0).all() and out[:, :, 1::2].abs().max() > 2.0 ** -6
+
+
+@pytest.mark.parametrize("power", [40, 100])
+def test_large_scales(device, power):
+    """Keys of zero beside a small state under a large scale."""
+    gen = torch.Generator().manual_seed(46)
+    q, k, v, log_decay, first = base.inputs(gen, 1, 2, 2, 150, 64, 64, F16, state=True)
+    k[:, :, :100] = 0
+    v *= 0
+    scale = 2.0 ** power
+    out, final = linear_attention(*base.on(device, q, k, v, log_decay), scale=scale, state=(first / scale).to(device))
+    base.check_forward(q, k, v, log_decay, first / scale, None, scale, out, final)
