@@ -123,9 +123,11 @@ template <typename T, int DIM, int THREADS, bool VEC> struct Tile {
             }
         } else {
             const T* const from = next + (reverse ? (CHUNK - count) * st : 0);
+            int thread = (int)threadIdx.x;
+            asm volatile("" : "+v"(thread));  // (what is made of it stays in the loop over the chunks: in front of it, each would take a register)
 #pragma unroll
             for (int u = 0; u < N; ++u) {
-                const int id = u * THREADS + (int)threadIdx.x, r = id / PIECES, c = id % PIECES * 8;
+                const int id = u * THREADS + thread, r = id / PIECES, c = id % PIECES * 8;
                 const unsigned short* raw = reinterpret_cast<const unsigned short*>(from + (int64_t)(reverse ? count - 1 - r : r) * st + c);
                 u32x4 words = {0, 0, 0, 0};
                 if (r < count && c + 8 <= dim) words = __builtin_bit_cast(u32x4, *reinterpret_cast<const Anywhere<8>*>(raw));
