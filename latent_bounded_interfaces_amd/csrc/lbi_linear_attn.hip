@@ -72,7 +72,8 @@ int check(const char* who, const lbi_linear_attention_call* call, bool pullback)
     if (c.T >= (int64_t)1 << 30 || c.B >= (int64_t)1 << 20 || c.H >= (int64_t)1 << 16 || basis >= (int64_t)1 << 20 ||
         MOST_CHAINS * c.B * c.H * basis > MOST_UNITS)
         return fail(LBI_ERR_UNSUPPORTED, "%s: too many sequences, heads and directions, or too many tokens", who);
-    if (!std::isfinite(c.scale) || c.scale == 0.0f) return fail(LBI_ERR_INVALID, "%s: scale must be finite and not zero", who);
+    if (!std::isfinite(c.scale) || !std::isfinite(1.0f / c.scale))  // the pullback's chains begin with the state's cotangent over the scale
+        return fail(LBI_ERR_INVALID, "%s: scale must be finite and not zero, and so must its inverse", who);
     return LBI_OK;
 }
 

@@ -13,6 +13,7 @@ grad mode on, or one with a tangent of forward-mode differentiation, raises.  No
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -165,8 +166,8 @@ def _check_attention(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
         raise ValueError(f"{what}: q, k and v must have one dtype")
     if log_decay.shape != (heads,) or log_decay.dtype != torch.float32:
         raise ValueError(f"{what}: log_decay must be [H] in fp32")
-    if scale == 0 or not math.isfinite(scale):
-        raise ValueError(f"{what}: scale must be finite and not zero")
+    if not 2.0 ** -128 < abs(ctypes.c_float(scale).value) < math.inf:  # NaN is neither
+        raise ValueError(f"{what}: scale must be finite and not zero, and so must its inverse, in fp32")
 
 
 def _check_states(what: str, name: str, t: torch.Tensor | None, shape: tuple[int, ...]) -> torch.Tensor | None:
@@ -215,7 +216,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     """``out_t = scale q_t S_t`` with ``S_t = exp(log_decay) S_{t-1} + k_t v_t^T`` and ``S_{-1} = state`` (zero by default).
 
     ``q [B, H, T, Dk]``, ``k [B, Hkv, T, Dk]``, ``v [B, Hkv, T, Dv]`` in fp16 or bf16, of any strides whose last one is 1; ``Hkv`` divides ``H`` and neighbouring
-    heads share; ``Dk, Dv <= 128``.  ``log_decay [H]`` in fp32 is the layer's constant, 0 or less.  ``lengths [B]`` (int32 or int64; clamped to
+    heads share; ``Dk, Dv <= 128``.  ``log_decay [H]`` in fp32 is the layer's constant, 0 or less.  ``scale`` and its inverse are finite in fp32.  ``lengths [B]`` (int32 or int64; clamped to
     ``0 ... T``): the tokens of each sequence that count; those behind them are not read, and the rows of ``out`` there are zero.
 
     Returns ``(out, S)``: ``out [B, H, T, Dv]`` in the dtype of ``q``, laid out as ``[B, T, H, Dv]`` (what an output projection reads, without a copy), and

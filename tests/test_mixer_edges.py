@@ -1,0 +1,46 @@
+"""What linear attention's entry points refuse at the ends of their ranges, without a device."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from latent_bounded_interfaces_amd import _lib
+from latent_bounded_interfaces_amd.hip.transformer import mixer
+
+OK = ctypes.c_void_p(256)  # never dereferenced
+
+
+def call(**changed):
+    sizes = dict(B=2, P=1, H=4, Hkv=2, T=100, Dk=64, Dv=64, q=256, k=256, v=256, q_stride=(25600, 6400, 64), k_stride=(12800, 6400, 64),
+                 v_stride=(12800, 6400, 64), log_decay=256, out=256, out_stride=(25600, 64, 256), state_out=256, g_out=256,
+                 g_out_stride=(25600, 25600, 6400, 64), dq=256, dk=256, dv=256, scale=1.0, dtype=_lib.LBI_BF16)
+    return _lib.LinearAttentionCall(**{**sizes, **changed})
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -128, -(2.0 ** -149), 1e-50, 0.0, math.inf, 1e39, math.nan])
+def test_a_scale_without_an_inverse(scale):
+    lib = _lib.load()
+    for entry in ("lbi_linear_attention", "lbi_linear_attention_pullback"):
+        # (of no sequences: what is not refused has nothing to do)
+        assert getattr(lib, entry)(ctypes.byref(call(B=0, scale=scale)), OK, 1 << 40, None) == -1 and b"scale" in lib.lbi_last_error(), entry
+    h = torch.bfloat16
+    q, k, v, log_decay = torch.zeros(2, 4, 5, 8, dtype=h), torch.zeros(2, 2, 5, 8, dtype=h), torch.zeros(2, 2, 5, 6, dtype=h), torch.zeros(4)
+    with pytest.raises(ValueError, match="scale"):
+        mixer.linear_attention(q, k, v, log_decay, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        mixer.linear_attention_input_pullback_basis(q, k, v, torch.zeros(2, 1, 4, 5, 6, dtype=h), log_decay, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        mixer.linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], log_decay, torch.zeros(2, 4, 8, 6), scale=scale)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -127, 2.0 ** -128 + 2.0 ** -149, -1e-38, 3e38])
+def test_a_scale_with_one(scale):
+    lib = _lib.load()
+    for entry in ("lbi_linear_attention", "lbi_linear_attention_pullback"):
+        assert getattr(lib, entry)(ctypes.byref(call(B=0, scale=scale)), OK, 1 << 40, None) == 0, entry
+    token = torch.zeros(2, 4, 8), torch.zeros(2, 4, 8), torch.zeros(2, 4, 6)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mixer.linear_attention_step(*token, torch.zeros(4), torch.zeros(2, 4, 8, 6), scale=scale)
