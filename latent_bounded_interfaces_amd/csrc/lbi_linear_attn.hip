@@ -19,7 +19,8 @@ int run_f16(const Call& call, hipStream_t stream);
 
 namespace {
 
-constexpr int64_t MOST_UNITS = (int64_t)1 << 28;  // chains of a call: a workgroup each, or a few of a hundred and less
+// Chains of a launch: a workgroup of 256 threads each (several of few only), in eights, and a launch has fewer than 2^32 threads.
+constexpr int64_t MOST_UNITS = ((int64_t)1 << 24) - 8;
 
 int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
     return dtype == LBI_F16 ? run_f16(call, stream) : run_bf16(call, exact_last, stream);
@@ -68,9 +69,9 @@ int check(const char* who, const lbi_linear_attention_call* call, bool pullback)
     if (c.H % c.Hkv) return fail(LBI_ERR_INVALID, "%s: H=%lld not a multiple of Hkv=%lld", who, (long long)c.H, (long long)c.Hkv);
     if (c.dtype != LBI_F16 && c.dtype != LBI_BF16) return fail(dtype_size(c.dtype) ? LBI_ERR_UNSUPPORTED : LBI_ERR_INVALID, "%s: bad dtype %d", who, c.dtype);
     if (c.Dk > MOST_DIM || c.Dv > MOST_DIM) return fail(LBI_ERR_UNSUPPORTED, "%s: head dims of up to %d", who, MOST_DIM);
-    const int64_t basis = pullback ? std::max<int64_t>(c.P, 1) : 1;
+    const int64_t basis = pullback ? std::max<int64_t>(c.P, 1) : 1, chains = !pullback ? 1 : c.Dk == c.Dv ? 3 : 2;
     if (c.T >= (int64_t)1 << 30 || c.B >= (int64_t)1 << 20 || c.H >= (int64_t)1 << 16 || basis >= (int64_t)1 << 20 ||
-        MOST_CHAINS * c.B * c.H * basis > MOST_UNITS)
+        chains * c.B * c.H * basis > MOST_UNITS)
         return fail(LBI_ERR_UNSUPPORTED, "%s: too many sequences, heads and directions, or too many tokens", who);
     if (!std::isfinite(c.scale) || !std::isfinite(1.0f / c.scale))  // the pullback's chains begin with the state's cotangent over the scale
         return fail(LBI_ERR_INVALID, "%s: scale must be finite and not zero, and so must its inverse", who);

@@ -44,3 +44,25 @@ def test_a_scale_with_one(scale):
     token = torch.zeros(2, 4, 8), torch.zeros(2, 4, 8), torch.zeros(2, 4, 6)
     with pytest.raises(RuntimeError, match="CUDA"):
         mixer.linear_attention_step(*token, torch.zeros(4), torch.zeros(2, 4, 8, 6), scale=scale)
+
+
+def test_more_chains_than_a_launch_has_workgroups_for():
+    lib = _lib.load()
+    least = 2 ** 24 - 8  # of 256 threads each, rounded up to eights: fewer than 2^32 threads
+
+    def status(entry, **sizes):
+        # (without log_decay: a call of sizes that are taken goes no further than that)
+        got = getattr(lib, entry)(ctypes.byref(call(**{**dict(T=1, Dk=8, Dv=8, log_decay=None), **sizes})), OK, 1 << 40, None)
+        return got, lib.lbi_last_error()
+
+    for entry, sizes in (("lbi_linear_attention", dict(B=1 << 19, H=64, Hkv=64)), ("lbi_linear_attention", dict(B=1 << 19, H=32, Hkv=1)),
+                         ("lbi_linear_attention_pullback", dict(B=1 << 10, H=16, P=1 << 9)), ("lbi_linear_attention_pullback", dict(B=1 << 10, H=16, P=512, Dv=4))):
+        got, why = status(entry, **sizes)
+        assert got == -2 and b"too many" in why, (entry, sizes)
+        assert getattr(lib, entry + "_workspace_bytes")(ctypes.byref(call(**{**dict(T=1, Dk=8, Dv=8), **sizes}))) == 0
+    for entry, sizes, chains in (("lbi_linear_attention", dict(B=6223, H=2696, Hkv=1), 1), ("lbi_linear_attention_pullback", dict(B=1 << 10, H=16, P=341), 3),
+                                 ("lbi_linear_attention_pullback", dict(B=1 << 10, H=16, P=511, Dv=4), 2)):
+        count = chains * sizes["B"] * sizes["H"] * sizes.get("P", 1)
+        assert 0.99 * least < count <= least
+        got, why = status(entry, **sizes)
+        assert got == -1 and b"null" in why, (entry, sizes)

@@ -132,3 +132,18 @@ def test_large_scales(device, power):
     scale = 2.0 ** power
     out, final = linear_attention(*base.on(device, q, k, v, log_decay), scale=scale, state=(first / scale).to(device))
     base.check_forward(q, k, v, log_decay, first / scale, None, scale, out, final)
+
+
+def test_as_many_chains_as_a_launch_takes(device):
+    """One token of 2^24 - 8 heads: out = scale q k v, state = k v."""
+    bsz, heads = 6223, 2696
+    assert bsz * heads == 2 ** 24 - 8
+    gen = torch.Generator().manual_seed(47)
+    q, k, v = (torch.randint(-8, 9, (bsz, heads, 1, 1), generator=gen).to(base.BF16).to(device) for _ in range(3))
+    log_decay = torch.full((heads,), -0.5, device=device)
+    out, state = linear_attention(q, k, v, log_decay, scale=0.5)
+    # whole numbers of up to 64 and 512, which the scores and the sums hold; one rounding in the results
+    assert torch.equal(state, (k.float() * v.float()))
+    assert torch.equal(out, (q.float() * k.float() * v.float() * 0.5).to(base.BF16))
+    with pytest.raises(RuntimeError, match="too many"):
+        linear_attention(*(torch.cat((t, t[:1])) for t in (q, k, v)), log_decay, scale=0.5)
