@@ -109,13 +109,14 @@ template <typename T, typename R, int GATE, bool MORE, bool TAIL, int NT, int PI
 __global__ __launch_bounds__(NT * SIDE<NT>) void gated_norm_pullback_kernel(const T* g_normed, const T* branch, const R* stream, const R* g_stream,
                                                                             const T* __restrict__ gate, const void* __restrict__ post_weight,
                                                                             const void* __restrict__ weight, T* g_branch, R* g_residual, T* g_gate,
-                                                                            Partials partials, int64_t per_gate, int slabs_per_gate, int slab, int D,
+                                                                            Partials partials, unsigned first_slab, int64_t per_gate, int slabs_per_gate, int slab, int D,
                                                                             float eps, float alpha, int post_wide, int wide) {
     extern __shared__ __align__(16) float lds[];  // SIDE > 1: [SIDE][D]
     __shared__ float spare[2][NT <= 64 ? 1 : NT / 64][3], spare2[2][NT <= 64 ? 1 : NT / 64][1];
     const int threads = NT <= 64 ? NT : (int)blockDim.x, t = threadIdx.x % threads, side = threadIdx.x / threads;
-    const int64_t group = blockIdx.x / slabs_per_gate, ends = (group + 1) * per_gate;
-    const int64_t first = group * per_gate + (int64_t)(blockIdx.x % slabs_per_gate) * slab, last = first + slab < ends ? first + slab : ends;
+    const unsigned own = first_slab + blockIdx.x;
+    const int64_t group = own / slabs_per_gate, ends = (group + 1) * per_gate;
+    const int64_t first = group * per_gate + (int64_t)(own % slabs_per_gate) * slab, last = first + slab < ends ? first + slab : ends;
     struct Row {
         Raw<R> x[PIECES], more[PIECES];
         Raw<T> g[PIECES], b[PIECES], k[PIECES];
@@ -234,13 +235,13 @@ __global__ __launch_bounds__(NT * SIDE<NT>) void gated_norm_pullback_kernel(cons
                 float sum = lds[c];
 #pragma unroll
                 for (int q = 1; q < SIDE<NT>; ++q) sum += lds[q * D + c];
-                to[(size_t)blockIdx.x * D + c] = sum;
+                to[(size_t)own * D + c] = sum;
             }
         } else {
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
                 const int c = (p * threads + t) * PIECE;
-                if (c < D) store8<TAIL>(to + (size_t)blockIdx.x * D + c, total[p], D - c);
+                if (c < D) store8<TAIL>(to + (size_t)own * D + c, total[p], D - c);
             }
         }
     };
@@ -288,12 +289,16 @@ template <typename T, typename R> int pullback(const Pullback& f, hipStream_t st
         constexpr int NT = decltype(form)::NT, PIECES = decltype(form)::PIECES, COUNT = SIDE<NT>;
         const auto launch = [&](auto kernel) {
             const size_t bytes = COUNT > 1 ? COUNT * (size_t)f.D * sizeof(float) : 0;  // 16 KiB at most
-            hipLaunchKernelGGL(kernel, dim3((unsigned)f.plan.slabs()), dim3((unsigned)(threads_of<NT, PIECES>(f.D) * COUNT)), bytes, stream,
-                               static_cast<const T*>(f.g_normed), static_cast<const T*>(f.branch), static_cast<const R*>(f.residual_out),
-                               static_cast<const R*>(f.g_residual_out), static_cast<const T*>(f.gate), f.post_weight, f.weight, static_cast<T*>(f.g_branch),
-                               static_cast<R*>(f.g_residual), static_cast<T*>(f.g_gate), f.partials, f.plan.per_gate, f.plan.slabs_per_gate, f.plan.slab,
-                               (int)f.D, f.eps, f.residual_scale, f.post_wide, f.wide);
-            LBI_HIP_CHECK(hipGetLastError());
+            const int threads = threads_of<NT, PIECES>(f.D) * COUNT;
+            const int64_t slabs = f.plan.slabs(), most = MOST_THREADS / threads;  // slabs of a launch
+            for (int64_t first = 0; first < slabs; first += most) {
+                hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(slabs - first, most)), dim3((unsigned)threads), bytes, stream,
+                                   static_cast<const T*>(f.g_normed), static_cast<const T*>(f.branch), static_cast<const R*>(f.residual_out),
+                                   static_cast<const R*>(f.g_residual_out), static_cast<const T*>(f.gate), f.post_weight, f.weight,
+                                   static_cast<T*>(f.g_branch), static_cast<R*>(f.g_residual), static_cast<T*>(f.g_gate), f.partials, (unsigned)first,
+                                   f.plan.per_gate, f.plan.slabs_per_gate, f.plan.slab, (int)f.D, f.eps, f.residual_scale, f.post_wide, f.wide);
+                LBI_HIP_CHECK(hipGetLastError());
+            }
             return (int)LBI_OK;
         };
         const auto by_gate = [&](auto more, auto tail) {
