@@ -119,20 +119,21 @@ def residual_rmsnorm_pullback(g_normed: torch.Tensor, residual_out: torch.Tensor
     return g_hidden, g_stream, g_weight
 
 
-def _rows_of_gate(what: str, gate: torch.Tensor | None, branch: torch.Tensor) -> int:
-    """Rows of ``branch [..., D]`` for each row of the gate; 0: each has its own."""
+def _rows_of_gate(what: str, gate: torch.Tensor | None, branch: torch.Tensor, sequence_gate: bool = False) -> int:
+    """Rows of ``branch [..., D]`` for each row of the gate; 0: each has its own.  ``sequence_gate``: a gate of the branch's own shape is not that of its rows
+    but of its sequences, which have one row each."""
     if gate is None:
         return 0
     if gate.dtype != branch.dtype:
         raise ValueError(f"{what}: gate must be in the dtype of the branch")
-    if gate.shape == branch.shape and gate.dim() > 1:
+    if gate.shape == branch.shape and gate.dim() > 1 and not sequence_gate:
         return 0
-    if gate.shape == branch.shape[-1:]:
+    if gate.shape == branch.shape[-1:] and not sequence_gate:
         return max(branch.numel() // max(branch.shape[-1], 1), 1)
     if gate.dim() == branch.dim() > 2 and gate.shape[0] == branch.shape[0] and gate.shape[-1] == branch.shape[-1] \
             and all(extent == 1 for extent in gate.shape[1:-1]):
         return max(branch[:1].numel() // max(branch.shape[-1], 1), 1)
-    raise ValueError(f"{what}: gate must be [D], [B, 1, ..., D] or shaped like the branch")
+    raise ValueError(f"{what}: gate must be " + ("[B, 1, ..., D]" if sequence_gate else "[D], [B, 1, ..., D] or shaped like the branch"))
 
 
 def gated_residual_rmsnorm(branch: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor, weight: torch.Tensor, eps: float, *,
@@ -168,14 +169,15 @@ def gated_residual_rmsnorm(branch: torch.Tensor, residual: torch.Tensor, post_we
 
 def gated_residual_rmsnorm_pullback(
         g_normed: torch.Tensor, branch: torch.Tensor, residual_out: torch.Tensor, post_weight: torch.Tensor, weight: torch.Tensor, eps: float, *,
-        gate: torch.Tensor | None = None, residual_scale: float = 1.0, g_residual: torch.Tensor | None = None
+        gate: torch.Tensor | None = None, residual_scale: float = 1.0, g_residual: torch.Tensor | None = None, sequence_gate: bool = False
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor, torch.Tensor]:
     """The cotangents of :func:`gated_residual_rmsnorm` from ``g_normed`` (of its ``y``) and ``g_residual`` (of its ``s``; ``None``: zero), at the
     ``branch`` that it was given and the ``residual_out`` that it returned as ``s``.
 
     Returns ``(g_branch, g_residual_in, g_gate, g_post_weight, g_weight)``: in the dtypes of ``branch`` and ``residual_out``, the gate's shaped like it
     (in its dtype for a gate of each position; otherwise summed over the rows that it gates, in fp32; ``None`` without one), and the weights' in fp32
-    ``[D]``, summed over all rows.  Sums run in a fixed order."""
+    ``[D]``, summed over all rows.  Sums run in a fixed order.  Where sequences have one position a gate of each sequence has the shape of one of each position
+    and is taken for that, unless ``sequence_gate`` says that it is each sequence's: its gradient is then fp32 for any number of positions."""
     what = "gated_residual_rmsnorm_pullback"
     if branch.dim() < 1 or g_normed.shape != branch.shape or residual_out.shape != branch.shape or post_weight.shape != branch.shape[-1:] \
             or weight.shape != branch.shape[-1:]:
@@ -184,7 +186,7 @@ def gated_residual_rmsnorm_pullback(
         raise ValueError(f"{what}: g_normed must be in the dtype of branch")
     if g_residual is not None and (g_residual.shape != branch.shape or g_residual.dtype != residual_out.dtype):
         raise ValueError(f"{what}: g_residual must have the shape and dtype of residual_out")
-    per_gate = _rows_of_gate(what, gate, branch)
+    per_gate = _rows_of_gate(what, gate, branch, sequence_gate)
     _one_device(what, g_normed, branch, residual_out, post_weight, weight, gate, g_residual)
     _lib.refuse_graph(what, g_normed, branch, residual_out, post_weight, weight, gate, g_residual)
     stream = residual_out.dtype

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from latent_bounded_interfaces_amd import _lib
-from latent_bounded_interfaces_amd.hip.transformer import mixer
+from latent_bounded_interfaces_amd.hip.transformer import block, mixer
 
 OK = ctypes.c_void_p(256)  # never dereferenced
 
@@ -66,3 +66,22 @@ def test_more_chains_than_a_launch_has_workgroups_for():
         assert 0.99 * least < count <= least
         got, why = status(entry, **sizes)
         assert got == -1 and b"null" in why, (entry, sizes)
+
+
+def test_how_many_rows_a_gate_has():
+    """The type of a gate's gradient goes by what the gate is of, not by the number of positions."""
+    d = 16
+    for positions in ((1,), (5,), (1, 1), (2, 3)):
+        branch = torch.zeros(3, *positions, d)
+        of_sequence = torch.zeros(3, *[1] * len(positions), d)
+        assert block._rows_of_gate("x", of_sequence, branch, True) == math.prod(positions)
+        assert block._rows_of_gate("x", branch, branch) == 0
+        for gate in (torch.zeros(d), torch.zeros(1, *[1] * len(positions), d), torch.zeros(3, *positions, 1), torch.zeros(3, d)):
+            with pytest.raises(ValueError, match="gate must be"):
+                block._rows_of_gate("x", gate, branch, True)
+    with pytest.raises(ValueError, match="gate must be"):
+        block._rows_of_gate("x", torch.zeros(3, d), torch.zeros(3, d), True)
+    assert block._rows_of_gate("x", None, branch, True) == 0
+    x, w = torch.zeros(2, 3, d), torch.ones(d)
+    with pytest.raises(ValueError, match="gate must be"):
+        block.gated_residual_rmsnorm_pullback(x, x, x, w, w, 1e-5, gate=x, sequence_gate=True)
