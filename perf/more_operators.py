@@ -181,7 +181,7 @@ def _run_own(s):
         return gated_residual_rmsnorm(s["branch"], s["residual"], s["post_weight"], s["weight"], _EPS, gate=s["gate"],
                                       residual_scale=s["residual_scale"])
     grads = gated_residual_rmsnorm_pullback(s["g_normed"], s["branch"], s["residual"], s["post_weight"], s["weight"], _EPS, gate=s["gate"],
-                                            residual_scale=s["residual_scale"], g_residual=s["g_residual"])
+                                            residual_scale=s["residual_scale"], g_residual=s["g_residual"], sequence_gate=case["gate"] == "sequence")
     return tuple(g for g in grads if g is not None)
 
 
