@@ -14,7 +14,7 @@
 namespace lbi {
 namespace linear_attn {
 
-int run_bf16(const Call& call, bool exact_last, hipStream_t stream);
+int run_bf16(const Call& call, bool exact, hipStream_t stream);
 int run_f16(const Call& call, hipStream_t stream);
 
 namespace {
@@ -22,8 +22,8 @@ namespace {
 // Chains of a launch: a workgroup of 256 threads each (several of few only), in eights, and a launch has fewer than 2^32 threads.
 constexpr int64_t MOST_UNITS = ((int64_t)1 << 24) - 8;
 
-int run(const Call& call, int dtype, bool exact_last, hipStream_t stream) {
-    return dtype == LBI_F16 ? run_f16(call, stream) : run_bf16(call, exact_last, stream);
+int run(const Call& call, int dtype, bool exact, hipStream_t stream) {
+    return dtype == LBI_F16 ? run_f16(call, stream) : run_bf16(call, exact, stream);
 }
 
 // Segments that a chain is cut into: as many as give a workgroup to each CU, since one alone on a CU takes a chunk in about 0.6 of the time of two that
@@ -205,7 +205,7 @@ extern "C" int lbi_linear_attention(const lbi_linear_attention_call* c, void* wo
     ch.scale = c->scale;
     ch.Da = (int)c->Dk, ch.Dc = (int)c->Dv, ch.reverse = 0, ch.shift = 0;
     cut(call, static_cast<float*>(workspace));
-    return run(call, c->dtype, c->state_out != nullptr, static_cast<hipStream_t>(stream));
+    return run(call, c->dtype, true, static_cast<hipStream_t>(stream));
 }
 
 extern "C" size_t lbi_linear_attention_pullback_workspace_bytes(const lbi_linear_attention_call* c) {

@@ -221,7 +221,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
     Returns ``(out, S)``: ``out [B, H, T, Dv]`` in the dtype of ``q``, laid out as ``[B, T, H, Dv]`` (what an output projection reads, without a copy), and
     the state ``[B, H, Dk, Dv]`` in fp32 after each sequence's last token, for :func:`linear_attention_step` or the next piece of the context (``None``
-    unless ``return_state``).  Sums are fp32; the decayed scores and a copy of the state are rounded to the dtype as operands.  A value that is
+    unless ``return_state``).  Sums are fp32; the decayed scores and a copy of the state are rounded to the dtype as operands, so ``out`` is
+    off by about 1.4 times what rounding it once would be.  A value that is
     not finite reaches the rows of its 64 tokens (those from a multiple of 64 on; in the pullback's ``dk`` and ``dv`` counted back from the last token),
     earlier ones among them."""
     what = "linear_attention"
@@ -285,7 +286,8 @@ def linear_attention_input_pullback_basis(
     Returns ``dq, dk [B, P, H, T, Dk]`` and ``dv [B, P, H, T, Dv]``, contiguous, in the dtype of ``q``, and the cotangent ``[B, P, H, Dk, Dv]`` of
     ``state`` (``None`` if no ``state`` was given).  Where heads share ``k`` and ``v`` there is a ``dk`` and ``dv`` for each query head, as
     ``attention_input_pullback_basis`` has them: :func:`rotary_heads_pullback` adds them up.  Nothing is kept from the forward pass; the states
-    are recomputed.  Types, strides, ``lengths`` (rows behind them are zero) and roundings as there; ``log_decay`` is a constant."""
+    are recomputed.  Types, strides, ``lengths`` (rows behind them are zero) and roundings as there, and in bf16 without ``state`` the decayed values that a
+    state adds up have 16 significant bits instead of 24; ``log_decay`` is a constant."""
     what = "linear_attention_input_pullback_basis"
     _check_attention(what, q, k, v, log_decay, scale, 1)
     _attention_types(what, q)

@@ -147,3 +147,14 @@ def test_as_many_chains_as_a_launch_takes(device):
     assert torch.equal(out, (q.float() * k.float() * v.float() * 0.5).to(base.BF16))
     with pytest.raises(RuntimeError, match="too many"):
         linear_attention(*(torch.cat((t, t[:1])) for t in (q, k, v)), log_decay, scale=0.5)
+
+
+@pytest.mark.parametrize("dtype", [base.BF16, F16])
+@pytest.mark.parametrize("shape", [(1, 2, 1, 65, 64, 64), (2, 2, 2, 500, 128, 128), (1, 1, 1, 1500, 33, 40), (4, 24, 24, 2100, 32, 24)])
+def test_results_do_not_go_by_whether_the_state_is_returned(device, shape, dtype):
+    gen = torch.Generator().manual_seed(50)
+    q, k, v, log_decay, first = base.on(device, *base.inputs(gen, *shape, dtype, state=True))
+    for state in (None, first):
+        out, _ = linear_attention(q, k, v, log_decay, scale=0.125, state=state)
+        again, nothing = linear_attention(q, k, v, log_decay, scale=0.125, state=state, return_state=False)
+        assert nothing is None and torch.equal(again, out)
