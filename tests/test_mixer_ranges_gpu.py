@@ -158,3 +158,41 @@ def test_results_do_not_go_by_whether_the_state_is_returned(device, shape, dtype
         out, _ = linear_attention(q, k, v, log_decay, scale=0.125, state=state)
         again, nothing = linear_attention(q, k, v, log_decay, scale=0.125, state=state, return_state=False)
         assert nothing is None and torch.equal(again, out)
+
+
+WIDTHS = [(128, 128), (80, 112), (33, 7), (64, 40)]  # the last two: off the 16-byte grid, on it in 64-wide tiles
+
+
+@pytest.mark.parametrize("dtype", [F16, base.BF16])
+@pytest.mark.parametrize("dk, dv", WIDTHS)
+# chains that are cut in two, whose states come in halves; in three; and in so many that a launch joins their states
+@pytest.mark.parametrize("bsz, heads, seqlen", [(4, 24, 2100), (5, 16, 1500), (5, 1, 2500)])
+def test_long_sequences_cut_in_two_in_three_and_in_many(device, bsz, heads, seqlen, dk, dv, dtype):
+    gen = torch.Generator().manual_seed(51)
+    lengths = torch.tensor([0, 1100, seqlen, 40, 700][:bsz])
+    q, k, v, log_decay, first = base.inputs(gen, bsz, heads, heads, seqlen, dk, dv, dtype, state=True)
+    for n in range(bsz):
+        k[n, :, int(lengths[n]):] = float("nan")
+    out, final = linear_attention(*base.on(device, q, k, v, log_decay), scale=0.3, state=first.to(device), lengths=lengths.to(device))
+    for n in range(bsz):
+        assert (out[n, :, int(lengths[n]):] == 0).all()
+    some = [0, heads - 1][:heads]  # each head is a chain of its own
+    base.check_forward(q[:, some], k[:, some], v[:, some], log_decay[some], first[:, some], lengths, 0.3, out[:, some], final[:, some])
+
+
+@pytest.mark.parametrize("dtype", [F16, base.BF16])
+@pytest.mark.parametrize("dk, dv", [(80, 112), (128, 64), (33, 7), (128, 128)])
+@pytest.mark.parametrize("bsz, heads, seqlen", [(4, 12, 2100), (3, 1, 2500)])
+def test_pullback_of_long_sequences_of_unequal_widths(device, bsz, heads, seqlen, dk, dv, dtype):
+    gen = torch.Generator().manual_seed(52)
+    lengths = torch.tensor([0, 1100, seqlen, 40][4 - bsz:])
+    q, k, v, log_decay, first = base.inputs(gen, bsz, heads, heads, seqlen, dk, dv, dtype, state=True)
+    g, g_state = base.rand(gen, bsz, 1, heads, seqlen, dv, dtype=dtype), base.rand(gen, bsz, 1, heads, dk, dv, dtype=F32)
+    for n in range(bsz):
+        q[n, :, int(lengths[n]):] = float("nan")
+        g[n, :, :, int(lengths[n]):] = float("inf")
+    got = linear_attention_input_pullback_basis(*base.on(device, q, k, v, g, log_decay), scale=0.2, state=first.to(device), g_state=g_state.to(device),
+                                                lengths=lengths.to(device))
+    last = [heads - 1]
+    base.check_pullback(q[:, last], k[:, last], v[:, last], g[:, :, last], log_decay[last], 0.2, first[:, last], g_state[:, :, last], lengths,
+                        [t[:, :, last] for t in got])
