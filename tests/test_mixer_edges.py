@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -85,3 +87,34 @@ def test_how_many_rows_a_gate_has():
     x, w = torch.zeros(2, 3, d), torch.ones(d)
     with pytest.raises(ValueError, match="gate must be"):
         block.gated_residual_rmsnorm_pullback(x, x, x, w, w, 1e-5, gate=x, sequence_gate=True)
+
+
+def test_a_packed_call_is_the_structure():
+    """The wrappers pack the call's bytes; the header's structure is what the entry points read."""
+    names = [(name, getattr(kind, "_length_", 1)) for name, kind in _lib.LinearAttentionCall._fields_]
+    whole = [n for n, count in names[:-3] for _ in range(count)]  # 8 bytes each
+    assert [n for n, _ in names[-3:]] == ["scale", "dtype", "lengths_wide"] and len(whole) == 37
+    packed = _lib.pack_linear_attention_call(*range(1000, 1037), 0.75, 2, 1)
+    assert len(packed) == ctypes.sizeof(_lib.LinearAttentionCall)
+    read = _lib.LinearAttentionCall.from_buffer_copy(packed)
+    values = [v for name, count in names[:-3] for v in (list(getattr(read, name)) if count > 1 else [getattr(read, name)])]
+    assert values == list(range(1000, 1037)) and (read.scale, read.dtype, read.lengths_wide) == (0.75, 2, 1)
+    # and in the order in which the wrappers give them
+    q, k, v = (torch.zeros(2, heads, 5, width, dtype=torch.bfloat16) for heads, width in ((4, 8), (2, 8), (2, 6)))
+    log_decay, state, g_state, d_state = torch.zeros(4), torch.zeros(2, 4, 8, 6), torch.zeros(2, 3, 4, 8, 6), torch.zeros(2, 3, 4, 8, 6)
+    lengths, out, state_out = torch.zeros(2, dtype=torch.int64), torch.zeros(2, 5, 4, 6).transpose(1, 2), torch.zeros(2, 4, 8, 6)
+    g, grads = torch.zeros(2, 3, 4, 5, 6), tuple(torch.zeros(2, 3, 4, 5, width) for width in (8, 8, 6))
+    read = _lib.LinearAttentionCall.from_buffer_copy(mixer._call(q, k, v, log_decay, 0.5, state, lengths, basis=3, out=out, state_out=state_out, g_out=g,
+                                                                 g_state=g_state, grads=grads, d_state=d_state))
+    assert [getattr(read, n) for n in ("B", "P", "H", "Hkv", "T", "Dk", "Dv")] == [2, 3, 4, 2, 5, 8, 6]
+    for name, t in dict(q=q, k=k, v=v, log_decay=log_decay, state=state, lengths=lengths, out=out, state_out=state_out, g_out=g, g_state=g_state, dq=grads[0],
+                        dk=grads[1], dv=grads[2], d_state=d_state).items():
+        assert getattr(read, name) == t.data_ptr(), name
+    for name, t in dict(q_stride=q, k_stride=k, v_stride=v, out_stride=out, g_out_stride=g).items():
+        assert list(getattr(read, name)) == list(t.stride()[:-1]), name
+    assert (read.scale, read.dtype, read.lengths_wide) == (0.5, _lib.LBI_BF16, 1)
+    # the header's own order
+    header = (Path(__file__).resolve().parents[1] / "include" / "lbi_hip.h").read_text()
+    body = re.search(r"typedef struct lbi_linear_attention_call \{(.*?)\}", header, re.S)[1]
+    declared = [(m[1], int(m[2] or 1)) for part in body.split(";") for m in re.finditer(r"(\w+)(?:\[(\d)\])?\s*(?:,|$)", part.strip())]
+    assert declared == names
