@@ -359,10 +359,14 @@ __global__ __launch_bounds__(64 * NT, 2) void scan_narrow_kernel(const Tin* __re
             constexpr int ahead_of = RING + (decltype(i)::value + NT - TPS) / NT - 1;   // steps down of the tile that is requested
             advance(i, matrix(r_top - ahead_of), std::integral_constant<int, RING * SPS - 1>{});
         });
-        // as many as the stores of the steps that the first waits count
+        // As many as the stores of the steps that the first waits count.  (The fences keep them apart: of equal stores the compiler makes one, and the first steps
+        // would not wait for their rows.)
         const __amdgpu_buffer_rsrc_t nothing = scan_planes::rows(out, 0);
 #pragma unroll
-        for (int x = 0; x < 4 * CT * RING; ++x) __builtin_amdgcn_raw_buffer_store_b32(0u, nothing, 0, 0, 0);
+        for (int x = 0; x < 4 * CT * RING; ++x) {
+            __builtin_amdgcn_raw_buffer_store_b32(0u, nothing, 0, 0, 0);
+            asm volatile("" ::: "memory");
+        }
     }
     // One step on the first TILES column tiles, the u-th of a trip; CARRY: with the vector, whose rows are dot products of the same
     // elements beside the matrix products.
