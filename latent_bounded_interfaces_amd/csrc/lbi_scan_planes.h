@@ -153,8 +153,10 @@ template <int BASE, int PER, int MOST> __device__ __forceinline__ void wait_youn
     else wait_younger<BASE, PER, MOST - 1>(n);
 }
 
+// (Four wait states and the move before: five lie between a vector instruction that writes a scalar, such as the v_readlane of a spilled one, and a memory instruction
+// that reads it.  The compiler does not see that one here.)
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t src, unsigned lane_offset, unsigned offset, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(lane_offset), "s"(src), "s"(offset)
                  : "memory");

@@ -84,3 +84,38 @@ def test_the_narrow_scans_first_waits_count_stores_that_are_there(listings):
             stores = len(re.findall(r"^\s*buffer_store_dword v\d+, off, s\[\d+:\d+\], 0\s*(?://.*)?$", body, re.M))
             assert stores >= 4 * int(m[2]) * int(m[3]), (symbol, stores)
     assert seen >= 20
+
+
+def _scalars(operand: str) -> range:
+    m = re.match(r"s(?:\[(\d+):(\d+)\]|(\d+))$", operand)
+    if m is None:
+        return range(0)
+    return range(int(m[3]), int(m[3]) + 1) if m[3] else range(int(m[1]), int(m[2]) + 1)
+
+
+def test_scalars_from_vector_instructions_reach_memory_instructions_in_time(listings):
+    """A scalar register that a vector instruction has written (a spilled one that comes back by v_readlane, a v_readfirstlane) may be read by a memory instruction
+    five wait states later at the earliest.  The compiler sees to it, but not for memory instructions in inline assembly."""
+    memory, found = ("buffer_", "global_", "scratch_", "flat_"), 0
+    from_vector = re.compile(r"^\s*v_read(?:first)?lane_b32 s(\d+), .*$", re.M)
+    for listing in listings:
+        text = listing.read_text()
+        for m in from_vector.finditer(text):
+            found += 1
+            register, states, at = int(m[1]), 0, m.end() + 1
+            while states < 5 and at < len(text):
+                end = text.find("\n", at)
+                line = text[at:end].split("//")[0].strip()
+                at = end + 1
+                if line.endswith(":"):
+                    continue
+                op, _, rest = line.partition(" ")
+                if op in ("", "s_endpgm"):
+                    break
+                operands = [part.split(" ")[0] for part in re.split(r",\s*", rest)]
+                if op.startswith(memory):
+                    assert not any(register in _scalars(operand) for operand in operands), (m[0].strip(), line, text[m.start():end])
+                elif op.startswith("s_") and register in _scalars(operands[0]) and not op.startswith("s_cmp"):
+                    break  # a scalar instruction's result is there at once
+                states += int(operands[0], 0) + 1 if op == "s_nop" else 1
+    assert found > 1000
