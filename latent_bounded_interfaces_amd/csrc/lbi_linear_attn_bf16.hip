@@ -9,7 +9,8 @@ namespace linear_attn {
 // is what their error goes by (us, 24 bits / 16: a basis of 4 for 64 heads of 4096 of 128 556 / 502, of 2 307 / 275, one direction for 96 of 1024 of 64 42 / 39; forwards,
 // 64 chains of 4096 of 128 103 / 89, 512 462 / 451, 96 of 1024 of 64 27 / 26).
 int run_bf16(const Call& call, bool exact, hipStream_t stream) {
-    return exact ? by_pieces<bf16_raw, 3>(call, stream) : by_pieces<bf16_raw, 2>(call, stream);
+    if (call.T <= MOST_TWICE) return by_pieces<bf16_raw, 3, true>(call, stream);
+    return exact ? by_pieces<bf16_raw, 3, false>(call, stream) : by_pieces<bf16_raw, 2, false>(call, stream);
 }
 
 }  // namespace linear_attn

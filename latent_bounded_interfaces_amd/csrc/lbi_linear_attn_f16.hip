@@ -4,7 +4,9 @@
 namespace lbi {
 namespace linear_attn {
 
-int run_f16(const Call& call, hipStream_t stream) { return by_pieces<_Float16, 2>(call, stream); }
+int run_f16(const Call& call, hipStream_t stream) {
+    return call.T <= MOST_TWICE ? by_pieces<_Float16, 2, true>(call, stream) : by_pieces<_Float16, 2, false>(call, stream);
+}
 
 }  // namespace linear_attn
 }  // namespace lbi

@@ -12,11 +12,15 @@
 // power and joins X with it taken out, a readout goes from the second's into the first's.  Without, an fp32 state of values of 1e-5 was off by 0.002 to 0.005 and
 // a column of 2^-39 of its neighbour was lost (us, without / with: 512 chains of 4096 tokens of 128 474 / 483, split ones 105 / 115, a basis of 4 587 / 622).
 // Below 2^-38 of the largest of its sum an operand is lost all the same.
+// The scores and the copy of the state are operands of 16 bits, one rounding each, as the inputs are: what they add to the results is as much as rounding the results
+// does (2-norm of the error, bf16 2.35e-3 where that alone is 1.66e-3, half precision 2.9e-4 and 2.1e-4).  In two planes each, results are as near as that one
+// rounding, at 44 more of 124 products a chunk (us, so / in one plane: 96 chains of 1024 tokens of 64 31 / 25, 64 of 4096 of 128 130 / 112, 512 521 / 487, the pullback below
+// 636 / 510); the scores alone in two leave 2.17e-3 (28, 117, 489, 546).  Calls of one chunk, which lose nothing by it, take two.
 // b has two tiles in LDS and the next chunk's comes in from the start of this one; a and c have one, which is free behind 2's barrier.  72 KB for heads of
 // 128, so that two workgroups share a CU, whose vector work then runs beside the other's products.
 //
-// Bound by memory in long calls that fill the chip: 512 chains of 4096 tokens of 128 457 us, 4.7 TB/s, 1024 of 2048 of 64 235 us, 4.6 TB/s, of the 4.9 that a copy
-// reaches.  The pullback of 4 directions for 4 x 16 heads of 4096 of 128, three chains each, takes 470 to 505 us (1.28 GB, 2.6 TB/s): 768 workgroups are one and a
+// Bound by memory in long calls that fill the chip: 512 chains of 4096 tokens of 128 457 to 487 us, 4.4 to 4.7 TB/s, 1024 of 2048 of 64 235 us, 4.6 TB/s, of the 4.9 that
+// a copy reaches.  The pullback of 4 directions for 4 x 16 heads of 4096 of 128, three chains each, takes 464 to 540 us, card by card (1.28 GB, 2.6 TB/s): 768 workgroups are one and a
 // half rounds of the 512 that fit, and a chunk's 124 products and 400 vector instructions a wave take 159 and 129 us of the SIMDs in all.  All tiles
 // asked for behind the last barrier had it at 541 us; a second tile of c instead of b's gained with one workgroup a CU
 // and lost with two; eight waves of 16 columns, priorities of waves, results past the caches (4 to 40 % slower) did not pay.
@@ -193,10 +197,12 @@ __device__ __forceinline__ bool unit_of(const Call& call, int segments, Unit& u)
 // Two tiles of b; of c one and a's and the scores, or two of c where only the state is wanted.
 template <int DA, int DC, bool OUT> constexpr int lds_bytes() { return CHUNK * 2 * (OUT ? 3 * DA + DC + CHUNK : 2 * (DA + DC)); }
 
-// OUT false: only the state that a segment, or half of one, leaves behind, from zero, into its slot.
-template <typename T, int DA, int DC, bool VEC, bool OUT, int PLANES>
+// OUT false: only the state that a segment, or half of one, leaves behind, from zero, into its slot.  TWICE: calls of one chunk, with the scores and the copy of the state in two
+// planes; the scores' second one has the place of b's second tile.
+template <typename T, int DA, int DC, bool VEC, bool OUT, int PLANES, bool TWICE>
 __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chunk_kernel(Call call) {
     constexpr bool HALF = std::is_same_v<T, _Float16>;
+    constexpr int OPERANDS = TWICE ? 2 : 1;  // planes of the scores and of the state's copy
     constexpr int KS = DA / 32, MT = DA / 16, NT = DC / 64;  // steps and tiles of the state: rows, this wave's columns
     constexpr int TILE_A = CHUNK * 2 * DA, TILE_C = CHUNK * 2 * DC, AT_C = 2 * TILE_A, AT_A = AT_C + TILE_C, AT_P = AT_A + TILE_A;
     extern __shared__ __align__(16) char lds[];  // b, b, c, a, the scores; b, b, c, c
@@ -309,11 +315,11 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
     auto chunk = [&](auto whole_tag) __attribute__((always_inline)) {
         constexpr bool WHOLE = decltype(whole_tag)::value;  // 64 tokens
         lds_barrier();  // this chunk's tiles are there
-        const lds_ptr tb = (lds_ptr)lds + stage * TILE_A, tc = (lds_ptr)lds + AT_C + (OUT ? 0 : stage * TILE_C), ta = (lds_ptr)lds + AT_A, tp = (lds_ptr)lds + AT_P;
+        const lds_ptr tb = (lds_ptr)lds + stage * TILE_A, tc = (lds_ptr)lds + AT_C + (OUT ? 0 : stage * TILE_C), ta = (lds_ptr)lds + AT_A, tp = (lds_ptr)lds + AT_P, tp2 = (lds_ptr)lds + TILE_A;
         // (what is made of them stays in this loop: in front of it, each would take a register)
         asm volatile("" : "+v"(in_a.nat_), "+v"(in_a.split_), "+v"(in_a.turned_), "+v"(in_p.nat_), "+v"(in_p.split_), "+v"(NT == 1 ? in_c.turned_ : in_c.halved_));
         const int count = WHOLE ? CHUNK : end - from;
-        const bool more_tokens = WHOLE && from + CHUNK < end;
+        const bool more_tokens = WHOLE && !TWICE && from + CHUNK < end;
         if (more_tokens) {
             bring_b(stage ^ 1, from + CHUNK);
             if (!OUT) bring_rest(stage ^ 1, from + CHUNK);
@@ -387,13 +393,21 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                     state_by[j] = into_range(over_rows_max(of_state));
                 }
             }
-            u32x4 state[2][NT];  // this step's rows of the state as an operand, and the next one's
+            u32x4 state[2][OPERANDS][NT];  // this step's rows of the state as an operand, and the next one's
             auto pack = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const float by = HALF ? state_by[j].down() : 1.0f;
                     const f32x4 lo = x[2 * ks][j] * by, hi = x[2 * ks + 1][j] * by;
-                    state[ks & 1][j] = u32x4{Mma<T>::pack2(lo[0], lo[1]), Mma<T>::pack2(lo[2], lo[3]), Mma<T>::pack2(hi[0], hi[1]), Mma<T>::pack2(hi[2], hi[3])};
+                    float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int q = 0; q < OPERANDS; ++q) {
+                            const unsigned word = Mma<T>::pack2(v[2 * e], v[2 * e + 1]);
+                            state[ks & 1][q][j][e] = word;
+                            v[2 * e] -= Mma<T>::lo(word), v[2 * e + 1] -= Mma<T>::hi(word);
+                        }
                 }
                 move_on(2 * ks);
                 move_on(2 * ks + 1);
@@ -420,8 +434,12 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                *(__attribute__((address_space(3))) u32x2*)(tp + (in_p.split_ ^ (t << 5)) + w * 32 * CHUNK) =
-                    u32x2{Mma<T>::pack2(s[t][0], s[t][1]), Mma<T>::pack2(s[t][2], s[t][3])};
+#pragma unroll
+                for (int q = 0; q < OPERANDS; ++q) {
+                    const u32x2 words = {Mma<T>::pack2(s[t][0], s[t][1]), Mma<T>::pack2(s[t][2], s[t][3])};
+                    *(__attribute__((address_space(3))) u32x2*)((q == 0 ? tp : tp2) + (in_p.split_ ^ (t << 5)) + w * 32 * CHUNK) = words;
+                    s[t] -= f32x4{Mma<T>::lo(words[0]), Mma<T>::hi(words[0]), Mma<T>::lo(words[1]), Mma<T>::hi(words[1])};
+                }
             if constexpr (HALF) {
                 decayed_into_range();
             }
@@ -440,9 +458,11 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
 #pragma unroll
                     for (int t = 0; t < EARLY; ++t) more[t] = in_a.split(ta, t, ks + 1);
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
+                for (int q = OPERANDS - 1; q >= 0; --q)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(state[ks & 1][j], tokens[t], acc[j][t]);
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(state[ks & 1][q][j], tokens[t], acc[j][t]);
                 if (ks + 1 < KS) pack(ks + 1);
 #pragma unroll
                 for (int p = ks * 4 * NT / KS; p < (ks + 1) * 4 * NT / KS; ++p) decay(0, p / 4, p % 4);
@@ -507,11 +527,13 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         if constexpr (OUT) {
             next_out += reverse ? -CHUNK * out_st : CHUNK * out_st;
             lds_barrier();  // the scores are there, and everyone is done with a and c
-            u32x4 scores[2][4];  // (read before the next tiles are asked for, which they would wait behind)
+            u32x4 scores[OPERANDS][2][4];  // (read before the next tiles are asked for, which they would wait behind)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+            for (int q = 0; q < OPERANDS; ++q)
 #pragma unroll
-                for (int t = 2 * ks; t < 4; ++t) scores[ks][t] = in_p.nat(tp, t, ks);
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int t = 2 * ks; t < 4; ++t) scores[q][ks][t] = in_p.nat(q == 0 ? tp : tp2, t, ks);
             LBI_PHASE_FENCE();
             if (more_tokens) bring_rest(0, from + CHUNK);
 #pragma unroll
@@ -524,11 +546,13 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
                 for (int j = 0; j < NT; ++j) acc[j][t] *= by;
             }
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+            for (int q = OPERANDS - 1; q >= 0; --q)
 #pragma unroll
-                for (int t = 2 * ks; t < 4; ++t)
+                for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(raw[ks][j], scores[ks][t], acc[j][t]);
+                    for (int t = 2 * ks; t < 4; ++t)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) acc[j][t] = Mma16<T>::mma(raw[ks][j], scores[q][ks][t], acc[j][t]);
             if constexpr (HALF) {
                 if constexpr (!VEC) LBI_PHASE_FENCE();
 #pragma unroll
@@ -540,6 +564,10 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
         // In half precision the sum of a chunk comes in the power of two of its decayed values: both steps of a row tile, then onto the state.
         const auto step_of = [](int step) __attribute__((always_inline)) { return HALF ? step % 2 : step / MT; };
         const auto tile_of = [](int step) __attribute__((always_inline)) { return HALF ? step / 2 : step % MT; };
+        if (TWICE)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) store(t);
+        if (TWICE && !ch.last.p) return;  // nobody wants the state behind the only chunk
         u32x4 rows = in_a.turned(tb, 0, 0);
         f32x4 added[HALF ? NT : 1];
 #pragma unroll
@@ -565,7 +593,7 @@ __global__ __launch_bounds__(256, OUT && DA == 64 && DC == 64 ? 3 : 2) void chun
             if (!HALF && ks == 0)
 #pragma unroll
                 for (int p = i * 4 * NT / MT; p < (i + 1) * 4 * NT / MT; ++p) decay(1, p / 4, p % 4);
-            if constexpr (OUT)
+            if constexpr (OUT && !TWICE)
                 if (ks == 1 && i < 4) store(i);
             if constexpr (WHOLE)
 #pragma unroll

@@ -196,3 +196,45 @@ def test_pullback_of_long_sequences_of_unequal_widths(device, bsz, heads, seqlen
     last = [heads - 1]
     base.check_pullback(q[:, last], k[:, last], v[:, last], g[:, :, last], log_decay[last], 0.2, first[:, last], g_state[:, :, last], lengths,
                         [t[:, :, last] for t in got])
+
+
+def within_one_rounding(got, want, a, b, c, first, sizes, scale, what):
+    """The result's own rounding and what two planes leave of the scores and of the state's copy: half a step twice over of each, fp32 sums, and in half
+    precision the lower end of the second planes, 2^-38 of the largest score or element of the state."""
+    u = base.half_step(got.dtype)
+    count = c.shape[-2] + c.shape[-1] + a.shape[-1] + 32
+    floor = 0.0
+    if got.dtype == F16:
+        floor = 2.0 ** -25 + 2.0 ** -38 * scale * (a.abs() @ b.abs().mT).amax((-2, -1), keepdim=True) * c.abs().sum(-2, keepdim=True)
+        if first is not None:
+            floor = floor + 2.0 ** -38 * scale * a.abs().sum(-1, keepdim=True) * first.abs().amax((-2, -1), keepdim=True)
+    base.close(got, want, u * want.abs() + (2 * u * u + count * STEP32) * sizes + floor, what)
+
+
+@pytest.mark.parametrize("dtype", [base.BF16, F16])
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("shape", [(1, 2, 2, 1, 64, 64), (3, 2, 2, 2, 128, 128), (2, 3, 3, 17, 33, 7), (1, 2, 2, 64, 128, 64), (2, 2, 2, 63, 48, 120), (1, 1, 1, 64, 1, 1)])
+def test_calls_of_one_chunk_round_their_results_once(device, shape, state, dtype):
+    gen = torch.Generator().manual_seed(53)
+    q, k, v, log_decay, first = base.inputs(gen, *shape, dtype, state=state)
+    bsz, heads, _, seqlen, dk, dv = shape
+    g = base.rand(gen, bsz, 2, heads, seqlen, dv, dtype=dtype)
+    g_state = base.rand(gen, bsz, 2, heads, dk, dv, dtype=F32) if state else None
+    scale = dk ** -0.5
+    dq, dk_, dv_, ds = base.d64(q, k, v, first)
+    want = oracle.linear_attention(dq, dk_, dv_, log_decay, scale=scale, state=ds)[0]
+    sizes = oracle.linear_attention(dq.abs(), dk_.abs(), dv_.abs(), log_decay, scale=scale, state=None if ds is None else ds.abs())[0]
+    moved = base.on(device, q, k, v, log_decay)
+    for return_state in (True, False):
+        out, _ = linear_attention(*moved, scale=scale, state=base.on(device, first)[0], return_state=return_state)
+        within_one_rounding(out, want, dq, dk_, dv_, ds, sizes, scale, "out")
+    got = linear_attention_input_pullback_basis(*moved[:3], g.to(device), moved[3], scale=scale, state=base.on(device, first)[0], g_state=base.on(device, g_state)[0])
+    for p in range(2):
+        results = []
+        for f in (lambda t: t, torch.abs):
+            leaves = [f(t).requires_grad_() for t in (dq.clone(), dk_.clone(), dv_.clone())]
+            o, s = oracle.linear_attention(*leaves, log_decay, scale=scale, state=None if ds is None else f(ds))
+            results.append(torch.autograd.grad((o * f(g[:, p].double())).sum() + (0.0 if g_state is None else (s * f(g_state[:, p].double())).sum()), leaves))
+        gp, gs = g[:, p].double(), None if g_state is None else g_state[:, p].double() / scale
+        for i, (a, b, c, x) in enumerate(((gp, dv_, dk_, None if ds is None else ds.mT), (dv_, gp, dq, None if gs is None else gs.mT), (dk_, dq, gp, gs))):
+            within_one_rounding(got[i][:, p], results[0][i], a, b, c, x, results[1][i], scale, ("dq", "dk", "dv")[i])
