@@ -532,10 +532,14 @@ int lbi_gated_residual_rmsnorm_pullback(const void* g_normed, const void* branch
  *   d_state [B,P,H,Dk,Dv], the cotangent of state (NULL: not wanted).  log_decay is a constant.
  *
  * Products on the 16-bit matrix cores, sums in fp32.  Rounded to 16 bits in between: the decayed scores and a copy of the state, each as an operand
- * (in fp16 brought into range by powers of two, one for each query's scores and each column of the state; what lies below 2^-38 of the largest of them is lost).  The state itself is fp32; the decayed values that it adds up have 24 significant bits, in
- * pullbacks without d_state 16; in fp16 always 22 down to 2^-16 of the largest of their column and 64 tokens, and 2^-38 of that below.  A value that is not finite reaches every row of its 64 tokens (of a multiple of 64 and the 63 behind it, for
- * dk and dv counted back from a sequence's last token), earlier ones too.
- * Dk, Dv up to 128; T below 2^30; B H, in the pullback 3 B P H (2 B P H where Dk and Dv differ), up to 2^24 - 8; scale finite and not 0, and so 1 / scale (g_state / scale is what a chain begins with).  Results overlap no other tensor.  Reruns are bit-identical.
+ * (in fp16 brought into range by powers of two, one for each query's scores and each column of the state; what lies below 2^-38 of the largest of
+ * them is lost); calls of up to 64 tokens keep 16 bits of each (22 in fp16).  The state itself is fp32;
+ * the decayed values that it adds up have 24 significant bits, in longer pullbacks without d_state 16; in fp16 always 22, down to 2^-16 of the largest
+ * of their column and 64 tokens, and 2^-38 of that below.  A value that is not finite reaches every row of its 64 tokens (of a multiple of 64 and
+ * the 63 behind it, for dk and dv counted back from a sequence's last token), earlier ones too.
+ *
+ * Dk, Dv up to 128; T below 2^30; B H, in the pullback 3 B P H (2 B P H where Dk and Dv differ), up to 2^24 - 8; scale finite and not 0, and so
+ * 1 / scale (g_state / scale is what a chain begins with).  Results overlap no other tensor.  Reruns are bit-identical.
  */
 typedef struct lbi_linear_attention_call {
     int64_t B, P, H, Hkv, T, Dk, Dv;

@@ -4,8 +4,9 @@ head, forwards and backwards.
     q, k, v = rotary_heads(in_proj(x));   S_t = exp(log_decay) S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t
 
 Stands beside the softmax attention of this package (``attention_input_pullback_basis``, ``attn_qkv_pullback``): the same tensors, heads and
-bases of cotangents, for a mixer whose state does not grow with the context.  (The reference's second and third backbone mix with a state that
-decays, too; its input pullback for a basis is a stub, cuda/mamba3/__init__.py:4-8.)  The turn is that of the reference's apply_rope
+bases of cotangents, for a mixer whose state does not grow with the context.  A head's decay is a constant of the layer, without a gradient; mixers whose decay depends
+on the token, as those of the reference's second and third backbone (whose input pullback for a basis is a stub there, cuda/mamba3/__init__.py:4-8), are
+not served by it.  The turn is that of the reference's apply_rope
 (backbones/transformer/rope.py:6-34), with part of a head, positions and stretched angles beside it.
 
 Plain functions with explicit pullbacks and no autograd nodes, as in :mod:`.block`: one that is given a tensor that requires grad, with
@@ -222,7 +223,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     Returns ``(out, S)``: ``out [B, H, T, Dv]`` in the dtype of ``q``, laid out as ``[B, T, H, Dv]`` (what an output projection reads, without a copy), and
     the state ``[B, H, Dk, Dv]`` in fp32 after each sequence's last token, for :func:`linear_attention_step` or the next piece of the context (``None``
     unless ``return_state``).  Sums are fp32; the decayed scores and a copy of the state are rounded to the dtype as operands, so ``out`` is
-    off by about 1.4 times what rounding it once would be.  A value that is
+    off by about 1.4 times what rounding it once would be (calls of up to 64 tokens round it once).  A value that is
     not finite reaches the rows of its 64 tokens (those from a multiple of 64 on; in the pullback's ``dk`` and ``dv`` counted back from the last token),
     earlier ones among them."""
     what = "linear_attention"
