@@ -54,5 +54,13 @@ struct Call {
     __host__ __device__ int slot_at(int s) const { return (s >> halved) * segment + (s & halved) * half; }  // the first token of slot s
 };
 
+// l^n x of `log` = n log l: x + x (l^n - 1) near 1, where rounding l^n would add up over many steps, and x l^n from a half on, where what it leaves of x
+// would be lost in the difference.
+struct Fade {
+    float by, kept;
+    __device__ __forceinline__ explicit Fade(float log) : by(log > -0.6931472f ? expm1f(log) : expf(log)), kept(log > -0.6931472f ? 1.0f : 0.0f) {}
+    __device__ __forceinline__ float of(float x) const { return fmaf(x, by, x * kept); }
+};
+
 }  // namespace linear_attn
 }  // namespace lbi

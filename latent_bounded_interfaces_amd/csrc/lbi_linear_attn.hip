@@ -127,15 +127,14 @@ __global__ __launch_bounds__(256) void step_kernel(const T* __restrict__ q, cons
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) vv[e] = to_f32(v[kv * Dv + col + e]);
-        const float l = log_decay[h], fade = expm1f(l);
+        const Fade fade(log_decay[h]);
 #pragma unroll
         for (int i = 0; i < ROUNDS; ++i) {
             const int row = row0 + i * SIDE;
             if (row >= Dk) continue;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                // x + x (l - 1): a decay near 1 is not rounded, which over many tokens would add up
-                x[i][e] = fmaf(kk[i], vv[e], fmaf(x[i][e], fade, x[i][e]));
+                x[i][e] = fmaf(kk[i], vv[e], fade.of(x[i][e]));
                 part[e] = fmaf(qq[i], x[i][e], part[e]);
             }
             *reinterpret_cast<vec*>(s + row * Dv + col) = x[i];

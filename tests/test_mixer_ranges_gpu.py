@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import test_mixer_gpu as base
-from latent_bounded_interfaces_amd.hip.transformer.mixer import linear_attention, linear_attention_input_pullback_basis
+from latent_bounded_interfaces_amd.hip.transformer.mixer import linear_attention, linear_attention_input_pullback_basis, linear_attention_step
 from oracle import mixer_half as oracle
 
 pytestmark = pytest.mark.gpu
@@ -238,3 +238,35 @@ def test_calls_of_one_chunk_round_their_results_once(device, shape, state, dtype
         gp, gs = g[:, p].double(), None if g_state is None else g_state[:, p].double() / scale
         for i, (a, b, c, x) in enumerate(((gp, dv_, dk_, None if ds is None else ds.mT), (dv_, gp, dq, None if gs is None else gs.mT), (dk_, dq, gp, gs))):
             within_one_rounding(got[i][:, p], results[0][i], a, b, c, x, results[1][i], scale, ("dq", "dk", "dv")[i])
+
+
+@pytest.mark.parametrize("dtype", [base.BF16, F16])
+@pytest.mark.parametrize("seqlen", [2, 64, 130, 700, 2500])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_what_a_decay_leaves_of_a_state_keeps_its_digits(device, seqlen, dim, dtype):
+    """Keys of zero: the state is its first times the decay, and the first's cotangent the last's, whatever little that leaves."""
+    gen = torch.Generator().manual_seed(54)
+    total = torch.tensor([-0.01, -0.5, -0.69, -0.7, -3.0, -12.0, -40.0])  # of a whole sequence, in logarithms
+    log_decay, heads = total / seqlen, len(total)
+    q, k, v, _, first = base.inputs(gen, 1, heads, heads, seqlen, dim, dim, dtype, state=True)
+    zero = torch.zeros_like(k)
+    left = (log_decay.double() * seqlen).exp()[:, None, None]
+    # for each of at most a chunk's 64 tokens or a segment: the product's rounding, its factor's (two steps at most), and its logarithm's, half a step of it
+    steps = 4 * (-(-seqlen // 64) + 16) + 2 * total.abs()[:, None, None]
+    _, final = linear_attention(*base.on(device, q, zero, v, log_decay), scale=0.125, state=first.to(device))
+    base.close(final, first.double() * left, steps * STEP32 * first.double().abs() * left, "state")
+    g, g_state = torch.zeros(1, 1, heads, seqlen, dim, dtype=dtype), base.rand(gen, 1, 1, heads, dim, dim, dtype=F32)
+    scale = 0.125  # a power of two: nothing is lost to it and back
+    d_state = linear_attention_input_pullback_basis(*base.on(device, q, k, v, g, log_decay), scale=scale, state=first.to(device), g_state=g_state.to(device))[3]
+    base.close(d_state, g_state.double() * left, steps * STEP32 * g_state.double().abs() * left, "d_state")
+
+
+@pytest.mark.parametrize("decay", [-1e-3, -0.6, -0.7, -2.0, -5.0])
+def test_what_a_decay_leaves_of_a_state_over_tokens(device, decay):
+    gen = torch.Generator().manual_seed(55)
+    q, v, state = base.rand(gen, 2, 3, 64, dtype=F32), base.rand(gen, 2, 3, 64, dtype=F32), base.rand(gen, 2, 3, 64, 64, dtype=F32)
+    mine, log_decay = state.to(device), torch.full((3,), decay)
+    for _ in range(10):
+        linear_attention_step(*base.on(device, q, torch.zeros_like(q), v, log_decay), mine, scale=1.0)
+    want = state.double() * (10 * log_decay[0].double()).exp()
+    base.close(mine, want, 10 * (4 + 2 * abs(decay)) * STEP32 * want.abs(), "state")
