@@ -119,3 +119,21 @@ def test_scalars_from_vector_instructions_reach_memory_instructions_in_time(list
                     break  # a scalar instruction's result is there at once
                 states += int(operands[0], 0) + 1 if op == "s_nop" else 1
     assert found > 1000
+
+
+def test_linear_attentions_waits_count_stores_that_are_there(listings):
+    """At a chunk's end the kernel waits until all but its last four memory operations are done: the results' four stores, behind which the next tiles were asked
+    for before.  Whole chunks and a last one have their own."""
+    seen = 0
+    for listing in listings:
+        if b"linear_attn12chunk_kernel" not in listing.read_bytes():
+            continue
+        for symbol, body in _kernels(listing):
+            m = re.search(r"chunk_kernelI\w+?Li(\d+)ELi(\d+)ELb(\d)ELb(\d)ELi\dELb(\d)E", symbol)
+            if m is None or m.groups()[2:] != ("1", "1", "0"):
+                continue
+            seen += 1
+            width = 4 if m[2] == "128" else 2
+            stores = len(re.findall(rf"^\s*buffer_store_dwordx{width} ", body, re.M))
+            assert stores == 8, (symbol, stores)
+    assert seen == 12  # four widths, three of types and planes

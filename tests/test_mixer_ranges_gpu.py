@@ -270,3 +270,27 @@ def test_what_a_decay_leaves_of_a_state_over_tokens(device, decay):
         linear_attention_step(*base.on(device, q, torch.zeros_like(q), v, log_decay), mine, scale=1.0)
     want = state.double() * (10 * log_decay[0].double()).exp()
     base.close(mine, want, 10 * (4 + 2 * abs(decay)) * STEP32 * want.abs(), "state")
+
+
+@pytest.mark.parametrize("dtype", [base.BF16, F16])
+@pytest.mark.parametrize("dk, dv", [(64, 80), (33, 128)])
+def test_calls_of_one_chunk_of_some_length(device, dk, dv, dtype):
+    gen = torch.Generator().manual_seed(56)
+    lengths, seqlen = torch.tensor([0, 1, 64, 37, 63]), 64
+    q, k, v, log_decay, first = base.inputs(gen, 5, 4, 2, seqlen, dk, dv, dtype, state=True)
+    g, g_state = base.rand(gen, 5, 2, 4, seqlen, dv, dtype=dtype), base.rand(gen, 5, 2, 4, dk, dv, dtype=F32)
+    for n in range(5):
+        for t in (q, k, v):
+            t[n, :, int(lengths[n]):] = float("nan")
+        g[n, :, :, int(lengths[n]):] = float("inf")
+    moved = base.on(device, q, k, v, log_decay)
+    out, final = linear_attention(*moved, scale=0.25, state=first.to(device), lengths=lengths.to(device))
+    base.check_forward(q, k, v, log_decay, first, lengths, 0.25, out, final)
+    for state, last in ((first, g_state), (None, g_state), (first, None)):
+        got = linear_attention_input_pullback_basis(*moved[:3], g.to(device), moved[3], scale=0.25, state=base.on(device, state)[0],
+                                                    g_state=base.on(device, last)[0], lengths=lengths.to(device))
+        base.check_pullback(q, k, v, g, log_decay, 0.25, state, last, lengths, got)
+        for n in range(5):
+            assert all((t[n, ..., int(lengths[n]):, :] == 0).all() for t in got[:3])
+    for n in range(5):
+        assert (out[n, :, int(lengths[n]):] == 0).all()
